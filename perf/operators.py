@@ -13,7 +13,7 @@ projection, with the cache held in 4 bits (VSL_DT_KV4) and with an RMSNorm on ev
 The 4-bit form: 32 consecutive head dims of a position are a block with a step d (7 significant bits, at
 least 2^-14) and a zero point z; the code n (0..15) stands for (n - z) d.  With lo = min(0, x), hi =
 max(0, x) over the block: d = the smallest such number >= (hi - lo) / 15, z = rint(-lo / d), n =
-clamp(rint(x / d) + z, 0, 15).  A cache of `cap` positions (rounded up to P, a multiple of 64) holds, from
+clamp(rint(x / d) + z, 0, 15).  A cache of `cap` positions (rounded up to P, a multiple of 128) holds, from
 its first byte, the codes and then, at a multiple of 256 bytes, the steps (binary16, z in the four low bits):
   K  codes [n_kv][P][hd / 8] words of 8 dims, steps [n_kv][P][hd / 32]
   V  codes [n_kv][P / 8][hd] words of 8 positions, steps [n_kv][P / 8][hd / 32][8]
@@ -138,7 +138,7 @@ def work(case):
 # the 4-bit form in plain torch
 # ---------------------------------------------------------------------------------------------
 def _positions(cap):
-    return (cap + 63) // 64 * 64
+    return (cap + 127) // 128 * 128
 
 
 def _steps_at(nkv, cap, hd):
