@@ -14,7 +14,7 @@
  *    asynchronous on that stream.
  *  - Device pointers are owned by the caller (normally suballocated from a vsl_arena); kernels do
  *    not allocate.  Workspaces are explicit arguments.
- *  - dtype codes: VSL_DT_F32 = 0, VSL_DT_F16 = 1 (IEEE binary16).
+ *  - dtype codes: VSL_DT_F32 = 0, VSL_DT_F16 = 1 (IEEE binary16), VSL_DT_KV4 = 7 (a KV cache in 4 bits).
  *  - Linear weights are row-major [out][in] ("GGUF ne0 = input dim"): y[o] = sum_i W[o*K+i] x[i]
  *    (final_linear.comp:63, feed_forward.comp:45).
  *  - Decode kernels take a device control block (vsl_ctrl) holding the current position, the
@@ -245,7 +245,9 @@ int vsl_qkv_rope_append(const float* x, const float* gamma, float eps, const voi
  * 0..ctrl->pos, GQA kv_head = head*n_kv/n_q): split-KV over `nsplit` chunks with online softmax,
  * then a combine launch.  Workspace: part_o [n_q][nsplit][hd] f32, part_ml [n_q][nsplit][2] f32.
  * fp16 caches of head_dim 128 with more than 8192 positions of capacity run the scores on the
- * matrix cores (the same results to fp32 rounding; faster from about 2K attended positions). */
+ * matrix cores (the same results to fp32 rounding; faster from about 2K attended positions).
+ * kv_dtype VSL_DT_F32, VSL_DT_F16 or VSL_DT_KV4 (both products on the matrix cores, q and the
+ * probabilities as hi / lo fp16 pairs, so |q * scale * log2(e)| < 65504; also below, _noalloc and _window). */
 int vsl_attn_decode(const float* q, const void* kcache, const void* vcache, int kv_dtype, uint32_t n_q,
                     uint32_t n_kv, uint32_t hd, uint32_t cap, float scale, uint32_t nsplit, float* part_o,
                     float* part_ml, float* out, vsl_ctrl* ctrl, void* stream);
@@ -272,6 +274,67 @@ int vsl_attn_decode_window(const float* q, const void* kcache, const void* vcach
                            uint32_t n_kv, uint32_t hd, uint32_t cap, float scale, uint32_t nsplit, float* part_o,
                            float* part_ml, float* out, vsl_ctrl* ctrl, uint32_t window, uint32_t n_global,
                            uint32_t threshold, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * KV cache in 4 bits (VSL_DT_KV4; no reference counterpart: the reference's caches are fp32,
+ * VulkanSymbioteEngine.cpp:22-61).  4.5 bits per value: 32768 positions of an 8-KV-head, 128-dim model
+ * take 37.7 MB per layer instead of 134 MB in fp16, and decode attention is bound by those bytes.
+ *
+ * A block is 32 consecutive head dims of one position.  With lo = min(0, x_i), hi = max(0, x_i) over it:
+ *   d  the smallest number of 7 significant bits >= (hi - lo) / 15, at least 2^-14
+ *   z = rint(-lo / d), 0..15     n_i = clamp(rint(x_i / d) + z, 0, 15)     (ties to even)
+ * and n_i stands for (n_i - z) d: within d / 2 of x_i, and exactly a binary16 value (4 bits times 7
+ * bits), so that the matrix cores multiply what the cache stands for.  A block that holds a NaN or an
+ * infinity, or whose hi - lo exceeds 65280, reads back as NaN in all 32 values.
+ * A K or V cache of `cap` positions, P = cap rounded up to a multiple of 128, is vsl_kv_cache_bytes long,
+ * 256-byte aligned: the codes, then at the next multiple of 256 bytes the steps, 16 bits each (d as
+ * binary16, z in its four low bits, which a d of 7 significant bits leaves free):
+ *   K  codes [n_kv][P][hd/8] words of 8 dims        steps [n_kv][P][hd/32]
+ *   V  codes [n_kv][P/8][hd] words of 8 positions   steps [n_kv][P/8][hd/32][8 positions]
+ * Value e of a word's eight is nibble e/2 + 4 (e%2).  head_dim 64 or 128.  Appends to one cache that may
+ * touch the same 8 positions are ordered by the caller (one stream); positions that a call does not
+ * append keep their bits.
+ * ------------------------------------------------------------------------------------------ */
+enum { VSL_DT_KV4 = 7 };
+/* bytes of one K or V cache: VSL_DT_KV4 as above, VSL_DT_F16 / VSL_DT_F32 [n_kv][cap][hd]; 0 for another
+ * dtype, and for VSL_DT_KV4 with another head_dim */
+uint64_t vsl_kv_cache_bytes(int kv_dtype, uint32_t n_kv, uint32_t cap, uint32_t hd);
+/* Positions pos0 .. pos0 + n - 1 of VSL_DT_KV4 caches as the values they stand for: k_out, v_out
+ * [n_kv][n][hd] fp16 or fp32 (16-byte aligned; exact in either).  A cache and its output may both be
+ * NULL. */
+int vsl_kv4_read(const void* kcache, const void* vcache, uint32_t n_kv, uint32_t cap, uint32_t hd, uint32_t pos0,
+                 uint32_t n, void* k_out, void* v_out, int out_dtype, void* stream);
+
+/* y[N] = W[N][K] RMSNorm(x, gamma) in fp32 (gamma NULL: no norm): the QKV projection of a decode step whose
+ * queries and keys are normed per head, and so cannot be rotated in the projection's epilogue.  W fp32,
+ * fp16 or a block-quantized pack; K % 8 == 0, K <= 32768.  ctrl may be NULL; with ctrl->done nothing is
+ * written. */
+int vsl_norm_gemv(const float* x, const float* gamma, float eps, const void* W, int wdtype, uint32_t N, uint32_t K,
+                  float* y, vsl_ctrl* ctrl, void* stream);
+
+/* Per-head norms of queries and keys, rotation and cache append of S rows of a QKV projection, qkv fp32
+ * [S][(n_q + 2 n_kv) hd], at positions pos0 .. pos0 + S - 1:
+ *   q, k <- q, k / sqrt(mean over hd of the square + eps) * gamma   (q_gamma, k_gamma fp32 [hd]; NULL: not normed)
+ *   q, k rotated by the tables' angles of the position (cos / sin [cap][hd/2], entry j for pair j):
+ *     VSL_ROPE_PAIRS   pairs (2j, 2j + 1), as the reference rotates (fused_matmul_rope.comp:48-81)
+ *     VSL_ROPE_HALVES  pairs (j, j + hd/2)
+ *   q -> q_out [S][n_q][hd] (VSL_DT_F32, VSL_DT_F16 or VSL_DT_F16X2), k and v -> the caches (VSL_DT_F32,
+ *   VSL_DT_F16 or VSL_DT_KV4).
+ * All of it is computed in 64 bits and rounded once: a cached code is that of the exact value, whatever the
+ * number of rows in the call.  head_dim 64 or 128; every pointer 16-byte aligned (VSL_DT_KV4 caches 256);
+ * positions past cap return VSL_E_CAPACITY before anything is launched. */
+enum { VSL_ROPE_PAIRS = 0, VSL_ROPE_HALVES = 1 };
+int vsl_qk_norm_rope_append(const float* qkv, uint32_t S, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t pos0,
+                            const float* q_gamma, const float* k_gamma, float eps, int rope, const float* rope_cos,
+                            const float* rope_sin, void* q_out, int q_dtype, void* kcache, void* vcache, int kv_dtype,
+                            uint32_t cap, void* stream);
+/* The same for the one row of a decode step, at position ctrl->pos: q -> q_out fp32 [n_q * hd].  As
+ * vsl_qkv_rope_append, nothing is written with ctrl->done, and a position past the capacity sets ctrl->done
+ * and ctrl->error instead. */
+int vsl_qk_norm_rope_append_decode(const float* qkv, uint32_t n_q, uint32_t n_kv, uint32_t hd, const float* q_gamma,
+                                   const float* k_gamma, float eps, int rope, const float* rope_cos, const float* rope_sin,
+                                   float* q_out, void* kcache, void* vcache, int kv_dtype, uint32_t cap, vsl_ctrl* ctrl,
+                                   void* stream);
 
 /* y[N] += W[N][K] x[K]  (O projection / FFN down projection with the residual add fused);
  * K % 8 == 0, K <= 32768 */
@@ -402,6 +465,16 @@ int vsl_attn_prefill_window(const void* q, int q_dtype, const void* kcache, cons
                             uint32_t pos0, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t cap, float scale,
                             void* out, int out_dtype, uint32_t window, uint32_t n_global, uint32_t threshold,
                             void* stream);
+
+/* vsl_attn_prefill over VSL_DT_KV4 caches (the rows' own keys and values appended before), and with the
+ * windowed mode.  Other arguments as there. */
+int vsl_attn_prefill_kv4(const void* q, int q_dtype, const void* kcache, const void* vcache, uint32_t S, uint32_t pos0,
+                         uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t cap, float scale, void* out, int out_dtype,
+                         void* stream);
+int vsl_attn_prefill_kv4_window(const void* q, int q_dtype, const void* kcache, const void* vcache, uint32_t S,
+                                uint32_t pos0, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t cap, float scale,
+                                void* out, int out_dtype, uint32_t window, uint32_t n_global, uint32_t threshold,
+                                void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * hipGraph helpers (each decode step is captured once and replayed).

@@ -23,6 +23,8 @@ ENGINE_LIB = os.path.join(LIB_DIR, "libvsl_engine.so")
 VSL_OK, VSL_E_INVALID, VSL_E_HIP, VSL_E_OOM, VSL_E_UNSUPPORTED, VSL_E_CAPACITY = 0, -100, -101, -102, -103, -104
 VSL_DT_F32, VSL_DT_F16, VSL_DT_F16X2, VSL_DT_F16F8 = 0, 1, 2, 3
 VSL_DT_Q8_0, VSL_DT_Q4_0, VSL_DT_Q4_1 = 4, 5, 6  # resident block-quantized weight packs
+VSL_DT_KV4 = 7  # a KV cache in 4 bits
+ROPE_PAIRS, ROPE_HALVES = 0, 1
 VSL_WF_F32, VSL_WF_F16, VSL_WF_Q4_0, VSL_WF_Q4_1, VSL_WF_Q8_0 = 0, 1, 2, 3, 4
 VSL_QL_REFERENCE, VSL_QL_GGML = 0, 1
 GEMM_A_X2, GEMM_C_X2, GEMM_A_F8, GEMM_C_F8 = 0x100, 0x200, 0x400, 0x800
@@ -171,6 +173,16 @@ _HIP_SIGS = {
                                              _P, _I32, _U32, _P, _P, _U64, _P]),
     "vsl_gemm_f16_resid_rmsnorm": (_I32, [_P, _P, _U32, _U32, _U32, _I32, _P, _P, _F32, _P, _I32, _P, _U64, _P]),
     "vsl_attn_prefill": (_I32, [_P, _I32, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _F32, _P, _I32, _P]),
+    "vsl_kv_cache_bytes": (_U64, [_I32, _U32, _U32, _U32]),
+    "vsl_kv4_read": (_I32, [_P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P, _I32, _P]),
+    "vsl_norm_gemv": (_I32, [_P, _P, _F32, _P, _I32, _U32, _U32, _P, _P, _P]),
+    "vsl_qk_norm_rope_append": (_I32, [_P, _U32, _U32, _U32, _U32, _U32, _P, _P, _F32, _I32, _P, _P, _P, _I32, _P, _P,
+                                       _I32, _U32, _P]),
+    "vsl_qk_norm_rope_append_decode": (_I32, [_P, _U32, _U32, _U32, _P, _P, _F32, _I32, _P, _P, _P, _P, _P, _I32, _U32,
+                                              _P, _P]),
+    "vsl_attn_prefill_kv4": (_I32, [_P, _I32, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _F32, _P, _I32, _P]),
+    "vsl_attn_prefill_kv4_window": (_I32, [_P, _I32, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _F32, _P, _I32, _U32,
+                                           _U32, _U32, _P]),
     "vsl_graph_begin": (_I32, [_P]),
     "vsl_graph_end": (_I32, [_P, ctypes.POINTER(_P)]),
     "vsl_graph_launch": (_I32, [_P, _P]),

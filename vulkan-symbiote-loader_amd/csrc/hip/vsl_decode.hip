@@ -1353,6 +1353,19 @@ void launch_attn_w(dim3 grid, hipStream_t s, const float* q, const void* kc, con
                                                                 pml, ctrl, w);
 }
 
+template <int HD>
+int launch_combine(hipStream_t s, uint32_t n_q, const float* po, const float* pml, uint32_t nsplit, float* out,
+                   const vsl_ctrl* ctrl) {
+    if (nsplit <= 32)
+        k_attn_combine<HD, 32><<<n_q, kCombineThreads, 0, s>>>(po, pml, nsplit, out, ctrl);
+    else if (nsplit <= (uint32_t)kFastSplits)
+        k_attn_combine<HD, kFastSplits><<<n_q, kCombineThreads, 0, s>>>(po, pml, nsplit, out, ctrl);
+    else
+        k_attn_combine<HD, 0><<<n_q, kCombineThreads, 0, s>>>(po, pml, nsplit, out, ctrl);
+    HIP_TRY(hipGetLastError());
+    return VSL_OK;
+}
+
 template <class KT, int HD>
 int launch_attn_g(uint32_t G, dim3 grid, hipStream_t s, const float* q, const void* kc, const void* vc, uint32_t n_q,
                   uint32_t n_kv, uint32_t cap, float scale, uint32_t nsplit, float* po, float* pml, float* out,
@@ -1369,14 +1382,7 @@ int launch_attn_g(uint32_t G, dim3 grid, hipStream_t s, const float* q, const vo
         default: return vsl_unsupported("vsl_attn_decode: GQA ratio %u (supported 1..8)", G);
     }
     HIP_TRY(hipGetLastError());
-    if (nsplit <= 32)
-        k_attn_combine<HD, 32><<<n_q, kCombineThreads, 0, s>>>(po, pml, nsplit, out, ctrl);
-    else if (nsplit <= (uint32_t)kFastSplits)
-        k_attn_combine<HD, kFastSplits><<<n_q, kCombineThreads, 0, s>>>(po, pml, nsplit, out, ctrl);
-    else
-        k_attn_combine<HD, 0><<<n_q, kCombineThreads, 0, s>>>(po, pml, nsplit, out, ctrl);
-    HIP_TRY(hipGetLastError());
-    return VSL_OK;
+    return launch_combine<HD>(s, n_q, po, pml, nsplit, out, ctrl);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -2897,7 +2903,17 @@ extern "C" int vsl_qkv_rope_append(const float* x, const float* gamma, float eps
     a.kc = kcache; a.vc = vcache; a.q_out = q_out; a.ctrl = ctrl;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (kv_dtype == VSL_DT_F16) return launch_gemv_w<2, EPI_QKV, WF16>(wdtype, a, 1u << 20, s, "vsl_qkv_rope_append");
+    if (kv_dtype != VSL_DT_F32) return vsl_unsupported("vsl_qkv_rope_append: kv dtype %d", kv_dtype);
     return launch_gemv_w<2, EPI_QKV, WF32>(wdtype, a, 1u << 20, s, "vsl_qkv_rope_append");
+}
+
+extern "C" int vsl_norm_gemv(const float* x, const float* gamma, float eps, const void* W, int wdtype, uint32_t N, uint32_t K,
+                             float* y, vsl_ctrl* ctrl, void* stream) {
+    if (!x || !W || !y) return vsl_invalid("vsl_norm_gemv: null pointer");
+    if (int rc = check_gemv_shape(N, K, "vsl_norm_gemv")) return rc;
+    GemvArgs a{};
+    a.W = W; a.N = N; a.K = K; a.x = x; a.gamma = gamma; a.eps = eps; a.y = y; a.ctrl = ctrl;
+    return launch_gemv_w<2, EPI_STORE>(wdtype, a, 1u << 20, static_cast<hipStream_t>(stream), "vsl_norm_gemv");
 }
 
 static int attn_decode(const float* q, const void* kcache, const void* vcache, int kv_dtype, uint32_t n_q,
@@ -2917,7 +2933,14 @@ static int attn_decode(const float* q, const void* kcache, const void* vcache, i
         if (hd == 128) return launch_attn_g<WF32, 128>(G, grid, s, q, kcache, vcache, n_q, n_kv, cap, scale, nsplit, part_o, part_ml, out, ctrl, w);
         if (hd == 64) return launch_attn_g<WF32, 64>(G, grid, s, q, kcache, vcache, n_q, n_kv, cap, scale, nsplit, part_o, part_ml, out, ctrl, w);
     }
-    return vsl_unsupported("vsl_attn_decode: head_dim %u / kv dtype %d (supported 64,128 / f16,f32)", hd, kv_dtype);
+    if (kv_dtype == VSL_DT_KV4 && (hd == 64 || hd == 128)) {
+        if (const int rc = vsl_kv4_attn_partials(q, kcache, vcache, n_q, n_kv, hd, cap, scale, nsplit, part_o, part_ml, ctrl,
+                                                 w.on, w.win, w.n_glob, w.thr, stream))
+            return rc;
+        return hd == 128 ? launch_combine<128>(s, n_q, part_o, part_ml, nsplit, out, ctrl)
+                         : launch_combine<64>(s, n_q, part_o, part_ml, nsplit, out, ctrl);
+    }
+    return vsl_unsupported("vsl_attn_decode: head_dim %u / kv dtype %d (supported 64,128 / f16,f32,kv4)", hd, kv_dtype);
 }
 
 extern "C" int vsl_attn_decode(const float* q, const void* kcache, const void* vcache, int kv_dtype, uint32_t n_q,

@@ -71,3 +71,9 @@ bool vsl_gemm_rows_direct(void* stream, const void* A, const void* B, uint32_t M
 // aligned, 2 <= B <= 16. Up to kSkinnyOneFragN rows its blocks take 16 rows and 16 waves.
 constexpr uint32_t kSkinnyOneFragN = 6128;
 void vsl_skinny_rows(const void* W, uint32_t N, uint32_t K, const void* X, uint32_t B, void* Y, bool y16, void* stream);
+
+// Decode attention over VSL_DT_KV4 caches (vsl_kv4.hip): the splits' partials as k_attn_decode leaves them. The caller
+// has checked the pointers, n_q % n_kv and nsplit.
+int vsl_kv4_attn_partials(const float* q, const void* kcache, const void* vcache, uint32_t n_q, uint32_t n_kv, uint32_t hd,
+                          uint32_t cap, float scale, uint32_t nsplit, float* part_o, float* part_ml, vsl_ctrl* ctrl, bool window,
+                          uint32_t win, uint32_t n_glob, uint32_t thr, void* stream);
