@@ -47,3 +47,12 @@ __device__ __forceinline__ half8 kv4_word(uint32_t w, const Kv4Step& s) {
 __device__ __forceinline__ half8 kv4_word(uint32_t w, const Kv4Step (&s)[4]) {
     return kv4_join(kv4_pair<0>(w, s[0]), kv4_pair<1>(w, s[1]), kv4_pair<2>(w, s[2]), kv4_pair<3>(w, s[3]));
 }
+
+// Two values rounded to binary16 in one instruction. The pair passes through an empty register asm, so that what is
+// used and what is subtracted from the values are the same rounding.
+__device__ __forceinline__ half2v pack_f16(float a, float b) {
+    typedef float float2v __attribute__((ext_vector_type(2)));
+    half2v h = __builtin_convertvector((float2v{a, b}), half2v);
+    asm volatile("" : "+v"(h));
+    return h;
+}

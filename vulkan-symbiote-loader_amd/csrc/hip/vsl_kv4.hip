@@ -44,6 +44,16 @@ __device__ __forceinline__ double group_sum64(double v) {
     return v;
 }
 
+// 1 / sqrt(x) to within an ulp or two: the hardware's estimate (26 bits or more) and two Newton steps, a third of the
+// instructions of a 64-bit square root and division. 0 for infinite x.
+__device__ __forceinline__ double rsqrt64(double x) {
+    const double r0 = __builtin_amdgcn_rsq(x);
+    double r = r0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) r = fma(0.5 * r, fma(-x * r, r, 1.0), r);
+    return r0 == 0.0 ? 0.0 : r;
+}
+
 // Four consecutive dims of a head's row in one lane (HD / 4 lanes a row): the head's norm and rotation, in 64
 // bits, as the choice of a 4-bit code hangs on values next to a border and is then the same for every number of rows
 // in a call (the vector pipes take 64-bit multiply-adds at the 32-bit rate).
@@ -64,7 +74,7 @@ __device__ __forceinline__ void norm_rotate(const float4v x, const float* gamma,
         double ss = 0.0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) ss = fma((double)x[i], (double)x[i], ss);
-        inv = 1.0 / sqrt(group_sum64<L>(ss) / HD + a.eps);
+        inv = rsqrt64(group_sum64<L>(ss) * (1.0 / HD) + a.eps);
     }
     const size_t row = (size_t)pos * (HD / 2);
     if (!a.halves) {
@@ -99,8 +109,16 @@ __device__ __forceinline__ void norm_rotate(const float4v x, const float* gamma,
     }
 }
 
+// rint(y / d), ties to even, from r = 1 / d to within an ulp or two (|y / d| <= 15): the remainder of the nearest
+// integer to y r is exact (d has 7 significant bits), and tells on which side of a border y / d lies.
+__device__ __forceinline__ double rint_quotient(double y, double d, double r) {
+    const double n = rint(y * r), rem = fma(-n, d, y), a = fabs(rem), h = 0.5 * d;
+    const bool off = a > h || (a == h && ((int)n & 1));
+    return off ? n + copysign(1.0, rem) : n;
+}
+
 // The 4-bit form of a block of 32 dims, four in each of 8 consecutive lanes: this lane's codes; returns the step
-// as stored. d = (hi - lo) / 15 rounded up to 7 significant bits, by a carry out of the 46 bits dropped.
+// as stored.
 __device__ __forceinline__ uint32_t kv4_quantize(const double (&y)[4], uint32_t (&n)[4]) {
     double lo = 0.0, hi = 0.0;
     bool bad = false;
@@ -117,16 +135,24 @@ __device__ __forceinline__ uint32_t kv4_quantize(const double (&y)[4], uint32_t 
     lo = fmin(lo, dpp64<kDppHalfMirror>(lo));
     hi = fmax(hi, dpp64<kDppHalfMirror>(hi));
     const uint64_t b = __builtin_amdgcn_ballot_w64(bad) >> (threadIdx.x & 56);
-    if ((b & 0xFF) != 0 || hi - lo > 65280.0) {
+    const double range = hi - lo;
+    if ((b & 0xFF) != 0 || range > 65280.0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) n[i] = 0;
         return kKv4NaN;
     }
-    constexpr uint64_t low = (1ull << 46) - 1;
-    const uint64_t u = (__builtin_bit_cast(uint64_t, (hi - lo) / 15.0) + low) & ~low;
-    const double d = fmax(__builtin_bit_cast(double, u), 0x1p-14), z = rint(-lo / d);
+    // d: the quotient by 15 cut to 7 significant bits, or the next such number where that is below it (15 times
+    // either is exact)
+    constexpr uint64_t one = 1ull << 46;
+    const uint64_t u = __builtin_bit_cast(uint64_t, range * (1.0 / 15.0)) & ~(one - 1);
+    const double cut = __builtin_bit_cast(double, u);
+    const double d = fmax(15.0 * cut >= range ? cut : __builtin_bit_cast(double, u + one), 0x1p-14);
+    double r = (double)__builtin_amdgcn_rcpf((float)d);  // 1 / d: 23 bits, then two Newton steps
+    r = fma(fma(-d, r, 1.0), r, r);
+    r = fma(fma(-d, r, 1.0), r, r);
+    const double z = rint_quotient(-lo, d, r);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) n[i] = (uint32_t)(int)fmin(fmax(rint(y[i] / d) + z, 0.0), 15.0);
+    for (int i = 0; i < 4; ++i) n[i] = (uint32_t)(int)fmin(fmax(rint_quotient(y[i], d, r) + z, 0.0), 15.0);
     const vsl_half dh = (vsl_half)(float)d;  // exact: 7 bits, 2^-14 .. 4352
     return (uint32_t)__builtin_bit_cast(uint16_t, dh) | (uint32_t)(int)z;
 }
@@ -171,96 +197,79 @@ __device__ __forceinline__ void store_kv(void* cache, size_t off, const double (
         *reinterpret_cast<half4*>(static_cast<vsl_half*>(cache) + off) =
             half4{(vsl_half)(float)y[0], (vsl_half)(float)y[1], (vsl_half)(float)y[2], (vsl_half)(float)y[3]};
 }
-// A lane's four codes of K in its word (two lanes a word: dims 0-3 and 4-7 of eight).
-__device__ __forceinline__ uint32_t k_word(const uint32_t (&n)[4], uint32_t c) {
+// A row of K in 4 bits, `at` its place among the cache's rows; two lanes a word (dims 0-3 and 4-7 of eight).
+template <int HD>
+__device__ __forceinline__ void store_k4(void* cache, uint64_t soff, size_t at, uint32_t c, const double (&y)[4]) {
+    uint32_t n[4];
+    const uint32_t step = kv4_quantize(y, n);
     const uint32_t own = (n[0] | n[1] << 16 | n[2] << 4 | n[3] << 20) << (c & 1 ? 8 : 0);
-    return own | (uint32_t)__builtin_amdgcn_update_dpp(0, (int)own, kDppPair, 0xF, 0xF, false);
+    const uint32_t w = own | (uint32_t)__builtin_amdgcn_update_dpp(0, (int)own, kDppPair, 0xF, 0xF, false);
+    if ((c & 1) == 0) static_cast<uint32_t*>(cache)[at * (HD / 8) + c / 2] = w;
+    if ((c & 7) == 0) reinterpret_cast<uint16_t*>(static_cast<char*>(cache) + soff)[at * (HD / 32) + c / 8] = (uint16_t)step;
 }
 
-// Prompt rows. An item is one head of 8 consecutive positions (an octet of the V words; the first and the last of a
-// call may be partly outside it), HD / 4 lanes, four dims each; consecutive items are consecutive heads, so a wave
-// reads a run of a row. All 8 rows are requested before the first is used.
+// Prompt rows, four dims a lane. The first v_waves waves take one 32-dim block of a V head at the 8 positions of an
+// octet each (8 lanes a position; the first and the last octet of a call may be partly outside it): the codes of a
+// column are joined to its word over the lanes. The others take rows of q and k heads (of all heads with fp16 and
+// fp32 caches), HD / 4 lanes each, neighbouring heads in neighbouring lanes.
 template <int HD, int QM, int KVM>
-__global__ __launch_bounds__(256) void k_append_rows(AppendArgs a) {
+__global__ __launch_bounds__(256) void k_append_rows(AppendArgs a, uint32_t v_waves) {
     constexpr uint32_t L = HD / 4, NB = HD / 32;
-    const uint32_t heads = a.n_q + 2 * a.n_kv, width = heads * HD;
-    const uint64_t t = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    const uint32_t o0 = a.pos0 / 8, n_oct = (a.pos0 + a.S - 1) / 8 - o0 + 1;
-    const uint64_t item = t / L;
-    if (item >= (uint64_t)n_oct * heads) return;
-    const uint32_t h = (uint32_t)(item % heads), oct = o0 + (uint32_t)(item / heads), c = (uint32_t)(t % L);
-    float4v x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const uint32_t s = oct * 8 + e - a.pos0;  // wraps below pos0
-        x[e] = float4v{0.f, 0.f, 0.f, 0.f};
-        if (s < a.S) x[e] = *reinterpret_cast<const float4v*>(a.qkv + (size_t)s * width + h * HD + 4 * c);
-    }
-    const bool is_q = h < a.n_q, is_k = !is_q && h < a.n_q + a.n_kv;
-    const uint32_t kvh = is_q ? 0 : is_k ? h - a.n_q : h - a.n_q - a.n_kv;
+    const uint32_t heads = a.n_q + 2 * a.n_kv, width = heads * HD, lane = threadIdx.x & 63;
     const uint64_t P = kv4_positions(a.cap), soff = kv4_steps_off(a.n_kv, a.cap, HD);
-    if (is_q) {
-        const size_t plane = (size_t)a.S * a.n_q * HD;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (KVM == KV_4 && wave < v_waves) {
+        const uint32_t blk = wave % NB, kvh = wave / NB % a.n_kv, oct = a.pos0 / 8 + wave / NB / a.n_kv;
+        const uint32_t e = lane >> 3, j = lane & 7, s = oct * 8 + e - a.pos0;  // wraps below pos0
+        const bool in = s < a.S;
+        float4v x = {0.f, 0.f, 0.f, 0.f};
+        if (in) x = *reinterpret_cast<const float4v*>(a.qkv + (size_t)s * width + (size_t)(a.n_q + a.n_kv + kvh) * HD + 32 * blk + 4 * j);
+        const double y[4] = {x[0], x[1], x[2], x[3]};
+        uint32_t n[4];
+        const uint32_t step = kv4_quantize(y, n);
+        u32x4 w;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t s = oct * 8 + e - a.pos0;
-            if (s >= a.S) continue;
-            double y[4];
-            norm_rotate<HD>(x[e], a.r.q_gamma, a.r, oct * 8 + e, c, y);
-            store_q<QM>(a.q_out, ((size_t)s * a.n_q + h) * HD + 4 * c, plane, y);
+        for (int i = 0; i < 4; ++i) {
+            uint32_t v = in ? n[i] << kv4_shift(e) : 0u;
+            v |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, false);  // lane ^ 8
+            const auto p16 = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+            v = p16[0] | p16[1];
+            const auto p32 = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+            w[i] = p32[0] | p32[1];
         }
+        if (lane < 8) {
+            u32x4* dst = reinterpret_cast<u32x4*>(static_cast<uint32_t*>(a.vc) + ((size_t)kvh * (P / 8) + oct) * HD + 32 * blk + 4 * j);
+            uint32_t mask = 0;  // of the octet's positions in this call; the others keep their codes
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) mask |= oct * 8 + i - a.pos0 < a.S ? 15u << kv4_shift(i) : 0u;
+            if (~mask) w |= *dst & ~mask;
+            *dst = w;
+        }
+        if (j == 0 && in)
+            reinterpret_cast<uint16_t*>(static_cast<char*>(a.vc) + soff)[(((size_t)kvh * (P / 8) + oct) * NB + blk) * 8 + e] =
+                (uint16_t)step;
         return;
     }
-    void* cache = is_k ? a.kc : a.vc;
-    if constexpr (KVM != KV_4) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t s = oct * 8 + e - a.pos0;
-            if (s >= a.S) continue;
-            double y[4] = {x[e][0], x[e][1], x[e][2], x[e][3]};
-            if (is_k) norm_rotate<HD>(x[e], a.r.k_gamma, a.r, oct * 8 + e, c, y);
-            store_kv<KVM>(cache, ((size_t)kvh * a.cap + oct * 8 + e) * HD + 4 * c, y);
-        }
-    } else {
-        uint16_t* steps = reinterpret_cast<uint16_t*>(static_cast<char*>(cache) + soff);
-        uint32_t step = 0;  // of position c % 8, this lane's to store
-        if (is_k) {
-            uint32_t* codes = static_cast<uint32_t*>(cache) + ((size_t)kvh * P + (size_t)oct * 8) * (HD / 8) + c / 2;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t s = oct * 8 + e - a.pos0;
-                if (s >= a.S) continue;
-                double y[4];
-                uint32_t n[4];
-                norm_rotate<HD>(x[e], a.r.k_gamma, a.r, oct * 8 + e, c, y);
-                const uint32_t st = kv4_quantize(y, n), w = k_word(n, c);
-                if ((c & 7) == (uint32_t)e) step = st;
-                if ((c & 1) == (e & 1u)) codes[e * (HD / 8)] = w;  // both lanes of a pair hold the word
-            }
-            const uint32_t e = c & 7;
-            if (oct * 8 + e - a.pos0 < a.S) steps[((size_t)kvh * P + (size_t)oct * 8 + e) * NB + c / 8] = (uint16_t)step;
-        } else {
-            uint32_t w[4] = {0, 0, 0, 0}, mask = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t s = oct * 8 + e - a.pos0;
-                if (s >= a.S) continue;
-                const double y[4] = {x[e][0], x[e][1], x[e][2], x[e][3]};
-                uint32_t n[4];
-                const uint32_t st = kv4_quantize(y, n);
-                if ((c & 7) == (uint32_t)e) step = st;
-                mask |= 15u << kv4_shift(e);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] |= n[i] << kv4_shift(e);
-            }
-            u32x4* dst = reinterpret_cast<u32x4*>(static_cast<uint32_t*>(cache) + ((size_t)kvh * (P / 8) + oct) * HD + 4 * c);
-            u32x4 v = {w[0], w[1], w[2], w[3]};
-            if (~mask) v |= *dst & ~mask;  // the octet's other positions keep their codes
-            *dst = v;
-            const uint32_t e = c & 7;
-            if (oct * 8 + e - a.pos0 < a.S) steps[(((size_t)kvh * (P / 8) + oct) * NB + c / 8) * 8 + e] = (uint16_t)step;
-        }
+    const uint32_t row_heads = KVM == KV_4 ? a.n_q + a.n_kv : heads, c = lane % L;
+    const uint32_t item = (KVM == KV_4 ? wave - v_waves : wave) * (64 / L);  // the wave's first row of a head
+    uint32_t s = item / row_heads, h = item % row_heads + lane / L;
+    while (h >= row_heads) {
+        h -= row_heads;
+        ++s;
     }
+    if (s >= a.S) return;
+    const uint32_t pos = a.pos0 + s;
+    const float4v x = *reinterpret_cast<const float4v*>(a.qkv + (size_t)s * width + (size_t)h * HD + 4 * c);
+    double y[4] = {x[0], x[1], x[2], x[3]};
+    if (h < a.n_q + a.n_kv) norm_rotate<HD>(x, h < a.n_q ? a.r.q_gamma : a.r.k_gamma, a.r, pos, c, y);
+    if (h < a.n_q) {
+        store_q<QM>(a.q_out, ((size_t)s * a.n_q + h) * HD + 4 * c, (size_t)a.S * a.n_q * HD, y);
+        return;
+    }
+    const bool is_k = h < a.n_q + a.n_kv;
+    const uint32_t kvh = is_k ? h - a.n_q : h - a.n_q - a.n_kv;
+    if constexpr (KVM != KV_4) store_kv<KVM>(is_k ? a.kc : a.vc, ((size_t)kvh * a.cap + pos) * HD + 4 * c, y);
+    else store_k4<HD>(a.kc, soff, (size_t)kvh * P + pos, c, y);
 }
 
 // One row at ctrl->pos, an item a head. The row, and for V the octet's words, are requested at once.
@@ -293,19 +302,19 @@ __global__ __launch_bounds__(64) void k_append_decode(AppendArgs a, vsl_ctrl* ct
     if constexpr (KVM != KV_4) {
         store_kv<KVM>(cache, ((size_t)kvh * a.cap + pos) * HD + 4 * c, y);
     } else {
-        const uint64_t P = kv4_positions(a.cap);
-        uint16_t* steps = reinterpret_cast<uint16_t*>(static_cast<char*>(cache) + kv4_steps_off(a.n_kv, a.cap, HD));
-        uint32_t n[4];
-        const uint32_t step = kv4_quantize(y, n);
+        const uint64_t P = kv4_positions(a.cap), soff = kv4_steps_off(a.n_kv, a.cap, HD);
         if (is_k) {
-            const uint32_t w = k_word(n, c);
-            if ((c & 1) == 0) static_cast<uint32_t*>(cache)[((size_t)kvh * P + pos) * (HD / 8) + c / 2] = w;
-            if ((c & 7) == 0) steps[((size_t)kvh * P + pos) * NB + c / 8] = (uint16_t)step;
+            store_k4<HD>(cache, soff, (size_t)kvh * P + pos, c, y);
         } else {
+            const size_t oct = (size_t)kvh * (P / 8) + pos / 8;
+            u32x4* dst = reinterpret_cast<u32x4*>(static_cast<uint32_t*>(cache) + oct * HD + 4 * c);
+            const u32x4 old = *dst;
             const uint32_t sh = kv4_shift(pos & 7);
-            u32x4* dst = reinterpret_cast<u32x4*>(static_cast<uint32_t*>(cache) + ((size_t)kvh * (P / 8) + pos / 8) * HD + 4 * c);
-            *dst = (*dst & ~(15u << sh)) | (u32x4{n[0], n[1], n[2], n[3]} << sh);
-            if ((c & 7) == 0) steps[(((size_t)kvh * (P / 8) + pos / 8) * NB + c / 8) * 8 + (pos & 7)] = (uint16_t)step;
+            uint32_t n[4];
+            const uint32_t step = kv4_quantize(y, n);
+            *dst = (old & ~(15u << sh)) | (u32x4{n[0], n[1], n[2], n[3]} << sh);
+            if ((c & 7) == 0)
+                reinterpret_cast<uint16_t*>(static_cast<char*>(cache) + soff)[(oct * NB + c / 8) * 8 + (pos & 7)] = (uint16_t)step;
         }
     }
 }
@@ -363,7 +372,10 @@ __global__ __launch_bounds__(256) void k_kv4_read(const char* __restrict__ kc, c
 // decode attention
 // ---------------------------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kDecWaves = 4;
+#ifndef KDEC
+#define KDEC 4
+#endif
+constexpr int kDecWaves = KDEC;
 
 // LDS traffic alone (global loads stay in flight).
 __device__ __forceinline__ void lds_barrier() {
@@ -497,7 +509,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_attn_decode_kv4(const float* __r
             qf[ks][e] = head < (uint32_t)G ? (col < 8 ? hi : lo16) : (vsl_half)0.f;
         }
     }
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, minus_plane = col < 8 ? 0.f : -1.f;
     float4v o[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) o[i] = float4v{0.f, 0.f, 0.f, 0.f};
@@ -541,15 +553,18 @@ __global__ __launch_bounds__(WAVES * 64) void k_attn_decode_kv4(const float* __r
             for (int i = 0; i < NC; ++i) o[i] *= corr;
             m = mn;
         }
+        // columns 0-7 take the hi plane, 8-15 what it leaves: fp16(p - plane * fp16(p)), plane 0 or 1
         half8 pf;
         const float ref = m == -INFINITY ? 0.f : m;  // no score seen yet: every s is -inf (or NaN)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float pr = fast_exp2(s[e] - ref);
-            l += pr;
-            vsl_half hi, lo16;
-            split_f16(pr, hi, lo16);
-            pf[e] = col < 8 ? hi : lo16;
+        for (int e = 0; e < 8; e += 2) {
+            const float p0 = fast_exp2(s[e] - ref), p1 = fast_exp2(s[e + 1] - ref);
+            l += p0;
+            l += p1;
+            const half2v hi = pack_f16(p0, p1);
+            const half2v w = pack_f16(fmaf((float)hi[0], minus_plane, p0), fmaf((float)hi[1], minus_plane, p1));
+            pf[e] = w[0];
+            pf[e + 1] = w[1];
         }
         Kv4Step st[4];
 #pragma unroll
@@ -652,10 +667,10 @@ int check_append(const char* fn, const float* qkv, uint32_t n_q, uint32_t n_kv, 
 }
 
 template <int HD, int QM>
-void launch_rows(uint32_t grid, hipStream_t s, const AppendArgs& a, int kv_dtype) {
-    if (kv_dtype == VSL_DT_KV4) k_append_rows<HD, QM, KV_4><<<grid, 256, 0, s>>>(a);
-    else if (kv_dtype == VSL_DT_F16) k_append_rows<HD, QM, KV_F16><<<grid, 256, 0, s>>>(a);
-    else k_append_rows<HD, QM, KV_F32><<<grid, 256, 0, s>>>(a);
+void launch_rows(uint32_t grid, hipStream_t s, const AppendArgs& a, int kv_dtype, uint32_t v_waves) {
+    if (kv_dtype == VSL_DT_KV4) k_append_rows<HD, QM, KV_4><<<grid, 256, 0, s>>>(a, v_waves);
+    else if (kv_dtype == VSL_DT_F16) k_append_rows<HD, QM, KV_F16><<<grid, 256, 0, s>>>(a, 0);
+    else k_append_rows<HD, QM, KV_F32><<<grid, 256, 0, s>>>(a, 0);
 }
 template <int HD>
 void launch_decode(uint32_t grid, hipStream_t s, const AppendArgs& a, int kv_dtype, vsl_ctrl* ctrl) {
@@ -688,16 +703,18 @@ extern "C" int vsl_qk_norm_rope_append(const float* qkv, uint32_t S, uint32_t n_
     if (S == 0) return VSL_OK;
     const AppendArgs a{qkv, S, n_q, n_kv, pos0, cap, RopeArgs{q_gamma, k_gamma, rope_cos, rope_sin, (double)eps, rope},
                        q_out, kcache, vcache};
-    const uint64_t items = (uint64_t)((pos0 + S - 1) / 8 - pos0 / 8 + 1) * (n_q + 2 * n_kv);
-    const uint64_t blocks = (items * (hd / 4) + 255) / 256;
-    if (blocks > 0x7FFFFFFFull) return vsl_invalid("%s: %u rows in one call", fn, S);
+    const bool kv4 = kv_dtype == VSL_DT_KV4;
+    const uint64_t v_waves = kv4 ? ((uint64_t)(pos0 + S - 1) / 8 - pos0 / 8 + 1) * n_kv * (hd / 32) : 0;
+    const uint64_t rows = (uint64_t)S * (n_q + (kv4 ? 1 : 2) * (uint64_t)n_kv), per_wave = 256 / hd;
+    const uint64_t blocks = (v_waves + (rows + per_wave - 1) / per_wave + 3) / 4;
+    if (blocks > 0x0FFFFFFEull) return vsl_unsupported("%s: %u rows in one call", fn, S);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const uint32_t grid = (uint32_t)blocks;
     auto go = [&](auto hdc) {
         constexpr int HD = decltype(hdc)::value;
-        if (q_dtype == VSL_DT_F32) launch_rows<HD, Q_F32>(grid, s, a, kv_dtype);
-        else if (q_dtype == VSL_DT_F16) launch_rows<HD, Q_F16>(grid, s, a, kv_dtype);
-        else launch_rows<HD, Q_F16X2>(grid, s, a, kv_dtype);
+        if (q_dtype == VSL_DT_F32) launch_rows<HD, Q_F32>(grid, s, a, kv_dtype, (uint32_t)v_waves);
+        else if (q_dtype == VSL_DT_F16) launch_rows<HD, Q_F16>(grid, s, a, kv_dtype, (uint32_t)v_waves);
+        else launch_rows<HD, Q_F16X2>(grid, s, a, kv_dtype, (uint32_t)v_waves);
     };
     if (hd == 128) go(std::integral_constant<int, 128>{});
     else go(std::integral_constant<int, 64>{});

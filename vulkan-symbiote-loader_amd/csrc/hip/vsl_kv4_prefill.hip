@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "vsl_device.h"
@@ -51,7 +52,10 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     const uint32_t h = kvh * G + (blockIdx.y % (G / GB)) * GB + wave % GB;
     const uint32_t s_base = qb * 32, my_s = s_base + (lane & 31), qw = n_q * HD;
     const size_t qplane = (size_t)S * qw;
-    const float sl2 = scale * kLog2e;
+    // scores are scaled within the exponential's argument, which the maximum then needs a positive factor for: a
+    // negative scale negates q, a zero one is a factor that leaves no difference
+    const float sl2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);
+    const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;
     const uint32_t last_s = min(S, s_base + 32) - 1;
     const uint32_t kv_end = pos0 + last_s + 1, my_pos = pos0 + my_s;
     const uint32_t n_tiles = (kv_end + TK - 1) / TK;
@@ -75,61 +79,70 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     const char* Vst = vc + soff + (uint64_t)kvh * P * NB * 2;
 
     // Pair i of a thread: K words 2w, 2w + 1 (16 dims) of a key row, V words of columns 2w, 2w + 1 of an octet.
-    struct Words {
-        uint2 k[NKW], v[NKW];
-        uint32_t ks[NKW];
-        u32x4 vs[NKW];
+    struct KWords {
+        uint2 k[NKW];
+        uint32_t s[NKW];
     };
-    auto k_at = [&](int i, int& row, int& w) {
-        const int P_ = i * NT + tid;
-        row = P_ / (HD / 16);
-        w = P_ % (HD / 16);
+    struct VWords {
+        uint2 v[NKW];
+        u32x4 s[NKW];
     };
-    auto v_at = [&](int i, int& oct, int& w) {
-        const int P_ = i * NT + tid;
-        oct = P_ / (HD / 2);
-        w = P_ % (HD / 2);
-    };
-    auto load = [&](Words& b, uint32_t t) {
+    auto load_k = [&](KWords& b, uint32_t t) {
 #pragma unroll
         for (int i = 0; i < NKW; ++i) {
-            int r, w;
-            k_at(i, r, w);
+            const int r = (i * NT + tid) / (HD / 16), w = (i * NT + tid) % (HD / 16);
             const uint64_t row = (uint64_t)t * TK + r;
             b.k[i] = *reinterpret_cast<const uint2*>(Kc + row * (HD / 2) + 8 * w);
-            b.ks[i] = *reinterpret_cast<const uint16_t*>(Kst + (row * NB + w / 2) * 2);
-            v_at(i, r, w);
-            const uint64_t oct = (uint64_t)t * (TK / 8) + r;
-            b.v[i] = *reinterpret_cast<const uint2*>(Vc + (oct * HD + 2 * w) * 4);
-            b.vs[i] = *reinterpret_cast<const u32x4*>(Vst + (oct * NB + w / 16) * 16);
+            b.s[i] = *reinterpret_cast<const uint16_t*>(Kst + (row * NB + w / 2) * 2);
         }
     };
-    // The tile's values into LDS. What lies past the block's last key is anything: its steps are taken as 0. So is a V
-    // block that stands for NaN, as a NaN would reach rows that do not see it through a product with 0: the
-    // block notes that there was one, and the rows that see it are found at the end.
-    auto expand = [&](const Words& b, int buf, uint32_t t) {
+    auto load_v = [&](VWords& b, uint32_t t) {
 #pragma unroll
         for (int i = 0; i < NKW; ++i) {
-            int r, w;
-            k_at(i, r, w);
-            const uint32_t kst = t * TK + r < kv_end ? b.ks[i] : 0u;
-            const Kv4Step s = kv4_step(kst | kst << 16);
+            const int r = (i * NT + tid) / (HD / 2), w = (i * NT + tid) % (HD / 2);
+            const uint64_t oct = (uint64_t)t * (TK / 8) + r;
+            b.v[i] = *reinterpret_cast<const uint2*>(Vc + (oct * HD + 2 * w) * 4);
+            b.s[i] = *reinterpret_cast<const u32x4*>(Vst + (oct * NB + w / 16) * 16);
+        }
+    };
+    // A tile's values into LDS. What lies past the block's last key is anything: its steps are taken as 0. So is a V
+    // block that stands for NaN, as a NaN would reach rows that do not see it through a product with 0: the
+    // block notes that there was one, and the rows that see it are found at the end.
+    auto expand_k = [&](const KWords& b, int buf, uint32_t t) {
+#pragma unroll
+        for (int i = 0; i < NKW; ++i) {
+            const int r = (i * NT + tid) / (HD / 16), w = (i * NT + tid) % (HD / 16);
+            const uint32_t st = t * TK + r < kv_end ? b.s[i] : 0u;
+            const Kv4Step s = kv4_step(st | st << 16);
             *reinterpret_cast<half8*>(&Ks[buf][sw<HD>(r, 2 * w)]) = kv4_word(b.k[i].x, s);
             *reinterpret_cast<half8*>(&Ks[buf][sw<HD>(r, 2 * w + 1)]) = kv4_word(b.k[i].y, s);
-            v_at(i, r, w);
-            Kv4Step vs[4];
-            bool nan = false;
+        }
+    };
+    auto expand_v = [&](const VWords& b, int buf, uint32_t t) {
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                uint32_t s2 = b.vs[i][p];
-                const uint32_t key = t * TK + 8 * r + 2 * p;
-                if (key >= kv_end) s2 = 0;
-                else if (key + 1 >= kv_end) s2 &= 0xFFFFu;
-                if ((s2 & 0xFFFFu) == kKv4NaN) { nan = true; s2 &= 0xFFFF0000u; }
-                if (s2 >> 16 == kKv4NaN) { nan = true; s2 &= 0xFFFFu; }
-                vs[p] = kv4_step(s2);
+        for (int i = 0; i < NKW; ++i) {
+            const int r = (i * NT + tid) / (HD / 2), w = (i * NT + tid) % (HD / 2);
+            u32x4 s = b.s[i];
+            if ((t + 1) * TK > kv_end) {  // block-uniform
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const uint32_t key = t * TK + 8 * r + 2 * p;
+                    s[p] = key >= kv_end ? 0u : key + 1 >= kv_end ? s[p] & 0xFFFFu : s[p];
+                }
             }
-            if (nan) s_nan = 1;
+            // an exponent of all ones carries into its half's top bit, which steps leave 0
+            const u32x4 c = s + 0x04000400u;
+            if (((c[0] | c[1] | c[2] | c[3]) & 0x80008000u) != 0) {
+                s_nan = 1;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    if ((s[p] & 0xFFFFu) == kKv4NaN) s[p] &= 0xFFFF0000u;
+                    if (s[p] >> 16 == kKv4NaN) s[p] &= 0xFFFFu;
+                }
+            }
+            Kv4Step vs[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) vs[p] = kv4_step(s[p]);
             *reinterpret_cast<half8*>(&Vs[buf][sw<TK>(2 * w, r)]) = kv4_word(b.v[i].x, vs);
             *reinterpret_cast<half8*>(&Vs[buf][sw<TK>(2 * w + 1, r)]) = kv4_word(b.v[i].y, vs);
         }
@@ -142,15 +155,17 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c) {
             const uint32_t row = my_s < S ? my_s : S - 1;  // rows past S are never stored
-            qf[p][c] = *reinterpret_cast<const half8*>(q + p * qplane + (size_t)row * qw + (size_t)h * HD + c * 16 +
-                                                       (lane >> 5) * 8);
+            const u32x4 x = *reinterpret_cast<const u32x4*>(q + p * qplane + (size_t)row * qw + (size_t)h * HD + c * 16 +
+                                                            (lane >> 5) * 8);
+            qf[p][c] = __builtin_bit_cast(half8, x ^ flip);
         }
     float16v o[HD / 32];
 #pragma unroll
     for (int t = 0; t < HD / 32; ++t)
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[t][v] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, minus_one = -1.f;
+    asm volatile("" : "+v"(minus_one));  // a register, so that value - (float)half is one mixed-precision multiply-add
     constexpr float kLazy = 8.f;  // the reference maximum is raised only by more than this (log2 units)
 
     const int krow = (lane & 19) | (lane & 4) << 1 | (lane & 8) >> 1;  // bits 2 and 3 of l % 32 exchanged
@@ -169,32 +184,27 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
                 for (int p = 0; p < QP; ++p) st[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[c], qf[p][c], st[kb], 0, 0, 0);
         }
     };
-    // scaled scores with the mask, where tile t reaches past the block's first row or begins before a row's window;
-    // returns the maximum of this lane's row. Element v of a fragment is key 16 (v / 8) + 8 (l / 32) + v % 8.
+    // the mask, where tile t reaches past the block's first row or begins before a row's window; returns the scaled
+    // maximum of this lane's row. Element v of a fragment is key 16 (v / 8) + 8 (l / 32) + v % 8.
     auto mask_max = [&](float16v (&st)[NKB], uint32_t t) {
-        float bm = -INFINITY;
-        if (t * TK + TK - 1 <= p_first && (t * TK >= lo_max || t * TK + TK <= n_glob)) {
-#pragma unroll
-            for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    st[kb][v] *= sl2;
-                    bm = fmaxf(bm, st[kb][v]);
-                }
-        } else {
+        if (!(t * TK + TK - 1 <= p_first && (t * TK >= lo_max || t * TK + TK <= n_glob))) {
 #pragma unroll
             for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
                     const uint32_t key = t * TK + (kbase + kb) * 32 + (v >> 3) * 16 + (lane >> 5) * 8 + (v & 7);
                     const bool seen = key <= my_pos && (key >= my_lo || key < n_glob);
-                    st[kb][v] = seen ? st[kb][v] * sl2 : -INFINITY;
-                    bm = fmaxf(bm, st[kb][v]);
+                    st[kb][v] = seen ? st[kb][v] : -INFINITY;
                 }
         }
+        float bm = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) bm = fmaxf(bm, st[kb][v]);
         float ba, bb;
         lane_pair<32>(bm, ba, bb);
-        return fmaxf(ba, bb);
+        return fmaxf(ba, bb) * sl2;
     };
     auto rescale = [&](float bm) {
         const bool raise = bm > m + kLazy;  // m = -inf: any finite tile maximum raises it
@@ -215,16 +225,17 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const float pv = fast_exp2(st[kb][v] - ref);
-                ps += pv;
+            for (int v = 0; v < 16; v += 2) {
+                const float p0 = fast_exp2(fmaf(st[kb][v], sl2, -ref)), p1 = fast_exp2(fmaf(st[kb][v + 1], sl2, -ref));
+                ps += p0;
+                ps += p1;
+                const half2v hi = pack_f16(p0, p1);
+                pf[0][kb][v >> 3][v & 7] = hi[0];
+                pf[0][kb][v >> 3][(v & 7) + 1] = hi[1];
                 if constexpr (QX2) {
-                    vsl_half hi, lo;
-                    split_f16(pv, hi, lo);
-                    pf[0][kb][v >> 3][v & 7] = hi;
-                    pf[QP - 1][kb][v >> 3][v & 7] = lo;
-                } else {
-                    pf[0][kb][v >> 3][v & 7] = (vsl_half)pv;
+                    const half2v lo = pack_f16(fmaf((float)hi[0], minus_one, p0), fmaf((float)hi[1], minus_one, p1));
+                    pf[QP - 1][kb][v >> 3][v & 7] = lo[0];
+                    pf[QP - 1][kb][v >> 3][(v & 7) + 1] = lo[1];
                 }
             }
         float pa, pb;
@@ -246,23 +257,39 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
                 }
     };
 
+    // Two buffers each for K and V, K one tile ahead. At the top of iteration t, K of t and t + 1 and V of t are in LDS
+    // and the scores of t in registers: the codes of K of t + 2 and V of t + 1 are requested, the scores of t + 1 are
+    // issued on the matrix cores while the vector pipe turns those of t into probabilities, then the products
+    // of t with V; the codes go into the buffers that K of t and V of t - 1 have left (both last read before the
+    // barrier that ended the previous iteration). Requests past the last tile repeat it.
+    auto tile = [&](uint32_t t) { return phys(t < n_vt ? t : n_vt - 1); };
     if (tid == 0) s_nan = 0;
     __syncthreads();
-    Words b;
-    load(b, phys(0));
-    expand(b, 0, phys(0));
+    KWords kw;
+    VWords vw;
+    load_k(kw, tile(0));
+    load_v(vw, tile(0));
+    expand_k(kw, 0, tile(0));
+    load_k(kw, tile(1));
+    expand_v(vw, 0, tile(0));
+    expand_k(kw, 1, tile(1));
     __syncthreads();
+    float16v st[NKB];
+    qk(0, st);
     for (uint32_t t = 0; t < n_vt; ++t) {
-        const uint32_t nt = phys(t + 1 < n_vt ? t + 1 : t);
-        load(b, nt);
-        float16v st[NKB];
-        qk((int)(t & 1), st);
+        load_k(kw, tile(t + 2));
+        load_v(vw, tile(t + 1));
         rescale(mask_max(st, phys(t)));
+        float16v sn[NKB];
+        qk((int)((t + 1) & 1), sn);
         half8 pf[QP][NKB][2];
         l += probs(st, pf);
         pv((int)(t & 1), pf);
-        // the other buffer was last read before the barrier that ended the previous tile
-        expand(b, (int)((t + 1) & 1), nt);
+        // every wave has its scores of t (taken in the previous iteration)
+        expand_k(kw, (int)(t & 1), tile(t + 2));
+        expand_v(vw, (int)((t + 1) & 1), tile(t + 1));
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) st[kb] = sn[kb];
         __syncthreads();
     }
     const uint32_t any_nan = s_nan;
@@ -375,13 +402,12 @@ void launch(hipStream_t s, const Args& a) {
         a.q, a.k, a.v, a.S, a.pos0, a.n_q, a.n_kv, a.cap, a.scale, a.out, a.om, a.win, a.n_glob, a.thr);
 }
 
-// Groups of a power of two of heads share a block, two waves a head up to four heads; other groups take blocks of
-// one or two heads (a block's threads divide a tile's words).
+// Up to four heads share a block, two waves a head: groups of a power of two, or pairs or single heads of the others
+// (a block's threads divide a tile's words).
 template <int HD, int G, bool QX2>
 void launch_group(hipStream_t s, const Args& a) {
-    constexpr bool pow2 = (G & (G - 1)) == 0;
-    constexpr int GB = pow2 ? G : G % 2 == 0 ? 2 : 1;
-    launch<HD, G, GB, QX2, GB <= 4 ? 2 : 1, 64 * 128 / HD>(s, a);
+    constexpr int GB = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
+    launch<HD, G, GB, QX2, 2, 64 * 128 / HD>(s, a);
 }
 
 template <int HD, int G>
@@ -403,6 +429,7 @@ int attn_prefill_kv4(const char* fn, const void* q, int q_dtype, const void* kca
     if (!aligned_to(kcache, 256) || !aligned_to(vcache, 256)) return vsl_invalid("%s: a 4-bit cache must be 256-byte aligned", fn);
     if (!aligned_to(q, 16) || !aligned_to(out, 16)) return vsl_invalid("%s: q and out must be 16-byte aligned", fn);
     if ((uint64_t)pos0 + S > cap) return vsl_capacity("%s: %u positions from %u exceed capacity %u", fn, S, pos0, cap);
+    if (!std::isfinite(scale)) return vsl_invalid("%s: scale is not finite", fn);
     if (cap > 0x80000000u) return vsl_unsupported("%s: capacity %u", fn, cap);
     if ((uint64_t)n_q * hd > 0x7FFFFFFFull || n_q > 65535u) return vsl_unsupported("%s: n_q=%u", fn, n_q);
     if (S == 0) return VSL_OK;
