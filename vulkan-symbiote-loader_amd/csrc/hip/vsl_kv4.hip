@@ -338,12 +338,13 @@ __global__ __launch_bounds__(256) void k_kv4_read(const char* __restrict__ kc, c
     const uint32_t o0 = pos0 / 8, n_oct = (pos0 + n - 1) / 8 - o0 + 1;
     const uint64_t nk = kc ? (uint64_t)n_kv * n * WPR : 0, nv = vc ? (uint64_t)n_kv * n_oct * WPR : 0;
     uint64_t t = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const Kv4Consts kc4 = kv4_consts();
     if (t < nk) {
         const uint32_t w = (uint32_t)(t % WPR);
         const uint64_t r = t / WPR, kvh = r / n, i = r % n, at = kvh * P + pos0 + i;
         const uint32_t word = reinterpret_cast<const uint32_t*>(kc)[at * WPR + w];
         const uint32_t s = reinterpret_cast<const uint16_t*>(kc + soff)[at * NB + w / 4];
-        store8(ko + (kvh * n + i) * HD + 8 * w, kv4_word(word, kv4_step(s | s << 16)));
+        store8(ko + (kvh * n + i) * HD + 8 * w, kv4_word(word, kv4_step(s | s << 16, kc4), kc4));
         return;
     }
     t -= nk;
@@ -355,10 +356,10 @@ __global__ __launch_bounds__(256) void k_kv4_read(const char* __restrict__ kc, c
     const u32x4 sp = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(vc + soff) + (at * NB + w / 4) * 8);
     Kv4Step st[4];
 #pragma unroll
-    for (int p = 0; p < 4; ++p) st[p] = kv4_step(sp[p]);
+    for (int p = 0; p < 4; ++p) st[p] = kv4_step(sp[p], kc4);
     half8 col[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) col[j] = kv4_word(j < 4 ? wa[j & 3] : wb[j & 3], st);
+    for (int j = 0; j < 8; ++j) col[j] = kv4_word(j < 4 ? wa[j & 3] : wb[j & 3], st, kc4);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const uint64_t i = oct * 8 + e - pos0;
@@ -402,7 +403,7 @@ __device__ __forceinline__ float add_lane8(float v) {
 // more than kLazy (probabilities stay below 2^kLazy). Masked positions get probability 0 and their V steps are set to
 // 0, so what the cache holds past the length never reaches a sum. Output as k_attn_decode's.
 template <int HD, int G, bool WIN, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void k_attn_decode_kv4(const float* __restrict__ q, const char* __restrict__ kcache,
+__global__ __launch_bounds__(WAVES * 64, 2) void k_attn_decode_kv4(const float* __restrict__ q, const char* __restrict__ kcache,
                                                                 const char* __restrict__ vcache, uint32_t n_kv, uint32_t cap,
                                                                 float scale, uint32_t nsplit, float* __restrict__ part_o,
                                                                 float* __restrict__ part_ml, vsl_ctrl* ctrl, uint32_t win,
@@ -418,6 +419,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_attn_decode_kv4(const float* __r
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t col = lane & 15, rg = lane >> 4, head = col & 7;
     const uint32_t h0 = kvh * G;
+    const Kv4Consts kc4 = kv4_consts();
     const uint64_t P = kv4_positions(cap), soff = kv4_steps_off(n_kv, cap, HD);
     const uint32_t all_tiles = (uint32_t)(P / TP);
     // this lane's part of tile 0
@@ -519,22 +521,23 @@ __global__ __launch_bounds__(WAVES * 64) void k_attn_decode_kv4(const float* __r
         float s[8];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const Kv4Step st = kv4_step(b.ks[t] | b.ks[t] << 16);
+            const Kv4Step st = kv4_step(b.ks[t] | b.ks[t] << 16, kc4);
             float4v d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
-                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_word(b.k[t][ks], st), qf[ks], d, 0, 0, 0);
+                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_word(b.k[t][ks], st, kc4), qf[ks], d, 0, 0, 0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[4 * t + i] = add_lane8(d[i]);
         }
         u32x4 vs = b.vs;
-        // wave-uniform: a tile that ends past the position, begins before the window, or is past the last
-        const bool whole = vt < n_vt && p0 + TP - 1 <= p && (!WIN || p0 >= lo || p0 + TP <= n_glob);
+        // wave-uniform: a tile that ends past the position or begins before the window
+        const bool whole = p0 + TP - 1 <= p && (!WIN || p0 >= lo || p0 + TP <= n_glob);
         if (!whole) {
+            asm volatile("");  // a branch, not selects in every tile
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const uint32_t k = p0 + 8 * rg + e;
-                const bool seen = vt < n_vt && k <= p && (!WIN || k >= lo || k < n_glob);
+                const bool seen = k <= p && (!WIN || k >= lo || k < n_glob);
                 s[e] = seen ? s[e] : -INFINITY;
                 if (!seen) vs[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
             }
@@ -568,26 +571,25 @@ __global__ __launch_bounds__(WAVES * 64) void k_attn_decode_kv4(const float* __r
         }
         Kv4Step st[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) st[i] = kv4_step(vs[i]);
+        for (int i = 0; i < 4; ++i) st[i] = kv4_step(vs[i], kc4);
 #pragma unroll
-        for (int i = 0; i < NC; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_word(b.v[i], st), pf, o[i], 0, 0, 0);
+        for (int i = 0; i < NC; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_word(b.v[i], st, kc4), pf, o[i], 0, 0, 0);
     };
 
-    // tiles in pairs, each buffer refilled right after it is consumed; the last pair is consumed without refills, and
-    // tiles past the wave's own are masked whole
-    const uint32_t first = vtile(0), stride = nsplit * WAVES;
-    const uint32_t mine = n_vt > first ? (n_vt - 1 - first) / stride + 1 : 0;
-    const uint32_t n_pairs = mine ? (mine + 1) / 2 : 1;
-    for (uint32_t pp = 0; pp + 1 < n_pairs; ++pp) {
-        consume(ta, vtile(2 * pp));
-        issue(ta, phys(vtile(2 * pp + 2)));
+    // two buffers, each refilled right after it is consumed (past the wave's last tile with tile 0)
+    const uint32_t stride = nsplit * WAVES;
+    for (uint32_t vt = vtile(0); vt < n_vt;) {
+        consume(ta, vt);
+        vt += stride;
+        if (vt >= n_vt) break;
+        issue(ta, phys(vt + stride));
         __builtin_amdgcn_sched_barrier(0);
-        consume(tb, vtile(2 * pp + 1));
-        issue(tb, phys(vtile(2 * pp + 3)));
+        consume(tb, vt);
+        vt += stride;
+        if (vt >= n_vt) break;
+        issue(tb, phys(vt + stride));
         __builtin_amdgcn_sched_barrier(0);
     }
-    consume(ta, vtile(2 * n_pairs - 2));
-    consume(tb, vtile(2 * n_pairs - 1));
 
     // the head's sums over the octets, the hi and lo columns joined; lane l holds head l % 8, dims
     // NC (4 (l / 16) + r) + i in o[i][r]
@@ -622,7 +624,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_attn_decode_kv4(const float* __r
         if (M != -INFINITY) {
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                const float fw = exp2f(s_ml[w][g][0] - M);
+                const float fw = fast_exp2(s_ml[w][g][0] - M);
                 L += s_ml[w][g][1] * fw;
                 A += s_acc[w][g][dd] * fw;
             }

@@ -73,6 +73,7 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     const uint32_t lo_max = (p_last + 1 > thr && p_last > win) ? p_last - win : 0;
 
     const uint64_t P = kv4_positions(cap), soff = kv4_steps_off(n_kv, cap, HD);
+    const Kv4Consts kc4 = kv4_consts();
     const char* Kc = kc + (uint64_t)kvh * P * (HD / 2);
     const char* Kst = kc + soff + (uint64_t)kvh * P * NB * 2;
     const char* Vc = vc + (uint64_t)kvh * P * (HD / 2);
@@ -113,9 +114,9 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
         for (int i = 0; i < NKW; ++i) {
             const int r = (i * NT + tid) / (HD / 16), w = (i * NT + tid) % (HD / 16);
             const uint32_t st = t * TK + r < kv_end ? b.s[i] : 0u;
-            const Kv4Step s = kv4_step(st | st << 16);
-            *reinterpret_cast<half8*>(&Ks[buf][sw<HD>(r, 2 * w)]) = kv4_word(b.k[i].x, s);
-            *reinterpret_cast<half8*>(&Ks[buf][sw<HD>(r, 2 * w + 1)]) = kv4_word(b.k[i].y, s);
+            const Kv4Step s = kv4_step(st | st << 16, kc4);
+            *reinterpret_cast<half8*>(&Ks[buf][sw<HD>(r, 2 * w)]) = kv4_word(b.k[i].x, s, kc4);
+            *reinterpret_cast<half8*>(&Ks[buf][sw<HD>(r, 2 * w + 1)]) = kv4_word(b.k[i].y, s, kc4);
         }
     };
     auto expand_v = [&](const VWords& b, int buf, uint32_t t) {
@@ -142,9 +143,9 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
             }
             Kv4Step vs[4];
 #pragma unroll
-            for (int p = 0; p < 4; ++p) vs[p] = kv4_step(s[p]);
-            *reinterpret_cast<half8*>(&Vs[buf][sw<TK>(2 * w, r)]) = kv4_word(b.v[i].x, vs);
-            *reinterpret_cast<half8*>(&Vs[buf][sw<TK>(2 * w + 1, r)]) = kv4_word(b.v[i].y, vs);
+            for (int p = 0; p < 4; ++p) vs[p] = kv4_step(s[p], kc4);
+            *reinterpret_cast<half8*>(&Vs[buf][sw<TK>(2 * w, r)]) = kv4_word(b.v[i].x, vs, kc4);
+            *reinterpret_cast<half8*>(&Vs[buf][sw<TK>(2 * w + 1, r)]) = kv4_word(b.v[i].y, vs, kc4);
         }
     };
 
