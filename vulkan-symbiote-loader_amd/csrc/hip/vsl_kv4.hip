@@ -373,6 +373,9 @@ __global__ __launch_bounds__(256) void k_kv4_read(const char* __restrict__ kc, c
 // decode attention
 // ---------------------------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
+#ifndef KBUF
+#define KBUF 2
+#endif
 #ifndef KDEC
 #define KDEC 4
 #endif
@@ -411,8 +414,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_decode_kv4(const float* 
     constexpr int KS = HD / 32, NB = HD / 32, NC = HD / 16;  // k-steps; blocks a row; V columns a lane (and O^T tiles)
     constexpr uint32_t TP = 32;
     constexpr float kLazy = 8.f;
+    constexpr int NBUF = KBUF;
     static_assert(G >= 1 && G <= 8, "GQA group of 1..8 heads");
-    __shared__ float s_ml[WAVES][G][2];
+    __shared__ __attribute__((aligned(8))) float s_ml[WAVES][G][2];
     __shared__ __attribute__((aligned(16))) float s_acc[WAVES][G][HD];
 
     const uint32_t kvh = blockIdx.y, split = blockIdx.x;
@@ -469,10 +473,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_decode_kv4(const float* 
         qa[ks][0] = *reinterpret_cast<const float4*>(qp);
         qa[ks][1] = *reinterpret_cast<const float4*>(qp + 4);
     }
-    Tile ta, tb;
+    Tile buf[NBUF];
     if constexpr (!WIN) {
-        issue(ta, vtile(0) < all_tiles ? vtile(0) : 0);
-        issue(tb, vtile(1) < all_tiles ? vtile(1) : 0);
+#pragma unroll
+        for (int i = 0; i < NBUF; ++i) issue(buf[i], vtile(i) < all_tiles ? vtile(i) : 0);
     }
     __builtin_amdgcn_sched_barrier(0);
     const uint32_t done = ctrl->done;
@@ -494,8 +498,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_decode_kv4(const float* 
         return vt < n_gt ? vt : vt - n_gt + t_lo;
     };
     if constexpr (WIN) {
-        issue(ta, phys(vtile(0)));
-        issue(tb, phys(vtile(1)));
+#pragma unroll
+        for (int i = 0; i < NBUF; ++i) issue(buf[i], phys(vtile(i)));
     }
 
     half8 qf[KS];
@@ -576,19 +580,21 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_decode_kv4(const float* 
         for (int i = 0; i < NC; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_word(b.v[i], st, kc4), pf, o[i], 0, 0, 0);
     };
 
-    // two buffers, each refilled right after it is consumed (past the wave's last tile with tile 0)
+    // each buffer is refilled right after it is consumed (past the wave's last tile with the one just consumed)
     const uint32_t stride = nsplit * WAVES;
-    for (uint32_t vt = vtile(0); vt < n_vt;) {
-        consume(ta, vt);
-        vt += stride;
-        if (vt >= n_vt) break;
-        issue(ta, phys(vt + stride));
-        __builtin_amdgcn_sched_barrier(0);
-        consume(tb, vt);
-        vt += stride;
-        if (vt >= n_vt) break;
-        issue(tb, phys(vt + stride));
-        __builtin_amdgcn_sched_barrier(0);
+    uint32_t vt = vtile(0);
+    bool more = vt < n_vt;
+    while (more) {
+#pragma unroll
+        for (int i = 0; i < NBUF; ++i) {
+            consume(buf[i], vt);
+            const uint32_t ahead = vt + NBUF * stride;
+            more = vt + stride < n_vt;
+            if (!more) break;
+            issue(buf[i], phys(ahead < n_vt ? ahead : vt));
+            __builtin_amdgcn_sched_barrier(0);
+            vt += stride;
+        }
     }
 
     // the head's sums over the octets, the hi and lo columns joined; lane l holds head l % 8, dims
@@ -615,29 +621,34 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_decode_kv4(const float* 
         }
     }
     lds_barrier();
-    for (uint32_t e = threadIdx.x; e < (uint32_t)(G * HD); e += WAVES * 64) {
-        const uint32_t g = e / HD, dd = e % HD;
-        float M = -INFINITY;
+    // four dims a thread; the waves' statistics and sums are read at once
+    static_assert(G * HD / 4 <= WAVES * 64, "one pass over the outputs");
+    const uint32_t g = threadIdx.x / (HD / 4), dd = threadIdx.x % (HD / 4) * 4;
+    if (g >= (uint32_t)G) return;
+    float2 ml[WAVES];
+    float4v acc[WAVES];
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) M = fmaxf(M, s_ml[w][g][0]);
-        float L = 0.f, A = 0.f;
-        if (M != -INFINITY) {
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                const float fw = fast_exp2(s_ml[w][g][0] - M);
-                L += s_ml[w][g][1] * fw;
-                A += s_acc[w][g][dd] * fw;
-            }
-        }
-        const size_t pidx = (size_t)(h0 + g) * nsplit + split;
-        if (!done) {
-            part_o[pidx * HD + dd] = A;
-            if (dd == 0) {
-                part_ml[pidx * 2 + 0] = M;
-                part_ml[pidx * 2 + 1] = L;
-            }
-        }
+    for (int w = 0; w < WAVES; ++w) {
+        ml[w] = *reinterpret_cast<const float2*>(&s_ml[w][g][0]);
+        acc[w] = *reinterpret_cast<const float4v*>(&s_acc[w][g][dd]);
     }
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) M = fmaxf(M, ml[w].x);
+    float L = 0.f;
+    float4v A = {0.f, 0.f, 0.f, 0.f};
+    const float ref = M == -INFINITY ? 0.f : M;  // no tile at all: every weight and sum is 0
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const float fw = fast_exp2(ml[w].x - ref);
+        L = fmaf(ml[w].y, fw, L);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) A[i] = fmaf(acc[w][i], fw, A[i]);
+    }
+    if (done) return;
+    const size_t pidx = (size_t)(h0 + g) * nsplit + split;
+    *reinterpret_cast<float4v*>(part_o + pidx * HD + dd) = A;
+    if (dd == 0) *reinterpret_cast<float2*>(part_ml + pidx * 2) = make_float2(M, L);
 }
 
 bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
