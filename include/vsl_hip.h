@@ -320,8 +320,8 @@ int vsl_norm_gemv(const float* x, const float* gamma, float eps, const void* W, 
  *     VSL_ROPE_HALVES  pairs (j, j + hd/2)
  *   q -> q_out [S][n_q][hd] (VSL_DT_F32, VSL_DT_F16 or VSL_DT_F16X2), k and v -> the caches (VSL_DT_F32,
  *   VSL_DT_F16 or VSL_DT_KV4).
- * All of it is computed in 64 bits and rounded once: a cached code is that of the exact value, whatever the
- * number of rows in the call.  head_dim 64 or 128; every pointer 16-byte aligned (VSL_DT_KV4 caches 256);
+ * Keys for a VSL_DT_KV4 cache are computed in 64 bits, so that a code is that of the exact value whatever the
+ * number of rows in the call; the rest in 32 bits, each output rounded once more if it has fewer. head_dim 64 or 128; every pointer 16-byte aligned (VSL_DT_KV4 caches 256);
  * positions past cap return VSL_E_CAPACITY before anything is launched. */
 enum { VSL_ROPE_PAIRS = 0, VSL_ROPE_HALVES = 1 };
 int vsl_qk_norm_rope_append(const float* qkv, uint32_t S, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t pos0,

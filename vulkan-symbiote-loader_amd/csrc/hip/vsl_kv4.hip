@@ -54,88 +54,130 @@ __device__ __forceinline__ double rsqrt64(double x) {
     return r0 == 0.0 ? 0.0 : r;
 }
 
-// Four consecutive dims of a head's row in one lane (HD / 4 lanes a row): the head's norm and rotation, in 64
-// bits, as the choice of a 4-bit code hangs on values next to a border and is then the same for every number of rows
-// in a call (the vector pipes take 64-bit multiply-adds at the 32-bit rate).
+// Four consecutive dims of a head's row in one lane (HD / 4 lanes a row): the head's norm and rotation. T: float; or
+// double for keys that become 4-bit codes, whose choice hangs on values next to a border: it is then the exact
+// value's, and the same for every number of rows in a call. (In 64 bits throughout, 2048 rows of the 8B shape took 29.5
+// us instead of 22.9: conversions and 64-bit operations, not memory, were the bound.)
 struct RopeArgs {
     const float* q_gamma;
     const float* k_gamma;
     const float* rc;
     const float* rs;
-    double eps;
+    float eps;
     int halves;
 };
+// What a lane reads for its four dims: the row, and the rotation's angles (pairs: two; halves: four, of the dims' half).
+struct RowIn {
+    float4v x, co, si;
+};
 template <int HD>
-__device__ __forceinline__ void norm_rotate(const float4v x, const float* gamma, const RopeArgs& a, uint32_t pos, uint32_t c,
-                                            double (&y)[4]) {
-    constexpr int L = HD / 4;
-    double inv = 1.0;
-    if (gamma) {
-        double ss = 0.0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ss = fma((double)x[i], (double)x[i], ss);
-        inv = rsqrt64(group_sum64<L>(ss) * (1.0 / HD) + a.eps);
-    }
+__device__ __forceinline__ void load_angles(const RopeArgs& a, uint32_t pos, uint32_t c, RowIn& r) {
     const size_t row = (size_t)pos * (HD / 2);
-    if (!a.halves) {
+    if (a.halves) {
+        const uint32_t j = 4 * (c & (HD / 8 - 1));
+        r.co = *reinterpret_cast<const float4v*>(a.rc + row + j);
+        r.si = *reinterpret_cast<const float4v*>(a.rs + row + j);
+    } else {
         const float2 co = *reinterpret_cast<const float2*>(a.rc + row + 2 * c);
         const float2 si = *reinterpret_cast<const float2*>(a.rs + row + 2 * c);
-        const float4v g = gamma ? *reinterpret_cast<const float4v*>(gamma + 4 * c) : float4v{1.f, 1.f, 1.f, 1.f};
-        double v[4];
+        r.co = float4v{co.x, co.y, 0.f, 0.f};
+        r.si = float4v{si.x, si.y, 0.f, 0.f};
+    }
+}
+// The gains of a lane's dims (ga; halves: of its dims of the first half ga, of the second gb).
+struct Gains {
+    float4v ga, gb;
+};
+template <int HD>
+__device__ __forceinline__ Gains load_gains(const RopeArgs& a, const float* gamma, uint32_t c) {
+    Gains g{{1.f, 1.f, 1.f, 1.f}, {1.f, 1.f, 1.f, 1.f}};
+    if (!gamma) return g;
+    const uint32_t j = a.halves ? 4 * (c & (HD / 8 - 1)) : 4 * c;
+    g.ga = *reinterpret_cast<const float4v*>(gamma + j);
+    if (a.halves) g.gb = *reinterpret_cast<const float4v*>(gamma + HD / 2 + j);
+    return g;
+}
+template <int HD, typename T>
+__device__ __forceinline__ void norm_rotate(const RowIn& r, bool norm, const Gains& g, const RopeArgs& a, uint32_t c, T (&y)[4]) {
+    constexpr int L = HD / 4;
+    T inv = 1;
+    if (norm) {
+        T ss = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (double)x[i] * inv * (double)g[i];
-        y[0] = v[0] * (double)co.x - v[1] * (double)si.x;
-        y[1] = v[0] * (double)si.x + v[1] * (double)co.x;
-        y[2] = v[2] * (double)co.y - v[3] * (double)si.y;
-        y[3] = v[2] * (double)si.y + v[3] * (double)co.y;
+        for (int i = 0; i < 4; ++i) ss = fma((T)r.x[i], (T)r.x[i], ss);
+        if constexpr (sizeof(T) == 8) {
+            inv = rsqrt64(group_sum64<L>(ss) * (1.0 / HD) + (double)a.eps);
+        } else {
+            ss = group_sum_dpp<16>(ss);
+            if constexpr (L == 32) {
+                float s0, s1;
+                lane_pair<16>(ss, s0, s1);
+                ss = s0 + s1;
+            }
+            inv = 1.f / sqrtf(ss / HD + a.eps);
+        }
+    }
+    if (!a.halves) {
+        T v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (T)r.x[i] * inv * (T)g.ga[i];
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const T co = (T)r.co[i / 2], si = (T)r.si[i / 2];
+            y[i] = v[i] * co - v[i + 1] * si;
+            y[i + 1] = v[i] * si + v[i + 1] * co;
+        }
     } else {
         // the other half's four dims are L / 2 lanes away
-        const uint32_t j = 4 * (c & (L / 2 - 1));
         const bool first = c < (uint32_t)(L / 2);
-        const float4v co = *reinterpret_cast<const float4v*>(a.rc + row + j);
-        const float4v si = *reinterpret_cast<const float4v*>(a.rs + row + j);
-        float4v ga = {1.f, 1.f, 1.f, 1.f}, gb = ga;
-        if (gamma) {
-            ga = *reinterpret_cast<const float4v*>(gamma + j);
-            gb = *reinterpret_cast<const float4v*>(gamma + HD / 2 + j);
-        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float xa, xb;
-            lane_pair<L / 2>(x[i], xa, xb);
-            const double va = (double)xa * inv * (double)ga[i], vb = (double)xb * inv * (double)gb[i];
-            y[i] = first ? va * (double)co[i] - vb * (double)si[i] : va * (double)si[i] + vb * (double)co[i];
+            lane_pair<L / 2>(r.x[i], xa, xb);
+            const T va = (T)xa * inv * (T)g.ga[i], vb = (T)xb * inv * (T)g.gb[i];
+            const T co = (T)r.co[i], si = (T)r.si[i];
+            y[i] = first ? va * co - vb * si : va * si + vb * co;
         }
     }
 }
 
-// rint(y / d), ties to even, from r = 1 / d to within an ulp or two (|y / d| <= 15): the remainder of the nearest
-// integer to y r is exact (d has 7 significant bits), and tells on which side of a border y / d lies.
-__device__ __forceinline__ double rint_quotient(double y, double d, double r) {
-    const double n = rint(y * r), rem = fma(-n, d, y), a = fabs(rem), h = 0.5 * d;
+// rint(y / d), ties to even, from r near 1 / d (an ulp or two; |y / d| <= 15): the remainder of the nearest integer to
+// y r is exact in either type (d has 7 significant bits), and tells on which side of a border y / d lies.
+template <typename T>
+__device__ __forceinline__ T rint_quotient(T y, T d, T r) {
+    const T n = rint(y * r), rem = fma(-n, d, y), a = fabs(rem), h = (T)0.5 * d;
     const bool off = a > h || (a == h && ((int)n & 1));
-    return off ? n + copysign(1.0, rem) : n;
+    return off ? n + copysign((T)1, rem) : n;
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_move(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_move(double v) {
+    return dpp64<CTRL>(v);
 }
 
 // The 4-bit form of a block of 32 dims, four in each of 8 consecutive lanes: this lane's codes; returns the step
 // as stored.
-__device__ __forceinline__ uint32_t kv4_quantize(const double (&y)[4], uint32_t (&n)[4]) {
-    double lo = 0.0, hi = 0.0;
+template <typename T>
+__device__ __forceinline__ uint32_t kv4_quantize(const T (&y)[4], uint32_t (&n)[4]) {
+    T lo = 0, hi = 0;
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         lo = fmin(lo, y[i]);
         hi = fmax(hi, y[i]);
-        bad |= !(fabs(y[i]) < (double)INFINITY);
+        bad |= !(fabs(y[i]) < (T)INFINITY);
     }
-    lo = fmin(lo, dpp64<kDppPair>(lo));
-    hi = fmax(hi, dpp64<kDppPair>(hi));
-    lo = fmin(lo, dpp64<kDppQuad>(lo));
-    hi = fmax(hi, dpp64<kDppQuad>(hi));
-    lo = fmin(lo, dpp64<kDppHalfMirror>(lo));
-    hi = fmax(hi, dpp64<kDppHalfMirror>(hi));
+    lo = fmin(lo, dpp_move<kDppPair>(lo));
+    hi = fmax(hi, dpp_move<kDppPair>(hi));
+    lo = fmin(lo, dpp_move<kDppQuad>(lo));
+    hi = fmax(hi, dpp_move<kDppQuad>(hi));
+    lo = fmin(lo, dpp_move<kDppHalfMirror>(lo));
+    hi = fmax(hi, dpp_move<kDppHalfMirror>(hi));
     const uint64_t b = __builtin_amdgcn_ballot_w64(bad) >> (threadIdx.x & 56);
-    const double range = hi - lo;
+    const double range = (double)hi - (double)lo;
     if ((b & 0xFF) != 0 || range > 65280.0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) n[i] = 0;
@@ -146,14 +188,17 @@ __device__ __forceinline__ uint32_t kv4_quantize(const double (&y)[4], uint32_t 
     constexpr uint64_t one = 1ull << 46;
     const uint64_t u = __builtin_bit_cast(uint64_t, range * (1.0 / 15.0)) & ~(one - 1);
     const double cut = __builtin_bit_cast(double, u);
-    const double d = fmax(15.0 * cut >= range ? cut : __builtin_bit_cast(double, u + one), 0x1p-14);
-    double r = (double)__builtin_amdgcn_rcpf((float)d);  // 1 / d: 23 bits, then two Newton steps
-    r = fma(fma(-d, r, 1.0), r, r);
-    r = fma(fma(-d, r, 1.0), r, r);
-    const double z = rint_quotient(-lo, d, r);
+    const double dd = fmax(15.0 * cut >= range ? cut : __builtin_bit_cast(double, u + one), 0x1p-14);
+    const T d = (T)dd;  // exact: 7 bits, 2^-14 .. 4352
+    T r = (T)__builtin_amdgcn_rcpf((float)dd);  // 1 / d to 23 bits, in 64 bits two Newton steps
+    if constexpr (sizeof(T) == 8) {
+        r = fma(fma(-d, r, 1.0), r, r);
+        r = fma(fma(-d, r, 1.0), r, r);
+    }
+    const T z = rint_quotient(-lo, d, r);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) n[i] = (uint32_t)(int)fmin(fmax(rint_quotient(y[i], d, r) + z, 0.0), 15.0);
-    const vsl_half dh = (vsl_half)(float)d;  // exact: 7 bits, 2^-14 .. 4352
+    for (int i = 0; i < 4; ++i) n[i] = (uint32_t)(int)fmin(fmax(rint_quotient(y[i], d, r) + z, (T)0), (T)15);
+    const vsl_half dh = (vsl_half)(float)dd;
     return (uint32_t)__builtin_bit_cast(uint16_t, dh) | (uint32_t)(int)z;
 }
 
@@ -170,17 +215,17 @@ enum { Q_F32 = 0, Q_F16 = 1, Q_F16X2 = 2 };
 enum { KV_F32 = 0, KV_F16 = 1, KV_4 = 2 };
 
 template <int QM>
-__device__ __forceinline__ void store_q(void* q_out, size_t off, size_t plane, const double (&y)[4]) {
+__device__ __forceinline__ void store_q(void* q_out, size_t off, size_t plane, const float (&y)[4]) {
     if constexpr (QM == Q_F32) {
         *reinterpret_cast<float4v*>(static_cast<float*>(q_out) + off) =
-            float4v{(float)y[0], (float)y[1], (float)y[2], (float)y[3]};
+            float4v{y[0], y[1], y[2], y[3]};
     } else {
         vsl_half* q = static_cast<vsl_half*>(q_out);
         half4 h, l;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             vsl_half hi, lo;
-            split_f16((float)y[i], hi, lo);
+            split_f16(y[i], hi, lo);
             h[i] = hi;
             l[i] = lo;
         }
@@ -189,13 +234,12 @@ __device__ __forceinline__ void store_q(void* q_out, size_t off, size_t plane, c
     }
 }
 template <int KVM>
-__device__ __forceinline__ void store_kv(void* cache, size_t off, const double (&y)[4]) {
+__device__ __forceinline__ void store_kv(void* cache, size_t off, const float (&y)[4]) {
     if constexpr (KVM == KV_F32)
-        *reinterpret_cast<float4v*>(static_cast<float*>(cache) + off) =
-            float4v{(float)y[0], (float)y[1], (float)y[2], (float)y[3]};
+        *reinterpret_cast<float4v*>(static_cast<float*>(cache) + off) = float4v{y[0], y[1], y[2], y[3]};
     else
         *reinterpret_cast<half4*>(static_cast<vsl_half*>(cache) + off) =
-            half4{(vsl_half)(float)y[0], (vsl_half)(float)y[1], (vsl_half)(float)y[2], (vsl_half)(float)y[3]};
+            half4{(vsl_half)y[0], (vsl_half)y[1], (vsl_half)y[2], (vsl_half)y[3]};
 }
 // A row of K in 4 bits, `at` its place among the cache's rows; two lanes a word (dims 0-3 and 4-7 of eight).
 template <int HD>
@@ -208,10 +252,13 @@ __device__ __forceinline__ void store_k4(void* cache, uint64_t soff, size_t at, 
     if ((c & 7) == 0) reinterpret_cast<uint16_t*>(static_cast<char*>(cache) + soff)[at * (HD / 32) + c / 8] = (uint16_t)step;
 }
 
-// Prompt rows, four dims a lane. The first v_waves waves take one 32-dim block of a V head at the 8 positions of an
-// octet each (8 lanes a position; the first and the last octet of a call may be partly outside it): the codes of a
-// column are joined to its word over the lanes. The others take rows of q and k heads (of all heads with fp16 and
-// fp32 caches), HD / 4 lanes each, neighbouring heads in neighbouring lanes.
+// Prompt rows, four dims a lane, everything that a lane reads requested before its first use. The first v_waves waves
+// take one 32-dim block of a V head at the 8 positions of an octet each (8 lanes a position; the first and the last octet
+// of a call may be partly outside it): the codes of a column are joined to its word over the lanes. The others take
+// rows of q and k heads (of all heads with fp16 and fp32 caches), HD / 4 lanes a head, neighbouring heads in
+// neighbouring lanes. Bound by memory in a large call: 2048 rows of the 8B shape with a split q (50 MB read, 36 MB
+// written) 22.9 us, 3.8 TB/s against the 5.3 of a large copy; 45 rows 3.5 us. Two and four rows a lane: 23.5 and 25.6,
+// 4.3 and 6.3 us; an octet of rows of one head a lane: 38.4 and 12.0 us.
 template <int HD, int QM, int KVM>
 __global__ __launch_bounds__(256) void k_append_rows(AppendArgs a, uint32_t v_waves) {
     constexpr uint32_t L = HD / 4, NB = HD / 32;
@@ -222,9 +269,9 @@ __global__ __launch_bounds__(256) void k_append_rows(AppendArgs a, uint32_t v_wa
         const uint32_t blk = wave % NB, kvh = wave / NB % a.n_kv, oct = a.pos0 / 8 + wave / NB / a.n_kv;
         const uint32_t e = lane >> 3, j = lane & 7, s = oct * 8 + e - a.pos0;  // wraps below pos0
         const bool in = s < a.S;
-        float4v x = {0.f, 0.f, 0.f, 0.f};
-        if (in) x = *reinterpret_cast<const float4v*>(a.qkv + (size_t)s * width + (size_t)(a.n_q + a.n_kv + kvh) * HD + 32 * blk + 4 * j);
-        const double y[4] = {x[0], x[1], x[2], x[3]};
+        const float4v x = *reinterpret_cast<const float4v*>(a.qkv + (size_t)(in ? s : 0) * width +
+                                                            (size_t)(a.n_q + a.n_kv + kvh) * HD + 32 * blk + 4 * j);
+        const float y[4] = {x[0], x[1], x[2], x[3]};
         uint32_t n[4];
         const uint32_t step = kv4_quantize(y, n);
         u32x4 w;
@@ -237,17 +284,17 @@ __global__ __launch_bounds__(256) void k_append_rows(AppendArgs a, uint32_t v_wa
             const auto p32 = __builtin_amdgcn_permlane32_swap(v, v, false, false);
             w[i] = p32[0] | p32[1];
         }
+        const size_t at = (size_t)kvh * (P / 8) + oct;
         if (lane < 8) {
-            u32x4* dst = reinterpret_cast<u32x4*>(static_cast<uint32_t*>(a.vc) + ((size_t)kvh * (P / 8) + oct) * HD + 32 * blk + 4 * j);
             uint32_t mask = 0;  // of the octet's positions in this call; the others keep their codes
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) mask |= oct * 8 + i - a.pos0 < a.S ? 15u << kv4_shift(i) : 0u;
+            u32x4* dst = reinterpret_cast<u32x4*>(static_cast<uint32_t*>(a.vc) + at * HD + 32 * blk + 4 * j);
             if (~mask) w |= *dst & ~mask;
             *dst = w;
         }
         if (j == 0 && in)
-            reinterpret_cast<uint16_t*>(static_cast<char*>(a.vc) + soff)[(((size_t)kvh * (P / 8) + oct) * NB + blk) * 8 + e] =
-                (uint16_t)step;
+            reinterpret_cast<uint16_t*>(static_cast<char*>(a.vc) + soff)[(at * NB + blk) * 8 + e] = (uint16_t)step;
         return;
     }
     const uint32_t row_heads = KVM == KV_4 ? a.n_q + a.n_kv : heads, c = lane % L;
@@ -258,18 +305,26 @@ __global__ __launch_bounds__(256) void k_append_rows(AppendArgs a, uint32_t v_wa
         ++s;
     }
     if (s >= a.S) return;
+    const bool is_q = h < a.n_q, is_k = !is_q && h < a.n_q + a.n_kv;
+    const float* gamma = is_q ? a.r.q_gamma : is_k ? a.r.k_gamma : nullptr;
     const uint32_t pos = a.pos0 + s;
-    const float4v x = *reinterpret_cast<const float4v*>(a.qkv + (size_t)s * width + (size_t)h * HD + 4 * c);
-    double y[4] = {x[0], x[1], x[2], x[3]};
-    if (h < a.n_q + a.n_kv) norm_rotate<HD>(x, h < a.n_q ? a.r.q_gamma : a.r.k_gamma, a.r, pos, c, y);
-    if (h < a.n_q) {
-        store_q<QM>(a.q_out, ((size_t)s * a.n_q + h) * HD + 4 * c, (size_t)a.S * a.n_q * HD, y);
-        return;
-    }
-    const bool is_k = h < a.n_q + a.n_kv;
+    RowIn in;
+    in.x = *reinterpret_cast<const float4v*>(a.qkv + (size_t)s * width + (size_t)h * HD + 4 * c);
+    const Gains g = load_gains<HD>(a.r, gamma, c);
+    if (is_q || is_k) load_angles<HD>(a.r, pos, c, in);
     const uint32_t kvh = is_k ? h - a.n_q : h - a.n_q - a.n_kv;
-    if constexpr (KVM != KV_4) store_kv<KVM>(is_k ? a.kc : a.vc, ((size_t)kvh * a.cap + pos) * HD + 4 * c, y);
-    else store_k4<HD>(a.kc, soff, (size_t)kvh * P + pos, c, y);
+    if constexpr (KVM == KV_4) {
+        if (is_k) {
+            double y[4];
+            norm_rotate<HD>(in, gamma != nullptr, g, a.r, c, y);
+            store_k4<HD>(a.kc, soff, (size_t)kvh * P + pos, c, y);
+            return;
+        }
+    }
+    float y[4] = {in.x[0], in.x[1], in.x[2], in.x[3]};
+    if (is_q || is_k) norm_rotate<HD>(in, gamma != nullptr, g, a.r, c, y);
+    if (is_q) store_q<QM>(a.q_out, ((size_t)s * a.n_q + h) * HD + 4 * c, (size_t)a.S * a.n_q * HD, y);
+    else if constexpr (KVM != KV_4) store_kv<KVM>(is_k ? a.kc : a.vc, ((size_t)kvh * a.cap + pos) * HD + 4 * c, y);
 }
 
 // One row at ctrl->pos, an item a head. The row, and for V the octet's words, are requested at once.
@@ -279,7 +334,10 @@ __global__ __launch_bounds__(64) void k_append_decode(AppendArgs a, vsl_ctrl* ct
     const uint32_t heads = a.n_q + 2 * a.n_kv;
     const uint32_t t = blockIdx.x * 64 + threadIdx.x, h = t / L, c = t % L;
     const bool in = h < heads;
+    const bool is_q = h < a.n_q, is_k = !is_q && h < a.n_q + a.n_kv;
+    const float* gamma = is_q ? a.r.q_gamma : is_k ? a.r.k_gamma : nullptr;
     const float4v x = *reinterpret_cast<const float4v*>(a.qkv + (in ? (size_t)h * HD + 4 * c : 0));
+    const Gains g = load_gains<HD>(a.r, gamma, c);
     const uint32_t done = ctrl->done, pos = ctrl->pos;
     if (done) return;
     if (pos >= a.cap) {
@@ -290,32 +348,35 @@ __global__ __launch_bounds__(64) void k_append_decode(AppendArgs a, vsl_ctrl* ct
         return;
     }
     if (!in) return;
-    const bool is_q = h < a.n_q, is_k = !is_q && h < a.n_q + a.n_kv;
     const uint32_t kvh = is_q ? 0 : is_k ? h - a.n_q : h - a.n_q - a.n_kv;
-    double y[4] = {x[0], x[1], x[2], x[3]};
-    if (is_q || is_k) norm_rotate<HD>(x, is_q ? a.r.q_gamma : a.r.k_gamma, a.r, pos, c, y);
+    const uint64_t P = kv4_positions(a.cap), soff = kv4_steps_off(a.n_kv, a.cap, HD);
+    RowIn in_row;
+    in_row.x = x;
+    if (is_q || is_k) load_angles<HD>(a.r, pos, c, in_row);
+    if constexpr (KVM == KV_4) {
+        if (is_k) {
+            double y[4];
+            norm_rotate<HD>(in_row, gamma != nullptr, g, a.r, c, y);
+            store_k4<HD>(a.kc, soff, (size_t)kvh * P + pos, c, y);
+            return;
+        }
+    }
+    float y[4] = {x[0], x[1], x[2], x[3]};
+    if (is_q || is_k) norm_rotate<HD>(in_row, gamma != nullptr, g, a.r, c, y);
     if (is_q) {
         store_q<Q_F32>(a.q_out, (size_t)h * HD + 4 * c, 0, y);
-        return;
-    }
-    void* cache = is_k ? a.kc : a.vc;
-    if constexpr (KVM != KV_4) {
-        store_kv<KVM>(cache, ((size_t)kvh * a.cap + pos) * HD + 4 * c, y);
+    } else if constexpr (KVM != KV_4) {
+        store_kv<KVM>(is_k ? a.kc : a.vc, ((size_t)kvh * a.cap + pos) * HD + 4 * c, y);
     } else {
-        const uint64_t P = kv4_positions(a.cap), soff = kv4_steps_off(a.n_kv, a.cap, HD);
-        if (is_k) {
-            store_k4<HD>(cache, soff, (size_t)kvh * P + pos, c, y);
-        } else {
-            const size_t oct = (size_t)kvh * (P / 8) + pos / 8;
-            u32x4* dst = reinterpret_cast<u32x4*>(static_cast<uint32_t*>(cache) + oct * HD + 4 * c);
-            const u32x4 old = *dst;
-            const uint32_t sh = kv4_shift(pos & 7);
-            uint32_t n[4];
-            const uint32_t step = kv4_quantize(y, n);
-            *dst = (old & ~(15u << sh)) | (u32x4{n[0], n[1], n[2], n[3]} << sh);
-            if ((c & 7) == 0)
-                reinterpret_cast<uint16_t*>(static_cast<char*>(cache) + soff)[(oct * NB + c / 8) * 8 + (pos & 7)] = (uint16_t)step;
-        }
+        const size_t oct = (size_t)kvh * (P / 8) + pos / 8;
+        u32x4* dst = reinterpret_cast<u32x4*>(static_cast<uint32_t*>(a.vc) + oct * HD + 4 * c);
+        const u32x4 old = *dst;
+        const uint32_t sh = kv4_shift(pos & 7);
+        uint32_t n[4];
+        const uint32_t step = kv4_quantize(y, n);
+        *dst = (old & ~(15u << sh)) | (u32x4{n[0], n[1], n[2], n[3]} << sh);
+        if ((c & 7) == 0)
+            reinterpret_cast<uint16_t*>(static_cast<char*>(a.vc) + soff)[(oct * NB + c / 8) * 8 + (pos & 7)] = (uint16_t)step;
     }
 }
 
@@ -373,13 +434,9 @@ __global__ __launch_bounds__(256) void k_kv4_read(const char* __restrict__ kc, c
 // decode attention
 // ---------------------------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
-#ifndef KBUF
-#define KBUF 2
-#endif
-#ifndef KDEC
-#define KDEC 4
-#endif
-constexpr int kDecWaves = KDEC;
+// Waves of a decode attention block, and tiles in flight a wave. With 8 waves, or 3 or 4 tiles, the 8B shape at 32 splits
+// took 6.1, 5.6 or 5.9 us over 778 positions instead of 4.9, and 11.4, 13.4 or 14.0 us over 32001 instead of 11.9.
+constexpr int kDecWaves = 4, kDecTiles = 2;
 
 // LDS traffic alone (global loads stay in flight).
 __device__ __forceinline__ void lds_barrier() {
@@ -414,7 +471,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_decode_kv4(const float* 
     constexpr int KS = HD / 32, NB = HD / 32, NC = HD / 16;  // k-steps; blocks a row; V columns a lane (and O^T tiles)
     constexpr uint32_t TP = 32;
     constexpr float kLazy = 8.f;
-    constexpr int NBUF = KBUF;
+    constexpr int NBUF = kDecTiles;
     static_assert(G >= 1 && G <= 8, "GQA group of 1..8 heads");
     __shared__ __attribute__((aligned(8))) float s_ml[WAVES][G][2];
     __shared__ __attribute__((aligned(16))) float s_acc[WAVES][G][HD];
@@ -680,8 +737,13 @@ int check_append(const char* fn, const float* qkv, uint32_t n_q, uint32_t n_kv, 
 }
 
 template <int HD, int QM>
-void launch_rows(uint32_t grid, hipStream_t s, const AppendArgs& a, int kv_dtype, uint32_t v_waves) {
-    if (kv_dtype == VSL_DT_KV4) k_append_rows<HD, QM, KV_4><<<grid, 256, 0, s>>>(a, v_waves);
+void launch_rows(hipStream_t s, const AppendArgs& a, int kv_dtype) {
+    const bool kv4 = kv_dtype == VSL_DT_KV4;
+    const uint64_t octets = ((uint64_t)a.pos0 + a.S - 1) / 8 - a.pos0 / 8 + 1;
+    const uint64_t v_waves = kv4 ? octets * a.n_kv * (HD / 32) : 0;
+    const uint64_t items = (uint64_t)a.S * (a.n_q + (kv4 ? 1 : 2) * (uint64_t)a.n_kv);
+    const uint32_t grid = (uint32_t)((v_waves + (items + 256 / HD - 1) / (256 / HD) + 3) / 4);
+    if (kv4) k_append_rows<HD, QM, KV_4><<<grid, 256, 0, s>>>(a, (uint32_t)v_waves);
     else if (kv_dtype == VSL_DT_F16) k_append_rows<HD, QM, KV_F16><<<grid, 256, 0, s>>>(a, 0);
     else k_append_rows<HD, QM, KV_F32><<<grid, 256, 0, s>>>(a, 0);
 }
@@ -714,20 +776,15 @@ extern "C" int vsl_qk_norm_rope_append(const float* qkv, uint32_t S, uint32_t n_
     if ((uint64_t)pos0 + S > cap)
         return vsl_capacity("%s: %u positions from %u exceed capacity %u", fn, S, pos0, cap);
     if (S == 0) return VSL_OK;
-    const AppendArgs a{qkv, S, n_q, n_kv, pos0, cap, RopeArgs{q_gamma, k_gamma, rope_cos, rope_sin, (double)eps, rope},
+    const AppendArgs a{qkv, S, n_q, n_kv, pos0, cap, RopeArgs{q_gamma, k_gamma, rope_cos, rope_sin, eps, rope},
                        q_out, kcache, vcache};
-    const bool kv4 = kv_dtype == VSL_DT_KV4;
-    const uint64_t v_waves = kv4 ? ((uint64_t)(pos0 + S - 1) / 8 - pos0 / 8 + 1) * n_kv * (hd / 32) : 0;
-    const uint64_t rows = (uint64_t)S * (n_q + (kv4 ? 1 : 2) * (uint64_t)n_kv), per_wave = 256 / hd;
-    const uint64_t blocks = (v_waves + (rows + per_wave - 1) / per_wave + 3) / 4;
-    if (blocks > 0x0FFFFFFEull) return vsl_unsupported("%s: %u rows in one call", fn, S);
+    if ((uint64_t)S * (n_q + 2 * n_kv) * hd >= 1ull << 37) return vsl_unsupported("%s: %u rows in one call", fn, S);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const uint32_t grid = (uint32_t)blocks;
     auto go = [&](auto hdc) {
         constexpr int HD = decltype(hdc)::value;
-        if (q_dtype == VSL_DT_F32) launch_rows<HD, Q_F32>(grid, s, a, kv_dtype, (uint32_t)v_waves);
-        else if (q_dtype == VSL_DT_F16) launch_rows<HD, Q_F16>(grid, s, a, kv_dtype, (uint32_t)v_waves);
-        else launch_rows<HD, Q_F16X2>(grid, s, a, kv_dtype, (uint32_t)v_waves);
+        if (q_dtype == VSL_DT_F32) launch_rows<HD, Q_F32>(s, a, kv_dtype);
+        else if (q_dtype == VSL_DT_F16) launch_rows<HD, Q_F16>(s, a, kv_dtype);
+        else launch_rows<HD, Q_F16X2>(s, a, kv_dtype);
     };
     if (hd == 128) go(std::integral_constant<int, 128>{});
     else go(std::integral_constant<int, 64>{});
@@ -744,7 +801,7 @@ extern "C" int vsl_qk_norm_rope_append_decode(const float* qkv, uint32_t n_q, ui
                                     kv_dtype, cap))
         return rc;
     if (!ctrl) return vsl_invalid("%s: null pointer", fn);
-    const AppendArgs a{qkv, 1, n_q, n_kv, 0, cap, RopeArgs{q_gamma, k_gamma, rope_cos, rope_sin, (double)eps, rope},
+    const AppendArgs a{qkv, 1, n_q, n_kv, 0, cap, RopeArgs{q_gamma, k_gamma, rope_cos, rope_sin, eps, rope},
                        q_out, kcache, vcache};
     const uint32_t grid = (uint32_t)(((uint64_t)(n_q + 2 * n_kv) * (hd / 4) + 63) / 64);
     hipStream_t s = static_cast<hipStream_t>(stream);
