@@ -66,6 +66,10 @@ typedef struct vsl_engine_options {
     uint32_t quant_decode;      /* 1 (default): block-quantized weights also stay resident as blocks
                                    (vsl_quant_pack) and the decode GEMVs read those; the prompt pass
                                    uses the expanded packs */
+    uint32_t kv4;               /* 1 = KV cache in 4 bits (VSL_DT_KV4: 4.5 bits a value instead of the weights' 16 or
+                                   32; head_dim 64 or 128) */
+    uint32_t rope_halves;       /* 1 = rotation of the pairs (j, j + head_dim / 2) instead of (2j, 2j + 1)
+                                   (VSL_ROPE_HALVES) */
 } vsl_engine_options;
 
 typedef struct vsl_gen_params {
@@ -157,6 +161,10 @@ int vsl_engine_pack(vsl_engine* e, uint64_t idx, vsl_pack_info* out, char* name,
  * convention 0 = the reference's tensor-type ids (F32 6, F16 48, Q4_0 13, Q4_1 14, Q8_0 17) and
  * block layout, 1 = ggml ids (F32 0, F16 1, Q4_0 2, Q4_1 3, Q8_0 8) and ggml's block layout. */
 int vsl_write_synthetic_gguf(const char* path, const vsl_model_spec* spec, uint64_t seed, int convention);
+/* the same with per-head norms of queries and keys (F32 "blk.N.attn_q_norm.weight" / "blk.N.attn_k_norm.weight" of
+ * head_dim gains, N(1, 0.1)); an engine opened from a file that has both tensors in every layer applies them before
+ * the rotation (vsl_qk_norm_rope_append).  No reference counterpart. */
+int vsl_write_synthetic_gguf_qk_norm(const char* path, const vsl_model_spec* spec, uint64_t seed, int convention);
 /* the same with a vocabulary: n_tokens strings (tokens[i], token_lens[i] bytes each, may hold any
  * byte) written as the array "tokenizer.ggml.tokens", or with keyed = 1 as one string key
  * "tokenizer.ggml.tokens.<i>" per token (the layout the reference's Tokenizer::from_gguf scans for,

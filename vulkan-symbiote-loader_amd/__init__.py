@@ -69,7 +69,7 @@ class EngineOptions(ctypes.Structure):
                 ("dequant_f32", ctypes.c_uint32), ("sparse_attention", ctypes.c_uint32),
                 ("sparse_window", ctypes.c_uint32), ("sparse_global", ctypes.c_uint32),
                 ("sparse_threshold", ctypes.c_uint32), ("prefill_lo8", ctypes.c_uint32),
-                ("quant_decode", ctypes.c_uint32)]
+                ("quant_decode", ctypes.c_uint32), ("kv4", ctypes.c_uint32), ("rope_halves", ctypes.c_uint32)]
 
 
 class GenParams(ctypes.Structure):
@@ -216,6 +216,7 @@ _ENGINE_SIGS = {
                                     ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),
     "vsl_engine_read_tensor": (_I32, [_P, ctypes.c_char_p, _P, _U64, ctypes.POINTER(ctypes.c_int)]),
     "vsl_write_synthetic_gguf": (_I32, [ctypes.c_char_p, ctypes.POINTER(ModelSpec), _U64, _I32]),
+    "vsl_write_synthetic_gguf_qk_norm": (_I32, [ctypes.c_char_p, ctypes.POINTER(ModelSpec), _U64, _I32]),
     "vsl_write_synthetic_gguf_vocab": (_I32, [ctypes.c_char_p, ctypes.POINTER(ModelSpec), _U64, _I32,
                                               ctypes.POINTER(ctypes.c_char_p), ctypes.POINTER(_U64), _U32, _I32]),
     "vsl_engine_pack_count": (_I32, [_P, ctypes.POINTER(_U64)]),
@@ -293,15 +294,19 @@ def make_spec(cfg, init_std=0.02):
     return s
 
 
-def write_synthetic_gguf(path, cfg, seed=0, convention="reference", init_std=0.02, vocab=None, keyed=False):
+def write_synthetic_gguf(path, cfg, seed=0, convention="reference", init_std=0.02, vocab=None, keyed=False,
+                         qk_norm=False):
     """cfg["dtype"]: VSL_WF_* storage of the 2-D weights. vocab: optional list of token strings or
     bytes, written as the array tokenizer.ggml.tokens (keyed=True: one key tokenizer.ggml.tokens.<id>
-    per token)."""
+    per token). qk_norm: per-head norms of queries and keys (no vocabulary then)."""
     lib = engine_lib()
     spec = make_spec(cfg, init_std)
     conv = {"reference": 0, "ggml": 1}[convention]
+    if vocab is not None and qk_norm:
+        raise ValueError("write_synthetic_gguf: qk_norm with a vocabulary")
     if vocab is None:
-        check(lib.vsl_write_synthetic_gguf(str(path).encode(), ctypes.byref(spec), seed, conv), lib)
+        write = lib.vsl_write_synthetic_gguf_qk_norm if qk_norm else lib.vsl_write_synthetic_gguf
+        check(write(str(path).encode(), ctypes.byref(spec), seed, conv), lib)
         return
     toks = [t if isinstance(t, bytes) else t.encode() for t in vocab]
     arr = (ctypes.c_char_p * max(len(toks), 1))(*toks)
@@ -365,10 +370,11 @@ class Engine:
 
     def __init__(self, gguf_path=None, spec=None, seed=0, device=0, kv_capacity=0, use_graph=True,
                  prefill_chunk=0, attn_splits=0, batched_prefill=True, init_std=0.02, prefill_split=None,
-                 dequant_f32=False, window=None, prefill_lo8=None, quant_decode=True):
+                 dequant_f32=False, window=None, prefill_lo8=None, quant_decode=True, kv4=False, rope_halves=False):
         """window: None (dense attention) or (sparse_window, sparse_global, sparse_threshold) for the
         windowed long-context mode; (512, 16, 8192) are the reference's values. prefill_split /
-        prefill_lo8: None keeps vsl_engine_default_options' stage masks."""
+        prefill_lo8: None keeps vsl_engine_default_options' stage masks. kv4: KV cache in 4 bits.
+        rope_halves: rotation of the pairs (j, j + head_dim / 2)."""
         self._lib = engine_lib()
         opt = EngineOptions()
         self._lib.vsl_engine_default_options(ctypes.byref(opt))
@@ -380,6 +386,7 @@ class Engine:
             opt.prefill_lo8 = prefill_lo8
         opt.dequant_f32 = int(bool(dequant_f32))
         opt.quant_decode = int(bool(quant_decode))
+        opt.kv4, opt.rope_halves = int(bool(kv4)), int(bool(rope_halves))
         if window is not None:
             opt.sparse_attention = 1
             opt.sparse_window, opt.sparse_global, opt.sparse_threshold = window

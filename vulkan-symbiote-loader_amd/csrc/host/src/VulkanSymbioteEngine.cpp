@@ -149,7 +149,12 @@ ExpectedVoid write_synthetic_gguf(const Path& path, const SyntheticSpec& spec, G
         for (uint64_t i = 0; i < d; ++i) f[i] = 1.0f;
         w.add_tensor(name, {d}, false, f, d * 4);
     };
-    store.reserve(4 + 9 * c.num_layers);
+    auto add_gains = [&](const std::string& name) {
+        store.emplace_back(hd * 4);
+        synthetic_fill_host(store.back().data(), false, hd, spec.seed, name, 1.0f, 0.1f);
+        w.add_tensor(name, {hd}, false, store.back().data(), hd * 4);
+    };
+    store.reserve(4 + 11 * c.num_layers);
     add_rand("token_embd.weight", d, V);
     for (uint32_t l = 0; l < c.num_layers; ++l) {
         add_ones(layer_name(l, "attn_norm.weight"));
@@ -157,6 +162,10 @@ ExpectedVoid write_synthetic_gguf(const Path& path, const SyntheticSpec& spec, G
         add_rand(layer_name(l, "attn_k.weight"), d, nkv * hd);
         add_rand(layer_name(l, "attn_v.weight"), d, nkv * hd);
         add_rand(layer_name(l, "attn_o.weight"), nq * hd, d);
+        if (spec.qk_norm) {
+            add_gains(layer_name(l, "attn_q_norm.weight"));
+            add_gains(layer_name(l, "attn_k_norm.weight"));
+        }
         add_ones(layer_name(l, "ffn_norm.weight"));
         add_rand(layer_name(l, "ffn_gate.weight"), d, F);
         add_rand(layer_name(l, "ffn_up.weight"), d, F);
@@ -204,6 +213,12 @@ VulkanSymbioteEngine::VulkanSymbioteEngine(const Path& model_path, const EngineO
         return static_cast<int>(options_.dequant_f32 ? VSL_DT_F32 : VSL_DT_F16);
     };
     tokenizer_ = Tokenizer::from_gguf(model_path);  // VulkanSymbioteEngine.cpp:1140
+    uint32_t norms = 0;
+    for (uint32_t l = 0; l < cfg.num_layers; ++l)
+        for (const char* n : {"attn_q_norm.weight", "attn_k_norm.weight"}) norms += loader_->get_tensor(layer_name(l, n)) != nullptr;
+    if (norms && norms != 2 * cfg.num_layers)
+        throw std::runtime_error("Failed to load model: query / key norms in some layers only");
+    qk_norm_ = norms != 0;
     try {
         plan_quant_gguf(cfg);
         init_device(cfg, pack_dtype(qf) == VSL_DT_F16, pack_dtype(ef));
@@ -321,7 +336,8 @@ void VulkanSymbioteEngine::init_device(const ModelConfig& cfg, bool fp16_weights
     if ((uint64_t)options_.sparse_window + options_.sparse_global >= 0x80000000ull)
         throw std::runtime_error("sparse window + global tokens too large");
     wdt_ = fp16_weights ? VSL_DT_F16 : VSL_DT_F32;
-    kvdt_ = wdt_;  // fp16 models keep an fp16 KV cache; fp32 models keep fp32
+    kvdt_ = options_.kv4 ? VSL_DT_KV4 : wdt_;  // fp16 models keep an fp16 KV cache; fp32 models keep fp32
+    append_apart_ = options_.kv4 || options_.rope_halves || qk_norm_;
     edt_ = embed_dtype;
     const uint32_t hd = config_.head_dim;
     if (hd != 64 && hd != 128) throw std::runtime_error("head_dim must be 64 or 128");
@@ -355,8 +371,8 @@ void VulkanSymbioteEngine::plan_and_allocate() {
     const ModelConfig& c = config_;
     const uint64_t d = c.hidden_size, hd = c.head_dim, nq = c.num_attention_heads, nkv = c.num_key_value_heads,
                    F = c.intermediate_size, V = c.vocab_size, L = c.num_layers, cap = cap_;
-    const uint64_t es = wdt_ == VSL_DT_F16 ? 2 : 4, kes = kvdt_ == VSL_DT_F16 ? 2 : 4, ees = edt_ == VSL_DT_F16 ? 2 : 4;
-    const bool batched = options_.batched_prefill && wdt_ == VSL_DT_F16 && kvdt_ == VSL_DT_F16 && d % 128 == 0 &&
+    const uint64_t es = wdt_ == VSL_DT_F16 ? 2 : 4, ees = edt_ == VSL_DT_F16 ? 2 : 4;
+    const bool batched = options_.batched_prefill && wdt_ == VSL_DT_F16 && kvdt_ != VSL_DT_F32 && d % 128 == 0 &&
                          ((nq + 2 * nkv) * hd) % 128 == 0 && (nq * hd) % 32 == 0 && F % 64 == 0 && d % 32 == 0 &&
                          F % 32 == 0;
     chunk_ = batched ? std::min<uint32_t>(options_.prefill_chunk ? options_.prefill_chunk : 2048, cap_) : 0;
@@ -374,6 +390,11 @@ void VulkanSymbioteEngine::plan_and_allocate() {
         Layer& y = layers_[l];
         add(d * 4, reinterpret_cast<void**>(&y.attn_norm));
         add(d * 4, reinterpret_cast<void**>(&y.ffn_norm));
+        if (qk_norm_) {
+            add(hd * 4, reinterpret_cast<void**>(&y.q_norm));
+            add(hd * 4, reinterpret_cast<void**>(&y.k_norm));
+            wbytes += 8 * hd;
+        }
         add((nq + 2 * nkv) * hd * d * es, &y.wqkv);
         add(d * nq * hd * es, &y.wo);
         add(2 * F * d * es, &y.wgu);
@@ -399,11 +420,13 @@ void VulkanSymbioteEngine::plan_and_allocate() {
     qadd(qfmt_out_, V, d, &out_q_, &out_qdt_);
     weight_bytes_ = wbytes;
     kv_bytes_ = 0;
+    const uint64_t kv = vsl_kv_cache_bytes(kvdt_, (uint32_t)nkv, (uint32_t)cap, (uint32_t)hd);
     for (uint64_t l = 0; l < L; ++l) {
-        add(nkv * cap * hd * kes, &layers_[l].kc);
-        add(nkv * cap * hd * kes, &layers_[l].vc);
-        kv_bytes_ += 2 * nkv * cap * hd * kes;
+        add(kv, &layers_[l].kc);
+        add(kv, &layers_[l].vc);
+        kv_bytes_ += 2 * kv;
     }
+    if (append_apart_) add((nq + 2 * nkv) * hd * 4, reinterpret_cast<void**>(&qkv_));
     add(cap * (hd / 2) * 4, reinterpret_cast<void**>(&rope_cos_));
     add(cap * (hd / 2) * 4, reinterpret_cast<void**>(&rope_sin_));
     add(d * 4, reinterpret_cast<void**>(&x_));
@@ -623,14 +646,14 @@ void VulkanSymbioteEngine::load_weights_from_gguf() {
         load_weight(dst, name, elems, wdt_, qt);
     };
     std::vector<std::vector<float>> norm_host;
-    norm_host.reserve(2 * c.num_layers + 1);
-    auto load_norm = [&](float* dst, const std::string& name) {
-        const GGUFTensorInfo& t = need(name, d);
+    norm_host.reserve(4 * c.num_layers + 1);
+    auto load_norm = [&](float* dst, const std::string& name, uint64_t n) {
+        const GGUFTensorInfo& t = need(name, n);
         auto r = g.read_tensor_data(t, true);  // F32 copied, F16 converted, blocks dequantized
-        if (!r.has_value() || r.value().size() != d) throw std::runtime_error("cannot read " + name);
+        if (!r.has_value() || r.value().size() != n) throw std::runtime_error("cannot read " + name);
         norm_host.push_back(std::move(r.value()));
-        check(vsl_copy_h2d(dst, norm_host.back().data(), d * 4, upload_stream_), "norm upload");
-        pack_manager_.register_pack(meta_of(name), dst, d * 4, VSL_DT_F32);
+        check(vsl_copy_h2d(dst, norm_host.back().data(), n * 4, upload_stream_), "norm upload");
+        pack_manager_.register_pack(meta_of(name), dst, n * 4, VSL_DT_F32);
     };
     load_weight(embed_, "token_embd.weight", V * d, edt_, QTarget{});
     for (uint32_t l = 0; l < c.num_layers; ++l) {
@@ -639,7 +662,11 @@ void VulkanSymbioteEngine::load_weights_from_gguf() {
         char* qkv = static_cast<char*>(y.wqkv);
         const uint32_t nr = (uint32_t)((nq + 2 * nkv) * hd);
         auto qt = [](void* pack, uint32_t rows, uint32_t K, uint32_t row0) { return QTarget{pack, rows, K, row0}; };
-        load_norm(y.attn_norm, layer_name(l, "attn_norm.weight"));
+        load_norm(y.attn_norm, layer_name(l, "attn_norm.weight"), d);
+        if (qk_norm_) {
+            load_norm(y.q_norm, layer_name(l, "attn_q_norm.weight"), hd);
+            load_norm(y.k_norm, layer_name(l, "attn_k_norm.weight"), hd);
+        }
         load_linear(qkv, layer_name(l, "attn_q.weight"), nq * hd * d, qt(y.qqkv, nr, (uint32_t)d, 0));
         load_linear(qkv + nq * hd * d * es, layer_name(l, "attn_k.weight"), nkv * hd * d,
                     qt(y.qqkv, nr, (uint32_t)d, (uint32_t)(nq * hd)));
@@ -648,14 +675,14 @@ void VulkanSymbioteEngine::load_weights_from_gguf() {
         const std::string oname = g.get_tensor(layer_name(l, "attn_o.weight")) ? layer_name(l, "attn_o.weight")
                                                                                : layer_name(l, "attn_output.weight");
         load_linear(y.wo, oname, d * nq * hd, qt(y.qo, (uint32_t)d, (uint32_t)(nq * hd), 0));
-        load_norm(y.ffn_norm, layer_name(l, "ffn_norm.weight"));
+        load_norm(y.ffn_norm, layer_name(l, "ffn_norm.weight"), d);
         load_linear(y.wgu, layer_name(l, "ffn_gate.weight"), F * d, qt(y.qgu, (uint32_t)(2 * F), (uint32_t)d, 0));
         load_linear(static_cast<char*>(y.wgu) + F * d * es, layer_name(l, "ffn_up.weight"), F * d,
                     qt(y.qgu, (uint32_t)(2 * F), (uint32_t)d, (uint32_t)F));
         load_linear(y.wdown, layer_name(l, "ffn_down.weight"), d * F, qt(y.qdown, (uint32_t)d, (uint32_t)F, 0));
     }
     if (g.get_tensor("output_norm.weight")) {
-        load_norm(out_norm_, "output_norm.weight");
+        load_norm(out_norm_, "output_norm.weight", d);
     } else {
         out_norm_ = nullptr;  // the reference has no final norm; a file without one runs without it
     }
@@ -674,17 +701,33 @@ void VulkanSymbioteEngine::load_weights_from_gguf() {
     vsl_host_pinned_free(stage[1]);
 }
 
+void VulkanSymbioteEngine::enqueue_qkv(const Layer& y) {
+    const ModelConfig& c = config_;
+    const uint32_t d = c.hidden_size, hd = c.head_dim, nq = c.num_attention_heads, nkv = c.num_key_value_heads;
+    const float eps = c.rms_epsilon;
+    // the operand's resident block-quantized pack where it has one, else its expanded pack
+    const void* w = y.qqkv ? y.qqkv : y.wqkv;
+    const int wdt = y.qqkv ? y.qdt_qkv : wdt_;
+    if (!append_apart_) {
+        check(vsl_qkv_rope_append(x_, y.attn_norm, eps, w, wdt, d, nq, nkv, hd, rope_cos_, rope_sin_, y.kc, y.vc, kvdt_, cap_,
+                                  q_, ctrl_, stream_),
+              "vsl_qkv_rope_append");
+        return;
+    }
+    check(vsl_norm_gemv(x_, y.attn_norm, eps, w, wdt, (nq + 2 * nkv) * hd, d, qkv_, ctrl_, stream_), "vsl_norm_gemv(qkv)");
+    check(vsl_qk_norm_rope_append_decode(qkv_, nq, nkv, hd, y.q_norm, y.k_norm, eps, rope(), rope_cos_, rope_sin_, q_, y.kc,
+                                         y.vc, kvdt_, cap_, ctrl_, stream_),
+          "vsl_qk_norm_rope_append_decode");
+}
+
 void VulkanSymbioteEngine::enqueue_layers(uint32_t l0, uint32_t l1) {
     const ModelConfig& c = config_;
-    const uint32_t d = c.hidden_size, hd = c.head_dim, nq = c.num_attention_heads, nkv = c.num_key_value_heads,
-                   F = c.intermediate_size;
+    const uint32_t d = c.hidden_size, hd = c.head_dim, nq = c.num_attention_heads, F = c.intermediate_size;
     const float eps = c.rms_epsilon, scale = 1.0f / std::sqrt((float)hd);
     for (uint32_t l = l0; l < l1; ++l) {
         const Layer& y = layers_[l];
         // each operand's resident block-quantized pack where it has one, else its expanded pack
-        check(vsl_qkv_rope_append(x_, y.attn_norm, eps, y.qqkv ? y.qqkv : y.wqkv, y.qqkv ? y.qdt_qkv : wdt_, d, nq,
-                                  nkv, hd, rope_cos_, rope_sin_, y.kc, y.vc, kvdt_, cap_, q_, ctrl_, stream_),
-              "vsl_qkv_rope_append");
+        enqueue_qkv(y);
         check(attend(y, scale), "vsl_attn_decode");
         check(vsl_gemv_residual(y.qo ? y.qo : y.wo, y.qo ? y.qdt_o : wdt_, d, nq * hd, attn_, x_, ctrl_, stream_),
               "vsl_gemv_residual(o)");
@@ -826,10 +869,26 @@ void VulkanSymbioteEngine::prefill_batched(uint32_t n_prompt, const SamplingPara
             const int a_o_l = a_o | (a_o == VSL_GEMM_A_F8 ? y.b8_o : 0);
             const int g_gu_l = g_gu | ((g_gu & VSL_GEMM_A_F8) ? y.b8_gu : 0);
             const int a_dn_l = a_dn | (a_dn == VSL_GEMM_A_F8 ? y.b8_down : 0);
-            check(vsl_gemm_f16_qkv_rope_append(pxn_, y.wqkv, S, d, a_qkv_l, nq, nkv, hd, c0, rope_cos_, rope_sin_, pq_,
-                                               qdt, y.kc, y.vc, kvdt_, cap_, pqkv_, gws_, gws_bytes_, stream_),
-                  "qkv + rope");
-            if (config_.use_sparse_attention)
+            if (append_apart_) {
+                check(vsl_gemm_f16_ws(pxn_, y.wqkv, S, wqkv, d, pqkv_, VSL_EPI_STORE_F32 | a_qkv_l, gws_, gws_bytes_, stream_),
+                      "gemm qkv");
+                check(vsl_qk_norm_rope_append(pqkv_, S, nq, nkv, hd, c0, y.q_norm, y.k_norm, eps, rope(), rope_cos_, rope_sin_,
+                                              pq_, qdt, y.kc, y.vc, kvdt_, cap_, stream_),
+                      "vsl_qk_norm_rope_append");
+            } else {
+                check(vsl_gemm_f16_qkv_rope_append(pxn_, y.wqkv, S, d, a_qkv_l, nq, nkv, hd, c0, rope_cos_, rope_sin_, pq_,
+                                                   qdt, y.kc, y.vc, kvdt_, cap_, pqkv_, gws_, gws_bytes_, stream_),
+                      "qkv + rope");
+            }
+            if (kvdt_ == VSL_DT_KV4 && config_.use_sparse_attention)
+                check(vsl_attn_prefill_kv4_window(pq_, qdt, y.kc, y.vc, S, c0, nq, nkv, hd, cap_, scale, pattn_, odt,
+                                                  config_.sparse_window_size, config_.sparse_global_tokens,
+                                                  config_.sparse_threshold, stream_),
+                      "vsl_attn_prefill_kv4_window");
+            else if (kvdt_ == VSL_DT_KV4)
+                check(vsl_attn_prefill_kv4(pq_, qdt, y.kc, y.vc, S, c0, nq, nkv, hd, cap_, scale, pattn_, odt, stream_),
+                      "vsl_attn_prefill_kv4");
+            else if (config_.use_sparse_attention)
                 check(vsl_attn_prefill_window(pq_, qdt, y.kc, y.vc, S, c0, nq, nkv, hd, cap_, scale, pattn_, odt,
                                               config_.sparse_window_size, config_.sparse_global_tokens,
                                               config_.sparse_threshold, stream_),
@@ -975,8 +1034,7 @@ int VulkanSymbioteEngine::generate_ids(const std::vector<uint32_t>& prompt, uint
 
 double VulkanSymbioteEngine::time_op(int op, uint32_t iterations) {
     const ModelConfig& c = config_;
-    const uint32_t d = c.hidden_size, hd = c.head_dim, nq = c.num_attention_heads, nkv = c.num_key_value_heads,
-                   F = c.intermediate_size;
+    const uint32_t d = c.hidden_size, hd = c.head_dim, nq = c.num_attention_heads, F = c.intermediate_size;
     const float eps = c.rms_epsilon, scale = 1.0f / std::sqrt((float)hd);
     if (gen_active_) synchronize();
     gen_active_ = false;
@@ -988,9 +1046,7 @@ double VulkanSymbioteEngine::time_op(int op, uint32_t iterations) {
         const Layer& y = layers_[l];
         switch (op) {
             case 0:
-                check(vsl_qkv_rope_append(x_, y.attn_norm, eps, y.qqkv ? y.qqkv : y.wqkv, y.qqkv ? y.qdt_qkv : wdt_, d,
-                                          nq, nkv, hd, rope_cos_, rope_sin_, y.kc, y.vc, kvdt_, cap_, q_, ctrl_,
-                                          stream_), "qkv");
+                enqueue_qkv(y);
                 break;
             case 1:
                 check(attend(y, scale), "attn");

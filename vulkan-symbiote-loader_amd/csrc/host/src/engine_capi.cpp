@@ -55,6 +55,8 @@ static EngineOptions to_options(const vsl_engine_options* o) {
     e.sparse_window = o->sparse_window;
     e.sparse_global = o->sparse_global;
     e.sparse_threshold = o->sparse_threshold;
+    e.kv4 = o->kv4 != 0;
+    e.rope_halves = o->rope_halves != 0;
     return e;
 }
 
@@ -339,10 +341,11 @@ extern "C" int vsl_engine_read_tensor(vsl_engine* e, const char* name, void* dst
     return VSL_OK;
 }
 
-extern "C" int vsl_write_synthetic_gguf(const char* path, const vsl_model_spec* spec, uint64_t seed, int convention) {
+static int write_gguf(const char* path, const vsl_model_spec* spec, uint64_t seed, int convention, bool qk_norm) {
     if (!path || !spec) return fail(VSL_E_INVALID, "vsl_write_synthetic_gguf: null argument");
     if (spec->dtype > VSL_WF_Q8_0) return fail(VSL_E_INVALID, "vsl_write_synthetic_gguf: unknown weight format");
     SyntheticSpec s;
+    s.qk_norm = qk_norm;
     s.config = to_config(spec);
     s.fp16 = spec->dtype == VSL_DT_F16;
     s.quant_format = spec->dtype >= VSL_WF_Q4_0 ? static_cast<int>(spec->dtype) : -1;
@@ -351,6 +354,14 @@ extern "C" int vsl_write_synthetic_gguf(const char* path, const vsl_model_spec* 
     auto r = write_synthetic_gguf(Path(path), s, convention == 1 ? GGUFConvention::GGML : GGUFConvention::REFERENCE);
     if (!r.has_value()) return fail(r.error(), "vsl_write_synthetic_gguf: write failed");
     return VSL_OK;
+}
+
+extern "C" int vsl_write_synthetic_gguf(const char* path, const vsl_model_spec* spec, uint64_t seed, int convention) {
+    return write_gguf(path, spec, seed, convention, false);
+}
+
+extern "C" int vsl_write_synthetic_gguf_qk_norm(const char* path, const vsl_model_spec* spec, uint64_t seed, int convention) {
+    return write_gguf(path, spec, seed, convention, true);
 }
 
 extern "C" int vsl_write_synthetic_gguf_vocab(const char* path, const vsl_model_spec* spec, uint64_t seed,

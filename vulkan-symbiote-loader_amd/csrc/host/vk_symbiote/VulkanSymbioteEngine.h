@@ -101,6 +101,11 @@ struct EngineOptions {
     uint32_t sparse_window = 512;
     uint32_t sparse_global = 16;
     uint32_t sparse_threshold = 8192;
+    // KV cache in 4 bits (VSL_DT_KV4, 4.5 bits a value) instead of the weights' 16 or 32: 8B decode attention over 32001
+    // positions reads 37 MB a layer instead of 131. Keys and values are rounded to 16 steps a 32-dim block.
+    bool kv4 = false;
+    // Rotation of the pairs (j, j + head_dim / 2) instead of (2j, 2j + 1).
+    bool rope_halves = false;
     bool verbose = false;
     static constexpr uint32_t kPrefillSplitAll = 0x1F;
     static constexpr uint32_t kPrefillLo8Stages = 0x1D;
@@ -121,6 +126,8 @@ struct SyntheticSpec {
     // or, with vocab_keyed, as one string key "tokenizer.ggml.tokens.<id>" per entry
     std::vector<std::string> vocab;
     bool vocab_keyed = false;
+    // write_synthetic_gguf only: per-head norms of queries and keys, gains ~ N(1, 0.1)
+    bool qk_norm = false;
     float init_std = 0.02f;
     uint64_t seed = 0;
 };
@@ -205,6 +212,8 @@ class VulkanSymbioteEngine {
     struct Layer {
         float* attn_norm = nullptr;
         float* ffn_norm = nullptr;
+        float* q_norm = nullptr;  // gains of the per-head norms of queries and keys (nullptr: none)
+        float* k_norm = nullptr;
         void* wqkv = nullptr;
         void* wo = nullptr;
         void* wgu = nullptr;
@@ -259,6 +268,7 @@ class VulkanSymbioteEngine {
     std::vector<Layer> layers_;
     float* rope_cos_ = nullptr;
     float* rope_sin_ = nullptr;
+    float* qkv_ = nullptr;  // a decode step's projection where the rotation is not in its epilogue
     float *x_ = nullptr, *q_ = nullptr, *attn_ = nullptr, *h_ = nullptr, *logits_ = nullptr;
     float* wrange_ = nullptr;  // [L][4] largest weight magnitudes (measure_weight_ranges)
     float *part_o_ = nullptr, *part_ml_ = nullptr;
@@ -300,6 +310,11 @@ class VulkanSymbioteEngine {
     vsl_graph* step_graph(const SamplingParams& p);
     void release();
     void check(int rc, const char* what) const;
+    // q / k norms, a 4-bit cache or the rotation by halves: the append is a launch of its own behind the projection
+    bool append_apart_ = false, qk_norm_ = false;
+    int rope() const { return options_.rope_halves ? 1 : 0; }  // VSL_ROPE_*
+    // the QKV projection of a decode step, rotated and appended to the layer's caches
+    void enqueue_qkv(const Layer& y);
     int attend(const Layer& y, float scale);  // decode attention of one layer (dense or windowed)
 };
 
