@@ -41,8 +41,9 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     constexpr int QP = QX2 ? 2 : 1;        // q planes; with split q the probabilities are split too
     static_assert(G % GB == 0 && NKB >= 1 && NKB * KSPLIT * 32 == TK, "a tile's fragments divide over a head's waves");
     static_assert(NKW >= 1 && NKW * NT * 16 == TK * HD, "a tile's words divide over the block");
-    __shared__ __attribute__((aligned(16))) vsl_half Ks[2][TK * HD];
-    __shared__ __attribute__((aligned(16))) vsl_half Vs[2][TK * HD];
+    __shared__ __attribute__((aligned(16))) vsl_half smem[4 * TK * HD];  // two buffers of K, two of V
+    auto Ks = [&](int buf) { return smem + buf * (TK * HD); };
+    auto Vs = [&](int buf) { return smem + (2 + buf) * (TK * HD); };
     __shared__ float s_stat[KSPLIT][GB][128];  // row statistics of the key shares, for their join
     __shared__ uint32_t s_nan;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -106,46 +107,38 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
             b.s[i] = *reinterpret_cast<const u32x4*>(Vst + (oct * NB + w / 16) * 16);
         }
     };
-    // A tile's values into LDS. What lies past the block's last key is anything: its steps are taken as 0. So is a V
-    // block that stands for NaN, as a NaN would reach rows that do not see it through a product with 0: the
-    // block notes that there was one, and the rows that see it are found at the end.
-    auto expand_k = [&](const KWords& b, int buf, uint32_t t) {
+    // A tile's values into LDS. A V block that stands for NaN (or holds no value of this cache: what lies past the
+    // block's last key is anything) would reach rows that do not see its key through a product with 0. Tiles that
+    // some row sees in part (EDGE) take such steps as 0; the block notes that there was a NaN, and the rows that see it
+    // are found at the end. (K needs none of this: what a key's row of scores holds is replaced where it is masked.)
+    auto expand_k = [&](const KWords& b, int buf) {
 #pragma unroll
         for (int i = 0; i < NKW; ++i) {
             const int r = (i * NT + tid) / (HD / 16), w = (i * NT + tid) % (HD / 16);
-            const uint32_t st = t * TK + r < kv_end ? b.s[i] : 0u;
-            const Kv4Step s = kv4_step(st | st << 16, kc4);
-            *reinterpret_cast<half8*>(&Ks[buf][sw<HD>(r, 2 * w)]) = kv4_word(b.k[i].x, s, kc4);
-            *reinterpret_cast<half8*>(&Ks[buf][sw<HD>(r, 2 * w + 1)]) = kv4_word(b.k[i].y, s, kc4);
+            const Kv4Step s = kv4_step(b.s[i] | b.s[i] << 16, kc4);
+            *reinterpret_cast<half8*>(Ks(buf) + sw<HD>(r, 2 * w)) = kv4_word(b.k[i].x, s, kc4);
+            *reinterpret_cast<half8*>(Ks(buf) + sw<HD>(r, 2 * w + 1)) = kv4_word(b.k[i].y, s, kc4);
         }
     };
-    auto expand_v = [&](const VWords& b, int buf, uint32_t t) {
+    auto expand_v = [&](const VWords& b, int buf, uint32_t t, auto edge) {
 #pragma unroll
         for (int i = 0; i < NKW; ++i) {
             const int r = (i * NT + tid) / (HD / 2), w = (i * NT + tid) % (HD / 2);
             u32x4 s = b.s[i];
-            if ((t + 1) * TK > kv_end) {  // block-uniform
+            if constexpr (decltype(edge)::value) {
 #pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    const uint32_t key = t * TK + 8 * r + 2 * p;
-                    s[p] = key >= kv_end ? 0u : key + 1 >= kv_end ? s[p] & 0xFFFFu : s[p];
-                }
-            }
-            // an exponent of all ones carries into its half's top bit, which steps leave 0
-            const u32x4 c = s + 0x04000400u;
-            if (((c[0] | c[1] | c[2] | c[3]) & 0x80008000u) != 0) {
-                s_nan = 1;
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    if ((s[p] & 0xFFFFu) == kKv4NaN) s[p] &= 0xFFFF0000u;
-                    if (s[p] >> 16 == kKv4NaN) s[p] &= 0xFFFFu;
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t x = s[e / 2] >> (16 * (e & 1)) & 0xFFFFu;
+                    if ((x & 0x7C00u) != 0x7C00u) continue;
+                    s[e / 2] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                    if (t * TK + 8 * r + e < kv_end) s_nan = 1;
                 }
             }
             Kv4Step vs[4];
 #pragma unroll
             for (int p = 0; p < 4; ++p) vs[p] = kv4_step(s[p], kc4);
-            *reinterpret_cast<half8*>(&Vs[buf][sw<TK>(2 * w, r)]) = kv4_word(b.v[i].x, vs, kc4);
-            *reinterpret_cast<half8*>(&Vs[buf][sw<TK>(2 * w + 1, r)]) = kv4_word(b.v[i].y, vs, kc4);
+            *reinterpret_cast<half8*>(Vs(buf) + sw<TK>(2 * w, r)) = kv4_word(b.v[i].x, vs, kc4);
+            *reinterpret_cast<half8*>(Vs(buf) + sw<TK>(2 * w + 1, r)) = kv4_word(b.v[i].y, vs, kc4);
         }
     };
 
@@ -170,25 +163,29 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     constexpr float kLazy = 8.f;  // the reference maximum is raised only by more than this (log2 units)
 
     const int krow = (lane & 19) | (lane & 4) << 1 | (lane & 8) >> 1;  // bits 2 and 3 of l % 32 exchanged
-    auto qk = [&](int buf, float16v (&st)[NKB]) {
+    auto read_k = [&](int buf, half8 (&kf)[NKB][HD / 16]) {
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c)
+                kf[kb][c] = *reinterpret_cast<const half8*>(Ks(buf) + sw<HD>((kbase + kb) * 32 + krow, 2 * c + (lane >> 5)));
+    };
+    auto qk = [&](const half8 (&kf)[NKB][HD / 16], float16v (&st)[NKB]) {
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) st[kb][v] = 0.f;
-            half8 kf[HD / 16];
-#pragma unroll
-            for (int c = 0; c < HD / 16; ++c)
-                kf[c] = *reinterpret_cast<const half8*>(&Ks[buf][sw<HD>((kbase + kb) * 32 + krow, 2 * c + (lane >> 5))]);
 #pragma unroll
             for (int c = 0; c < HD / 16; ++c)
 #pragma unroll
-                for (int p = 0; p < QP; ++p) st[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[c], qf[p][c], st[kb], 0, 0, 0);
+                for (int p = 0; p < QP; ++p)
+                    st[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[kb][c], qf[p][c], st[kb], 0, 0, 0);
         }
     };
-    // the mask, where tile t reaches past the block's first row or begins before a row's window; returns the scaled
-    // maximum of this lane's row. Element v of a fragment is key 16 (v / 8) + 8 (l / 32) + v % 8.
-    auto mask_max = [&](float16v (&st)[NKB], uint32_t t) {
-        if (!(t * TK + TK - 1 <= p_first && (t * TK >= lo_max || t * TK + TK <= n_glob))) {
+    // the mask of a tile that some row sees in part; returns the scaled maximum of this lane's row. Element v of a
+    // fragment is key 16 (v / 8) + 8 (l / 32) + v % 8.
+    auto mask_max = [&](float16v (&st)[NKB], uint32_t t, auto edge) {
+        if constexpr (decltype(edge)::value) {
 #pragma unroll
             for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
@@ -251,7 +248,7 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
 #pragma unroll
                 for (int hi = 0; hi < 2; ++hi) {
                     const half8 af = *reinterpret_cast<const half8*>(
-                        &Vs[buf][sw<TK>(tt * 32 + (lane & 31), (kbase + kb) * 4 + 2 * hi + (lane >> 5))]);
+                        Vs(buf) + sw<TK>(tt * 32 + (lane & 31), (kbase + kb) * 4 + 2 * hi + (lane >> 5)));
 #pragma unroll
                     for (int p = 0; p < QP; ++p)
                         o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af, pf[p][kb][hi], o[tt], 0, 0, 0);
@@ -262,83 +259,95 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     // and the scores of t in registers: the codes of K of t + 2 and V of t + 1 are requested, the scores of t + 1 are
     // issued on the matrix cores while the vector pipe turns those of t into probabilities, then the products
     // of t with V; the codes go into the buffers that K of t and V of t - 1 have left (both last read before the
-    // barrier that ended the previous iteration). Requests past the last tile repeat it.
-    auto tile = [&](uint32_t t) { return phys(t < n_vt ? t : n_vt - 1); };
-    if (tid == 0) s_nan = 0;
-    __syncthreads();
+    // barrier that ended the previous iteration). Tiles that every row of the block sees whole come first (without a
+    // window): they run without masks and checks, in one straight block of code past the rescale.
+    float16v st[NKB];
     KWords kw;
     VWords vw;
-    load_k(kw, tile(0));
-    load_v(vw, tile(0));
-    expand_k(kw, 0, tile(0));
-    load_k(kw, tile(1));
-    expand_v(vw, 0, tile(0));
-    expand_k(kw, 1, tile(1));
-    __syncthreads();
-    float16v st[NKB];
-    qk(0, st);
-    for (uint32_t t = 0; t < n_vt; ++t) {
-        load_k(kw, tile(t + 2));
-        load_v(vw, tile(t + 1));
-        rescale(mask_max(st, phys(t)));
+    auto body = [&](uint32_t t, auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
+        const bool one = !EDGE || t + 1 < n_vt, two = t + 2 < n_vt;
+        if (!EDGE || two) load_k(kw, phys(two ? t + 2 : t));
+        if (one) load_v(vw, phys(t + 1));
+        half8 kf[NKB][HD / 16];
+        if (one) read_k((int)((t + 1) & 1), kf);
+        if constexpr (!EDGE) __builtin_amdgcn_sched_barrier(0);
+        rescale(mask_max(st, phys(t), edge));
         float16v sn[NKB];
-        qk((int)((t + 1) & 1), sn);
+        if (one) qk(kf, sn);
         half8 pf[QP][NKB][2];
         l += probs(st, pf);
         pv((int)(t & 1), pf);
-        // every wave has its scores of t (taken in the previous iteration)
-        expand_k(kw, (int)(t & 1), tile(t + 2));
-        expand_v(vw, (int)((t + 1) & 1), tile(t + 1));
+        if (!EDGE || two) expand_k(kw, (int)(t & 1));  // every wave has its scores of t
+        if (one) expand_v(vw, (int)((t + 1) & 1), phys(t + 1), edge);
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb) st[kb] = sn[kb];
         __syncthreads();
+    };
+    if (tid == 0) s_nan = 0;
+    __syncthreads();
+    load_k(kw, phys(0));
+    load_v(vw, phys(0));
+    expand_k(kw, 0);
+    if (n_vt > 1) load_k(kw, phys(1));
+    expand_v(vw, 0, phys(0), std::true_type{});
+    if (n_vt > 1) expand_k(kw, 1);
+    __syncthreads();
+    {
+        half8 kf[NKB][HD / 16];
+        read_k(0, kf);
+        qk(kf, st);
     }
+    const uint32_t n_whole = lo_max ? 0 : (p_first + 1) / TK;
+    uint32_t t = 0;
+    for (; t + 1 < n_whole; ++t) body(t, std::false_type{});
+    for (; t < n_vt; ++t) body(t, std::true_type{});
     const uint32_t any_nan = s_nan;
 
+    // The key shares of each head, joined in LDS (the tile buffers are done with): wave ksp of a head takes the 32-dim
+    // fragments f with f % KSPLIT = ksp from all of them, brought to the largest maximum, and stores them.
+    constexpr int NF = HD / 32;
     if constexpr (KSPLIT > 1) {
-        // the key shares of each head, joined in LDS (the tile buffers are done with): waves with ksp > 0 leave their
-        // accumulators and row statistics, the ksp = 0 wave brings all to the largest maximum
-        constexpr int SLOT = HD / 32 * 16 * 64;          // accumulator floats of a wave
-        constexpr int PER = 2 * TK * HD * 2 / 4 / SLOT;  // slots in each of the two buffer sets
-        static_assert(2 * PER >= (KSPLIT - 1) * GB, "the join does not fit in the tile buffers");
+        constexpr int FS = 16 * 64;  // floats of a fragment
+        static_assert(GB * NF * (KSPLIT - 1) * FS * 4 <= 4 * TK * HD * 2, "the join does not fit in the tile buffers");
         const int hw = wave % GB;
-        auto slot = [&](int j) {
-            const int i = (j - 1) * GB + hw;
-            return reinterpret_cast<float*>(i < PER ? &Ks[0][0] : &Vs[0][0]) + (i % PER) * SLOT;
+        // fragment f as share j leaves it to its taker (j is not the taker)
+        auto slot = [&](int f, int j) {
+            return reinterpret_cast<float*>(smem) + ((hw * NF + f) * (KSPLIT - 1) + (j < f % KSPLIT ? j : j - 1)) * FS + lane;
         };
-        if (ksp > 0) {
-            float* xo = slot(ksp);
 #pragma unroll
-            for (int tt = 0; tt < HD / 32; ++tt)
+        for (int f = 0; f < NF; ++f)
+            if (f % KSPLIT != ksp) {
 #pragma unroll
-                for (int v = 0; v < 16; ++v) xo[(tt * 16 + v) * 64 + lane] = o[tt][v];
-            s_stat[ksp][hw][lane] = m;
-            s_stat[ksp][hw][64 + lane] = l;
-        }
+                for (int v = 0; v < 16; ++v) slot(f, ksp)[v * 64] = o[f][v];
+            }
+        s_stat[ksp][hw][lane] = m;
+        s_stat[ksp][hw][64 + lane] = l;
         __syncthreads();
-        if (ksp > 0) return;
-        float mm = m;
+        float mj[KSPLIT], wj[KSPLIT], mm = -INFINITY;
 #pragma unroll
-        for (int j = 1; j < KSPLIT; ++j) mm = fmaxf(mm, s_stat[j][hw][lane]);
-        if (mm == -INFINITY) mm = 0.f;  // only NaN scores: their sums are kept (below)
-        // a share that saw no score has l = 0, or NaN from NaN scores: either way it joins with weight 1 or less
-        auto weight = [&](float mj) { return mj == -INFINITY ? 1.f : fast_exp2(mj - mm); };
-        const float c0 = weight(m);
-        l *= c0;
+        for (int j = 0; j < KSPLIT; ++j) mm = fmaxf(mm, mj[j] = s_stat[j][hw][lane]);
+        if (mm == -INFINITY) mm = 0.f;  // only NaN scores
+        l = 0.f;
 #pragma unroll
-        for (int tt = 0; tt < HD / 32; ++tt)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) o[tt][v] *= c0;
-#pragma unroll
-        for (int j = 1; j < KSPLIT; ++j) {
-            const float* xo = slot(j);
-            const float cj = weight(s_stat[j][hw][lane]);
-            l += s_stat[j][hw][64 + lane] * cj;
-#pragma unroll
-            for (int tt = 0; tt < HD / 32; ++tt)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) o[tt][v] += xo[(tt * 16 + v) * 64 + lane] * cj;
+        for (int j = 0; j < KSPLIT; ++j) {
+            // a share that saw no score has sums of 0, or of NaN from NaN scores, which are kept
+            wj[j] = mj[j] == -INFINITY ? 1.f : fast_exp2(mj[j] - mm);
+            l = fmaf(s_stat[j][hw][64 + lane], wj[j], l);
         }
+        const float own = m == -INFINITY ? 1.f : fast_exp2(m - mm);
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+            if (f % KSPLIT == ksp) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[f][v] *= own;
+#pragma unroll
+                for (int j = 0; j < KSPLIT; ++j)
+                    if (j != ksp) {
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) o[f][v] = fmaf(slot(f, j)[v * 64], wj[j], o[f][v]);
+                    }
+            }
     }
 
     if (my_s >= S) return;
@@ -355,7 +364,8 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     vsl_half* orow = out + (size_t)my_s * qw + (size_t)h * HD;
     // element v of O^T fragment t is dim 32 t + 8 (v / 4) + 4 (l / 32) + v % 4: runs of four dims, one store a plane
 #pragma unroll
-    for (int t = 0; t < HD / 32; ++t) {
+    for (int t = 0; t < NF; ++t) {
+        if (KSPLIT > 1 && t % KSPLIT != ksp) continue;
         const float f = nan_blocks >> t & 1 ? __builtin_nanf("") : inv;
 #pragma unroll
         for (int v0 = 0; v0 < 16; v0 += 4) {
@@ -403,11 +413,28 @@ void launch(hipStream_t s, const Args& a) {
         a.q, a.k, a.v, a.S, a.pos0, a.n_q, a.n_kv, a.cap, a.scale, a.out, a.om, a.win, a.n_glob, a.thr);
 }
 
-// Up to four heads share a block, two waves a head: groups of a power of two, or pairs or single heads of the others
-// (a block's threads divide a tile's words).
+// Enough blocks for every CU: up to four heads share a block and its expanded tiles, two waves a head (groups of a power
+// of two; pairs or single heads of the others: a block's threads divide a tile's words). Otherwise blocks of fewer
+// heads, four waves a head on tiles of 128 keys, as long as a CU holds every block: a chain of half or less the tiles, for
+// expanding them once a block. Split q, 8B shape (head_dim 128, 4 heads a group), blocks of 4 heads / 2 / 1: 45 rows
+// 10.7 / 11.0 / 9.3 us (one tile of 64 keys, 2 waves a head: 8.0), 128 rows 13.4 / 11.1 / 9.9, 400 rows 19.9 / 18.4 / 29.8,
+// 45 rows at 3000 77 / 60 / 52; 1B shape (64), one plane, 512 rows 13.0 / 10.8 / 13.2.
 template <int HD, int G, bool QX2>
 void launch_group(hipStream_t s, const Args& a) {
     constexpr int GB = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
+    constexpr uint64_t kCUs = 256;  // MI355X compute units
+    const uint64_t groups = (uint64_t)((a.S + 31) / 32) * a.n_kv;
+    if (groups * G <= kCUs) {
+        if (a.pos0 + a.S <= 64) launch<HD, G, 1, QX2, 2, 64>(s, a);
+        else launch<HD, G, 1, QX2, 4, 128>(s, a);
+        return;
+    }
+    if constexpr (GB == 4) {
+        if (groups * (G / 2) <= kCUs) {
+            launch<HD, G, 2, QX2, 4, 128>(s, a);
+            return;
+        }
+    }
     launch<HD, G, GB, QX2, 2, 64 * 128 / HD>(s, a);
 }
 
