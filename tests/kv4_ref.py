@@ -121,14 +121,20 @@ def attend(q, K, V, p0, scale, window=None):
     S, n_q, hd = q.shape
     n_kv, n = K.shape[:2]
     out = np.empty((S, n_q, hd))
+    ok = np.stack([seen(p0 + s, n, window) for s in range(S)])
+    whole = np.isfinite(K).all() and np.isfinite(V).all()
     with np.errstate(all="ignore"):
-        for s in range(S):
-            ok = seen(p0 + s, n, window)
-            for h in range(n_q):
-                k, v = K[h * n_kv // n_q][ok], V[h * n_kv // n_q][ok]
-                x = (k @ q[s, h]) * scale
+        for h in range(n_q):
+            k, v = K[h * n_kv // n_q], V[h * n_kv // n_q]
+            if whole:
+                x = np.where(ok, (q[:, h] @ k.T) * scale, -np.inf)
+                w = np.exp(x - x.max(1, keepdims=True))
+                out[:, h] = (w @ v) / w.sum(1, keepdims=True)
+                continue
+            for s in range(S):  # what is not seen takes no part, whatever it holds
+                x = (k[ok[s]] @ q[s, h]) * scale
                 w = np.exp(x - np.max(x))
-                out[s, h] = (w @ v) / w.sum()
+                out[s, h] = (w @ v[ok[s]]) / w.sum()
     return out
 
 

@@ -438,7 +438,11 @@ PROMPT = [  # hd, n_q, n_kv, S, pos0, cap
     (128, 32, 8, 45, 0, 4096), (64, 32, 8, 70, 0, 128), (128, 4, 1, 33, 95, 128), (64, 4, 4, 1, 0, 1), (128, 6, 2, 31, 1, 1000),
     (64, 8, 1, 100, 29, 300), (128, 8, 1, 64, 64, 128), (128, 5, 1, 32, 7, 40), (64, 7, 1, 40, 120, 260), (64, 3, 1, 3, 500, 503),
     (128, 2, 1, 129, 0, 129), (64, 2, 2, 65, 63, 200), (64, 6, 1, 20, 200, 400), (128, 1, 1, 5, 251, 256), (128, 7, 1, 9, 60, 100),
-    (64, 5, 1, 34, 94, 128), (128, 3, 1, 10, 310, 400), (64, 1, 1, 50, 300, 384)]
+    (64, 5, 1, 34, 94, 128), (128, 3, 1, 10, 310, 400), (64, 1, 1, 50, 300, 384),
+    # more heads times row blocks than CUs: blocks that share expanded tiles, two heads, four, and as the group divides
+    (128, 32, 8, 300, 21, 400), (64, 32, 8, 290, 0, 300), (128, 64, 8, 270, 130, 400), (64, 64, 8, 270, 3, 273),
+    (128, 40, 8, 225, 100, 330), (64, 36, 12, 230, 1, 256), (128, 48, 8, 200, 64, 264), (64, 32, 32, 257, 0, 257),
+    (128, 32, 16, 280, 40, 320), (64, 56, 8, 170, 200, 384), (128, 32, 32, 260, 3, 300)]
 
 
 @pytest.mark.parametrize("x2,odt", [(True, 2), (True, 1), (True, 3), (False, 1), (False, 2)])
@@ -457,7 +461,9 @@ def test_prompt(vsl, dev, H, shape, x2, odt):
 
 @pytest.mark.parametrize("hd,n_q,n_kv,S,pos0,cap,window", [
     (128, 4, 1, 100, 300, 512, (50, 16, 100)), (64, 4, 2, 70, 129, 256, (10, 3, 150)), (128, 2, 2, 40, 500, 640, (0, 0, 1)),
-    (64, 8, 1, 33, 400, 512, (200, 130, 64)), (128, 3, 1, 64, 0, 128, (8, 1, 30)), (64, 1, 1, 96, 190, 300, (33, 70, 200))])
+    (64, 8, 1, 33, 400, 512, (200, 130, 64)), (128, 3, 1, 64, 0, 128, (8, 1, 30)), (64, 1, 1, 96, 190, 300, (33, 70, 200)),
+    (128, 32, 8, 300, 200, 512, (150, 20, 260)), (64, 64, 8, 280, 111, 400, (70, 130, 120)), (128, 64, 8, 270, 0, 300, (40, 3, 100)),
+    (64, 40, 8, 240, 250, 500, (0, 65, 300))])
 def test_prompt_window(vsl, dev, H, hd, n_q, n_kv, S, pos0, cap, window):
     rng = np.random.default_rng(hd + S + pos0)
     n = pos0 + S
@@ -470,7 +476,7 @@ def test_prompt_window(vsl, dev, H, hd, n_q, n_kv, S, pos0, cap, window):
 
 
 @pytest.mark.parametrize("window", [None, (20, 4, 30)])
-@pytest.mark.parametrize("hd,n_q,n_kv", [(128, 4, 1), (64, 3, 1), (64, 8, 1)])
+@pytest.mark.parametrize("hd,n_q,n_kv", [(128, 4, 1), (64, 3, 1), (64, 8, 1), (128, 96, 24), (64, 176, 22), (128, 180, 36)])
 def test_prompt_nan_rows(vsl, dev, H, hd, n_q, n_kv, window):
     """NaN keys and values reach exactly the rows (and, for values, the 32 columns) that see them."""
     rng = np.random.default_rng(hd + n_q)
@@ -487,9 +493,10 @@ def test_prompt_nan_rows(vsl, dev, H, hd, n_q, n_kv, window):
         want = np.zeros((S, n_q, hd), bool)
         for s in range(S):
             see = kv4_ref.seen(pos0 + s, n, window)
-            want[s] |= bool(see[bad_k].any())
+            G = n_q // n_kv  # the heads that read KV head 0
+            want[s, :G] |= bool(see[bad_k].any())
             for p, b in bad_v:
-                want[s, :, 32 * b:32 * b + 32] |= bool(see[p])
+                want[s, :G, 32 * b:32 * b + 32] |= bool(see[p])
         assert np.array_equal(np.isnan(got), want)
         ref = kv4_ref.attend(used, np.nan_to_num(Kv), np.nan_to_num(Vv), pos0, 0.1, window)
         tol = attn_tol(used, np.nan_to_num(Kv), np.nan_to_num(Vv), 0.1) + out_tol(ref, 2)

@@ -393,6 +393,267 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     }
 }
 
+// The same for few rows, where a block for a head and 32 rows leaves CUs idle and no tile is shared: block (row block,
+// head) of WAVES waves that go through the keys by themselves, wave w the tiles of 32 keys w, w + WAVES, ..., straight from
+// the cache into registers (two tiles in flight, no barrier before the join). As above but for the orders of dims, which
+// follow the cache's words so that a lane reads its codes by 16 bytes: lane group g = l / 32 takes the dims HD/2 g + 8 c ..
+// of the scores' step c, and row r of the product's fragment f is dim NF r + f. Join: every wave leaves its sums in LDS,
+// and takes two of their 16 registers from all of them.
+template <int HD, bool QX2, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void k_attn_prefill_kv4_few(
+    const vsl_half* __restrict__ q, const char* __restrict__ kc, const char* __restrict__ vc, uint32_t S, uint32_t pos0,
+    uint32_t n_q, uint32_t n_kv, uint32_t cap, float scale, vsl_half* __restrict__ out, int om, uint32_t win,
+    uint32_t n_glob, uint32_t thr) {
+    constexpr int NB = HD / 32, NF = HD / 32, NS = HD / 16, QP = QX2 ? 2 : 1, VPW = 16 / WAVES;
+    constexpr uint32_t TK = 32;
+    typedef float fragv __attribute__((ext_vector_type(NF)));
+    __shared__ __attribute__((aligned(16))) fragv s_o[WAVES][16][64];
+    __shared__ float s_stat[WAVES][2][64];
+    __shared__ uint32_t s_nan;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
+    const uint32_t h = blockIdx.y, kvh = h / (n_q / n_kv);
+    const uint32_t s_base = blockIdx.x * 32, my_s = s_base + (lane & 31), qw = n_q * HD;
+    const size_t qplane = (size_t)S * qw;
+    const float sl2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);  // see above
+    const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;
+    const uint32_t last_s = min(S, s_base + 32) - 1;
+    const uint32_t p_first = pos0 + s_base, p_last = pos0 + last_s, my_pos = pos0 + my_s, kv_end = p_last + 1;
+    const uint32_t n_tiles = (kv_end + TK - 1) / TK;
+    uint32_t n_gt = n_tiles, t_lo = n_tiles;
+    if (p_first + 1 > thr && p_first > win) {
+        t_lo = (p_first - win) / TK;
+        n_gt = min((n_glob + TK - 1) / TK, t_lo);
+    }
+    const uint32_t n_vt = n_gt + (n_tiles - t_lo);
+    auto phys = [&](uint32_t vt) { return vt < n_gt ? vt : vt - n_gt + t_lo; };
+    const uint32_t my_lo = (my_pos + 1 > thr && my_pos > win) ? my_pos - win : 0;
+    const uint32_t lo_max = (p_last + 1 > thr && p_last > win) ? p_last - win : 0;
+
+    const uint64_t P = kv4_positions(cap), soff = kv4_steps_off(n_kv, cap, HD);
+    const Kv4Consts kc4 = kv4_consts();
+    const uint32_t krow = (lane & 19) | (lane & 4) << 1 | (lane & 8) >> 1;  // bits 2 and 3 of l % 32 exchanged
+    const char* Kc = kc + ((uint64_t)kvh * P + krow) * (HD / 2) + g * (HD / 4);
+    const char* Kst = kc + soff + (((uint64_t)kvh * P + krow) * NB + g * NB / 2) * 2;
+    const char* Vc = vc + (((uint64_t)kvh * (P / 8) + g) * HD + NF * (lane & 31)) * 4;
+    const char* Vst0 = vc + soff + (uint64_t)kvh * P * NB * 2;
+    const char* Vst = Vst0 + ((uint64_t)g * NB + NF * (lane & 31) / 32) * 16;
+
+    struct Tile {
+        uint32_t k[NS], ks, v[2][NF];
+        u32x4 vs[2];
+    };
+    auto issue = [&](Tile& b, uint32_t t) {
+        const uint64_t p0 = (uint64_t)t * TK;
+        const u32x4* kp = reinterpret_cast<const u32x4*>(Kc + p0 * (HD / 2));
+#pragma unroll
+        for (int i = 0; i < NS / 4; ++i) {
+            const u32x4 w = kp[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b.k[4 * i + j] = w[j];
+        }
+        if constexpr (NB == 4) b.ks = *reinterpret_cast<const uint32_t*>(Kst + p0 * NB * 2);
+        else b.ks = *reinterpret_cast<const uint16_t*>(Kst + p0 * NB * 2);
+#pragma unroll
+        for (int hi = 0; hi < 2; ++hi) {
+            const uint64_t oct = p0 / 8 + 2 * hi;
+            if constexpr (NF == 4) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(Vc + oct * HD * 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) b.v[hi][j] = w[j];
+            } else {
+                const uint2 w = *reinterpret_cast<const uint2*>(Vc + oct * HD * 4);
+                b.v[hi][0] = w.x;
+                b.v[hi][1] = w.y;
+            }
+            b.vs[hi] = *reinterpret_cast<const u32x4*>(Vst + oct * NB * 16);
+        }
+    };
+
+    half8 qf[QP][NS];
+#pragma unroll
+    for (int p = 0; p < QP; ++p)
+#pragma unroll
+        for (int c = 0; c < NS; ++c) {
+            const uint32_t row = my_s < S ? my_s : S - 1;  // rows past S are never stored
+            const u32x4 x = *reinterpret_cast<const u32x4*>(q + p * qplane + (size_t)row * qw + (size_t)h * HD + g * (HD / 2) + 8 * c);
+            qf[p][c] = __builtin_bit_cast(half8, x ^ flip);
+        }
+    float16v o[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[f][v] = 0.f;
+    float m = -INFINITY, l = 0.f, minus_one = -1.f;
+    asm volatile("" : "+v"(minus_one));
+    constexpr float kLazy = 8.f;
+    if (threadIdx.x == 0) s_nan = 0;
+    __syncthreads();
+
+    auto consume = [&](Tile& b, uint32_t vt) {
+        const uint32_t p0 = phys(vt) * TK;
+        float16v st;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) st[v] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NS; ++c) {
+            // a lane group's dims: one or two blocks
+            const uint32_t x = c < 4 ? b.ks & 0xFFFFu : b.ks >> 16;
+            const half8 kf = kv4_word(b.k[c], kv4_step(x | x << 16, kc4), kc4);
+#pragma unroll
+            for (int p = 0; p < QP; ++p) st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[p][c], st, 0, 0, 0);
+        }
+        if (!(p0 + TK - 1 <= p_first && (p0 >= lo_max || p0 + TK <= n_glob))) {  // some row sees the tile in part
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const uint32_t key = p0 + (v >> 3) * 16 + g * 8 + (v & 7);
+                st[v] = key <= my_pos && (key >= my_lo || key < n_glob) ? st[v] : -INFINITY;
+            }
+#pragma unroll
+            for (int hi = 0; hi < 2; ++hi)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t x = b.vs[hi][e / 2] >> (16 * (e & 1)) & 0xFFFFu;
+                    if ((x & 0x7C00u) != 0x7C00u) continue;
+                    b.vs[hi][e / 2] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                    if (p0 + 16 * hi + 8 * g + e < kv_end) s_nan = 1;
+                }
+        }
+        float bm = st[0];
+#pragma unroll
+        for (int v = 1; v < 16; ++v) bm = fmaxf(bm, st[v]);
+        float ba, bb;
+        lane_pair<32>(bm, ba, bb);
+        bm = fmaxf(ba, bb) * sl2;
+        const bool raise = bm > m + kLazy;  // m = -inf: any finite tile maximum raises it
+        if (__builtin_amdgcn_ballot_w64(raise)) {
+            const float mn = raise ? bm : m;
+            const float corr = mn == -INFINITY ? 1.f : fast_exp2(m - mn);  // m = -inf: 0
+            l *= corr;
+            m = mn;
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[f][v] *= corr;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        half8 pf[QP][2];
+#pragma unroll
+        for (int v = 0; v < 16; v += 2) {
+            const float p_0 = fast_exp2(fmaf(st[v], sl2, -ref)), p_1 = fast_exp2(fmaf(st[v + 1], sl2, -ref));
+            l += p_0;
+            l += p_1;
+            const half2v hi = pack_f16(p_0, p_1);
+            pf[0][v >> 3][v & 7] = hi[0];
+            pf[0][v >> 3][(v & 7) + 1] = hi[1];
+            if constexpr (QX2) {
+                const half2v lo = pack_f16(fmaf((float)hi[0], minus_one, p_0), fmaf((float)hi[1], minus_one, p_1));
+                pf[QP - 1][v >> 3][v & 7] = lo[0];
+                pf[QP - 1][v >> 3][(v & 7) + 1] = lo[1];
+            }
+        }
+#pragma unroll
+        for (int hi = 0; hi < 2; ++hi) {
+            Kv4Step vs[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) vs[p] = kv4_step(b.vs[hi][p], kc4);
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                const half8 vf = kv4_word(b.v[hi][f], vs, kc4);
+#pragma unroll
+                for (int p = 0; p < QP; ++p) o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[p][hi], o[f], 0, 0, 0);
+            }
+        }
+    };
+    Tile ta, tb;
+    uint32_t vt = wave;
+    if (vt < n_vt) issue(ta, phys(vt));
+    if (vt + WAVES < n_vt) issue(tb, phys(vt + WAVES));
+    while (vt < n_vt) {
+        consume(ta, vt);
+        vt += WAVES;
+        if (vt >= n_vt) break;
+        issue(ta, phys(vt + WAVES < n_vt ? vt + WAVES : vt));  // past the wave's last tile the one just read
+        __builtin_amdgcn_sched_barrier(0);
+        consume(tb, vt);
+        vt += WAVES;
+        if (vt >= n_vt) break;
+        issue(tb, phys(vt + WAVES < n_vt ? vt + WAVES : vt));
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    float l0, l1;
+    lane_pair<32>(l, l0, l1);
+    l = l0 + l1;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+        fragv x;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) x[f] = o[f][v];
+        s_o[wave][v][lane] = x;
+    }
+    s_stat[wave][0][lane] = m;
+    s_stat[wave][1][lane] = l;
+    __syncthreads();
+    if (my_s >= S) return;
+    float w[WAVES], mm = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < WAVES; ++j) mm = fmaxf(mm, w[j] = s_stat[j][0][lane]);
+    if (mm == -INFINITY) mm = 0.f;  // only NaN scores
+    l = 0.f;
+#pragma unroll
+    for (int j = 0; j < WAVES; ++j) {
+        // a wave that saw no score has sums of 0, or of NaN from NaN scores, which are kept
+        w[j] = w[j] == -INFINITY ? 1.f : fast_exp2(w[j] - mm);
+        l = fmaf(s_stat[j][1][lane], w[j], l);
+    }
+    uint32_t nan_blocks = 0;  // 32-dim blocks of V in which this row sees a NaN
+    if (s_nan) {
+        const uint16_t* vs = reinterpret_cast<const uint16_t*>(Vst0);
+        for (uint32_t key = 0; key <= my_pos; ++key) {
+            if (key < my_lo && key >= n_glob) continue;
+            for (int bl = 0; bl < NB; ++bl)
+                if (vs[((size_t)(key / 8) * NB + bl) * 8 + key % 8] == kKv4NaN) nan_blocks |= 1u << bl;
+        }
+    }
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int i = 0; i < VPW; ++i) {
+        const int v = VPW * wave + i;
+        fragv x;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) x[f] = 0.f;
+#pragma unroll
+        for (int j = 0; j < WAVES; ++j) {
+            const fragv y = s_o[j][v][lane];
+#pragma unroll
+            for (int f = 0; f < NF; ++f) x[f] = fmaf(y[f], w[j], x[f]);
+        }
+        const uint32_t dim = NF * ((v >> 2) * 8 + g * 4 + (v & 3));  // dims dim .. dim + NF - 1
+        x *= nan_blocks >> (dim / 32) & 1 ? __builtin_nanf("") : inv;
+        const size_t at = (size_t)my_s * qw + (size_t)h * HD + dim;
+        typedef vsl_half halfn __attribute__((ext_vector_type(NF)));
+        halfn hv, lv;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            vsl_half hi, lo;
+            split_f16(x[f], hi, lo);
+            hv[f] = hi;
+            lv[f] = lo;
+        }
+        *reinterpret_cast<halfn*>(out + at) = hv;
+        if (om == 1) *reinterpret_cast<halfn*>(out + qplane + at) = lv;
+        if (om == 2) {
+            uint8_t* lo8 = reinterpret_cast<uint8_t*>(out + qplane) + (size_t)my_s * qw + lo8_pos(h * HD + dim);
+            if constexpr (NF == 4) {
+                *reinterpret_cast<uint32_t*>(lo8) = lo8_code4(x[0] - (float)hv[0], x[1] - (float)hv[1], x[2] - (float)hv[2],
+                                                              x[3] - (float)hv[3]);
+            } else {
+                *reinterpret_cast<uint16_t*>(lo8) =
+                    (uint16_t)lo8_code4(x[0] - (float)hv[0], x[1] - (float)hv[1], 0.f, 0.f);
+            }
+        }
+    }
+}
+
 bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 struct Args {
@@ -425,8 +686,14 @@ void launch_group(hipStream_t s, const Args& a) {
     constexpr uint64_t kCUs = 256;  // MI355X compute units
     const uint64_t groups = (uint64_t)((a.S + 31) / 32) * a.n_kv;
     if (groups * G <= kCUs) {
+#ifdef KOLD
         if (a.pos0 + a.S <= 64) launch<HD, G, 1, QX2, 2, 64>(s, a);
         else launch<HD, G, 1, QX2, 4, 128>(s, a);
+#else
+        constexpr int W = 8;
+        k_attn_prefill_kv4_few<HD, QX2, W><<<dim3((a.S + 31) / 32, a.n_q), W * 64, 0, s>>>(
+            a.q, a.k, a.v, a.S, a.pos0, a.n_q, a.n_kv, a.cap, a.scale, a.out, a.om, a.win, a.n_glob, a.thr);
+#endif
         return;
     }
     if constexpr (GB == 4) {
