@@ -247,7 +247,8 @@ int vsl_qkv_rope_append(const float* x, const float* gamma, float eps, const voi
  * fp16 caches of head_dim 128 with more than 8192 positions of capacity run the scores on the
  * matrix cores (the same results to fp32 rounding; faster from about 2K attended positions).
  * kv_dtype VSL_DT_F32, VSL_DT_F16 or VSL_DT_KV4 (both products on the matrix cores, q and the
- * probabilities as hi / lo fp16 pairs, so |q * scale * log2(e)| < 65504; also below, _noalloc and _window). */
+ * probabilities as hi / lo fp16 pairs, so |q * scale * log2(e)| < 65504; q and part_o 16-byte, part_ml 8-byte aligned; also
+ * below, _noalloc and _window). */
 int vsl_attn_decode(const float* q, const void* kcache, const void* vcache, int kv_dtype, uint32_t n_q,
                     uint32_t n_kv, uint32_t hd, uint32_t cap, float scale, uint32_t nsplit, float* part_o,
                     float* part_ml, float* out, vsl_ctrl* ctrl, void* stream);

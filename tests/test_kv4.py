@@ -104,6 +104,8 @@ def test_attention_refusals(vsl, H):
     assert decode(nsplit=0) == -100
     assert decode(nq=18) == -103
     assert decode(hd=32) == -103
+    for q, po, ml in [(ptr(off=8), ptr(), ptr()), (ptr(), ptr(off=8), ptr()), (ptr(), ptr(), ptr(off=4))]:
+        assert H.vsl_attn_decode(q, ptr(), ptr(), vsl.VSL_DT_KV4, 8, 2, 128, 64, 0.1, 4, po, ml, ptr(), ptr(), None) == -100
     # the fused projection writes fp16 and fp32 caches only
     assert H.vsl_qkv_rope_append(ptr(), ptr(), 1e-5, ptr(), 1, 256, 4, 4, 64, ptr(), ptr(), ptr(), ptr(), vsl.VSL_DT_KV4, 64,
                                  ptr(), ptr(), None) == -103

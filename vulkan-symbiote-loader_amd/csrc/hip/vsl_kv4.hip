@@ -462,6 +462,9 @@ __device__ __forceinline__ float add_lane8(float v) {
 // Softmax with a reference maximum m per head that is raised, for the whole wave, only when some score exceeds it by
 // more than kLazy (probabilities stay below 2^kLazy). Masked positions get probability 0 and their V steps are set to
 // 0, so what the cache holds past the length never reaches a sum. Output as k_attn_decode's.
+// Bound by latency at short lengths (8B shape, 32 splits, 778 positions 4.9 us: loads 1.0, one tile's chain 1.1, the waves'
+// join and the partials 0.9, the launch), and by the expansion's vector instructions at long ones: 32001 positions 11.9 us,
+// of which the loads alone, by the same pattern, take 8.6 (37 MB, 4.3 TB/s), against 22.4 for the fp16 cache's kernel.
 template <int HD, int G, bool WIN, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_decode_kv4(const float* __restrict__ q, const char* __restrict__ kcache,
                                                                 const char* __restrict__ vcache, uint32_t n_kv, uint32_t cap,
@@ -849,6 +852,8 @@ int vsl_kv4_attn_partials(const float* q, const void* kcache, const void* vcache
                           uint32_t win, uint32_t n_glob, uint32_t thr, void* stream) {
     if (const int rc = check_kv4("vsl_attn_decode", kcache, vcache, hd)) return rc;
     if (cap == 0) return vsl_invalid("vsl_attn_decode: capacity 0");
+    if (!aligned_to(q, 16) || !aligned_to(part_o, 16) || !aligned_to(part_ml, 8))
+        return vsl_invalid("vsl_attn_decode: a 4-bit cache needs q and part_o 16-byte, part_ml 8-byte aligned");
     const dim3 grid(nsplit, n_kv);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const char* kc = static_cast<const char*>(kcache);

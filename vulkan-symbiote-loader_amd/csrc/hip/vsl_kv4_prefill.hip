@@ -29,7 +29,10 @@ __device__ __forceinline__ int sw(int r, int c) {
 // v_mfma_f32_32x32x16_f16, the online softmax of its 32 rows (a lane owns a row with lane ^ 32), and O^T += V^T P^T.
 // MFMA row r of a 32-key fragment is the key with bits 2 and 3 of r exchanged, so that the scores a lane holds are
 // octets of consecutive keys: the probabilities are the B operand as they are, and V^T's operand one 16-byte LDS read.
-// The next tile's codes are in flight while a tile is computed.
+// The next tiles' codes are in flight while a tile is computed.
+// Bound by the matrix cores at large sizes: 2048 rows at 6144 of the 8B shape with a split q (two products a plane: 0.48
+// TFLOP) 470 us, 1.02 PFLOP/s, against 1.25 of a large fp16 library product on the same card; the expansion costs 80 of
+// the 470 us (412 us without it in the loop), the exponentials 20.
 template <int HD, int G, int GB, bool QX2, int KSPLIT, int TK>
 __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     const vsl_half* __restrict__ q, const char* __restrict__ kc, const char* __restrict__ vc, uint32_t S, uint32_t pos0,
@@ -674,26 +677,22 @@ void launch(hipStream_t s, const Args& a) {
         a.q, a.k, a.v, a.S, a.pos0, a.n_q, a.n_kv, a.cap, a.scale, a.out, a.om, a.win, a.n_glob, a.thr);
 }
 
-// Enough blocks for every CU: up to four heads share a block and its expanded tiles, two waves a head (groups of a power
-// of two; pairs or single heads of the others: a block's threads divide a tile's words). Otherwise blocks of fewer
-// heads, four waves a head on tiles of 128 keys, as long as a CU holds every block: a chain of half or less the tiles, for
-// expanding them once a block. Split q, 8B shape (head_dim 128, 4 heads a group), blocks of 4 heads / 2 / 1: 45 rows
-// 10.7 / 11.0 / 9.3 us (one tile of 64 keys, 2 waves a head: 8.0), 128 rows 13.4 / 11.1 / 9.9, 400 rows 19.9 / 18.4 / 29.8,
-// 45 rows at 3000 77 / 60 / 52; 1B shape (64), one plane, 512 rows 13.0 / 10.8 / 13.2.
+// As long as a CU holds every block of one head and 32 rows, those (k_attn_prefill_kv4_few). Past that up to four heads
+// share a block and its expanded tiles, two waves a head (groups of a power of two; pairs or single heads of the others: a
+// block's threads divide a tile's words), or, while that leaves CUs idle, two heads with four waves each on tiles of 128 keys:
+// twice the blocks, half the tiles in a chain. Measured, split q unless said: blocks of several heads / of one, 8B shape
+// (head_dim 128, 4 heads a group) 128 rows 9.8 / 9.1 us, 45 rows at 3000 51.5 / 30.4, 250 rows at 500 23.2 / 15.2, 300 rows at
+// 1000 36.8 / 34.6, 400 rows 18.2 / 20.6, one plane 700 rows 23.0 / 29.2, 1B shape (64), one plane, 512 rows 10.8 / 13.3; four
+// heads a block / two: 1B shape, one plane, 512 rows 12.7 / 10.8.
 template <int HD, int G, bool QX2>
 void launch_group(hipStream_t s, const Args& a) {
     constexpr int GB = G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;
     constexpr uint64_t kCUs = 256;  // MI355X compute units
     const uint64_t groups = (uint64_t)((a.S + 31) / 32) * a.n_kv;
     if (groups * G <= kCUs) {
-#ifdef KOLD
-        if (a.pos0 + a.S <= 64) launch<HD, G, 1, QX2, 2, 64>(s, a);
-        else launch<HD, G, 1, QX2, 4, 128>(s, a);
-#else
         constexpr int W = 8;
         k_attn_prefill_kv4_few<HD, QX2, W><<<dim3((a.S + 31) / 32, a.n_q), W * 64, 0, s>>>(
             a.q, a.k, a.v, a.S, a.pos0, a.n_q, a.n_kv, a.cap, a.scale, a.out, a.om, a.win, a.n_glob, a.thr);
-#endif
         return;
     }
     if constexpr (GB == 4) {
