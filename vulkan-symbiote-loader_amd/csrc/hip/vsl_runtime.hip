@@ -364,7 +364,8 @@ struct vsl_graph {
     int device = -1;                          // the direct kernels' device
 };
 
-// The kernels of a graph that is one chain of at most kDirectNodes kernel nodes, in order; else empty.
+// The kernels of a graph that is one chain of at most kDirectNodes kernel nodes, in order; else empty. Only kernels that
+// hipLaunchKernel can launch as the capture did: known by a host symbol (not a module's function), not cooperative.
 static std::vector<hipKernelNodeParams> kernel_chain(hipGraph_t graph) {
     size_t n = 0, n_edges = 0;
     if (hipGraphGetNodes(graph, nullptr, &n) != hipSuccess || n == 0 || n > kDirectNodes) return {};
@@ -384,6 +385,11 @@ static std::vector<hipKernelNodeParams> kernel_chain(hipGraph_t graph) {
         hipKernelNodeParams p{};
         if (hipGraphNodeGetType(at, &type) != hipSuccess || type != hipGraphNodeTypeKernel) return {};
         if (hipGraphKernelNodeGetParams(at, &p) != hipSuccess || !p.func || !p.kernelParams || p.extra) return {};
+        hipFuncAttributes fa;
+        hipKernelNodeAttrValue coop{};
+        if (hipFuncGetAttributes(&fa, p.func) != hipSuccess) return {};
+        if (hipGraphKernelNodeGetAttribute(at, hipKernelNodeAttributeCooperative, &coop) != hipSuccess || coop.cooperative)
+            return {};
         chain.push_back(p);
         hipGraphNode_t next = nullptr;
         for (size_t e = 0; e < n_edges; ++e) {
@@ -418,6 +424,7 @@ extern "C" int vsl_graph_end(void* stream, vsl_graph** out) {
     }
     g->direct = kernel_chain(g->graph);
     if (hipGetDevice(&g->device) != hipSuccess) g->direct.clear();
+    if (g->direct.empty()) (void)hipGetLastError();  // what a query above reported of a node that it does not cover
     *out = g;
     return VSL_OK;
 }
