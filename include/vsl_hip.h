@@ -246,9 +246,9 @@ int vsl_qkv_rope_append(const float* x, const float* gamma, float eps, const voi
  * then a combine launch.  Workspace: part_o [n_q][nsplit][hd] f32, part_ml [n_q][nsplit][2] f32.
  * fp16 caches of head_dim 128 with more than 8192 positions of capacity run the scores on the
  * matrix cores (the same results to fp32 rounding; faster from about 2K attended positions).
- * kv_dtype VSL_DT_F32, VSL_DT_F16 or VSL_DT_KV4 (both products on the matrix cores, q and the
- * probabilities as hi / lo fp16 pairs, so |q * scale * log2(e)| < 65504; q and part_o 16-byte, part_ml 8-byte aligned; also
- * below, _noalloc and _window). */
+ * kv_dtype VSL_DT_F32, VSL_DT_F16 or VSL_DT_KV4 (here, in _noalloc and in _window).  With VSL_DT_KV4 both
+ * products run on the matrix cores, q and the probabilities as hi / lo fp16 pairs: |q * scale * log2(e)| <
+ * 65504; q and part_o 16-byte, part_ml 8-byte aligned. */
 int vsl_attn_decode(const float* q, const void* kcache, const void* vcache, int kv_dtype, uint32_t n_q,
                     uint32_t n_kv, uint32_t hd, uint32_t cap, float scale, uint32_t nsplit, float* part_o,
                     float* part_ml, float* out, vsl_ctrl* ctrl, void* stream);
@@ -302,7 +302,7 @@ enum { VSL_DT_KV4 = 7 };
 uint64_t vsl_kv_cache_bytes(int kv_dtype, uint32_t n_kv, uint32_t cap, uint32_t hd);
 /* Positions pos0 .. pos0 + n - 1 of VSL_DT_KV4 caches as the values they stand for: k_out, v_out
  * [n_kv][n][hd] fp16 or fp32 (16-byte aligned; exact in either).  A cache and its output may both be
- * NULL. */
+ * NULL.  Up to 1.9e9 / (n_kv * hd / 8) positions a call. */
 int vsl_kv4_read(const void* kcache, const void* vcache, uint32_t n_kv, uint32_t cap, uint32_t hd, uint32_t pos0,
                  uint32_t n, void* k_out, void* v_out, int out_dtype, void* stream);
 
@@ -322,8 +322,9 @@ int vsl_norm_gemv(const float* x, const float* gamma, float eps, const void* W, 
  *   q -> q_out [S][n_q][hd] (VSL_DT_F32, VSL_DT_F16 or VSL_DT_F16X2), k and v -> the caches (VSL_DT_F32,
  *   VSL_DT_F16 or VSL_DT_KV4).
  * Keys for a VSL_DT_KV4 cache are computed in 64 bits, so that a code is that of the exact value whatever the
- * number of rows in the call; the rest in 32 bits, each output rounded once more if it has fewer. head_dim 64 or 128; every pointer 16-byte aligned (VSL_DT_KV4 caches 256);
- * positions past cap return VSL_E_CAPACITY before anything is launched. */
+ * number of rows in the call; the rest in 32 bits, each output rounded once more if it has fewer.  head_dim 64
+ * or 128; every pointer 16-byte aligned (VSL_DT_KV4 caches 256); at most 2^33 values of qkv in a call; positions
+ * past cap return VSL_E_CAPACITY before anything is launched.  Inputs and outputs do not overlap. */
 enum { VSL_ROPE_PAIRS = 0, VSL_ROPE_HALVES = 1 };
 int vsl_qk_norm_rope_append(const float* qkv, uint32_t S, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t pos0,
                             const float* q_gamma, const float* k_gamma, float eps, int rope, const float* rope_cos,
@@ -468,7 +469,7 @@ int vsl_attn_prefill_window(const void* q, int q_dtype, const void* kcache, cons
                             void* stream);
 
 /* vsl_attn_prefill over VSL_DT_KV4 caches (the rows' own keys and values appended before), and with the
- * windowed mode.  Other arguments as there. */
+ * windowed mode.  Other arguments as there; GQA ratio 1..8, q and out 16-byte aligned. */
 int vsl_attn_prefill_kv4(const void* q, int q_dtype, const void* kcache, const void* vcache, uint32_t S, uint32_t pos0,
                          uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t cap, float scale, void* out, int out_dtype,
                          void* stream);

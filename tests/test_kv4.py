@@ -64,6 +64,9 @@ def test_append_refusals_of_one_entry(vsl, H):
     assert _append(vsl, H, S=65) == -104
     assert _append(vsl, H, S=0) == 0
     assert _append_decode(vsl, H, ctrl=None) == -100
+    # more values than a launch has lanes for
+    assert _append(vsl, H, S=1 << 26, nq=32, nkv=8, hd=128, cap=1 << 27) == -103
+    assert _append(vsl, H, S=0xFFFFFFFF, nq=1, nkv=1, hd=128, cap=0xFFFFFFFF) == -103
 
 
 def test_read_refusals(vsl, H):
@@ -76,6 +79,7 @@ def test_read_refusals(vsl, H):
         assert read(**kw) == -100, kw
     assert read(hd=32) == -103
     assert read(dt=2) == -103
+    assert read(nkv=8, hd=128, n=1 << 27, cap=1 << 28) == -103
     assert read(pos0=62) == -104
     assert read(pos0=0xFFFFFFFF, n=2) == -104
 

@@ -781,7 +781,7 @@ extern "C" int vsl_qk_norm_rope_append(const float* qkv, uint32_t S, uint32_t n_
     if (S == 0) return VSL_OK;
     const AppendArgs a{qkv, S, n_q, n_kv, pos0, cap, RopeArgs{q_gamma, k_gamma, rope_cos, rope_sin, eps, rope},
                        q_out, kcache, vcache};
-    if ((uint64_t)S * (n_q + 2 * n_kv) * hd >= 1ull << 37) return vsl_unsupported("%s: %u rows in one call", fn, S);
+    if ((uint64_t)S * (n_q + 2 * n_kv) * hd > 1ull << 33) return vsl_unsupported("%s: %u rows in one call", fn, S);  // 2^31 lanes
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto go = [&](auto hdc) {
         constexpr int HD = decltype(hdc)::value;
@@ -826,13 +826,13 @@ extern "C" int vsl_kv4_read(const void* kcache, const void* vcache, uint32_t n_k
     if (n == 0) return VSL_OK;
     const uint64_t n_oct = (pos0 + n - 1) / 8 - pos0 / 8 + 1;
     const uint64_t items = (uint64_t)n_kv * (hd / 8) * ((kcache ? n : 0) + (vcache ? n_oct : 0));
-    const uint64_t blocks = (items + 255) / 256;
-    if (blocks > 0x7FFFFFFFull) return vsl_invalid("%s: %u positions in one call", fn, n);
+    if (items > 1ull << 31) return vsl_unsupported("%s: %u positions in one call", fn, n);
+    const uint32_t blocks = (uint32_t)((items + 255) / 256);
     const char* kc = static_cast<const char*>(kcache);
     const char* vc = static_cast<const char*>(vcache);
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto go = [&](auto kernel, auto* ko, auto* vo) {
-        kernel<<<(uint32_t)blocks, 256, 0, s>>>(kc, vc, n_kv, cap, pos0, n, ko, vo);
+        kernel<<<blocks, 256, 0, s>>>(kc, vc, n_kv, cap, pos0, n, ko, vo);
     };
     if (out_dtype == VSL_DT_F16) {
         vsl_half *ko = static_cast<vsl_half*>(k_out), *vo = static_cast<vsl_half*>(v_out);
