@@ -98,6 +98,7 @@ def test_attention_refusals(vsl, H):
     for kw in (dict(hd=96), dict(nq=18), dict(qdt=0), dict(odt=0), dict(qdt=3)):
         assert prefill(**kw) == -103, kw
     assert prefill(pos0=61) == -104
+    assert prefill(S=1 << 24, cap=1 << 25) == -103
 
     def decode(kc=ptr(), vc=ptr(), nq=8, nkv=2, hd=128, cap=64, nsplit=4, dt=vsl.VSL_DT_KV4):
         return H.vsl_attn_decode(ptr(), kc, vc, dt, nq, nkv, hd, cap, 0.1, nsplit, ptr(), ptr(), ptr(), ptr(), None)

@@ -30,9 +30,11 @@ __device__ __forceinline__ int sw(int r, int c) {
 // MFMA row r of a 32-key fragment is the key with bits 2 and 3 of r exchanged, so that the scores a lane holds are
 // octets of consecutive keys: the probabilities are the B operand as they are, and V^T's operand one 16-byte LDS read.
 // The next tiles' codes are in flight while a tile is computed.
-// Bound by the matrix cores at large sizes: 2048 rows at 6144 of the 8B shape with a split q (two products a plane: 0.48
-// TFLOP) 470 us, 1.02 PFLOP/s, against 1.25 of a large fp16 library product on the same card; the expansion costs 80 of
-// the 470 us (412 us without it in the loop), the exponentials 20.
+// Bound by power at large sizes, 2048 rows at 6144 of the 8B shape with a split q (0.48 TFLOP on the matrix cores): 427 us,
+// 1.13 PFLOP/s, against 1.25 of a large fp16 library product on the same card. The clock is at 1.9 GHz then; with the two waves
+// of a SIMD in opposite phases (one in its products, one in its probabilities and expansion, a barrier each) it falls to 1.75
+// and the time stays (425 us; smaller calls lose 5-25 %). Before the order of blocks was what it is, 470 us fell to 412
+// without the expansion in the loop and to 398 without the exponentials too.
 template <int HD, int G, int GB, bool QX2, int KSPLIT, int TK>
 __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     const vsl_half* __restrict__ q, const char* __restrict__ kc, const char* __restrict__ vc, uint32_t S, uint32_t pos0,
@@ -50,10 +52,13 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     __shared__ float s_stat[KSPLIT][GB][128];  // row statistics of the key shares, for their join
     __shared__ uint32_t s_nan;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t qb = gridDim.x - 1 - blockIdx.x;  // the longest (latest) query blocks start first
-    const uint32_t kvh = blockIdx.y / (G / GB);
+    // the longest (latest) query blocks of every head start first; neighbouring blocks, which go to different XCDs, take
+    // different KV heads (with 8 of them each XCD's L2 holds one). Head by head instead, the last head's longest blocks start
+    // in the second round: 2048 rows at 6144 458 us instead of 427, 1B shape 1500 rows at 500 55 instead of 44.
+    const uint32_t hb = n_q / GB, qb = gridDim.x / hb - 1 - blockIdx.x / hb;
+    const uint32_t kvh = blockIdx.x % hb % n_kv;
     const int ksp = wave / GB, kbase = ksp * NKB;
-    const uint32_t h = kvh * G + (blockIdx.y % (G / GB)) * GB + wave % GB;
+    const uint32_t h = kvh * G + (blockIdx.x % hb / n_kv) * GB + wave % GB;
     const uint32_t s_base = qb * 32, my_s = s_base + (lane & 31), qw = n_q * HD;
     const size_t qplane = (size_t)S * qw;
     // scores are scaled within the exponential's argument, which the maximum then needs a positive factor for: a
@@ -414,8 +419,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_prefill_kv4_few(
     __shared__ float s_stat[WAVES][2][64];
     __shared__ uint32_t s_nan;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
-    const uint32_t h = blockIdx.y, kvh = h / (n_q / n_kv);
-    const uint32_t s_base = blockIdx.x * 32, my_s = s_base + (lane & 31), qw = n_q * HD;
+    const uint32_t kvh = blockIdx.x % n_q % n_kv, h = kvh * (n_q / n_kv) + blockIdx.x % n_q / n_kv;  // order: see above
+    const uint32_t s_base = blockIdx.x / n_q * 32, my_s = s_base + (lane & 31), qw = n_q * HD;
     const size_t qplane = (size_t)S * qw;
     const float sl2 = fmaxf(fabsf(scale) * kLog2e, 1e-30f);  // see above
     const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;
@@ -672,7 +677,7 @@ struct Args {
 
 template <int HD, int G, int GB, bool QX2, int KSPLIT, int TK>
 void launch(hipStream_t s, const Args& a) {
-    const dim3 grid((a.S + 31) / 32, a.n_kv * (G / GB));
+    const uint32_t grid = (a.S + 31) / 32 * (a.n_q / GB);
     k_attn_prefill_kv4<HD, G, GB, QX2, KSPLIT, TK><<<grid, 64 * GB * KSPLIT, 0, s>>>(
         a.q, a.k, a.v, a.S, a.pos0, a.n_q, a.n_kv, a.cap, a.scale, a.out, a.om, a.win, a.n_glob, a.thr);
 }
@@ -691,7 +696,7 @@ void launch_group(hipStream_t s, const Args& a) {
     const uint64_t groups = (uint64_t)((a.S + 31) / 32) * a.n_kv;
     if (groups * G <= kCUs) {
         constexpr int W = 8;
-        k_attn_prefill_kv4_few<HD, QX2, W><<<dim3((a.S + 31) / 32, a.n_q), W * 64, 0, s>>>(
+        k_attn_prefill_kv4_few<HD, QX2, W><<<(a.S + 31) / 32 * a.n_q, W * 64, 0, s>>>(
             a.q, a.k, a.v, a.S, a.pos0, a.n_q, a.n_kv, a.cap, a.scale, a.out, a.om, a.win, a.n_glob, a.thr);
         return;
     }
@@ -725,7 +730,8 @@ int attn_prefill_kv4(const char* fn, const void* q, int q_dtype, const void* kca
     if ((uint64_t)pos0 + S > cap) return vsl_capacity("%s: %u positions from %u exceed capacity %u", fn, S, pos0, cap);
     if (!std::isfinite(scale)) return vsl_invalid("%s: scale is not finite", fn);
     if (cap > 0x80000000u) return vsl_unsupported("%s: capacity %u", fn, cap);
-    if ((uint64_t)n_q * hd > 0x7FFFFFFFull || n_q > 65535u) return vsl_unsupported("%s: n_q=%u", fn, n_q);
+    if ((uint64_t)n_q * hd > 0x7FFFFFFFull) return vsl_unsupported("%s: n_q=%u", fn, n_q);
+    if (((uint64_t)S + 31) / 32 * n_q >= 1ull << 22) return vsl_unsupported("%s: %u rows in one call", fn, S);  // 2^30 lanes
     if (S == 0) return VSL_OK;
     const Args a{static_cast<const vsl_half*>(q), static_cast<const char*>(kcache), static_cast<const char*>(vcache), S, pos0,
                  n_q, n_kv, cap, scale, static_cast<vsl_half*>(out),
