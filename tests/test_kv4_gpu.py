@@ -602,3 +602,57 @@ def test_token_loop(vsl, dev, H, hd, n_q, n_kv, halves, window):
     assert np.array_equal(dev.get(dk), kb) and np.array_equal(dev.get(dv), vb)
     vsl.check(H.vsl_graph_destroy(g))
     vsl.check(H.vsl_stream_destroy(s))
+
+
+def test_two_calls_at_once(vsl, dev, H):
+    """Prompt attention (both kernels) and decode attention over the same caches on three streams without a wait between,
+    a few times over, and a captured prompt call replayed beside eager ones: bit for bit what each gives alone."""
+    hd, n_q, n_kv, cap, n = 128, 32, 8, 900, 800
+    rng = np.random.default_rng(91)
+    kb, vb, _, _ = filled(rng, rng.normal(0, 1, (n_kv, n, hd)), rng.normal(0, 1, (n_kv, n, hd)), cap)
+    dk, dv = dev.put(kb), dev.put(vb)
+    streams = [ctypes.c_void_p() for _ in range(3)]
+    for s in streams:
+        vsl.check(H.vsl_stream_create(ctypes.byref(s)))
+    few, many, nsplit = 40, 300, 16
+    dq = {S: dev.put(rng.normal(0, 1, (2, S, n_q * hd)).astype(np.float16)) for S in (few, many)}
+    q1 = dev.put(rng.normal(0, 1, n_q * hd).astype(np.float32))
+    ctrl = dev.empty((8,), np.int32)
+    vsl.check(H.vsl_ctrl_reset(dev.p(ctrl), n - 1, 4, 0, cap, None))
+    po, pml = dev.empty((n_q * nsplit * hd,), np.float32), dev.empty((n_q * nsplit * 2,), np.float32)
+
+    def prompt(S, out, s):
+        vsl.check(H.vsl_attn_prefill_kv4(dev.p(dq[S]), 2, dev.p(dk), dev.p(dv), S, n - S, n_q, n_kv, hd, cap, 0.1, dev.p(out), 2, s))
+
+    def token(out, s):
+        vsl.check(H.vsl_attn_decode(dev.p(q1), dev.p(dk), dev.p(dv), 7, n_q, n_kv, hd, cap, 0.1, nsplit, dev.p(po), dev.p(pml),
+                                    dev.p(out), dev.p(ctrl), s))
+
+    outs = lambda: [dev.empty((2, few, n_q * hd), np.float16), dev.empty((2, many, n_q * hd), np.float16),
+                    dev.empty((n_q * hd,), np.float32)]
+    alone = outs()
+    dev.sync()
+    prompt(few, alone[0], None)
+    prompt(many, alone[1], None)
+    token(alone[2], None)
+    alone = [dev.get(o) for o in alone]
+    assert all(np.isfinite(a).all() and a.any() for a in alone)
+    graph_out, g = dev.empty((2, many, n_q * hd), np.float16), ctypes.c_void_p()
+    vsl.check(H.vsl_graph_begin(streams[0]))
+    prompt(many, graph_out, streams[0])
+    vsl.check(H.vsl_graph_end(streams[0], ctypes.byref(g)))
+    for _ in range(4):
+        got = outs()
+        graph_out.fill_(0)
+        dev.sync()
+        vsl.check(H.vsl_graph_launch(g, streams[0]))
+        prompt(few, got[0], streams[0])
+        prompt(many, got[1], streams[1])
+        token(got[2], streams[2])
+        for s in streams:
+            vsl.check(H.vsl_stream_sync(s))
+        assert all(np.array_equal(dev.get(o), a) for o, a in zip(got, alone))
+        assert np.array_equal(dev.get(graph_out), alone[1])
+    vsl.check(H.vsl_graph_destroy(g))
+    for s in streams:
+        vsl.check(H.vsl_stream_destroy(s))
