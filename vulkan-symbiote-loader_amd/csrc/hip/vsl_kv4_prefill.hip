@@ -267,8 +267,9 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     // and the scores of t in registers: the codes of K of t + 2 and V of t + 1 are requested, the scores of t + 1 are
     // issued on the matrix cores while the vector pipe turns those of t into probabilities, then the products
     // of t with V; the codes go into the buffers that K of t and V of t - 1 have left (both last read before the
-    // barrier that ended the previous iteration). Tiles that every row of the block sees whole come first (without a
-    // window): they run without masks and checks, in one straight block of code past the rescale.
+    // barrier that ended the previous iteration; K of tile 0 before one of its own). Tiles that every row of the block
+    // sees whole come first (without a window): they run without masks and checks, in one straight block of code past
+    // the rescale.
     float16v st[NKB];
     KWords kw;
     VWords vw;
@@ -304,6 +305,7 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     {
         half8 kf[NKB][HD / 16];
         read_k(0, kf);
+        __syncthreads();  // body(0) writes K of tile 2 where this read K of tile 0
         qk(kf, st);
     }
     const uint32_t n_whole = lo_max ? 0 : (p_first + 1) / TK;
