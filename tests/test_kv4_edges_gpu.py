@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import kv4_ref
-from test_kv4_gpu import H, _dev, attn_tol, dev, filled, out_tol, prefill  # noqa: F401 (fixtures)
+from test_kv4_gpu import H, _dev, attn_tol, decode, dev, filled, out_tol, prefill  # noqa: F401 (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +40,72 @@ def test_prompt_tiles_are_kept_apart(vsl, dev, H, shape):
     assert np.all(np.abs(first[:, fin] - ref) <= tol)
     for _ in range(6):
         assert np.array_equal(prefill(vsl, dev, H, q, True, dk, dv, n_kv, cap, pos0, 2, scale)[0], first, equal_nan=True)
+
+
+# ------------------------------------------------------------------------------------------
+# positions that no append wrote
+# ------------------------------------------------------------------------------------------
+FILLS = ["random", 0x7BF0, 0x7000, 0x6C50, 0xFBF0, 0x7C00, 0xFFFF, 0x6C4F]  # against all NaN, as filled() leaves them
+
+
+def refill(rng, buf, kept, n_kv, cap, hd, is_v, fill):
+    """The cache's bytes with other codes and steps wherever `kept` (a truth value a position) is False."""
+    w, s = kv4_ref.views(buf, n_kv, cap, hd, is_v)
+    new = np.zeros_like(buf)
+    nw, ns = kv4_ref.views(new, n_kv, cap, hd, is_v)
+    nw[:] = rng.integers(0, 1 << 32, nw.shape, dtype=np.uint32)
+    ns[:] = rng.integers(0, 1 << 16, ns.shape, dtype=np.uint16) if fill == "random" else fill
+    at = np.flatnonzero(kept)
+    if is_v:
+        for p in at:
+            m = np.uint32(15 << kv4_ref.SHIFT[p % 8])
+            nw[:, p // 8] = (nw[:, p // 8] & ~m) | (w[:, p // 8] & m)
+            ns[:, p // 8, :, p % 8] = s[:, p // 8, :, p % 8]
+    else:
+        nw[:, at], ns[:, at] = w[:, at], s[:, at]
+    return new
+
+
+STALE = [  # hd, n_q, n_kv, S, pos0, window: a row block's own waves; two heads, four, and as the group divides share tiles
+    (128, 32, 8, 45, 0, None), (64, 8, 2, 33, 70, None), (64, 3, 1, 3, 0, None), (128, 64, 8, 160, 201, None),
+    (64, 32, 8, 290, 0, None), (128, 64, 8, 270, 131, None), (64, 64, 8, 270, 3, None), (128, 48, 8, 200, 65, None),
+    (128, 40, 8, 225, 100, None), (64, 56, 8, 170, 201, None), (128, 8, 2, 40, 300, (50, 16, 100)),
+    (64, 6, 2, 70, 333, (33, 3, 64)), (128, 64, 8, 270, 400, (70, 20, 100)), (64, 40, 8, 240, 450, (20, 70, 300))]
+
+
+@pytest.mark.parametrize("shape", STALE, ids=str)
+def test_prompt_over_what_was_left_in_the_cache(vsl, dev, H, shape):
+    """What a cache holds past the last key, and where a window hides a position from every row, reaches no output, whatever
+    the bits: infinite, negative and other steps that no append stores, too."""
+    hd, n_q, n_kv, S, pos0, window = shape
+    rng = np.random.default_rng(sum(shape[:5]))
+    n, cap = pos0 + S, pos0 + S + 40
+    kb, vb, K, V = filled(rng, rng.normal(0, 1, (n_kv, n, hd)), rng.normal(0, 1.3, (n_kv, n, hd)), cap)
+    q = rng.normal(0, 1, (S, n_q, hd)).astype(np.float32)
+    scale = 1.0 / math.sqrt(hd)
+    kept = np.zeros(kv4_ref.positions(cap), bool)
+    for s in range(S):
+        kept[:n] |= kv4_ref.seen(pos0 + s, n, window)
+    want, used = prefill(vsl, dev, H, q, True, dev.put(kb), dev.put(vb), n_kv, cap, pos0, 2, scale, window)
+    ref = kv4_ref.attend(used, K, V, pos0, scale, window)
+    assert np.all(np.abs(want - ref) <= attn_tol(used, K, V, scale) + out_tol(ref, 2))
+    for fill in FILLS:
+        dk, dv = (dev.put(refill(rng, b, kept, n_kv, cap, hd, is_v, fill)) for b, is_v in ((kb, False), (vb, True)))
+        got, _ = prefill(vsl, dev, H, q, True, dk, dv, n_kv, cap, pos0, 2, scale, window)
+        assert np.array_equal(got, want), fill
+
+
+@pytest.mark.parametrize("hd,n_q,n_kv,n,nsplit,window", [(128, 8, 2, 45, 4, None), (64, 5, 1, 300, 7, None), (128, 32, 8, 778, 32, None),
+                                                         (64, 8, 1, 500, 3, (40, 5, 100)), (128, 4, 4, 700, 8, (100, 33, 64))])
+def test_decode_over_what_was_left_in_the_cache(vsl, dev, H, hd, n_q, n_kv, n, nsplit, window):
+    rng = np.random.default_rng(n + hd)
+    cap = n + 40
+    kb, vb, _, _ = filled(rng, rng.normal(0, 1, (n_kv, n, hd)), rng.normal(0, 1.3, (n_kv, n, hd)), cap)
+    q = rng.normal(0, 1, (n_q, hd)).astype(np.float32)
+    kept = np.zeros(kv4_ref.positions(cap), bool)
+    kept[:n] = kv4_ref.seen(n - 1, n, window)
+    want = decode(vsl, dev, H, q, dev.put(kb), dev.put(vb), n_kv, cap, n - 1, nsplit, window)
+    assert np.isfinite(want).all() and want.any()
+    for fill in FILLS:
+        dk, dv = (dev.put(refill(rng, b, kept, n_kv, cap, hd, is_v, fill)) for b, is_v in ((kb, False), (vb, True)))
+        assert np.array_equal(decode(vsl, dev, H, q, dk, dv, n_kv, cap, n - 1, nsplit, window), want), fill

@@ -13,6 +13,9 @@ __device__ __host__ __forceinline__ constexpr uint64_t kv4_bytes(uint32_t n_kv, 
 }
 
 constexpr uint32_t kKv4NaN = 0x7E00;  // the step of a block that reads back as NaN
+// The largest other step that an append stores: d = 4352 (a range of 65280), z = 15. Past it (n - z) d may overflow, and
+// so may what stands for a position that no append wrote, whose bits are anything.
+constexpr uint32_t kKv4MaxStep = 0x6C4F;
 
 // Shift of value e's nibble in a word of eight: values 2p and 2p + 1 lie 16 bits apart, so that one mask takes
 // both into the halves of a register.

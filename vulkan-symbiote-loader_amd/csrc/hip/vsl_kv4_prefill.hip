@@ -115,10 +115,11 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
             b.s[i] = *reinterpret_cast<const u32x4*>(Vst + (oct * NB + w / 16) * 16);
         }
     };
-    // A tile's values into LDS. A V block that stands for NaN (or holds no value of this cache: what lies past the
-    // block's last key is anything) would reach rows that do not see its key through a product with 0. Tiles that
-    // some row sees in part (EDGE) take such steps as 0; the block notes that there was a NaN, and the rows that see it
-    // are found at the end. (K needs none of this: what a key's row of scores holds is replaced where it is masked.)
+    // A tile's values into LDS. A V block that stands for NaN would reach rows that do not see its key through a product
+    // with 0, and so would an infinity from a step that no append stored (the bits past the block's last key, and of
+    // positions that a window hides from all its rows, are anything). Tiles that some row sees in part (EDGE) take such
+    // steps as 0; the block notes that there was a NaN, and the rows that see it are found at the end. (K needs none
+    // of this: what a key's row of scores holds is replaced where it is masked.)
     auto expand_k = [&](const KWords& b, int buf) {
 #pragma unroll
         for (int i = 0; i < NKW; ++i) {
@@ -137,7 +138,7 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const uint32_t x = s[e / 2] >> (16 * (e & 1)) & 0xFFFFu;
-                    if ((x & 0x7C00u) != 0x7C00u) continue;
+                    if (x <= kKv4MaxStep) continue;
                     s[e / 2] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
                     if (t * TK + 8 * r + e < kv_end) s_nan = 1;
                 }
@@ -523,7 +524,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_prefill_kv4_few(
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const uint32_t x = b.vs[hi][e / 2] >> (16 * (e & 1)) & 0xFFFFu;
-                    if ((x & 0x7C00u) != 0x7C00u) continue;
+                    if (x <= kKv4MaxStep) continue;
                     b.vs[hi][e / 2] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
                     if (p0 + 16 * hi + 8 * g + e < kv_end) s_nan = 1;
                 }
