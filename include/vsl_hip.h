@@ -479,9 +479,9 @@ int vsl_attn_prefill_kv4_window(const void* q, int q_dtype, const void* kcache, 
                                 void* stream);
 
 /* ------------------------------------------------------------------------------------------
- * hipGraph helpers (each decode step is captured once and replayed).  A graph that is a chain of up to four kernels
- * is replayed as launches of its own, with the parameters it was captured with.  Replays of one graph share the memory it
- * names: the caller orders them, on one stream or by events.  vsl_graph_launch is called on the device of the capture.
+ * hipGraph helpers (each decode step is captured once and replayed).  A replay is one operation on its stream: what
+ * other threads enqueue there comes before or after it.  Replays of one graph share the memory it names: on different
+ * streams they may run at the same time, and the caller orders them by events.
  * ------------------------------------------------------------------------------------------ */
 typedef struct vsl_graph vsl_graph;
 int vsl_graph_begin(void* stream);

@@ -7,7 +7,6 @@
 #include <map>
 #include <mutex>
 #include <string>
-#include <vector>
 
 #include "vsl_device.h"
 #include "vsl_hip.h"
@@ -352,56 +351,10 @@ extern "C" int vsl_ctrl_reset(vsl_ctrl* ctrl, uint32_t pos, uint32_t max_steps, 
 // ------------------------------------------------------------------------------------------
 // hipGraph helpers
 // ------------------------------------------------------------------------------------------
-// A captured graph. Up to kDirectNodes kernels in a chain (a decode step's attention stage, say) are replayed as
-// launches of their own, with the parameters that the graph holds: hipGraphLaunch takes the host 14 us whatever the
-// size up to there, a launch 2.7 us (chains of 1 / 2 / 3 / 4 small kernels: 14.6 / 14.5 / 14.1 / 13.8 us a replay by
-// hipGraphLaunch, 2.7 / 5.3 / 8.5 / 11.0 us by launches; 8: 19.9 / 22.1).
-constexpr size_t kDirectNodes = 4;
 struct vsl_graph {
     hipGraph_t graph = nullptr;
     hipGraphExec_t exec = nullptr;
-    std::vector<hipKernelNodeParams> direct;  // in order; empty: replayed by hipGraphLaunch
-    int device = -1;                          // the direct kernels' device
 };
-
-// The kernels of a graph that is one chain of at most kDirectNodes kernel nodes, in order; else empty. Only kernels that
-// hipLaunchKernel can launch as the capture did: known by a host symbol (not a module's function), not cooperative.
-static std::vector<hipKernelNodeParams> kernel_chain(hipGraph_t graph) {
-    size_t n = 0, n_edges = 0;
-    if (hipGraphGetNodes(graph, nullptr, &n) != hipSuccess || n == 0 || n > kDirectNodes) return {};
-    if (hipGraphGetEdges(graph, nullptr, nullptr, &n_edges) != hipSuccess || n_edges != n - 1) return {};
-    hipGraphNode_t nodes[kDirectNodes], from[kDirectNodes], to[kDirectNodes], at = nullptr;
-    if (hipGraphGetNodes(graph, nodes, &n) != hipSuccess) return {};
-    if (n_edges && hipGraphGetEdges(graph, from, to, &n_edges) != hipSuccess) return {};
-    for (size_t i = 0; i < n; ++i) {  // the node that no edge ends at
-        bool first = true;
-        for (size_t e = 0; e < n_edges; ++e) first &= to[e] != nodes[i];
-        if (first && at) return {};
-        if (first) at = nodes[i];
-    }
-    std::vector<hipKernelNodeParams> chain;
-    while (at && chain.size() < n) {
-        hipGraphNodeType type;
-        hipKernelNodeParams p{};
-        if (hipGraphNodeGetType(at, &type) != hipSuccess || type != hipGraphNodeTypeKernel) return {};
-        if (hipGraphKernelNodeGetParams(at, &p) != hipSuccess || !p.func || !p.kernelParams || p.extra) return {};
-        hipFuncAttributes fa;
-        hipKernelNodeAttrValue coop{};
-        if (hipFuncGetAttributes(&fa, p.func) != hipSuccess) return {};
-        if (hipGraphKernelNodeGetAttribute(at, hipKernelNodeAttributeCooperative, &coop) != hipSuccess || coop.cooperative)
-            return {};
-        chain.push_back(p);
-        hipGraphNode_t next = nullptr;
-        for (size_t e = 0; e < n_edges; ++e) {
-            if (from[e] != at) continue;
-            if (next) return {};
-            next = to[e];
-        }
-        at = next;
-    }
-    if (at || chain.size() != n) return {};
-    return chain;
-}
 
 extern "C" int vsl_graph_begin(void* stream) {
     HIP_TRY(hipStreamBeginCapture(static_cast<hipStream_t>(stream), hipStreamCaptureModeThreadLocal));
@@ -422,22 +375,12 @@ extern "C" int vsl_graph_end(void* stream, vsl_graph** out) {
         delete g;
         return vsl_hip_fail(e, "hipGraphInstantiate", __FILE__, __LINE__);
     }
-    g->direct = kernel_chain(g->graph);
-    if (hipGetDevice(&g->device) != hipSuccess) g->direct.clear();
-    if (g->direct.empty()) (void)hipGetLastError();  // what a query above reported of a node that it does not cover
     *out = g;
     return VSL_OK;
 }
 
 extern "C" int vsl_graph_launch(vsl_graph* g, void* stream) {
     if (!g) return vsl_invalid("vsl_graph_launch: null graph");
-    int device = -1;
-    if (!g->direct.empty() && hipGetDevice(&device) == hipSuccess && device == g->device) {
-        for (const hipKernelNodeParams& p : g->direct)
-            HIP_TRY(hipLaunchKernel(p.func, p.gridDim, p.blockDim, p.kernelParams, p.sharedMemBytes,
-                                    static_cast<hipStream_t>(stream)));
-        return VSL_OK;
-    }
     HIP_TRY(hipGraphLaunch(g->exec, static_cast<hipStream_t>(stream)));
     return VSL_OK;
 }
