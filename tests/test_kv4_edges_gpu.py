@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import kv4_ref
-from test_kv4_gpu import H, _dev, attn_tol, decode, dev, filled, out_tol, prefill  # noqa: F401 (fixtures)
+from test_kv4_gpu import H, U, _dev, attn_tol, decode, dev, filled, out_tol, prefill  # noqa: F401 (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,75 @@ def test_decode_over_what_was_left_in_the_cache(vsl, dev, H, hd, n_q, n_kv, n, n
     for fill in FILLS:
         dk, dv = (dev.put(refill(rng, b, kept, n_kv, cap, hd, is_v, fill)) for b, is_v in ((kb, False), (vb, True)))
         assert np.array_equal(decode(vsl, dev, H, q, dk, dv, n_kv, cap, n - 1, nsplit, window), want), fill
+
+
+# ------------------------------------------------------------------------------------------
+# one key with nearly all the weight, and a long tail
+# ------------------------------------------------------------------------------------------
+# The tail's keys have a score of 0, G (in powers of two) below that of key 3, whose value is 0, and one value v: exactly
+#   out = t w v / (1 + t w),  w = 2^-G,  t tail keys.
+# Probabilities are passed to the second product in binary16, as hi / lo pairs or alone, 2^7 times as large as the reference
+# maximum's share (at most 2^8 more): half a subnormal step, 2^-25, is 2^-32 of it, t 2^-32 v of the output. Alone they
+# are also rounded by 2^-11 of themselves where they are not subnormal. Relative to the output: a score is off by
+# G (2^-22 + (hd + 1) U) as in attn_tol, the exponentials by 2^-22, sums over the keys by 2 n U.
+TAIL_GAPS = [25.6, 28.0]
+
+
+def tail(rng, hd, n_kv, n, cap):
+    K, V = np.zeros((n_kv, n, hd)), np.ones((n_kv, n, hd))
+    K[:, 3, 0], V[:, 3] = 2.0, 0.0
+    return filled(rng, K, V, cap)
+
+
+def tail_check(got, score, v, t, hd, split, extra):
+    """got [..., n_q, hd] of rows that see t tail keys (an array over the leading axes)."""
+    w = 2.0 ** -score
+    t = np.asarray(t, np.float64).reshape(-1, *[1] * (got.ndim - 1))
+    ref = t * w * v / (1 + t * w)
+    rel = 2 * (math.log(2) * score * (2.0 ** -22 + (hd + 1) * U) + 2.0 ** -22 + (t + 1) * U) + (0 if split else 2.0 ** -11)
+    assert np.all(np.abs(got - ref) <= t * 2.0 ** -32 * v + rel * ref + extra(ref))
+
+
+@pytest.mark.parametrize("gap", TAIL_GAPS)
+@pytest.mark.parametrize("hd,n_q,n_kv,n,nsplit", [(128, 4, 1, 16000, 1), (64, 8, 2, 16001, 1), (128, 8, 1, 30000, 4)])
+def test_decode_keeps_a_tail(vsl, dev, H, hd, n_q, n_kv, n, nsplit, gap):
+    rng = np.random.default_rng(n)
+    cap, scale = n + 9, 1.0 / math.sqrt(hd)
+    kb, vb, K, V = tail(rng, hd, n_kv, n, cap)
+    a = K[0, 3, 0] * scale * math.log2(math.e)
+    q = np.zeros((n_q, hd), np.float32)
+    q[:, 0] = gap / a
+    got = decode(vsl, dev, H, q, dev.put(kb), dev.put(vb), n_kv, cap, n - 1, nsplit)
+    tail_check(got[None], float(q[0, 0]) * a, V[0, 0, 0], n - 1, hd, True, lambda r: 0.0)
+
+
+@pytest.mark.parametrize("gap", TAIL_GAPS)
+@pytest.mark.parametrize("x2", [True, False])
+@pytest.mark.parametrize("hd,n_q,n_kv,S,n", [(128, 8, 2, 3, 16000), (64, 4, 1, 40, 16000), (128, 64, 8, 130, 8000), (64, 64, 8, 130, 8000),
+                                             (128, 64, 8, 270, 8000), (64, 64, 8, 270, 8000), (128, 40, 8, 225, 8000)])
+def test_prompt_keeps_a_tail(vsl, dev, H, hd, n_q, n_kv, S, n, x2, gap):
+    rng = np.random.default_rng(n + S)
+    cap, scale, pos0 = n + 9, 1.0 / math.sqrt(hd), n - S
+    kb, vb, K, V = tail(rng, hd, n_kv, n, cap)
+    a = K[0, 3, 0] * scale * math.log2(math.e)
+    q = np.zeros((S, n_q, hd), np.float32)
+    q[:, :, 0] = gap / a
+    got, used = prefill(vsl, dev, H, q, x2, dev.put(kb), dev.put(vb), n_kv, cap, pos0, 2, scale)
+    tail_check(got, used[0, 0, 0] * a, V[0, 0, 0], pos0 + np.arange(S), hd, x2, lambda r: out_tol(r, 2))
+
+
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 18, 2.0 ** 23])
+@pytest.mark.parametrize("hd,n_q,n_kv,S", [(128, 8, 2, 40), (128, 64, 8, 140), (64, 64, 8, 270)])
+def test_scores_of_any_size_stay_finite(vsl, dev, H, hd, n_q, n_kv, S, size):
+    """Scores so large that fp32 holds them to whole powers of two: the outputs are means of the values all the same."""
+    rng = np.random.default_rng(S)
+    n, cap, scale = S + 300, S + 320, 1.0 / math.sqrt(hd)
+    kb, vb, K, V = filled(rng, rng.normal(0, 1, (n_kv, n, hd)), rng.normal(0, 1, (n_kv, n, hd)), cap)
+    q = rng.normal(0, 1, (S, n_q, hd)).astype(np.float32)
+    big = size / (np.abs(K).max() * hd ** 0.5 * 4)
+    dk, dv = dev.put(kb), dev.put(vb)
+    for x2 in (True, False):
+        got, _ = prefill(vsl, dev, H, q, x2, dk, dv, n_kv, cap, 300, 2, scale * big)
+        assert np.abs(got).max() <= 1.01 * np.abs(V).max()
+    one = decode(vsl, dev, H, q[0] * np.float32(min(big, 2.0 ** 12)), dk, dv, n_kv, cap, n - 1, 4)
+    assert np.abs(one).max() <= 1.01 * np.abs(V).max()

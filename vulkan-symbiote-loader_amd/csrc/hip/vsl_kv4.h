@@ -61,6 +61,14 @@ __device__ __forceinline__ half8 kv4_word(uint32_t w, const Kv4Step (&s)[4], con
     return kv4_join(kv4_pair<0>(w, s[0], c), kv4_pair<1>(w, s[1], c), kv4_pair<2>(w, s[2], c), kv4_pair<3>(w, s[3], c));
 }
 
+// Softmax against a reference m per row (log2 units) that is raised, to kKv4Room below the largest score seen, only when
+// some score exceeds it by more than kKv4Room + kKv4Lazy: probabilities stay up to 2^15, within binary16, and what the pair
+// of planes (or the one plane) drops of each, half a subnormal step 2^-25, is 2^-32 of the largest or less. (With m
+// at the largest score it is 2^-25, and a tail of 16000 keys just below that share, 5e-4 of an output, is lost.) The
+// excess is taken as the difference that the exponential gets, so the bound holds for scores that fp32 holds to whole
+// powers of two, too.
+constexpr float kKv4Lazy = 8.f, kKv4Room = 7.f;
+
 // Two values rounded to binary16 in one instruction. The pair passes through an empty register asm, so that what is
 // used and what is subtracted from the values are the same rounding.
 __device__ __forceinline__ half2v pack_f16(float a, float b) {

@@ -459,9 +459,8 @@ __device__ __forceinline__ float add_lane8(float v) {
 //    octet l / 16, which is the B operand P^T of O^T += V^T P^T when V's words are octets of positions: the lanes of
 //    the columns 0-7 pass the probabilities' hi plane, the others the lo plane;
 //  - lane l expands the V columns HD/16 (l % 16) .. + HD/16 - 1 of octet l / 16, whose steps are one 16-byte load.
-// Softmax with a reference maximum m per head that is raised, for the whole wave, only when some score exceeds it by
-// more than kLazy (probabilities stay below 2^kLazy). Masked positions get probability 0 and their V steps are set to
-// 0, so what the cache holds past the length never reaches a sum. Output as k_attn_decode's.
+// Softmax against a reference per head (kKv4Room), raised for the whole wave. Masked positions get probability 0 and
+// their V steps are set to 0, so what the cache holds past the length never reaches a sum. Output as k_attn_decode's.
 // Bound by latency at short lengths (8B shape, 32 splits, 778 positions 4.9 us: loads 1.0, one tile's chain 1.1, the waves'
 // join and the partials 0.9, the launch), and by the expansion's vector instructions at long ones: 32001 positions 11.9 us,
 // of which the loads alone, by the same pattern, take 8.6 (37 MB, 4.3 TB/s), against 22.4 for the fp16 cache's kernel.
@@ -473,7 +472,6 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_decode_kv4(const float* 
                                                                 uint32_t n_glob, uint32_t thr) {
     constexpr int KS = HD / 32, NB = HD / 32, NC = HD / 16;  // k-steps; blocks a row; V columns a lane (and O^T tiles)
     constexpr uint32_t TP = 32;
-    constexpr float kLazy = 8.f;
     constexpr int NBUF = kDecTiles;
     static_assert(G >= 1 && G <= 8, "GQA group of 1..8 heads");
     __shared__ __attribute__((aligned(8))) float s_ml[WAVES][G][2];
@@ -609,11 +607,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_decode_kv4(const float* 
         float bm = s[0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) bm = fmaxf(bm, s[e]);
-        if (__builtin_amdgcn_ballot_w64(bm > m + kLazy)) {  // m = -inf: any finite score raises it
+        if (__builtin_amdgcn_ballot_w64(bm - m > kKv4Lazy + kKv4Room)) {  // m = -inf: any finite score raises it
             float a0, a1;
             lane_pair<16>(bm, a0, a1);
             lane_pair<32>(fmaxf(a0, a1), a0, a1);
-            const float mn = fmaxf(m, fmaxf(a0, a1));
+            const float mn = fmaxf(m, fmaxf(a0, a1) - kKv4Room);
             const float corr = mn == -INFINITY ? 1.f : fast_exp2(m - mn);  // m = -inf: 0
             l *= corr;
 #pragma unroll

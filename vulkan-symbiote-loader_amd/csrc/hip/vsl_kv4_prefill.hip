@@ -169,7 +169,6 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
         for (int v = 0; v < 16; ++v) o[t][v] = 0.f;
     float m = -INFINITY, l = 0.f, minus_one = -1.f;
     asm volatile("" : "+v"(minus_one));  // a register, so that value - (float)half is one mixed-precision multiply-add
-    constexpr float kLazy = 8.f;  // the reference maximum is raised only by more than this (log2 units)
 
     const int krow = (lane & 19) | (lane & 4) << 1 | (lane & 8) >> 1;  // bits 2 and 3 of l % 32 exchanged
     auto read_k = [&](int buf, half8 (&kf)[NKB][HD / 16]) {
@@ -191,7 +190,7 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
                     st[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[kb][c], qf[p][c], st[kb], 0, 0, 0);
         }
     };
-    // the mask of a tile that some row sees in part; returns the scaled maximum of this lane's row. Element v of a
+    // the mask of a tile that some row sees in part; returns the maximum of this lane's row. Element v of a
     // fragment is key 16 (v / 8) + 8 (l / 32) + v % 8.
     auto mask_max = [&](float16v (&st)[NKB], uint32_t t, auto edge) {
         if constexpr (decltype(edge)::value) {
@@ -211,12 +210,12 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
             for (int v = 0; v < 16; ++v) bm = fmaxf(bm, st[kb][v]);
         float ba, bb;
         lane_pair<32>(bm, ba, bb);
-        return fmaxf(ba, bb) * sl2;
+        return fmaxf(ba, bb);
     };
     auto rescale = [&](float bm) {
-        const bool raise = bm > m + kLazy;  // m = -inf: any finite tile maximum raises it
+        const bool raise = fmaf(bm, sl2, -m) > kKv4Lazy + kKv4Room;  // m = -inf: any finite tile maximum raises it
         if (__builtin_amdgcn_ballot_w64(raise)) {
-            const float mn = raise ? bm : m;
+            const float mn = raise ? fmaf(bm, sl2, -kKv4Room) : m;
             const float corr = mn == -INFINITY ? 1.f : fast_exp2(m - mn);  // m = -inf: 0
             l *= corr;
             m = mn;
@@ -496,7 +495,6 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_prefill_kv4_few(
         for (int v = 0; v < 16; ++v) o[f][v] = 0.f;
     float m = -INFINITY, l = 0.f, minus_one = -1.f;
     asm volatile("" : "+v"(minus_one));
-    constexpr float kLazy = 8.f;
     if (threadIdx.x == 0) s_nan = 0;
     __syncthreads();
 
@@ -534,10 +532,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_prefill_kv4_few(
         for (int v = 1; v < 16; ++v) bm = fmaxf(bm, st[v]);
         float ba, bb;
         lane_pair<32>(bm, ba, bb);
-        bm = fmaxf(ba, bb) * sl2;
-        const bool raise = bm > m + kLazy;  // m = -inf: any finite tile maximum raises it
+        bm = fmaxf(ba, bb);
+        const bool raise = fmaf(bm, sl2, -m) > kKv4Lazy + kKv4Room;  // m = -inf: any finite tile maximum raises it
         if (__builtin_amdgcn_ballot_w64(raise)) {
-            const float mn = raise ? bm : m;
+            const float mn = raise ? fmaf(bm, sl2, -kKv4Room) : m;
             const float corr = mn == -INFINITY ? 1.f : fast_exp2(m - mn);  // m = -inf: 0
             l *= corr;
             m = mn;
