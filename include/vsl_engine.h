@@ -163,7 +163,8 @@ int vsl_engine_pack(vsl_engine* e, uint64_t idx, vsl_pack_info* out, char* name,
 int vsl_write_synthetic_gguf(const char* path, const vsl_model_spec* spec, uint64_t seed, int convention);
 /* the same with per-head norms of queries and keys (F32 "blk.N.attn_q_norm.weight" / "blk.N.attn_k_norm.weight" of
  * head_dim gains, N(1, 0.1)); an engine opened from a file that has both tensors in every layer applies them before
- * the rotation (vsl_qk_norm_rope_append).  No reference counterpart. */
+ * the rotation (vsl_qk_norm_rope_append), and refuses one whose "general.architecture" is not "llama" (geometry keys and
+ * rotation of other architectures are not read).  No reference counterpart. */
 int vsl_write_synthetic_gguf_qk_norm(const char* path, const vsl_model_spec* spec, uint64_t seed, int convention);
 /* the same with a vocabulary: n_tokens strings (tokens[i], token_lens[i] bytes each, may hold any
  * byte) written as the array "tokenizer.ggml.tokens", or with keyed = 1 as one string key

@@ -219,6 +219,11 @@ VulkanSymbioteEngine::VulkanSymbioteEngine(const Path& model_path, const EngineO
     if (norms && norms != 2 * cfg.num_layers)
         throw std::runtime_error("Failed to load model: query / key norms in some layers only");
     qk_norm_ = norms != 0;
+    // the geometry is read from "llama.*" keys, and the rotation is that of llama files: another architecture with such
+    // norms has keys and a rotation of its own, and would run to wrong text
+    if (qk_norm_ && !cfg.model_type.empty() && cfg.model_type != "llama")
+        throw std::runtime_error("Failed to load model: query / key norms in a file of architecture \"" + cfg.model_type +
+                                 "\" (only \"llama\" geometry keys and rotation are read)");
     try {
         plan_quant_gguf(cfg);
         init_device(cfg, pack_dtype(qf) == VSL_DT_F16, pack_dtype(ef));
