@@ -57,7 +57,7 @@ __device__ __forceinline__ double rsqrt64(double x) {
 // Four consecutive dims of a head's row in one lane (HD / 4 lanes a row): the head's norm and rotation. T: float; or
 // double for keys that become 4-bit codes, whose choice hangs on values next to a border: it is then the exact
 // value's, and the same for every number of rows in a call. (In 64 bits throughout, 2048 rows of the 8B shape took 29.5
-// us instead of 22.9: conversions and 64-bit operations, not memory, were the bound.)
+// us instead of 22.9, side by side: conversions and 64-bit operations, not memory, were the bound.)
 struct RopeArgs {
     const float* q_gamma;
     const float* k_gamma;
@@ -257,8 +257,8 @@ __device__ __forceinline__ void store_k4(void* cache, uint64_t soff, size_t at, 
 // of a call may be partly outside it): the codes of a column are joined to its word over the lanes. The others take
 // rows of q and k heads (of all heads with fp16 and fp32 caches), HD / 4 lanes a head, neighbouring heads in
 // neighbouring lanes. Bound by memory in a large call: 2048 rows of the 8B shape with a split q (50 MB read, 36 MB
-// written) 22.9 us, 3.8 TB/s against the 5.3 of a large copy; 45 rows 3.5 us. Two and four rows a lane: 23.5 and 25.6,
-// 4.3 and 6.3 us; an octet of rows of one head a lane: 38.4 and 12.0 us.
+// written) 22.5 us (median of a trace; the least 19.8), 3.8 TB/s against the 5.3 of a large copy; 45 rows 3.5 us. Two
+// and four rows a lane: 23.5 and 25.6, 4.3 and 6.3 us; an octet of rows of one head a lane: 38.4 and 12.0 us.
 template <int HD, int QM, int KVM>
 __global__ __launch_bounds__(256) void k_append_rows(AppendArgs a, uint32_t v_waves) {
     constexpr uint32_t L = HD / 4, NB = HD / 32;
@@ -463,7 +463,8 @@ __device__ __forceinline__ float add_lane8(float v) {
 // their V steps are set to 0, so what the cache holds past the length never reaches a sum. Output as k_attn_decode's.
 // Bound by latency at short lengths (8B shape, 32 splits, 778 positions 4.9 us: loads 1.0, one tile's chain 1.1, the waves'
 // join and the partials 0.9, the launch), and by the expansion's vector instructions at long ones: 32001 positions 11.9 us,
-// of which the loads alone, by the same pattern, take 8.6 (37 MB, 4.3 TB/s), against 22.4 for the fp16 cache's kernel.
+// of which the loads alone, by the same pattern, take 8.6 (37 MB, 4.3 TB/s), against 22.4 for the fp16 cache's kernel
+// (11.6 to 13 in a trace, where a launch starts on an idle card).
 template <int HD, int G, bool WIN, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void k_attn_decode_kv4(const float* __restrict__ q, const char* __restrict__ kcache,
                                                                 const char* __restrict__ vcache, uint32_t n_kv, uint32_t cap,

@@ -43,7 +43,10 @@ __global__ __launch_bounds__(64 * GB * KSPLIT) void k_attn_prefill_kv4(
     constexpr int NT = 64 * GB * KSPLIT, NB = HD / 32;
     constexpr int NKB = TK / 32 / KSPLIT;  // 32-key fragments of a tile per wave
     constexpr int NKW = TK * HD / 16 / NT; // pairs of words per thread and tile, of K and of V
-    constexpr int QP = QX2 ? 2 : 1;        // q planes; with split q the probabilities are split too
+    // q planes; with a split q the probabilities are split too. A caller who passes one plane has q in fp16 already: the
+    // probabilities are then rounded to it as well, 2^-11 of each (512 rows of the 1B shape: 2.5e-4 from the exact values,
+    // of which the fp16 output alone is 2.0e-4), for half the matrix work: 2048 rows at 6144 296 us, split 429.
+    constexpr int QP = QX2 ? 2 : 1;
     static_assert(G % GB == 0 && NKB >= 1 && NKB * KSPLIT * 32 == TK, "a tile's fragments divide over a head's waves");
     static_assert(NKW >= 1 && NKW * NT * 16 == TK * HD, "a tile's words divide over the block");
     __shared__ __attribute__((aligned(16))) vsl_half smem[4 * TK * HD];  // two buffers of K, two of V
@@ -688,7 +691,8 @@ void launch(hipStream_t s, const Args& a) {
 // block's threads divide a tile's words), or, while that leaves CUs idle, two heads with four waves each on tiles of 128 keys:
 // twice the blocks, half the tiles in a chain. Measured, split q unless said: blocks of several heads / of one, 8B shape
 // (head_dim 128, 4 heads a group) 128 rows 9.8 / 9.1 us, 45 rows at 3000 51.5 / 30.4, 250 rows at 500 23.2 / 15.2, 300 rows at
-// 1000 36.8 / 34.6, 400 rows 18.2 / 20.6, one plane 700 rows 23.0 / 29.2, 1B shape (64), one plane, 512 rows 10.8 / 13.3; four
+// 1000 36.8 / 34.6, behind longer caches (traced) 45 rows at 12000 206 / 92, 128 at 30000 503 / 226, 250 at 30000
+// 506 / 271; 400 rows 18.2 / 20.6, one plane 700 rows 23.0 / 29.2, 1B shape (64), one plane, 512 rows 10.8 / 13.3; four
 // heads a block / two: 1B shape, one plane, 512 rows 12.7 / 10.8.
 template <int HD, int G, bool QX2>
 void launch_group(hipStream_t s, const Args& a) {
