@@ -338,6 +338,47 @@ int vsl_qk_norm_rope_append_decode(const float* qkv, uint32_t n_q, uint32_t n_kv
                                    float* q_out, void* kcache, void* vcache, int kv_dtype, uint32_t cap, vsl_ctrl* ctrl,
                                    void* stream);
 
+/* Rotary tables of scaled frequencies (the reference knows theta alone, fused_matmul_rope.comp:48-81): entry [r][j] of
+ * rope_cos / rope_sin (fp32 [rows][rot/2]) is the cosine / sine of (pos0 + r) f_j, times the scale, with
+ *   f_j = theta^(-2 j / rot) / freq_factors[j]   (freq_factors fp32 [rot/2] in device memory; NULL: 1)
+ *   VSL_ROPE_SCALE_NONE    as it is
+ *   VSL_ROPE_SCALE_LINEAR  f_j / factor
+ *   VSL_ROPE_SCALE_TURNS   by the turns n_j = orig_ctx f_j / (2 pi): a f_j + (1 - a) f_j / factor with
+ *                          a = (n_j - low) / (high - low) within 0..1
+ *   VSL_ROPE_SCALE_YARN    by the pair's index: (1 - b) f_j + b f_j / factor with b = (j - lo) / max(hi - lo, 0.001) within
+ *                          0..1, lo = floor(c(high)), hi = ceil(c(low)), both within 0..rot - 1,
+ *                          c(n) = rot ln(orig_ctx / (2 pi n)) / (2 ln theta)
+ * The scale is mscale; with mscale = 0 it is 1, and for VSL_ROPE_SCALE_YARN with a factor above 1 0.1 ln(factor) + 1.
+ * Angles are computed in 64 bits.  rot even, up to 512; pos0 + rows <= 2^31. */
+enum { VSL_ROPE_SCALE_NONE = 0, VSL_ROPE_SCALE_LINEAR = 1, VSL_ROPE_SCALE_TURNS = 2, VSL_ROPE_SCALE_YARN = 3 };
+typedef struct vsl_rope_scaling { /* host memory, read during the call */
+    int32_t type;              /* VSL_ROPE_SCALE_* */
+    float theta, factor;       /* factor: not read without scaling */
+    float orig_ctx, low, high; /* TURNS, YARN: the first context's positions; turns from which / up to which scaling fades */
+    float mscale;
+} vsl_rope_scaling;
+int vsl_rope_tables(uint32_t rot, uint32_t pos0, uint32_t rows, const vsl_rope_scaling* scaling, const float* freq_factors,
+                    float* rope_cos, float* rope_sin, void* stream);
+
+/* vsl_qk_norm_rope_append without norms, for models that rotate the first `rot` dims of each head only (the others pass
+ * unchanged; rot = 0: none, tables unused) and for rows whose rotary position is not their place in the cache (packed
+ * documents): row s is appended at pos0 + s and rotated by the tables' row positions[s] (device memory; NULL: pos0 + s).
+ * VSL_ROPE_PAIRS rotates (2j, 2j + 1), VSL_ROPE_HALVES (j, j + rot/2), j < rot/2.  Tables [table_rows][rot/2]; a position
+ * at or past table_rows makes the row's rotated dims NaN.  head_dim a multiple of 8 up to 512, rot even; caches
+ * VSL_DT_F32 or VSL_DT_F16; pointers 16-byte aligned (positions 4); S rows of ceil((n_q + 2 n_kv) hd / 1024) blocks, at
+ * most 2^23 blocks a call.  32 bits, each output rounded once more if it has fewer. */
+int vsl_rope_part_append(const float* qkv, uint32_t S, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t rot, int rope,
+                         uint32_t pos0, const uint32_t* positions, const float* rope_cos, const float* rope_sin,
+                         uint32_t table_rows, void* q_out, int q_dtype, void* kcache, void* vcache, int kv_dtype,
+                         uint32_t cap, void* stream);
+/* The same for the one row of a decode step, at ctrl->pos (rotated by *position, device memory; NULL: ctrl->pos): q ->
+ * q_out fp32 [n_q * hd].  With ctrl->done nothing is written; a position past the capacity sets ctrl->done and
+ * ctrl->error instead. */
+int vsl_rope_part_append_decode(const float* qkv, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t rot, int rope,
+                                const uint32_t* position, const float* rope_cos, const float* rope_sin, uint32_t table_rows,
+                                float* q_out, void* kcache, void* vcache, int kv_dtype, uint32_t cap, vsl_ctrl* ctrl,
+                                void* stream);
+
 /* y[N] += W[N][K] x[K]  (O projection / FFN down projection with the residual add fused);
  * K % 8 == 0, K <= 32768 */
 int vsl_gemv_residual(const void* W, int wdtype, uint32_t N, uint32_t K, const float* x, float* resid,
@@ -369,6 +410,27 @@ uint32_t vsl_lm_head_ws_blocks(void);
  * exposed for the sampler parity tests.  out: one u32.  Sampler limits as above. */
 int vsl_sample_logits(const float* logits, uint32_t V, vsl_sampler sampler, uint64_t step,
                       uint32_t* out, void* stream);
+
+/* One token for each of `rows` rows of logits (fp32 or fp16, row r at logits + r * stride elements), by the row's own
+ * parameters and uniform number, both in device memory, so that a captured call serves changing ones.  With
+ * w_i = exp((l_i - max l) / temperature), the kept tokens are
+ *   the first top_k in the order (logit descending, index ascending)          top_k = 0 or past V: all
+ *   of those, in that order, the shortest run whose w reach top_p of their sum   top_p >= 1 or NaN: all
+ *   of those, the ones with w_i >= min_p                                      min_p <= 0 or NaN: all
+ * and always the first.  The token is the first one by index whose running sum of kept w exceeds u times their total; its
+ * share w / total goes to probs (may be NULL).  temperature <= 0 or NaN, top_k = 1, top_p <= 0 and min_p > 1 give the first
+ * maximum, with share 1.  u below 0 or NaN counts as 0, 1 and above as the largest float below 1.  NaN logits count as
+ * -infinity, +infinity as the largest float; a row of -infinity gives token 0 with share 0.  Weights below about 2^-91
+ * of the largest may count as 0.  Weights are summed in 64 bits.  V up to 2^20, up to 65535 rows; workspace 16-byte aligned,
+ * vsl_sample_rows_ws_bytes(rows, V) bytes (0 for sizes that are not served). */
+typedef struct vsl_row_sampler {
+    float temperature;
+    uint32_t top_k;
+    float top_p, min_p;
+} vsl_row_sampler;
+int vsl_sample_rows(const void* logits, int dtype, uint32_t rows, uint32_t V, uint64_t stride, const vsl_row_sampler* params,
+                    const float* u, uint32_t* tokens, float* probs, void* workspace, uint64_t ws_bytes, void* stream);
+uint64_t vsl_sample_rows_ws_bytes(uint32_t rows, uint32_t V);
 
 /* Host-side reset of the control block (device memory) for a new generation. */
 int vsl_ctrl_reset(vsl_ctrl* ctrl, uint32_t pos, uint32_t max_steps, uint32_t stop_on_eos,
@@ -477,6 +539,36 @@ int vsl_attn_prefill_kv4_window(const void* q, int q_dtype, const void* kcache, 
                                 uint32_t pos0, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t cap, float scale,
                                 void* out, int out_dtype, uint32_t window, uint32_t n_global, uint32_t threshold,
                                 void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Attention with modified scores (no reference counterpart).  With s_k = scale q.k over the keys k of the row at position p:
+ *   softcap > 0     s_k <- softcap tanh(s_k / softcap)
+ *   slopes          s_k <- s_k - slopes[head] |p - k|       (fp32 [n_q] in device memory; NULL: no bias)
+ *   ranges          the row attends to the keys begin <= k < end of its pair (uint32 [S][2] in device memory: packed
+ *                   documents, prefixes that see themselves whole, windows, padding; NULL: 0 <= k <= p)
+ * then softmax over the keys attended to.  `end` counts up to the positions that the call can know: pos0 + S in
+ * vsl_attn_prefill_mods, ctrl->pos + 1 in vsl_attn_decode_mods.  A row without keys gives zeros.  What masked
+ * positions hold, infinities and NaN among it, reaches no result; an infinity or a NaN among the values attended to makes
+ * the outputs that it reaches infinite or NaN.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct vsl_attn_mods { /* host memory, read during the call; NULL for the call: no modification */
+    float softcap;             /* 0: none */
+    uint32_t pad;
+    const float* slopes;
+    const uint32_t* ranges;
+} vsl_attn_mods;
+/* vsl_attn_decode with modified scores: arguments as there; caches VSL_DT_F16 or VSL_DT_F32, head_dim 64 or 128, any GQA
+ * ratio 1..8, 1..1024 splits; over fp16 caches |q| < 65504 (two fp16 planes); q, caches, part_o and out 16-byte, part_ml 8-byte aligned. */
+int vsl_attn_decode_mods(const float* q, const void* kcache, const void* vcache, int kv_dtype, uint32_t n_q, uint32_t n_kv,
+                         uint32_t hd, uint32_t cap, float scale, uint32_t nsplit, float* part_o, float* part_ml, float* out,
+                         vsl_ctrl* ctrl, const vsl_attn_mods* mods, void* stream);
+/* vsl_attn_prefill with modified scores: arguments as there, all pointers 16-byte aligned (slopes 4, ranges 8).  With a
+ * workspace of vsl_attn_prefill_mods_ws_bytes calls of few rows split the keys over more blocks and join their sums in
+ * a second launch; with less (NULL, 0) they run unsplit. */
+int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kcache, const void* vcache, uint32_t S, uint32_t pos0,
+                          uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t cap, float scale, void* out, int out_dtype,
+                          const vsl_attn_mods* mods, void* workspace, uint64_t ws_bytes, void* stream);
+uint64_t vsl_attn_prefill_mods_ws_bytes(uint32_t S, uint32_t pos0, uint32_t n_q, uint32_t n_kv, uint32_t hd);
 
 /* ------------------------------------------------------------------------------------------
  * hipGraph helpers (each decode step is captured once and replayed).  A replay is one operation on its stream: what

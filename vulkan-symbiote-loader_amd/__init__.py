@@ -25,6 +25,7 @@ VSL_DT_F32, VSL_DT_F16, VSL_DT_F16X2, VSL_DT_F16F8 = 0, 1, 2, 3
 VSL_DT_Q8_0, VSL_DT_Q4_0, VSL_DT_Q4_1 = 4, 5, 6  # resident block-quantized weight packs
 VSL_DT_KV4 = 7  # a KV cache in 4 bits
 ROPE_PAIRS, ROPE_HALVES = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_TURNS, ROPE_SCALE_YARN = 0, 1, 2, 3
 VSL_WF_F32, VSL_WF_F16, VSL_WF_Q4_0, VSL_WF_Q4_1, VSL_WF_Q8_0 = 0, 1, 2, 3, 4
 VSL_QL_REFERENCE, VSL_QL_GGML = 0, 1
 GEMM_A_X2, GEMM_C_X2, GEMM_A_F8, GEMM_C_F8 = 0x100, 0x200, 0x400, 0x800
@@ -96,6 +97,23 @@ class Sampler(ctypes.Structure):
 class Ctrl(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint32) for n in
                 ("pos", "step", "done", "stop_on_eos", "max_steps", "token", "capacity", "error")]
+
+
+class RopeScaling(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("theta", ctypes.c_float), ("factor", ctypes.c_float),
+                ("orig_ctx", ctypes.c_float), ("low", ctypes.c_float), ("high", ctypes.c_float),
+                ("mscale", ctypes.c_float)]
+
+
+class AttnMods(ctypes.Structure):
+    """slopes and ranges: device addresses or None."""
+    _fields_ = [("softcap", ctypes.c_float), ("pad", ctypes.c_uint32), ("slopes", ctypes.c_void_p),
+                ("ranges", ctypes.c_void_p)]
+
+
+class RowSampler(ctypes.Structure):
+    _fields_ = [("temperature", ctypes.c_float), ("top_k", ctypes.c_uint32), ("top_p", ctypes.c_float),
+                ("min_p", ctypes.c_float)]
 
 
 # model configurations named by the workloads they run
@@ -183,6 +201,18 @@ _HIP_SIGS = {
     "vsl_attn_prefill_kv4": (_I32, [_P, _I32, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _F32, _P, _I32, _P]),
     "vsl_attn_prefill_kv4_window": (_I32, [_P, _I32, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _F32, _P, _I32, _U32,
                                            _U32, _U32, _P]),
+    "vsl_rope_tables": (_I32, [_U32, _U32, _U32, ctypes.POINTER(RopeScaling), _P, _P, _P, _P]),
+    "vsl_rope_part_append": (_I32, [_P, _U32, _U32, _U32, _U32, _U32, _I32, _U32, _P, _P, _P, _U32, _P, _I32, _P, _P, _I32,
+                                    _U32, _P]),
+    "vsl_rope_part_append_decode": (_I32, [_P, _U32, _U32, _U32, _U32, _I32, _P, _P, _P, _U32, _P, _P, _P, _I32, _U32, _P,
+                                           _P]),
+    "vsl_attn_decode_mods": (_I32, [_P, _P, _P, _I32, _U32, _U32, _U32, _U32, _F32, _U32, _P, _P, _P, _P,
+                                    ctypes.POINTER(AttnMods), _P]),
+    "vsl_attn_prefill_mods": (_I32, [_P, _I32, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _F32, _P, _I32,
+                                     ctypes.POINTER(AttnMods), _P, _U64, _P]),
+    "vsl_attn_prefill_mods_ws_bytes": (_U64, [_U32, _U32, _U32, _U32, _U32]),
+    "vsl_sample_rows": (_I32, [_P, _I32, _U32, _U32, _U64, _P, _P, _P, _P, _P, _U64, _P]),
+    "vsl_sample_rows_ws_bytes": (_U64, [_U32, _U32]),
     "vsl_graph_begin": (_I32, [_P]),
     "vsl_graph_end": (_I32, [_P, ctypes.POINTER(_P)]),
     "vsl_graph_launch": (_I32, [_P, _P]),

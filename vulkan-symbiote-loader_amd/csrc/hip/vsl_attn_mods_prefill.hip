@@ -1,0 +1,551 @@
+// vsl_attn_mods_prefill.hip -- prompt attention with capped scores, a distance bias and a range of keys for each row
+// (vsl_attn_prefill_mods). No reference counterpart.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "vsl_attn_mods.h"
+#include "vsl_internal.h"
+
+using namespace attn_mods;
+
+namespace {
+
+constexpr int kTiles = 4;   // query tiles of a block: 32 rows of one head each
+constexpr int kShares = 2;  // waves of a query tile, each with one 32-key half of every key tile
+constexpr int kTK = 64, kBufs = 3, kThreads = 64 * kTiles * kShares;
+
+struct PrefillArgs {
+    const vsl_half* q;
+    const vsl_half* kc;
+    const vsl_half* vc;
+    uint32_t S, pos0, n_q, n_kv, cap, G, n_chunk;
+    float to_u;    // |scale| / softcap, or |scale| * log2(e) without a cap
+    float from_u;  // softcap * log2(e)
+    int negative;  // scale < 0: q is taken with the other sign
+    int out_mode;  // 0 fp16, 1 hi / lo fp16 planes, 2 fp16 + fp8 planes
+    const float* slopes;
+    const uint32_t* ranges;
+    vsl_half* out;
+    float* part_o;   // [n_chunk][S][n_q][HD], where the keys are split over blocks
+    float* part_ml;  // [n_chunk][S][n_q][2]
+};
+
+// row of D of a 32 x 32 product in register v
+__device__ __forceinline__ int d_row(int v, int lane) { return (v >> 2) * 8 + (lane >> 5) * 4 + (v & 3); }
+
+// o * inv (four consecutive dims of a head's row) as the output's type
+template <int HD>
+__device__ __forceinline__ void store4(const PrefillArgs& a, uint32_t s, uint32_t h, int dim, const float (&y)[4]) {
+    const size_t qw = (size_t)a.n_q * HD, plane = (size_t)a.S * qw, at = (size_t)s * qw + (size_t)h * HD + dim;
+    half4 hv, lv;
+    if (a.out_mode == 2) {
+        uint32_t lo8;
+        split4_f16_f8(y[0], y[1], y[2], y[3], hv, lo8);
+        *reinterpret_cast<half4*>(a.out + at) = hv;
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(a.out + plane) + (size_t)s * qw + lo8_pos(h * HD + dim)) = lo8;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        vsl_half hi, lo;
+        split_f16(y[i], hi, lo);
+        hv[i] = hi;
+        lv[i] = lo;
+    }
+    *reinterpret_cast<half4*>(a.out + at) = hv;
+    if (a.out_mode == 1) *reinterpret_cast<half4*>(a.out + plane + at) = lv;
+}
+
+// keys [lo, hi) of row s
+__device__ __forceinline__ void row_range(const PrefillArgs& a, uint32_t s, uint32_t& lo, uint32_t& hi) {
+    lo = 0;
+    hi = a.pos0 + s + 1;
+    if (a.ranges) {
+        const uint2 r = reinterpret_cast<const uint2*>(a.ranges)[s];
+        lo = r.x;
+        hi = min(r.y, a.pos0 + a.S);
+        if (lo >= hi) lo = hi = 0;
+    }
+}
+
+// The rows of a query tile over the keys k0 .. k1 - 1 without matrix products: a wave takes one row after the other, a lane a
+// key for the scores and HD / 64 dims for the sums, and multiplies no masked key's V. (A call: within the kernel it would cost
+// the tiles' loop 50 registers spilled.)
+template <int HD, bool QX2, bool CAP>
+__device__ __noinline__ void rows_one_by_one(const PrefillArgs& a, uint32_t rb, uint32_t h, uint32_t chunk, uint32_t k0, uint32_t k1) {
+    constexpr int D = HD / 64;
+    const uint32_t lane = threadIdx.x & 63, qw = a.n_q * HD, kvh = h / a.G;
+    const vsl_half* Kb = a.kc + (size_t)kvh * a.cap * HD;
+    const vsl_half* Vb = a.vc + (size_t)kvh * a.cap * HD;
+    const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.f;
+    for (uint32_t s = rb * 32; s < min(rb * 32 + 32, a.S); ++s) {
+        uint32_t lo, hi;
+        row_range(a, s, lo, hi);
+        lo = max(lo, k0);
+        hi = min(hi, k1);
+        const vsl_half* q = a.q + (size_t)s * qw + (size_t)h * HD;
+        float m = -INFINITY, l = 0.f, acc[D];
+#pragma unroll
+        for (int i = 0; i < D; ++i) acc[i] = 0.f;
+        for (uint32_t kb = lo; kb < hi; kb += 64) {
+            const uint32_t k = kb + lane;
+            float sc = 0.f;
+            if (k < hi) {
+                for (int d = 0; d < HD; ++d) {
+                    float x = (float)q[d];
+                    if constexpr (QX2) x += (float)q[(size_t)a.S * qw + d];
+                    sc = fmaf(a.negative ? -x : x, (float)Kb[(size_t)k * HD + d], sc);
+                }
+            }
+            sc *= a.to_u;
+            if constexpr (CAP) sc = tanh_any(sc) * a.from_u;
+            sc = fmaf(-slope, fabsf((float)((int)k - (int)(a.pos0 + s))), sc);
+            if (k >= hi) sc = -INFINITY;
+            const float mn = fmaxf(m, wave_max_dpp(sc)), ref = mn == -INFINITY ? 0.f : mn, corr = fast_exp2(m - ref);
+            const float w = fast_exp2(sc - ref);
+            l = fmaf(l, corr, wave_sum_dpp(w));
+            m = mn;
+#pragma unroll
+            for (int i = 0; i < D; ++i) acc[i] *= corr;
+            for (uint32_t j = 0; j < min(64u, hi - kb); ++j) {
+                const float wj = __shfl(w, (int)j, 64);
+#pragma unroll
+                for (int i = 0; i < D; ++i) acc[i] = fmaf(wj, (float)Vb[(size_t)(kb + j) * HD + 64 * i + lane], acc[i]);
+            }
+        }
+        if (m == -INFINITY && l != 0.f) m = 0.f;
+        if (a.n_chunk > 1) {
+            const size_t at = ((size_t)chunk * a.S + s) * a.n_q + h;
+#pragma unroll
+            for (int i = 0; i < D; ++i) a.part_o[at * HD + 64 * i + lane] = acc[i];
+            if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+            continue;
+        }
+        // four consecutive dims in every fourth lane, for the output's types
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = __shfl(acc[i], (int)((lane & ~3u) + j), 64) * inv;
+            if ((lane & 3) == 0) store4<HD>(a, s, h, 64 * i + (int)lane, y);
+        }
+    }
+}
+
+// Block: four query tiles (32 rows of one head) of one KV head, numbered row block by row block with the group's heads
+// within; two waves each, a wave the one 32-key half of every 64-key tile. Key tiles go from the cache straight into LDS
+// (three buffers, two tiles ahead), shared by the four query tiles. Per tile a wave takes S^T = K Q^T (its D: a lane has 16
+// keys of one row), turns the scores into probabilities, which are the operand of O^T += V^T P^T as they lie, and the next
+// tile's S^T is issued under this one's softmax. The halves are joined through LDS at the end.
+// A row's keys are a range [lo, hi); tiles that lie within the ranges of all of a wave's rows take no masks, and tiles
+// outside all of them are skipped. In the others a masked probability is 0; where V then holds an infinity or a NaN, whose
+// product with 0 would reach the sums, the query tile's rows are computed again, one by one (rows_one_by_one).
+template <int HD, bool QX2, bool CAP>
+__global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
+    constexpr int CPR = HD / 8, NCH = kTK * CPR / kThreads, QP = QX2 ? 2 : 1, ND = HD / 32;
+    static_assert(NCH >= 1 && kTK * CPR % kThreads == 0, "a tile divides over the block");
+    __shared__ __attribute__((aligned(16))) vsl_half Ks[kBufs][kTK * HD];
+    __shared__ __attribute__((aligned(16))) vsl_half Vs[kBufs][kTK * HD];
+    __shared__ uint32_t s_lo[kTiles * kShares], s_hi[kTiles * kShares];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // blocks in the order of their rows, the last (longest under the causal mask) first, KV heads next to each other
+    const uint32_t n_rb = (a.S + 31) / 32, n_qt = n_rb * a.G, n_grp = (n_qt + kTiles - 1) / kTiles;
+    const uint32_t kvh = blockIdx.x % a.n_kv, grp = n_grp - 1 - blockIdx.x / a.n_kv, chunk = blockIdx.y;
+    const uint32_t qt = grp * kTiles + wave / kShares;
+    const bool active = qt < n_qt;
+    const int share = wave % kShares;
+    const uint32_t rb = active ? qt / a.G : 0, h = kvh * a.G + (active ? qt % a.G : 0);
+    const uint32_t my_s = rb * 32 + (lane & 31), row = min(my_s, a.S - 1);  // rows past S are those of row S - 1, not stored
+    const uint32_t qw = a.n_q * HD;
+    const size_t qplane = (size_t)a.S * qw;
+    const uint32_t my_pos = a.pos0 + row;
+
+    // this row's keys [lo, lo + n); the wave's: within some row's and within all rows'
+    uint32_t lo, hi;
+    row_range(a, row, lo, hi);
+    uint32_t some_lo = hi > lo ? lo : 0xFFFFFFFFu, some_hi = hi, all_lo = hi > lo ? lo : 0xFFFFFFFFu, all_hi = hi;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {  // the two half waves hold the same rows
+        some_lo = min(some_lo, (uint32_t)__shfl_xor((int)some_lo, o, 64));
+        some_hi = max(some_hi, (uint32_t)__shfl_xor((int)some_hi, o, 64));
+        all_lo = max(all_lo, (uint32_t)__shfl_xor((int)all_lo, o, 64));
+        all_hi = min(all_hi, (uint32_t)__shfl_xor((int)all_hi, o, 64));
+    }
+    if (!active) {
+        some_lo = 0xFFFFFFFFu;
+        some_hi = 0;
+    }
+    some_lo = __builtin_amdgcn_readfirstlane(some_lo);
+    some_hi = __builtin_amdgcn_readfirstlane(some_hi);
+    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+    if (lane == 0) {
+        s_lo[wave] = some_lo;
+        s_hi[wave] = some_hi;
+    }
+    __syncthreads();
+    uint32_t blk_lo = 0xFFFFFFFFu, blk_hi = 0;
+#pragma unroll
+    for (int w = 0; w < kTiles * kShares; ++w) {
+        blk_lo = min(blk_lo, s_lo[w]);
+        blk_hi = max(blk_hi, s_hi[w]);
+    }
+    blk_lo = __builtin_amdgcn_readfirstlane(blk_lo);
+    blk_hi = __builtin_amdgcn_readfirstlane(blk_hi);
+    // the block's key tiles, or its chunk of them
+    uint32_t t0 = 0, t1 = 0;
+    if (blk_hi > blk_lo) {
+        t0 = blk_lo / kTK;
+        t1 = (blk_hi + kTK - 1) / kTK;
+        const uint32_t n = t1 - t0, per = n / a.n_chunk, rest = n % a.n_chunk;
+        t0 += chunk * per + min(chunk, rest);
+        t1 = t0 + per + (chunk < rest ? 1 : 0);
+    }
+
+    const vsl_half* Kb = a.kc + (size_t)kvh * a.cap * HD;
+    const vsl_half* Vb = a.vc + (size_t)kvh * a.cap * HD;
+    // Tile copy: LDS chunk i * kThreads + tid holds row r, and of it the chunk whose swizzled place that is. Positions past
+    // the block's keys read the last of them.
+    uint32_t coff[NCH];
+    int crow[NCH];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int P = i * kThreads + tid, r = P / CPR;
+        crow[i] = r;
+        coff[i] = (uint32_t)(swizzle<HD>(r, P % CPR) - r * HD);
+    }
+    auto issue = [&](int buf, uint32_t t) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const size_t at = (size_t)min(t * kTK + crow[i], blk_hi - 1) * HD + coff[i];
+            lds_load16(Kb + at, 0, &Ks[buf][(i * kThreads + wave * 64) * 8]);
+            lds_load16(Vb + at, 0, &Vs[buf][(i * kThreads + wave * 64) * 8]);
+        }
+    };
+
+    // Q^T as the B operand: lane holds row lane % 32, dims 16 c + 8 (lane / 32) ..
+    half8 qf[QP][HD / 16];
+#pragma unroll
+    for (int p = 0; p < QP; ++p)
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) {
+            qf[p][c] = *reinterpret_cast<const half8*>(a.q + p * qplane + (size_t)row * qw + (size_t)h * HD + c * 16 + (lane >> 5) * 8);
+            if (a.negative) qf[p][c] = -qf[p][c];
+        }
+    const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.f;
+    float16v o[ND];
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[t][v] = 0.f;
+    float m = -INFINITY, l = 0.f;
+
+    auto qk = [&](int buf, float16v& st) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) st[v] = 0.f;
+        half8 kf[HD / 16];
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c)
+            kf[c] = *reinterpret_cast<const half8*>(&Ks[buf][swizzle<HD>(share * 32 + (lane & 31), 2 * c + (lane >> 5))]);
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c)
+#pragma unroll
+            for (int p = 0; p < QP; ++p) st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[c], qf[p][c], st, 0, 0, 0);
+    };
+    // scores of tile t in log2 units, modified, masked where the tile is not within all rows' ranges
+    auto modify = [&](float16v& st, uint32_t t, bool whole) {
+        if constexpr (CAP) {
+            float um = 0.f;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                st[v] *= a.to_u;
+                um = fmaxf(um, fabsf(st[v]));
+            }
+            if (__builtin_amdgcn_ballot_w64(um > kTanhNear)) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) st[v] = tanh_any(st[v]) * a.from_u;
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) st[v] = tanh_near(st[v]) * a.from_u;
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) st[v] *= a.to_u;
+        }
+        const uint32_t k0 = t * kTK + share * 32;
+        if (a.slopes) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                st[v] = fmaf(-slope, fabsf((float)((int)(k0 + d_row(v, lane)) - (int)my_pos)), st[v]);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) st[v] = k0 + d_row(v, lane) - lo < hi - lo ? st[v] : -INFINITY;
+        }
+    };
+    auto raise = [&](const float16v& st) {
+        float bm = st[0];
+#pragma unroll
+        for (int v = 1; v < 16; ++v) bm = fmaxf(bm, st[v]);
+        if (__builtin_amdgcn_ballot_w64(bm - m > kLazy + kRoom)) {  // m = -inf: any finite score raises it
+            float a0, a1;
+            lane_pair<32>(bm, a0, a1);
+            const float mn = fmaxf(m, fmaxf(a0, a1) - kRoom);
+            const float corr = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+            l *= corr;
+#pragma unroll
+            for (int t = 0; t < ND; ++t)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[t][v] *= corr;
+            m = mn;
+        }
+    };
+    auto probs = [&](const float16v& st, half8 (&pf)[QP][2]) {
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int v = 0; v < 16; v += 2) {
+            const float p0 = fast_exp2(st[v] - ref), p1 = fast_exp2(st[v + 1] - ref);
+            l += p0;
+            l += p1;
+            const half2v hi2 = round2(p0, p1);
+            pf[0][v >> 3][v & 7] = hi2[0];
+            pf[0][v >> 3][(v & 7) + 1] = hi2[1];
+            if constexpr (QX2) {
+                const half2v lo2 = round2(p0 - (float)hi2[0], p1 - (float)hi2[1]);
+                pf[QP - 1][v >> 3][v & 7] = lo2[0];
+                pf[QP - 1][v >> 3][(v & 7) + 1] = lo2[1];
+            }
+        }
+    };
+    // V^T operand of dims 32 tt .., keys 16 half ..: slots of P^T are the keys (v / 4) 8 + (lane / 32) 4 + v % 4, which the
+    // transpose reads match: lane i of 16 addresses V[r0 + i / 4][d0 + 4 (i % 4) ..] and receives V[r0 + j][d0 + i] as value j
+    const int gi = lane & 15, gdim = ((lane >> 4) & 1) * 16 + 4 * (gi & 3);
+    auto v_frag = [&](int buf, int tt, int half) {
+        const int d = tt * 32 + gdim, r = share * 32 + half * 16 + (lane >> 5) * 4 + (gi >> 2);
+        const half4 x0 = lds_read_tr16(&Vs[buf][swizzle<HD>(r, d >> 3) + (d & 7)]);
+        const half4 x1 = lds_read_tr16(&Vs[buf][swizzle<HD>(r + 8, d >> 3) + (d & 7)]);
+        return half8{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+    };
+    auto pv = [&](int buf, const half8 (&pf)[QP][2]) {
+#pragma unroll
+        for (int tt = 0; tt < ND; ++tt)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const half8 af = v_frag(buf, tt, half);
+#pragma unroll
+                for (int p = 0; p < QP; ++p) o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af, pf[p][half], o[tt], 0, 0, 0);
+            }
+    };
+    // infinities and NaN in this wave's half of the tile's V
+    uint32_t odd = 0;
+    auto note_odd = [&](int buf) {
+#pragma unroll 1
+        for (int tt = 0; tt < ND; ++tt)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const u32x4 w = __builtin_bit_cast(u32x4, v_frag(buf, tt, half));
+                odd |= odd_halfs(w[0]) | odd_halfs(w[1]) | odd_halfs(w[2]) | odd_halfs(w[3]);
+            }
+        asm volatile("" ::: "memory");  // the products read V again: nothing of it is kept in registers here
+    };
+
+    // Tiles t and t + 1 are in LDS and the scores of t in registers at the top of iteration t; t + 2 goes where t - 1 was.
+    // Each wave waits for its own copies, then the block meets: all copies have landed and all waves are done with buffer t.
+    if (t1 > t0) {
+        auto buf_of = [&](uint32_t t) { return (int)((t - t0) % kBufs); };
+        issue(0, t0);
+        issue(1, min(t0 + 1, t1 - 1));
+        VSL_VMCNT_WAIT(0);
+        __syncthreads();
+        float16v st;
+        qk(0, st);
+        for (uint32_t t = t0; t < t1; ++t) {
+            issue(buf_of(t + 2), min(t + 2, t1 - 1));
+            const uint32_t k0 = t * kTK + share * 32;
+            const bool any = k0 < some_hi && k0 + 32 > some_lo, whole = k0 >= all_lo && k0 + 32 <= all_hi;  // wave-uniform
+            if (any && whole) {
+                float16v sn;
+                modify(st, t, true);
+                raise(st);
+                qk(buf_of(t + 1), sn);
+                half8 pf[QP][2];
+                probs(st, pf);
+                pv(buf_of(t), pf);
+                st = sn;
+            } else {
+                if (any) {
+                    modify(st, t, false);
+                    raise(st);
+                    half8 pf[QP][2];
+                    probs(st, pf);
+                    note_odd(buf_of(t));
+                    pv(buf_of(t), pf);
+                }
+                qk(buf_of(t + 1), st);
+            }
+            VSL_VMCNT_WAIT(0);
+            __syncthreads();
+        }
+    }
+    // a row's weights lie in two lanes
+    {
+        float a0, a1;
+        lane_pair<32>(l, a0, a1);
+        l = a0 + a1;
+        if (m == -INFINITY && l != 0.f) m = 0.f;  // only NaN scores: keep the sum in the join
+    }
+    // the halves of each query tile joined: the second leaves its sums in the tile buffers (every read and copy is over)
+    const bool any_odd = __builtin_amdgcn_ballot_w64(odd != 0) != 0;
+    constexpr int OSZ = ND * 16 * 64, SLOT = OSZ + 128;
+    static_assert(kTiles / 2 * SLOT * 4 <= kBufs * kTK * HD * 2, "two query tiles' sums in each set of buffers");
+    {
+        const int w = wave / kShares;
+        float* x = reinterpret_cast<float*>(w < kTiles / 2 ? &Ks[0][0] : &Vs[0][0]) + (w % (kTiles / 2)) * SLOT;
+        if (share) {
+#pragma unroll
+            for (int t = 0; t < ND; ++t)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) x[(t * 16 + v) * 64 + lane] = o[t][v];
+            x[OSZ + lane] = m;
+            x[OSZ + 64 + lane] = l;
+            if (lane == 0) s_lo[wave] = any_odd;
+        }
+        __syncthreads();
+        if (share) return;
+        if (any_odd || s_lo[wave + 1]) {
+            if (active) rows_one_by_one<HD, QX2, CAP>(a, rb, h, chunk, t0 * kTK, t1 * kTK);
+            return;
+        }
+        const float mb = x[OSZ + lane], mm = fmaxf(m, mb), ref = mm == -INFINITY ? 0.f : mm;
+        const float ca = fast_exp2(m - ref), cb = fast_exp2(mb - ref);
+        l = l * ca + x[OSZ + 64 + lane] * cb;
+        m = mm;
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[t][v] = o[t][v] * ca + x[(t * 16 + v) * 64 + lane] * cb;
+    }
+    if (!active || my_s >= a.S) return;
+    if (a.n_chunk > 1) {
+        const size_t at = ((size_t)chunk * a.S + my_s) * a.n_q + h;
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+            for (int v = 0; v < 16; v += 4)
+                *reinterpret_cast<float4v*>(a.part_o + at * HD + t * 32 + d_row(v, lane)) = float4v{o[t][v], o[t][v + 1], o[t][v + 2], o[t][v + 3]};
+        if (lane < 32) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; v += 4) {
+            const float y[4] = {o[t][v] * inv, o[t][v + 1] * inv, o[t][v + 2] * inv, o[t][v + 3] * inv};
+            store4<HD>(a, my_s, h, t * 32 + d_row(v, lane), y);
+        }
+}
+
+// The chunks' sums of a row and head joined: HD / 4 lanes each.
+template <int HD>
+__global__ __launch_bounds__(256) void k_join_prefill(PrefillArgs a) {
+    constexpr uint32_t LPR = HD / 4;
+    const uint64_t at = (uint64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR, n = (uint64_t)a.S * a.n_q;
+    if (at >= n) return;
+    const int dim = threadIdx.x % LPR * 4;
+    float M = -INFINITY;
+    for (uint32_t c = 0; c < a.n_chunk; ++c) M = fmaxf(M, a.part_ml[(c * n + at) * 2]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float L = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t c = 0; c < a.n_chunk; ++c) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (c * n + at) * 2);
+        const float4v v = *reinterpret_cast<const float4v*>(a.part_o + (c * n + at) * HD + dim);
+        const float f = fast_exp2(ml.x - ref);
+        L = fmaf(ml.y, f, L);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = fmaf(v[i], f, y[i]);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] *= inv;
+    store4<HD>(a, (uint32_t)(at / a.n_q), (uint32_t)(at % a.n_q), dim, y);
+}
+
+uint32_t blocks_of(uint32_t S, uint32_t n_q, uint32_t n_kv) {
+    const uint64_t n_qt = (uint64_t)((S + 31) / 32) * (n_q / n_kv);
+    return (uint32_t)((n_qt + kTiles - 1) / kTiles * n_kv);
+}
+
+// Key chunks: as many as fill the CUs, none shorter than four tiles of the longest rows.
+uint32_t chunks_of(uint32_t S, uint32_t pos0, uint32_t n_q, uint32_t n_kv) {
+    const uint64_t blocks = blocks_of(S, n_q, n_kv), tiles = ((uint64_t)pos0 + S + kTK - 1) / kTK;
+    if (blocks >= 256) return 1;
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({256 / blocks, tiles / 4, 32}));
+}
+
+bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+}  // namespace
+
+extern "C" uint64_t vsl_attn_prefill_mods_ws_bytes(uint32_t S, uint32_t pos0, uint32_t n_q, uint32_t n_kv, uint32_t hd) {
+    if (S == 0 || n_kv == 0 || n_q == 0 || n_q % n_kv || (hd != 64 && hd != 128)) return 0;
+    const uint64_t c = chunks_of(S, pos0, n_q, n_kv);
+    return c > 1 ? c * S * n_q * (hd + 2) * 4 : 0;
+}
+
+extern "C" int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kcache, const void* vcache, uint32_t S,
+                                     uint32_t pos0, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t cap, float scale,
+                                     void* out, int out_dtype, const vsl_attn_mods* mods, void* workspace, uint64_t ws_bytes,
+                                     void* stream) {
+    const char* fn = "vsl_attn_prefill_mods";
+    if (!q || !kcache || !vcache || !out) return vsl_invalid("%s: null pointer", fn);
+    if (n_kv == 0 || n_q == 0 || n_q % n_kv) return vsl_invalid("%s: n_q=%u not a multiple of n_kv=%u", fn, n_q, n_kv);
+    if ((q_dtype != VSL_DT_F16 && q_dtype != VSL_DT_F16X2) ||
+        (out_dtype != VSL_DT_F16 && out_dtype != VSL_DT_F16X2 && out_dtype != VSL_DT_F16F8))
+        return vsl_unsupported("%s: dtypes %d/%d", fn, q_dtype, out_dtype);
+    if (hd != 64 && hd != 128) return vsl_unsupported("%s: head_dim %u (64 or 128)", fn, hd);
+    const uint32_t G = n_q / n_kv;
+    if (G > 8) return vsl_unsupported("%s: GQA ratio %u (supported 1..8)", fn, G);
+    if (cap > 0x7FFFFFFFu) return vsl_invalid("%s: capacity %u", fn, cap);
+    if ((uint64_t)pos0 + S > cap) return vsl_capacity("%s: %u positions from %u exceed capacity %u", fn, S, pos0, cap);
+    for (const void* p : {q, kcache, vcache, static_cast<const void*>(out), static_cast<const void*>(workspace)})
+        if (!aligned_to(p, 16)) return vsl_invalid("%s: pointers must be 16-byte aligned", fn);
+    const vsl_attn_mods none{};
+    const vsl_attn_mods& md = mods ? *mods : none;
+    if (!aligned_to(md.slopes, 4) || !aligned_to(md.ranges, 8)) return vsl_invalid("%s: misaligned pointer", fn);
+    if (!(md.softcap >= 0.f) || md.softcap == INFINITY) return vsl_invalid("%s: softcap %g", fn, (double)md.softcap);
+    if (S == 0) return VSL_OK;
+    const uint64_t blocks = ((uint64_t)((S + 31) / 32) * G + kTiles - 1) / kTiles * n_kv;
+    if (blocks > 1u << 23 || (uint64_t)S * n_q > 1u << 26) return vsl_unsupported("%s: %u rows in one call", fn, S);
+    const bool capped = md.softcap > 0.f;
+    const float mag = std::fabs(scale);
+    uint32_t chunks = workspace ? chunks_of(S, pos0, n_q, n_kv) : 1;
+    if (chunks > 1 && ws_bytes < (uint64_t)chunks * S * n_q * (hd + 2) * 4) chunks = 1;
+    PrefillArgs a{static_cast<const vsl_half*>(q), static_cast<const vsl_half*>(kcache), static_cast<const vsl_half*>(vcache),
+                  S, pos0, n_q, n_kv, cap, G, chunks, capped ? mag / md.softcap : mag * kLog2e, md.softcap * kLog2e, scale < 0.f,
+                  out_dtype == VSL_DT_F16X2 ? 1 : out_dtype == VSL_DT_F16F8 ? 2 : 0, md.slopes, md.ranges,
+                  static_cast<vsl_half*>(out), static_cast<float*>(workspace),
+                  static_cast<float*>(workspace) + (size_t)chunks * S * n_q * hd};
+    const dim3 grid((uint32_t)blocks, chunks);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    auto go = [&](auto hdc, auto x2, auto cc) {
+        constexpr int HD = decltype(hdc)::value;
+        k_prefill_mods<HD, decltype(x2)::value, decltype(cc)::value><<<grid, kThreads, 0, s>>>(a);
+        if (chunks > 1) k_join_prefill<HD><<<(uint32_t)(((uint64_t)S * n_q + 1024 / HD - 1) / (1024 / HD)), 256, 0, s>>>(a);
+    };
+    auto pick = [&](auto hdc) {
+        if (q_dtype == VSL_DT_F16X2) {
+            if (capped) go(hdc, std::true_type{}, std::true_type{});
+            else go(hdc, std::true_type{}, std::false_type{});
+        } else {
+            if (capped) go(hdc, std::false_type{}, std::true_type{});
+            else go(hdc, std::false_type{}, std::false_type{});
+        }
+    };
+    if (hd == 128) pick(std::integral_constant<int, 128>{});
+    else pick(std::integral_constant<int, 64>{});
+    HIP_TRY(hipGetLastError());
+    return VSL_OK;
+}
