@@ -8,16 +8,18 @@
 // index. Weights are summed in 64 bits (fixed point where atomics add them, so that no order of arrival matters): the
 // token is that of exact sums but where u falls within about 1e-12 of a border.
 //
-// Two launches. k_rows_scan reads the row's slices (a block each) once and leaves, by what the row asks for,
+// Three launches. k_rows_scan reads the row's slices (a block each) once and leaves, by what the row asks for,
 //   GREEDY  the slice's maximum
 //   TOPK    (k <= kLeanK) the slice's tokens that can be among the k largest: at least k of them lie at or above the k-th
 //           largest of the block's per-thread maxima
 //   SUM     (no cut but min-p) the maximum
 //   HIST    (top-p, or a larger k) counts and weights by bins of 1/8 in l / T, whose grid is the same for every slice, so
 //           that no slice has to know the row's maximum
-// k_rows_pick ends GREEDY and TOPK rows in one block; for SUM its blocks sum the kept weights of the slices, for HIST they
-// collect the tokens of the bins in which a cut falls, and the last block to arrive draws. Where ties or ranges make a
-// list too long, that block narrows the cuts down over the whole row instead.
+// k_rows_cut ends GREEDY and TOPK rows in one block; for SUM its blocks sum the kept weights of the slices, for HIST each
+// joins the slices' bins, which tells in which bins a cut falls, and collects its tokens of those. k_rows_draw, a block a
+// row, finds the cuts among the collected tokens, the slice in which u falls and the token there. Where ties or ranges make
+// a list too long, it narrows the cuts down over the whole row instead. (The last block of the second kernel to arrive
+// took the draw at first: its fences write the L2 caches back, and a pass over one row of 131072 took 66 us.)
 #include <float.h>
 
 #include <cmath>
@@ -27,12 +29,14 @@
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr uint32_t kMaxSlices = 128, kMaxEpt = 8;
+constexpr int kThreads = 256, kDrawThreads = 1024;
+constexpr uint32_t kMaxSlices = 128, kMaxEpt = 32;
 constexpr uint32_t kMaxRowsV = kMaxSlices * kMaxEpt * kThreads;  // 2^20 tokens
-constexpr uint32_t kLeanK = 256;   // TOPK up to this k
-constexpr uint32_t kLeanCap = 512;  // tokens a slice's list holds
-constexpr uint32_t kListCap = 4096;  // tokens a row's list holds, in LDS too
+constexpr uint32_t kLeanK = 128;     // TOPK up to this k
+constexpr uint32_t kLeanCap = 256;   // TOPK: tokens a slice's list holds
+constexpr int kLeanRegs = 4, kDrawRegs = 8;  // tokens of a list that a thread holds
+constexpr uint32_t kLeanList = kLeanRegs * kThreads, kListCap = kDrawRegs * kDrawThreads;  // tokens of a row's list
+constexpr uint32_t kFinish = 256;    // keys that are left to a key a thread
 constexpr uint32_t kBins = 512;     // of 1/8 in l / T; the last one takes all below e^-63.9 of the largest, never drawn
 constexpr double kBinSpan = 0.11751;  // above 1 - exp(-1/8), the most that a weight lies below its bin's upper edge
 constexpr int kBinFrac = 36;        // weights in a bin: what they lie below it, in units of 2^-36
@@ -42,7 +46,7 @@ constexpr int kCountShift = 46;     // 8192 of them stay below 2^46; the count a
 // below it, a draw has passed a border a little above it.
 constexpr double kBinNoise = 4e-11;
 constexpr double kMaxTop = 16384.0;  // l / T up to which the grid's rounding (2^-39) is far below a weight's
-constexpr double kListOne = 0x1p50, kRowOne = 0x1p42;  // fixed point of weights in lists (<= 2^13 tokens) and rows (<= 2^20)
+constexpr double kListOne = 0x1p48, kRowOne = 0x1p42;  // fixed point of weights in lists (<= 2^15 tokens) and rows (<= 2^20)
 
 enum { MODE_GREEDY = 0, MODE_TOPK = 1, MODE_SUM = 2, MODE_HIST = 3 };
 
@@ -69,16 +73,25 @@ __device__ __forceinline__ RowParams row_params(const vsl_row_sampler& s, uint32
 
 struct SliceRec {
     uint64_t top;     // the largest rank key (0: nothing above -inf)
-    uint32_t count;   // TOPK: tokens found (kLeanCap of them stored)
+    uint32_t count;   // TOPK: tokens found (kLeanCap of them stored); HIST: bins up to the last one that holds a token
     float floor_v;    // TOPK: all tokens of the slice at or above this value are in its list, and there are k of them (-inf: all)
-    double sum;       // SUM: kept weights
+    double sum;       // weights kept for sure
     uint64_t pad;
+};
+
+struct RowRec {
+    uint32_t kb, plo, phi, sure;  // HIST: the bin of the k-th token, those in which the top-p cut can fall, those kept whole
+    uint32_t cut_k, k_left;       // whether k ends within its bin, and how many of that bin's tokens count
+    double lo_total, hi_total;    // the first k tokens' weights, without and with the k-th's bin
+    uint32_t whole, pad;          // TOPK: the lists do not hold the tokens
+    double cum_w[kBins];          // HIST: weights up to and with each bin
 };
 
 struct Work {
     SliceRec* rec;       // [rows][nsl]
-    uint32_t* counters;  // [rows][2]: the row list's length, blocks that have arrived
-    uint64_t* lists;     // [rows][max(nsl * kLeanCap, kListCap)]
+    RowRec* row;         // [rows]
+    uint32_t* counters;  // [rows]: the row list's length
+    uint64_t* lists;     // [rows][list_stride]
     uint64_t* hist;      // [rows][nsl][kBins]
     uint32_t list_stride;
 };
@@ -100,187 +113,240 @@ __device__ __forceinline__ float value_of(uint64_t rank) {
 }
 __device__ __forceinline__ uint32_t index_of(uint64_t rank) { return ~(uint32_t)rank; }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
-    return (uint64_t)__shfl_xor((uint32_t)(v >> 32), m, 64) << 32 | __shfl_xor((uint32_t)v, m, 64);
+// Waves: scans and reductions of 64-bit values by DPP lane moves (rows of 16 by shifts, then row 0 into 1, 2 into 3, and both
+// into the upper half); lanes that a move does not reach read 0.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_move64(uint64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+    return (uint64_t)hi << 32 | lo;
 }
+template <class T, class Op>
+__device__ __forceinline__ T wave_steps(T v, Op op) {
+    auto step = [&](auto ctrl, auto rows) {
+        v = op(v, __builtin_bit_cast(T, dpp_move64<decltype(ctrl)::value, decltype(rows)::value>(__builtin_bit_cast(uint64_t, v))));
+    };
+    using std::integral_constant;
+    step(integral_constant<int, 0x111>(), integral_constant<int, 0xF>());  // row_shr:1
+    step(integral_constant<int, 0x112>(), integral_constant<int, 0xF>());
+    step(integral_constant<int, 0x114>(), integral_constant<int, 0xF>());
+    step(integral_constant<int, 0x118>(), integral_constant<int, 0xF>());
+    step(integral_constant<int, 0x142>(), integral_constant<int, 0xA>());  // row_bcast:15 into rows 1 and 3
+    step(integral_constant<int, 0x143>(), integral_constant<int, 0xC>());  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+template <class T>
+__device__ __forceinline__ T last_lane(T v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 63);
+    return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {  // inclusive
+    return wave_steps(v, [](T a, T b) { return a + b; });
+}
+template <class T>
+__device__ __forceinline__ T wave_add(T v) { return last_lane(wave_scan(v)); }
 __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        const uint64_t x = shfl_xor64(v, o);
-        v = x > v ? x : v;
-    }
-    return v;
+    return last_lane(wave_steps(v, [](uint64_t a, uint64_t b) { return a > b ? a : b; }));
 }
-template <class T>
-__device__ __forceinline__ T wave_add(T v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __builtin_bit_cast(T, shfl_xor64(__builtin_bit_cast(uint64_t, v), o));
-    return v;
-}
-// Inclusive sum over the wave's lanes below and at this one.
-template <class T>
-__device__ __forceinline__ T wave_scan(T v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t b = __builtin_bit_cast(uint64_t, v);
-        const uint64_t x = (uint64_t)__shfl_up((uint32_t)(b >> 32), o, 64) << 32 | __shfl_up((uint32_t)b, o, 64);
-        if (lane >= o) v += __builtin_bit_cast(T, x);
-    }
-    return v;
+__device__ __forceinline__ uint64_t wave_or64(uint64_t v) {
+    return last_lane(wave_steps(v, [](uint64_t a, uint64_t b) { return a | b; }));
 }
 
+struct Keyed {
+    uint64_t key, weight;
+};
 struct Shared {
-    uint64_t red[kWaves + 1];
+    uint64_t red[2 * kDrawThreads / 64];
     uint64_t digits[256];
     uint32_t counts[256];
+    __attribute__((aligned(16))) Keyed keyed[kFinish];
     uint64_t sel_key, sel_left;
-    uint32_t sel_count, sel_done;
+    uint32_t sel_count, n;
 };
 
 // Block-wide sums, maxima and scans of 64-bit values, every thread ending with the result. All threads call.
-template <class T>
-__device__ T block_add(Shared& sh, T v) {
+template <int NT, class T>
+__device__ __forceinline__ T block_add(Shared& sh, T v) {
     v = wave_add(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = __builtin_bit_cast(uint64_t, v);
     __syncthreads();
     T s = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) s += __builtin_bit_cast(T, sh.red[w]);
+    for (int w = 0; w < NT / 64; ++w) s += __builtin_bit_cast(T, sh.red[w]);
     return s;
 }
-__device__ uint64_t block_max64(Shared& sh, uint64_t v) {
-    v = wave_max64(v);
+// Two maxima at once.
+template <int NT>
+__device__ __forceinline__ void block_max2(Shared& sh, uint64_t& a, uint64_t& b) {
+    a = wave_max64(a);
+    b = wave_max64(b);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) {
+        sh.red[threadIdx.x >> 6] = a;
+        sh.red[NT / 64 + (threadIdx.x >> 6)] = b;
+    }
     __syncthreads();
-    uint64_t s = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) s = sh.red[w] > s ? sh.red[w] : s;
-    return s;
+    for (int w = 0; w < NT / 64; ++w) {
+        a = sh.red[w] > a ? sh.red[w] : a;
+        b = sh.red[NT / 64 + w] > b ? sh.red[NT / 64 + w] : b;
+    }
 }
-template <class T>
-__device__ T block_scan(Shared& sh, T v) {
+// Inclusive scan; `total`: the sum over the block.
+template <int NT, class T>
+__device__ __forceinline__ T block_scan(Shared& sh, T v, T& total) {
     v = wave_scan(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 63) sh.red[threadIdx.x >> 6] = __builtin_bit_cast(uint64_t, v);
     __syncthreads();
     const int wave = threadIdx.x >> 6;
     T before = 0;
+    total = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-        if (w < wave) before += __builtin_bit_cast(T, sh.red[w]);
+    for (int w = 0; w < NT / 64; ++w) {
+        const T x = __builtin_bit_cast(T, sh.red[w]);
+        if (w < wave) before += x;
+        total += x;
+    }
     return before + v;
 }
 
 // The last key of the shortest run of keys, in descending order, whose measures reach `target` (the smallest key of all if
-// they do not). src(i, key, measure) for i < n: false where the element takes no part; measure is an integer, keys differ.
-// Digits of 8 bits from the highest bit in which keys differ; ends early when a digit holds one key. All threads call;
-// 0 without elements.
-template <class Src>
-__device__ uint64_t select_key(Shared& sh, uint32_t n, uint64_t target, Src src) {
+// they do not). visit(f) calls f(rank) for each of the thread's elements; map(rank, key, measure) is false where one takes no
+// part; measures are integers, keys differ and are not 0. `n` bounds the elements that take part. Narrowed down by
+// digits of 8 bits, from the highest bit in which keys differ, until kFinish keys are left, whose threads sum up the
+// measures before their own. All threads call; 0 without elements.
+template <int NT, class Visit, class Map>
+__device__ __forceinline__ uint64_t select_key(Shared& sh, uint32_t n, uint64_t target, Visit visit, Map map) {
     const uint32_t t = threadIdx.x;
-    uint64_t all_or = 0, all_and = ~0ull;
-    for (uint32_t i = t; i < n; i += kThreads) {
-        uint64_t key, w;
-        if (src(i, key, w)) {
-            all_or |= key;
-            all_and &= key;
-        }
-    }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        all_or |= shfl_xor64(all_or, o);
-        all_and &= shfl_xor64(all_and, o);
-    }
-    __syncthreads();
-    if ((t & 63) == 0) {
-        sh.digits[t >> 6] = all_or;
-        sh.digits[kWaves + (t >> 6)] = all_and;
-    }
-    __syncthreads();
-    all_or = 0;
-    all_and = ~0ull;
-    for (int w = 0; w < kWaves; ++w) {
-        all_or |= sh.digits[w];
-        all_and &= sh.digits[kWaves + w];
-    }
-    __syncthreads();
-    if (all_or == 0) return 0;
-    const uint64_t diff = all_or ^ all_and;  // keys that differ somewhere (one key: none)
-    if (diff == 0) return all_or;
-    const int top = 64 - __builtin_clzll(diff);  // bits 0 .. top - 1 differ
-    int shift = top > 8 ? top - 8 : 0;
-    uint64_t prefix = top >= 64 ? 0 : all_and >> top << top, mask = top >= 64 ? 0 : ~0ull << top;
-    for (;;) {
-        for (uint32_t i = t; i < 256; i += kThreads) {
-            sh.digits[i] = 0;
-            sh.counts[i] = 0;
-        }
-        __syncthreads();
-        for (uint32_t i = t; i < n; i += kThreads) {
+    uint64_t prefix = 0, mask = 0;
+    if (n > kFinish) {
+        uint64_t all_or = 0, none_or = 0;  // bits that some key has, that some key lacks
+        visit([&](uint64_t rank) {
             uint64_t key, w;
-            if (src(i, key, w) && (key & mask) == prefix) {
-                const uint32_t d = (uint32_t)(key >> shift) & 255u;
-                atomicAdd(reinterpret_cast<unsigned long long*>(&sh.digits[d]), (unsigned long long)w);
-                atomicAdd(&sh.counts[d], 1u);
+            if (map(rank, key, w)) {
+                all_or |= key;
+                none_or |= ~key;
             }
+        });
+        all_or = wave_or64(all_or);
+        none_or = wave_or64(none_or);
+        __syncthreads();
+        if ((t & 63) == 0) {
+            sh.red[t >> 6] = all_or;
+            sh.red[NT / 64 + (t >> 6)] = none_or;
         }
         __syncthreads();
-        if (t < 64) {  // lane t: digits 255 - 4 t .. 252 - 4 t, descending
-            uint64_t d4[4], s = 0;
-            uint32_t c4[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                d4[j] = sh.digits[255 - 4 * t - j];
-                c4[j] = sh.counts[255 - 4 * t - j];
-                s += d4[j];
-            }
-            const uint64_t incl = wave_scan(s);
-            uint64_t run = incl - s;
-            int hit = -1, last = -1;
-            uint64_t left = target, last_run = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (c4[j]) {
-                    last = j;
-                    last_run = run;
-                }
-                if (hit < 0 && c4[j] && run + d4[j] >= target) {
-                    hit = j;
-                    left = target - run;
-                }
-                run += d4[j];
-            }
-            const uint64_t reach = __builtin_amdgcn_ballot_w64(hit >= 0), some = __builtin_amdgcn_ballot_w64(last >= 0);
-            const bool none = reach == 0;  // the sums fall short of the target: the smallest key
-            const int who = none ? 63 - __builtin_clzll(some) : __builtin_ctzll(reach);
-            if ((int)t == who) {
-                const int j = none ? last : hit;
-                sh.sel_left = none ? (target > last_run ? target - last_run : 0) : left;
-                sh.sel_key = 255 - 4 * t - j;
-                sh.sel_count = c4[j == 0 ? 0 : j == 1 ? 1 : j == 2 ? 2 : 3];
-            }
+        for (int w = 0; w < NT / 64; ++w) {
+            all_or |= sh.red[w];
+            none_or |= sh.red[NT / 64 + w];
         }
-        __syncthreads();
-        prefix |= sh.sel_key << shift;
-        mask |= 255ull << shift;
-        target = sh.sel_left;
-        const uint32_t count = sh.sel_count;
-        __syncthreads();
-        if (count == 1 || shift == 0) break;
-        shift = shift > 8 ? shift - 8 : 0;
+        const uint64_t diff = all_or & none_or;
+        if (diff == 0) return all_or;              // one key, or none
+        const int top = 64 - __builtin_clzll(diff);  // bits 0 .. top - 1 differ
+        int shift = top > 8 ? top - 8 : 0;
+        if (top < 64) {
+            mask = ~0ull << top;
+            prefix = all_or & mask;
+        }
+        for (;;) {
+            __syncthreads();
+            if (t < 256) {
+                sh.digits[t] = 0;
+                sh.counts[t] = 0;
+            }
+            __syncthreads();
+            visit([&](uint64_t rank) {
+                uint64_t key, w;
+                if (map(rank, key, w) && (key & mask) == prefix) {
+                    const uint32_t d = (uint32_t)(key >> shift) & 255u;
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&sh.digits[d]), (unsigned long long)w);
+                    atomicAdd(&sh.counts[d], 1u);
+                }
+            });
+            __syncthreads();
+            if (t < 64) {  // lane t: digits 255 - 4 t .. 252 - 4 t, descending
+                uint64_t d4[4], s = 0;
+                uint32_t c4[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    d4[j] = sh.digits[255 - 4 * t - j];
+                    c4[j] = sh.counts[255 - 4 * t - j];
+                    s += d4[j];
+                }
+                uint64_t run = wave_scan(s) - s, left = 0, last_left = 0;
+                uint32_t hit = 0, last = 0, hit_n = 0, last_n = 0;  // digit + 1
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (c4[j]) {
+                        last = 256 - 4 * t - j;
+                        last_n = c4[j];
+                        last_left = target > run ? target - run : 0;
+                        if (!hit && run + d4[j] >= target) {
+                            hit = last;
+                            hit_n = last_n;
+                            left = last_left;
+                        }
+                    }
+                    run += d4[j];
+                }
+                const uint64_t reach = __builtin_amdgcn_ballot_w64(hit != 0), some = __builtin_amdgcn_ballot_w64(last != 0);
+                // the first digit that reaches the target; where none does, the smallest
+                const int who = reach ? __builtin_ctzll(reach) : 63 - __builtin_clzll(some | 1);
+                if ((int)t == who) {
+                    sh.sel_key = (reach ? hit : last) - 1;
+                    sh.sel_left = reach ? left : last_left;
+                    sh.sel_count = reach ? hit_n : last_n;
+                }
+            }
+            __syncthreads();
+            prefix |= sh.sel_key << shift;
+            mask |= 255ull << shift;
+            target = sh.sel_left;
+            if (sh.sel_count <= kFinish || shift == 0) break;
+            shift = shift > 8 ? shift - 8 : 0;
+        }
     }
-    // the one key with that prefix
-    for (uint32_t i = t; i < n; i += kThreads) {
+    __syncthreads();
+    if (t < kFinish) sh.keyed[t] = Keyed{0, 0};
+    if (t == 0) {
+        sh.n = 0;
+        sh.sel_key = 0;
+        sh.sel_left = 0;
+    }
+    __syncthreads();
+    visit([&](uint64_t rank) {
         uint64_t key, w;
-        if (src(i, key, w) && (key & mask) == prefix) sh.sel_key = key;
+        if (map(rank, key, w) && (key & mask) == prefix) {
+            const uint32_t at = atomicAdd(&sh.n, 1u);
+            if (at < kFinish) sh.keyed[at] = Keyed{key, w};
+        }
+    });
+    __syncthreads();
+    const uint32_t m = min(sh.n, kFinish);
+    if (t < m) {
+        const Keyed mine = sh.keyed[t];
+        uint64_t before = 0;
+        bool least = true;
+        for (uint32_t j0 = 0; j0 < m; j0 += 8) {
+            Keyed x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = sh.keyed[j0 + j];  // zeros behind the last
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                before += x[j].key > mine.key ? x[j].weight : 0;
+                least &= x[j].key == 0 || x[j].key >= mine.key;
+            }
+        }
+        if (before < target && before + mine.weight >= target) sh.sel_key = mine.key;
+        if (least) sh.sel_left = mine.key;
     }
     __syncthreads();
-    const uint64_t key = sh.sel_key;
-    __syncthreads();
-    return key;
+    return sh.sel_key ? sh.sel_key : sh.sel_left;
 }
 
 struct RowOut {
@@ -294,64 +360,69 @@ __device__ __forceinline__ void put(const RowOut& o, uint32_t token, double prob
 
 __device__ __forceinline__ double weight_of(float v, double vmax, double inv_t) { return exp(((double)v - vmax) * inv_t); }
 
-// The draw over elements elem(i) -> rank key (0: none), i < n, that hold every token of the first k: the three cuts, then
-// the index at which the running sum passes u. `one`: the fixed point of weights.
-template <class Elem>
-__device__ void draw_exact(Shared& sh, uint32_t n, const RowParams& rp, double vmax, double u, double one, const RowOut& out,
-                           bool cut_k, Elem elem) {
+// The draw over elements (visit and n as for select_key) that hold every token of the first k: the three cuts, then the index
+// at which the running sum passes u. `one`: the fixed point of weights.
+template <int NT, class Visit>
+__device__ __forceinline__ void draw_exact(Shared& sh, uint32_t n, const RowParams& rp, double vmax, double u, double one, const RowOut& out,
+                           bool cut_k, Visit visit) {
     auto fixed = [&](uint64_t rank) { return (uint64_t)(weight_of(value_of(rank), vmax, rp.inv_t) * one + 0.5); };
     uint64_t low = 1;  // the smallest kept rank key
-    if (cut_k) low = select_key(sh, n, rp.k, [&](uint32_t i, uint64_t& key, uint64_t& w) {
-        key = elem(i);
+    if (cut_k) low = select_key<NT>(sh, n, rp.k, visit, [&](uint64_t rank, uint64_t& key, uint64_t& w) {
+        key = rank;
         w = 1;
-        return key != 0;
+        return true;
     });
-    auto total_of = [&](auto kept) {
-        uint64_t s = 0;
-        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-            const uint64_t key = elem(i);
-            if (key >= low && kept(key)) s += fixed(key);
-        }
-        return block_add(sh, s);
-    };
     if (rp.cut_p) {
-        const uint64_t total = total_of([](uint64_t) { return true; });
-        const uint64_t target = (uint64_t)ceil((double)total * rp.p);
-        low = select_key(sh, n, target, [&](uint32_t i, uint64_t& key, uint64_t& w) {
-            key = elem(i);
-            w = key >= low ? fixed(key) : 0;
-            return key >= low;
+        uint64_t s = 0;
+        visit([&](uint64_t rank) { s += rank >= low ? fixed(rank) : 0; });
+        const uint64_t target = (uint64_t)ceil((double)block_add<NT>(sh, s) * rp.p);
+        low = select_key<NT>(sh, n, target, visit, [&](uint64_t rank, uint64_t& key, uint64_t& w) {
+            key = rank;
+            w = rank >= low ? fixed(rank) : 0;
+            return rank >= low;
         });
     }
     // min-p: the weight itself decides
-    auto heavy = [&](uint64_t key) { return weight_of(value_of(key), vmax, rp.inv_t) >= rp.m; };
-    const uint64_t total = total_of(heavy);
+    auto heavy = [&](uint64_t rank) { return weight_of(value_of(rank), vmax, rp.inv_t) >= rp.m; };
+    uint64_t s = 0;
+    visit([&](uint64_t rank) { s += rank >= low && heavy(rank) ? fixed(rank) : 0; });
+    const uint64_t total = block_add<NT>(sh, s);
     uint64_t target = (uint64_t)((double)total * u) + 1;
     if (target > total) target = total;
-    const uint64_t at = select_key(sh, n, target, [&](uint32_t i, uint64_t& key, uint64_t& w) {
-        const uint64_t rank = elem(i);
+    const uint64_t at = select_key<NT>(sh, n, target, visit, [&](uint64_t rank, uint64_t& key, uint64_t& w) {
         if (rank < low || !heavy(rank)) return false;
         w = fixed(rank);
         key = (rank & 0xFFFFFFFFull) + 1;  // the inverted index: ascending indices are descending keys (+ 1: not 0)
         return w != 0;
     });
     const uint32_t idx = ~(uint32_t)(at - 1);
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-        const uint64_t rank = elem(i);
-        if (rank && index_of(rank) == idx) put(out, idx, (double)fixed(rank) / (double)total);
-    }
+    visit([&](uint64_t rank) {
+        if (index_of(rank) == idx) put(out, idx, (double)fixed(rank) / (double)total);
+    });
 }
 
 // Bin of a value on the grid that all slices share: floor(8 l / T), as a double (exact to 2^53, and monotone above).
 __device__ __forceinline__ double bin_of(float v, double inv_t) { return floor((double)v * inv_t * 8.0); }
 __device__ __forceinline__ uint32_t bin_below(double top_bin, double bin) { return (uint32_t)fmin(top_bin - bin, (double)(kBins - 1)); }
+// 1 - exp(y) for -1/8 <= y <= 0, to 2^-45 (the series' first eight terms).
+__device__ __forceinline__ double one_less_exp(double y) {
+    double p = 1.0 / 40320.0;
+    p = fma(p, y, 1.0 / 5040.0);
+    p = fma(p, y, 1.0 / 720.0);
+    p = fma(p, y, 1.0 / 120.0);
+    p = fma(p, y, 1.0 / 24.0);
+    p = fma(p, y, 1.0 / 6.0);
+    p = fma(p, y, 0.5);
+    p = fma(p, y, 1.0);
+    return -p * y;
+}
 
 template <class T, int EPT>
 __global__ __launch_bounds__(kThreads) void k_rows_scan(const T* __restrict__ logits, uint32_t V, uint64_t stride,
                                                         const vsl_row_sampler* __restrict__ params, Work ws) {
     __shared__ Shared sh;
     __shared__ uint64_t s_hist[kBins];
-    __shared__ uint32_t s_n;
+    __shared__ uint32_t s_n, s_low;
     const uint32_t row = blockIdx.y, slice = blockIdx.x, nsl = gridDim.x, t = threadIdx.x;
     const T* l = logits + (size_t)row * stride;
     const uint32_t first = slice * (EPT * kThreads);
@@ -362,131 +433,136 @@ __global__ __launch_bounds__(kThreads) void k_rows_scan(const T* __restrict__ lo
         v[i] = e < V ? load_logit(l, e) : -INFINITY;
     }
     const RowParams rp = row_params(params[row], V);
-    if (slice == 0 && t < 2) ws.counters[2 * row + t] = 0;
-    uint64_t best = 0;
+    if (slice == 0 && t == 0) ws.counters[row] = 0;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-        const uint64_t r = rank_of(v[i], first + i * kThreads + t);
-        best = r > best ? r : best;
+    for (uint32_t b = 0; b < kBins; b += kThreads) s_hist[b + t] = 0;
+    if (t == 0) {
+        s_n = 0;
+        s_low = 0xFFFFFFFFu;
+        sh.sel_count = kBins - 1;
     }
-    const uint64_t top = block_max64(sh, best);
+    float mx = v[0];
+    int arg = 0;
+#pragma unroll
+    for (int i = 1; i < EPT; ++i)
+        if (v[i] > mx) {
+            mx = v[i];
+            arg = i;
+        }
+    const uint64_t best = rank_of(mx, first + arg * kThreads + t);
+    uint64_t top = best, low_key = best ? ~(best | 0xFFFFFFFFull) : 0;  // the smallest of the threads' maxima, inverted
+    block_max2<kThreads>(sh, top, low_key);
     SliceRec* rec = ws.rec + (size_t)row * nsl + slice;
     if (t == 0) rec->top = top;
     if (rp.mode == MODE_GREEDY || rp.mode == MODE_SUM) return;
-    for (uint32_t b = t; b < kBins; b += kThreads) s_hist[b] = 0;
-    if (t == 0) s_n = 0;
     if (rp.mode == MODE_TOPK) {
         // threads' maxima in 512 bins between their largest and their smallest: the bin of the k-th bounds the k-th token
-        const float vmax = top ? value_of(top) : 0.f, mine = best ? value_of(best) : INFINITY;
-        const uint64_t low_key = block_max64(sh, best ? ~(best | 0xFFFFFFFFull) : 0);
-        const float vmin = top ? value_of(~low_key) : 0.f, range = vmax - vmin;
+        const float vmax = top ? value_of(top) : 0.f, vmin = top ? value_of(~low_key) : 0.f, range = vmax - vmin;
         const float step = range > 0.f ? (float)(kBins - 2) / range : 0.f;
         auto bin = [&](float x) {
             const float b = (vmax - x) * step;
             return b < (float)(kBins - 1) ? (uint32_t)b : kBins - 1;  // NaN (an infinite range): the last
         };
-        if (best) atomicAdd(reinterpret_cast<unsigned long long*>(&s_hist[bin(mine)]), 1ull);
+        uint32_t* count = reinterpret_cast<uint32_t*>(s_hist);
+        if (best) atomicAdd(&count[bin(mx)], 1u);
         __syncthreads();
-        uint64_t c = t < kBins ? s_hist[t] : 0;
-        const uint64_t incl = block_scan(sh, c);
-        if (t == 0) sh.sel_count = kBins - 1;
+        if (t < 64) {
+            uint32_t c[kBins / 64];
+            uint64_t s = 0;
+#pragma unroll
+            for (int j = 0; j < (int)kBins / 64; ++j) {
+                c[j] = count[t * (kBins / 64) + j];
+                s += c[j];
+            }
+            uint64_t run = wave_scan(s) - s;
+#pragma unroll
+            for (int j = 0; j < (int)kBins / 64; ++j) {
+                if (run < rp.k && run + c[j] >= rp.k) sh.sel_count = t * (kBins / 64) + j;
+                run += c[j];
+            }
+        }
         __syncthreads();
-        if (t < kBins && incl >= rp.k && incl - c < rp.k) sh.sel_count = t;
-        __syncthreads();
-        const uint32_t cut = sh.sel_count;
-        float lowest = INFINITY;
+        const uint32_t cut = sh.sel_count;  // the last bin: fewer than k threads hold a token
         uint64_t* list = ws.lists + (size_t)row * ws.list_stride + (size_t)slice * kLeanCap;
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
             if (v[i] == -INFINITY || bin(v[i]) > cut) continue;
             const uint32_t at = atomicAdd(&s_n, 1u);
-            if (at < kLeanCap) list[at] = rank_of(v[i], first + i * kThreads + t);
-            lowest = fminf(lowest, v[i]);
+            const uint64_t r = rank_of(v[i], first + i * kThreads + t);
+            if (at < kLeanCap) list[at] = r;
+            atomicMin(&s_low, (uint32_t)(r >> 32));
         }
+        __syncthreads();
         // the list's smallest value: with k tokens in it, no token below that value is among the row's k largest
-        const uint64_t lk = block_max64(sh, lowest < INFINITY ? ~(rank_of(lowest, 0) | 0xFFFFFFFFull) : 0);
         if (t == 0) {
             rec->count = s_n;
-            rec->floor_v = s_n >= rp.k ? value_of(~lk) : -INFINITY;
+            rec->floor_v = s_n >= rp.k ? value_of((uint64_t)s_low << 32) : -INFINITY;
         }
         return;
     }
-    __syncthreads();
     const double top_bin = top ? bin_of(value_of(top), rp.inv_t) : 0.0;
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
         if (v[i] == -INFINITY) continue;
         const double x = (double)v[i] * rp.inv_t, b = floor(x * 8.0);
         const uint32_t r = bin_below(top_bin, b);
-        const double d = 1.0 - exp(x - (b + 1.0) * 0.125);
-        const uint64_t add = (1ull << kCountShift) + (r < kBins - 1 ? (uint64_t)(fmin(fmax(d, 0.0), kBinSpan) * (double)(1ull << kBinFrac) + 0.5) : 0);
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s_hist[r]), (unsigned long long)add);
+        const double d = fmin(fmax(one_less_exp(x - (b + 1.0) * 0.125), 0.0), kBinSpan);
+        if (r < kBins - 1)
+            atomicAdd(reinterpret_cast<unsigned long long*>(&s_hist[r]),
+                      (unsigned long long)((1ull << kCountShift) + (uint64_t)(d * (double)(1ull << kBinFrac) + 0.5)));
     }
     __syncthreads();
     uint64_t* h = ws.hist + ((size_t)row * nsl + slice) * kBins;
-    for (uint32_t b = t; b < kBins; b += kThreads) h[b] = s_hist[b];
-}
-
-// Draws from one slice: the token at which the kept weights' running sum, by index, passes `target`.
-template <class T, int EPT, class Kept>
-__device__ void walk_slice(Shared& sh, const T* l, uint32_t V, uint32_t first, double target, double total, double vmax,
-                           double inv_t, const RowOut& out, Kept kept) {
-    const uint32_t t = threadIdx.x, from = first + t * EPT;
-    double w[EPT], mine = 0.0;
-    uint64_t last = 0;  // the last kept index + 1
+    uint64_t used = 0, unused = 0;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-        w[i] = 0.0;
-        if (from + i >= V) continue;
-        const float v = load_logit(l, from + i);
-        const double x = v == -INFINITY ? 0.0 : weight_of(v, vmax, inv_t);
-        if (v == -INFINITY || !kept(rank_of(v, from + i), x)) continue;
-        w[i] = x;
-        mine += x;
-        if (x > 0.0) last = from + i + 1;
+    for (uint32_t b = 0; b < kBins; b += kThreads) {
+        const uint64_t x = s_hist[b + t];
+        h[b + t] = x;  // the last one is 0: what lies outside the bins is read from there
+        if (x) used = b + t + 1;
     }
-    const double incl = block_scan(sh, mine), before = incl - mine;
-    // the first thread whose sum passes the target (rounding may leave none: the last kept token)
-    const uint64_t hit = block_max64(sh, incl > target && mine > 0.0 ? ~(uint64_t)t : 0);
-    const uint64_t end = block_max64(sh, last);
-    const uint32_t who = hit ? (uint32_t)~hit : (uint32_t)(end - 1 - first) / EPT;
-    if (end == 0 || t != who) return;
-    double run = before;
-    uint32_t token = 0;
-    double weight = 0.0;
-    bool found = false;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-        run += w[i];
-        if (w[i] > 0.0 && !found) {
-            token = from + i;
-            weight = w[i];
-            found = hit && run > target;
-        }
-    }
-    put(out, token, weight / total);
+    block_max2<kThreads>(sh, used, unused);
+    if (t == 0) rec->count = (uint32_t)used;
 }
 
 template <class T, int EPT>
-__global__ __launch_bounds__(kThreads) void k_rows_pick(const T* __restrict__ logits, uint32_t V, uint64_t stride,
-                                                        const vsl_row_sampler* __restrict__ params, const float* __restrict__ us,
-                                                        Work ws, uint32_t* __restrict__ tokens, float* __restrict__ probs) {
+__global__ __launch_bounds__(kThreads) void k_rows_cut(const T* __restrict__ logits, uint32_t V, uint64_t stride,
+                                                       const vsl_row_sampler* __restrict__ params, const float* __restrict__ us,
+                                                       Work ws, uint32_t* __restrict__ tokens, float* __restrict__ probs) {
+    constexpr int NT = kThreads;
     __shared__ Shared sh;
-    __shared__ uint64_t s_list[kListCap];
-    __shared__ double s_cum_w[kBins];
+    __shared__ uint64_t s_list[kLeanList];
+    __shared__ double s_cum_w[kBins], s_edge[kBins];
     __shared__ uint32_t s_cum_n[kBins];
-    __shared__ uint64_t s_slice[kMaxSlices];
-    __shared__ uint32_t s_n, s_plo, s_phi, s_kb;
-    __shared__ bool s_last;
-    const uint32_t row = blockIdx.y, slice = blockIdx.x, nsl = gridDim.x, t = threadIdx.x;
+    __shared__ uint32_t s_count[kMaxSlices], s_off[kMaxSlices], s_n, s_plo, s_phi, s_kb, s_base;
+    const uint32_t row = blockIdx.y, slice = blockIdx.x, nsl = gridDim.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const RowParams rp = row_params(params[row], V);
     if (rp.mode <= MODE_TOPK && slice != 0) return;
-    const SliceRec* rec = ws.rec + (size_t)row * nsl;
+    SliceRec* rec = ws.rec + (size_t)row * nsl;
     const T* l = logits + (size_t)row * stride;
+    const uint32_t first = slice * (EPT * kThreads);
+    float v[EPT];
+    if (rp.mode >= MODE_SUM) {
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) {
+            const uint32_t e = first + i * kThreads + t;
+            v[i] = e < V ? load_logit(l, e) : -INFINITY;
+        }
+    }
     const RowOut out{tokens + row, probs ? probs + row : nullptr};
-    const float uf = us[row];
-    const double u = uf > 0.f ? fmin((double)uf, 1.0 - 0x1p-24) : 0.0;  // NaN and below 0: 0; 1 and above: the float below 1
-    const uint64_t top = block_max64(sh, t < nsl ? rec[t].top : 0);
+    uint64_t my_top = 0, top, bound = 0;
+    uint32_t my_count = 0;
+    if (t < nsl) {
+        my_top = rec[t].top;
+        if (rp.mode == MODE_TOPK || rp.mode == MODE_HIST) my_count = rec[t].count;
+        if (rp.mode == MODE_TOPK) bound = rank_of(rec[t].floor_v, 0xFFFFFFFFu);  // the smallest rank of that value
+    }
+    if (t < kMaxSlices) s_count[t] = my_count;
+    if (t == 0) {
+        s_n = 0;
+        s_kb = s_plo = s_phi = kBins - 1;
+    }
+    top = my_top;
+    block_max2<NT>(sh, top, bound);
     if (top == 0) {  // nothing above -inf
         if (slice == 0 && t == 0) put(out, 0, 0.0);
         return;
@@ -496,237 +572,363 @@ __global__ __launch_bounds__(kThreads) void k_rows_pick(const T* __restrict__ lo
         return;
     }
     const double vmax = (double)value_of(top);
-    auto whole_row = [&] {
-        draw_exact(sh, V, rp, vmax, u, kRowOne, out, rp.k < V, [&](uint32_t i) { return rank_of(load_logit(l, i), i); });
-    };
 
     if (rp.mode == MODE_TOPK) {
-        // tokens at or above the highest of the slices' bounds
-        float bound = -INFINITY;
-        for (uint32_t s = 0; s < nsl; ++s) bound = fmaxf(bound, rec[s].floor_v);
-        if (t == 0) s_n = 0;
-        __syncthreads();
+        // the slices' tokens at or above the highest of their bounds
         const uint64_t* lists = ws.lists + (size_t)row * ws.list_stride;
-        bool whole = false;
-        for (uint32_t i = t; i < nsl * kLeanCap; i += kThreads) {
-            const uint32_t s = i / kLeanCap, c = rec[s].count;
-            whole |= c > kLeanCap;
-            if (i % kLeanCap >= min(c, kLeanCap)) continue;
-            const uint64_t r = lists[i];
-            if (value_of(r) < bound) continue;
+        auto take = [&](uint64_t r) {
+            if (r < bound || r == 0) return;
             const uint32_t at = atomicAdd(&s_n, 1u);
-            if (at < kListCap) s_list[at] = r;
-        }
-        if (__syncthreads_or(whole) || s_n > kListCap) {
-            whole_row();
-            return;
-        }
-        draw_exact(sh, s_n, rp, vmax, u, kListOne, out, s_n > rp.k, [&](uint32_t i) { return s_list[i]; });
-        return;
-    }
-
-    const uint32_t first = slice * (EPT * kThreads);
-    uint32_t* counters = ws.counters + 2 * row;
-    auto last_block = [&] {
-        __threadfence();
-        __syncthreads();
-        if (t == 0) s_last = atomicAdd(&counters[1], 1u) == nsl - 1;
-        __syncthreads();
-        __threadfence();
-        return s_last;
-    };
-    // the slice in which the running sum of s_slice (fixed point kRowOne) passes u; then the walk
-    auto draw_slice = [&](double u, auto kept) {
-        __syncthreads();
-        if (t < 64) {
-            const uint64_t a = 2 * t < nsl ? s_slice[2 * t] : 0, b = 2 * t + 1 < nsl ? s_slice[2 * t + 1] : 0;
-            const uint64_t incl = wave_scan(a + b);
-            if (t == 63) sh.sel_left = incl;
-            const uint64_t sum = (uint64_t)__shfl((uint32_t)(incl >> 32), 63, 64) << 32 | __shfl((uint32_t)incl, 63, 64);
-            const double target = (double)sum * u;
-            const uint64_t before = incl - a - b;
-            const bool in_a = a && (double)(before + a) > target, in_b = b && (double)incl > target;
-            const uint64_t hit = __builtin_amdgcn_ballot_w64(in_a || in_b);
-            const uint64_t some = __builtin_amdgcn_ballot_w64(a || b);
-            const int who = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some | 1);
-            if ((int)t == who) {
-                const bool second = hit ? !in_a : b != 0;
-                sh.sel_count = 2 * t + (second ? 1 : 0);
-                sh.sel_key = second ? before + a : before;
+            if (at < kLeanList) s_list[at] = r;
+        };
+        for (uint32_t s0 = wave; s0 < nsl; s0 += 4 * (NT / 64)) {  // four slices' first 64 entries at a time
+            uint64_t r[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t s = s0 + j * (NT / 64);
+                r[j] = s < nsl && lane < s_count[s] ? lists[(size_t)s * kLeanCap + lane] : 0;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t s = s0 + j * (NT / 64);
+                take(r[j]);
+                if (s < nsl)
+                    for (uint32_t i = 64 + lane; i < min(s_count[s], kLeanCap); i += 64) take(lists[(size_t)s * kLeanCap + i]);
             }
         }
-        __syncthreads();
-        const double total = (double)sh.sel_left / kRowOne, before = (double)sh.sel_key / kRowOne;
-        const uint32_t s = sh.sel_count;
-        __syncthreads();
-        walk_slice<T, EPT>(sh, l, V, s * (EPT * kThreads), total * u - before, total, vmax, rp.inv_t, out, kept);
-    };
+        const bool over = __syncthreads_or(my_count > kLeanCap);
+        const uint32_t n = s_n;
+        const bool whole = over || n > kLeanList;
+        if (t == 0) ws.row[row].whole = whole;
+        if (whole) return;
+        uint64_t r[kLeanRegs];
+#pragma unroll
+        for (int i = 0; i < kLeanRegs; ++i) r[i] = i * NT + t < n ? s_list[i * NT + t] : 0;
+        const float uf = us[row];
+        const double u = uf > 0.f ? fmin((double)uf, 1.0 - 0x1p-24) : 0.0;
+        draw_exact<NT>(sh, n, rp, vmax, u, kListOne, out, n > rp.k, [&](auto f) {
+#pragma unroll
+            for (int i = 0; i < kLeanRegs; ++i)
+                if (r[i]) f(r[i]);
+        });
+        return;
+    }
 
     if (rp.mode == MODE_SUM) {
         double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
-            const uint32_t e = first + i * kThreads + t;
-            const float v = e < V ? load_logit(l, e) : -INFINITY;
-            const double w = v == -INFINITY ? 0.0 : weight_of(v, vmax, rp.inv_t);
+            const double w = v[i] == -INFINITY ? 0.0 : weight_of(v[i], vmax, rp.inv_t);
             if (w >= rp.m) sum += w;
         }
-        sum = block_add(sh, sum);
-        if (t == 0) ws.rec[(size_t)row * nsl + slice].sum = sum;
-        if (!last_block()) return;
-        if (t < nsl) s_slice[t] = (uint64_t)(rec[t].sum * kRowOne + 0.5);
-        draw_slice(u, [&](uint64_t, double w) { return w >= rp.m; });
+        sum = block_add<NT>(sh, sum);
+        if (t == 0) rec[slice].sum = sum;
         return;
     }
 
-    if (fabs(vmax * rp.inv_t) > kMaxTop) {
-        if (slice == 0) whole_row();
-        return;
-    }
-    // HIST: the slices' bins on the row's grid, thread b bin b below the row's top bin
+    if (fabs(vmax * rp.inv_t) > kMaxTop) return;  // drawn from the whole row
+    // HIST: the slices' bins on the row's grid, thread t the bins 2 t and 2 t + 1 below the row's top bin
     const double top_bin = bin_of(value_of(top), rp.inv_t);
     const uint64_t* hist = ws.hist + (size_t)row * nsl * kBins;
-    // weight of bin b's upper edge relative to the largest token
-    auto edge = [&](uint32_t b) { return exp((top_bin + 1.0 - (double)b) * 0.125 - vmax * rp.inv_t); };
-    auto bin_weight = [](uint64_t h) {  // of a bin's tokens, relative to its upper edge
-        return (double)(h >> kCountShift) - (double)(h & ((1ull << kCountShift) - 1)) * (1.0 / (double)(1ull << kBinFrac));
-    };
-    auto offset_of = [&](uint32_t s) {  // bins between the row's top and the slice's
-        return rec[s].top ? bin_below(top_bin, bin_of(value_of(rec[s].top), rp.inv_t)) : kBins - 1;
-    };
-    uint64_t n = 0;
-    double w = 0.0;
-    if (t < kBins - 1) {
-        for (uint32_t s = 0; s < nsl; ++s) {
-            const uint32_t o = offset_of(s);
-            if (t < o) continue;
-            const uint64_t h = hist[(size_t)s * kBins + t - o];
-            n += h >> kCountShift;
-            w += bin_weight(h);
+    constexpr uint64_t kLess = (1ull << kCountShift) - 1;
+    constexpr double kUnit = 1.0 / (double)(1ull << kBinFrac);
+    // bins between the row's top and the slice's, and those that hold something
+    uint64_t used = 0, unused = 0;
+    if (t < nsl) {
+        const uint32_t o = my_top ? bin_below(top_bin, bin_of(value_of(my_top), rp.inv_t)) : kBins - 1;
+        s_off[t] = o;
+        used = min(o + my_count, kBins - 1);
+    }
+    // weights of the bins' upper edges relative to the largest token
+    const double top_edge = (top_bin + 1.0) * 0.125 - vmax * rp.inv_t;
+#pragma unroll
+    for (uint32_t b = 0; b < kBins; b += kThreads) s_edge[b + t] = exp(top_edge - 0.125 * (double)(b + t));
+    block_max2<NT>(sh, used, unused);
+    uint32_t n2[2] = {0, 0};
+    uint64_t less[2] = {0, 0};
+    if (2 * t < (uint32_t)used) {
+        for (uint32_t s0 = 0; s0 < nsl; s0 += 16) {
+            uint64_t h[16][2];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const uint32_t s = min(s0 + j, nsl - 1), at = 2 * t - s_off[s];  // wraps below the slice's top
+                const bool in = s0 + j < nsl;
+                const uint64_t* hs = hist + (size_t)s * kBins;
+                h[j][0] = hs[in && at < kBins ? at : kBins - 1];
+                h[j][1] = hs[in && at + 1 < kBins ? at + 1 : kBins - 1];
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    n2[i] += (uint32_t)(h[j][i] >> kCountShift);
+                    less[i] += h[j][i] & kLess;
+                }
         }
-        w *= edge(t);
     }
-    const uint64_t cum_n = block_scan(sh, n);
-    const double cum_w = block_scan(sh, w);
-    if (t < kBins) {
-        s_cum_n[t] = (uint32_t)cum_n;
-        s_cum_w[t] = cum_w;
-    }
-    if (t == 0) {
-        s_kb = kBins - 1;
-        s_plo = s_phi = kBins - 1;
-    }
-    __syncthreads();
+    if (2 * t + 1 == kBins - 1) n2[1] = 0, less[1] = 0;  // below all bins that count
+    double w2[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w2[i] = ((double)n2[i] - (double)less[i] * kUnit) * s_edge[2 * t + i];
+    uint64_t all_n;
+    double all_w;
+    const uint64_t cn1 = block_scan<NT>(sh, (uint64_t)n2[0] + n2[1], all_n), cn0 = cn1 - n2[1];
+    const double cw1 = block_scan<NT>(sh, w2[0] + w2[1], all_w), cw0 = cw1 - w2[1];
+    s_cum_n[2 * t] = (uint32_t)cn0;
+    s_cum_n[2 * t + 1] = (uint32_t)cn1;
+    s_cum_w[2 * t] = cw0;
+    s_cum_w[2 * t + 1] = cw1;
     // the bin of the k-th token (kBins - 1: below all bins that count) and the bins in which the top-p cut can fall
-    if (t < kBins - 1 && n && cum_n >= rp.k && cum_n - n < rp.k) s_kb = t;
+    if (n2[0] && cn0 >= rp.k && cn0 - n2[0] < rp.k) s_kb = 2 * t;
+    if (n2[1] && cn1 >= rp.k && cn0 < rp.k) s_kb = 2 * t + 1;
     __syncthreads();
     const uint32_t kb = s_kb;
     const bool cut_k = kb < kBins - 1 && s_cum_n[kb] != rp.k;
-    const double hi_total = s_cum_w[min(kb, kBins - 2)], lo_total = cut_k ? (kb ? s_cum_w[kb - 1] : 0.0) : hi_total;
-    if (rp.cut_p && t < kBins - 1 && n) {
-        if (cum_w >= lo_total * rp.p * (1.0 - kBinNoise)) atomicMin(&s_plo, t);
-        if (cum_w >= hi_total * rp.p * (1.0 - kBinNoise)) atomicMin(&s_phi, t);
+    const double hi_total = s_cum_w[kb], lo_total = cut_k ? (kb ? s_cum_w[kb - 1] : 0.0) : hi_total;
+    if (rp.cut_p) {
+        const double lo = lo_total * rp.p * (1.0 - kBinNoise), hi = hi_total * rp.p * (1.0 - kBinNoise);
+        if (n2[0] && cw0 >= lo) atomicMin(&s_plo, 2 * t);
+        if (n2[1] && cw1 >= lo) atomicMin(&s_plo, 2 * t + 1);
+        if (n2[0] && cw0 >= hi) atomicMin(&s_phi, 2 * t);
+        if (n2[1] && cw1 >= hi) atomicMin(&s_phi, 2 * t + 1);
     }
     __syncthreads();
     const uint32_t plo = s_plo, phi = s_phi;
     const uint32_t mb = rp.m > 0.0 ? bin_below(top_bin, fmin(floor((vmax * rp.inv_t + log(rp.m)) * 8.0), top_bin)) : kBins - 1;
-    auto row_bin = [&](float v) { return bin_below(top_bin, bin_of(v, rp.inv_t)); };
     auto wanted = [&](uint32_t b) {
         return b < kBins - 1 && ((cut_k && b == kb) || (rp.cut_p && b >= plo && b <= phi) || b == mb);
     };
-    // this slice's tokens in those bins
-    uint64_t* list = ws.lists + (size_t)row * ws.list_stride;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-        const uint32_t e = first + i * kThreads + t;
-        const float v = e < V ? load_logit(l, e) : -INFINITY;
-        if (v == -INFINITY || !wanted(row_bin(v))) continue;
-        const uint32_t at = atomicAdd(&counters[0], 1u);
-        if (at < kListCap) list[at] = rank_of(v, e);
+    // Bins that are kept whole whatever the cuts turn out to be: those before the first in which one can fall (all bins up to
+    // that of the last one kept are then wanted ones). This slice's weight in them, and its tokens in the wanted bins.
+    const uint32_t sure = min(min(rp.cut_p ? plo : kBins - 1, mb), kb < kBins - 1 ? (cut_k ? kb : kb + 1) : kBins - 1);
+    if (slice == 0) {
+        RowRec& r = ws.row[row];
+        r.cum_w[2 * t] = cw0;
+        r.cum_w[2 * t + 1] = cw1;
+        if (t == 0) {
+            r.kb = kb;
+            r.plo = plo;
+            r.phi = phi;
+            r.sure = sure;
+            r.cut_k = cut_k;
+            r.k_left = rp.k - (cut_k && kb ? s_cum_n[kb - 1] : 0);
+            r.lo_total = lo_total;
+            r.hi_total = hi_total;
+        }
     }
-    if (!last_block()) return;
-    const uint32_t n_list = __hip_atomic_load(&counters[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (n_list > kListCap) {
-        whole_row();
+    {
+        const uint64_t* hs = hist + (size_t)slice * kBins;
+        const uint32_t o = s_off[slice];
+        double sum = 0.0;
+#pragma unroll
+        for (uint32_t b0 = 0; b0 < kBins; b0 += kThreads) {
+            const uint32_t b = b0 + t;
+            if (b < o || b >= sure) continue;
+            const uint64_t h = hs[b - o];
+            sum += ((double)(h >> kCountShift) - (double)(h & kLess) * kUnit) * s_edge[b];
+        }
+        sum = block_add<NT>(sh, sum);
+        if (t == 0) rec[slice].sum = sum;
+    }
+    uint64_t* list = ws.lists + (size_t)row * ws.list_stride;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i)
+        if (v[i] != -INFINITY && wanted(bin_below(top_bin, bin_of(v[i], rp.inv_t)))) mine |= 1u << i;
+    uint64_t total;
+    const uint64_t c = __builtin_popcount(mine);
+    uint32_t at = (uint32_t)(block_scan<NT>(sh, c, total) - c);
+    if (total == 0) return;
+    if (t == 0) s_base = atomicAdd(&ws.counters[row], (uint32_t)total);
+    __syncthreads();
+    at += s_base;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i)
+        if (mine >> i & 1) {
+            if (at < kListCap) list[at] = rank_of(v[i], first + i * kThreads + t);
+            ++at;
+        }
+}
+
+// A block a row of mode SUM or HIST, or of one whose lists overflowed. SL: tokens a slice.
+template <class T, int SL>
+__global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict__ logits, uint32_t V, uint64_t stride,
+                                                            const vsl_row_sampler* __restrict__ params, const float* __restrict__ us,
+                                                            uint32_t nsl, Work ws, uint32_t* __restrict__ tokens,
+                                                            float* __restrict__ probs) {
+    constexpr int NT = kDrawThreads, E = SL / NT;
+    __shared__ Shared sh;
+    __shared__ uint64_t s_slice[kMaxSlices];
+    const uint32_t row = blockIdx.x, t = threadIdx.x;
+    const RowParams rp = row_params(params[row], V);
+    const RowRec& rr = ws.row[row];
+    if (rp.mode == MODE_GREEDY || (rp.mode == MODE_TOPK && !rr.whole)) return;
+    const T* l = logits + (size_t)row * stride;
+    const RowOut out{tokens + row, probs ? probs + row : nullptr};
+    const float uf = us[row];
+    const double u = uf > 0.f ? fmin((double)uf, 1.0 - 0x1p-24) : 0.0;  // NaN and below 0: 0; 1 and above: the float below 1
+    const uint32_t n_list = rp.mode == MODE_HIST ? ws.counters[row] : 0;
+    const SliceRec* rec = ws.rec + (size_t)row * nsl;
+    uint64_t top = 0, none = 0;
+    double slice_sum = 0.0;
+    if (t < nsl) {
+        top = rec[t].top;
+        slice_sum = rec[t].sum;
+    }
+    const uint64_t* list = ws.lists + (size_t)row * ws.list_stride;
+    uint64_t r[kDrawRegs];
+#pragma unroll
+    for (int i = 0; i < kDrawRegs; ++i) r[i] = 0;
+    if (n_list <= kListCap) {
+#pragma unroll
+        for (int i = 0; i < kDrawRegs; ++i)
+            if (i * NT + t < n_list) r[i] = list[i * NT + t];
+    }
+    block_max2<NT>(sh, top, none);
+    if (top == 0) return;
+    const double vmax = (double)value_of(top);
+    if (rp.mode == MODE_TOPK || (rp.mode == MODE_HIST && (n_list > kListCap || fabs(vmax * rp.inv_t) > kMaxTop))) {
+        draw_exact<NT>(sh, V, rp, vmax, u, kRowOne, out, rp.k < V, [&](auto f) {
+            for (uint32_t i0 = t; i0 < V; i0 += 8 * NT) {
+                uint64_t x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = i0 + j * NT < V ? rank_of(load_logit(l, i0 + j * NT), i0 + j * NT) : 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (x[j]) f(x[j]);
+            }
+        });
         return;
     }
-    for (uint32_t i = t; i < n_list; i += kThreads) s_list[i] = list[i];
-    __syncthreads();
-    auto fixed = [&](uint64_t rank) { return (uint64_t)(weight_of(value_of(rank), vmax, rp.inv_t) * kListOne + 0.5); };
-    uint64_t low = 1;
-    double total = hi_total;
-    if (cut_k) {
-        low = select_key(sh, n_list, rp.k - (kb ? s_cum_n[kb - 1] : 0), [&](uint32_t i, uint64_t& key, uint64_t& w1) {
-            key = s_list[i];
-            w1 = 1;
-            return row_bin(value_of(key)) == kb;
-        });
-        uint64_t part = 0;
-        for (uint32_t i = t; i < n_list; i += kThreads)
-            if (s_list[i] >= low && row_bin(value_of(s_list[i])) == kb) part += fixed(s_list[i]);
-        total = lo_total + (double)block_add(sh, part) / kListOne;
-    }
-    if (rp.cut_p) {
-        const double target = total * rp.p * (1.0 - kBinNoise);
-        uint32_t pb = plo;
-        while (pb < phi && s_cum_w[pb] < target) ++pb;
-        const double base = pb ? s_cum_w[pb - 1] : 0.0;
-        const uint64_t left = target > base ? (uint64_t)ceil((target - base) * kListOne) : 1;
-        const uint64_t cut = select_key(sh, n_list, left, [&](uint32_t i, uint64_t& key, uint64_t& w1) {
-            key = s_list[i];
-            if (key < low || row_bin(value_of(key)) != pb) return false;
-            w1 = fixed(key);
-            return true;
-        });
-        if (cut > low) low = cut;
-    }
-    // whole bins above the cut's, and of its own bin the list's tokens
-    uint32_t cb = low > 1 ? row_bin(value_of(low)) : kBins - 1;
-    if (low <= 1 && kb < kBins - 1) cb = kb + 1;  // k ends with a whole bin
-    const uint32_t whole_bins = min(cb, mb);
-    auto kept = [&](uint64_t rank, double wt) {
-        return rank >= low && wt >= rp.m && row_bin(value_of(rank)) <= cb - (low > 1 ? 0 : 1);
+    auto visit = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < kDrawRegs; ++i) {
+            if ((uint32_t)i * NT >= n_list) break;
+            if (r[i]) f(r[i]);
+        }
     };
-    const uint32_t lane = t & 63;
-    for (uint32_t s = t >> 6; s < nsl; s += kWaves) {
-        const uint32_t o = offset_of(s);
-        double sum = 0.0;
-        for (uint32_t b = o + lane; b < whole_bins; b += 64) sum += bin_weight(hist[(size_t)s * kBins + b - o]) * edge(b);
-        sum = wave_add(sum);
-        if (lane == 0) s_slice[s] = (uint64_t)(sum * kRowOne + 0.5);
+    const double top_bin = bin_of(value_of(top), rp.inv_t);
+    auto row_bin = [&](float x) { return bin_below(top_bin, bin_of(x, rp.inv_t)); };
+    auto fixed = [&](uint64_t rank) { return (uint64_t)(weight_of(value_of(rank), vmax, rp.inv_t) * kListOne + 0.5); };
+    uint64_t low = 1;  // the smallest kept rank key
+    uint32_t cb = kBins - 2, sure = 0;  // the last bin that keeps a token; the bins kept whole are in the slices' sums
+    const bool hist = rp.mode == MODE_HIST;
+    if (hist) {
+        const uint32_t kb = rr.kb, plo = rr.plo, phi = rr.phi;
+        sure = rr.sure;
+        double total = rr.hi_total;
+        if (rr.cut_k) {
+            low = select_key<NT>(sh, n_list, rr.k_left, visit, [&](uint64_t rank, uint64_t& key, uint64_t& w) {
+                key = rank;
+                w = 1;
+                return row_bin(value_of(rank)) == kb;
+            });
+            if (rp.cut_p) {
+                uint64_t part = 0;
+                visit([&](uint64_t rank) { part += rank >= low && row_bin(value_of(rank)) == kb ? fixed(rank) : 0; });
+                total = rr.lo_total + (double)block_add<NT>(sh, part) / kListOne;
+            }
+        }
+        if (rp.cut_p) {
+            const double target = total * rp.p * (1.0 - kBinNoise);
+            uint32_t pb = plo;
+            while (pb < phi && rr.cum_w[pb] < target) ++pb;
+            const double base = pb ? rr.cum_w[pb - 1] : 0.0;
+            const uint64_t left = target > base ? (uint64_t)ceil((target - base) * kListOne) : 1;
+            const uint64_t cut = select_key<NT>(sh, n_list, left, visit, [&](uint64_t rank, uint64_t& key, uint64_t& w) {
+                if (rank < low || row_bin(value_of(rank)) != pb) return false;
+                key = rank;
+                w = fixed(rank);
+                return true;
+            });
+            if (cut > low) low = cut;
+        }
+        cb = low > 1 ? row_bin(value_of(low)) : kb < kBins - 1 ? kb : kBins - 2;
+    }
+    auto kept = [&](uint64_t rank, double w) { return rank >= low && w >= rp.m && (!hist || row_bin(value_of(rank)) <= cb); };
+    // the slices' kept weights, in fixed point; of the bins that a cut divides, the list's tokens
+    if (t < kMaxSlices) s_slice[t] = (uint64_t)(slice_sum * kRowOne + 0.5);
+    __syncthreads();
+    visit([&](uint64_t rank) {
+        const double w = weight_of(value_of(rank), vmax, rp.inv_t);
+        if (row_bin(value_of(rank)) >= sure && kept(rank, w))
+            atomicAdd(reinterpret_cast<unsigned long long*>(&s_slice[index_of(rank) / SL]), (unsigned long long)(w * kRowOne + 0.5));
+    });
+    __syncthreads();
+    // the slice in which their running sum passes u
+    if (t < 64) {
+        const uint64_t a = s_slice[2 * t], b = s_slice[2 * t + 1];
+        const uint64_t incl = wave_scan(a + b), sum = last_lane(incl), before = incl - a - b;
+        const double target = (double)sum * (hist ? u * (1.0 + kBinNoise) : u);
+        const bool in_a = a && (double)(before + a) > target, in_b = b && (double)incl > target;
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(in_a || in_b), some = __builtin_amdgcn_ballot_w64(a || b);
+        const int who = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some | 1);
+        if ((int)t == who) {
+            const bool second = hit ? !in_a : b != 0;
+            sh.sel_count = 2 * t + (second ? 1 : 0);
+            sh.sel_key = second ? before + a : before;
+            sh.sel_left = sum;
+        }
     }
     __syncthreads();
-    for (uint32_t i = t; i < n_list; i += kThreads) {
-        const uint64_t r = s_list[i];
-        const double wt = weight_of(value_of(r), vmax, rp.inv_t);
-        const uint32_t b = row_bin(value_of(r));
-        if (b < whole_bins || !kept(r, wt)) continue;
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s_slice[index_of(r) / (EPT * kThreads)]), (unsigned long long)(wt * kRowOne + 0.5));
+    // the token in it: thread t takes E neighbours
+    const double total = (double)sh.sel_left / kRowOne;
+    const double target = total * (hist ? u * (1.0 + kBinNoise) : u) - (double)sh.sel_key / kRowOne;
+    const uint32_t first = sh.sel_count * SL, from = first + t * E;
+    double w[E], mine = 0.0, all;
+    uint64_t last = 0;  // the last kept index + 1
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const float x = from + i < V ? load_logit(l, from + i) : -INFINITY;
+        const double wx = weight_of(x, vmax, rp.inv_t);
+        w[i] = x != -INFINITY && kept(rank_of(x, from + i), wx) ? wx : 0.0;
+        mine += w[i];
+        if (w[i] > 0.0) last = from + i + 1;
     }
-    draw_slice(u * (1.0 + kBinNoise), kept);
+    const double incl = block_scan<NT>(sh, mine, all);
+    // the first thread whose sum passes the target (rounding may leave none: the last kept token)
+    uint64_t hit = incl > target && mine > 0.0 ? ~(uint64_t)t : 0, end = last;
+    block_max2<NT>(sh, hit, end);
+    const uint32_t who = hit ? (uint32_t)~hit : (uint32_t)(end - 1 - first) / E;
+    if (end == 0 || t != who) return;
+    double run = incl - mine, share = 0.0;
+    uint32_t token = 0;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        run += w[i];
+        if (w[i] > 0.0 && !found) {
+            token = from + i;
+            share = w[i];
+            found = hit && run > target;
+        }
+    }
+    put(out, token, share / total);
 }
 
 uint64_t up256(uint64_t b) { return (b + 255) & ~255ull; }
 
 // Elements a thread: enough slices to fill the CUs with the rows there are, at most kMaxSlices of them.
 uint32_t elements_per_thread(uint32_t rows, uint32_t V) {
-    for (uint32_t e : {2u, 4u})
-        if ((uint64_t)rows * ((V + e * kThreads - 1) / (e * kThreads)) <= 256 && (V + e * kThreads - 1) / (e * kThreads) <= kMaxSlices)
+    for (uint32_t e : {8u, 16u})
+        if ((uint64_t)rows * ((V + e * kThreads - 1) / (e * kThreads)) <= 1024 && (V + e * kThreads - 1) / (e * kThreads) <= kMaxSlices)
             return e;
     return kMaxEpt;
 }
 
 struct Layout {
     uint32_t ept, nsl, list_stride;
-    uint64_t counters, lists, hist, bytes;
+    uint64_t row, counters, lists, hist, bytes;
 };
 Layout layout(uint32_t rows, uint32_t V) {
     Layout y;
     y.ept = elements_per_thread(rows, V);
     y.nsl = (V + y.ept * kThreads - 1) / (y.ept * kThreads);
-    y.list_stride = y.nsl * kLeanCap > kListCap ? y.nsl * kLeanCap : kListCap;
-    y.counters = up256((uint64_t)rows * y.nsl * sizeof(SliceRec));
-    y.lists = y.counters + up256((uint64_t)rows * 8);
+    const uint32_t wide = V < kListCap ? V : kListCap;
+    y.list_stride = y.nsl * kLeanCap > wide ? y.nsl * kLeanCap : wide;
+    y.row = up256((uint64_t)rows * y.nsl * sizeof(SliceRec));
+    y.counters = y.row + up256((uint64_t)rows * sizeof(RowRec));
+    y.lists = y.counters + up256((uint64_t)rows * 4);
     y.hist = y.lists + up256((uint64_t)rows * y.list_stride * 8);
     y.bytes = y.hist + up256((uint64_t)rows * y.nsl * kBins * 8);
     return y;
@@ -737,7 +939,8 @@ void launch(hipStream_t s, const Layout& y, const T* logits, uint32_t rows, uint
             const vsl_row_sampler* params, const float* u, const Work& w, uint32_t* tokens, float* probs) {
     const dim3 grid(y.nsl, rows);
     k_rows_scan<T, EPT><<<grid, kThreads, 0, s>>>(logits, V, stride, params, w);
-    k_rows_pick<T, EPT><<<grid, kThreads, 0, s>>>(logits, V, stride, params, u, w, tokens, probs);
+    k_rows_cut<T, EPT><<<grid, kThreads, 0, s>>>(logits, V, stride, params, u, w, tokens, probs);
+    k_rows_draw<T, EPT * kThreads><<<rows, kDrawThreads, 0, s>>>(logits, V, stride, params, u, y.nsl, w, tokens, probs);
 }
 
 }  // namespace
@@ -766,13 +969,13 @@ extern "C" int vsl_sample_rows(const void* logits, int dtype, uint32_t rows, uin
         return vsl_capacity("%s: workspace of %llu bytes, %llu needed", fn, (unsigned long long)ws_bytes,
                             (unsigned long long)y.bytes);
     char* base = static_cast<char*>(workspace);
-    const Work w{reinterpret_cast<SliceRec*>(base), reinterpret_cast<uint32_t*>(base + y.counters),
+    const Work w{reinterpret_cast<SliceRec*>(base), reinterpret_cast<RowRec*>(base + y.row), reinterpret_cast<uint32_t*>(base + y.counters),
                  reinterpret_cast<uint64_t*>(base + y.lists), reinterpret_cast<uint64_t*>(base + y.hist), y.list_stride};
     hipStream_t s = static_cast<hipStream_t>(stream);
     auto go = [&](auto* l) {
-        if (y.ept == 2) launch<std::remove_const_t<std::remove_pointer_t<decltype(l)>>, 2>(s, y, l, rows, V, stride, params, u, w, tokens, probs);
-        else if (y.ept == 4) launch<std::remove_const_t<std::remove_pointer_t<decltype(l)>>, 4>(s, y, l, rows, V, stride, params, u, w, tokens, probs);
-        else launch<std::remove_const_t<std::remove_pointer_t<decltype(l)>>, 8>(s, y, l, rows, V, stride, params, u, w, tokens, probs);
+        if (y.ept == 8) launch<std::remove_const_t<std::remove_pointer_t<decltype(l)>>, 8>(s, y, l, rows, V, stride, params, u, w, tokens, probs);
+        else if (y.ept == 16) launch<std::remove_const_t<std::remove_pointer_t<decltype(l)>>, 16>(s, y, l, rows, V, stride, params, u, w, tokens, probs);
+        else launch<std::remove_const_t<std::remove_pointer_t<decltype(l)>>, 32>(s, y, l, rows, V, stride, params, u, w, tokens, probs);
     };
     if (dtype == VSL_DT_F32) go(static_cast<const float*>(logits));
     else go(static_cast<const vsl_half*>(logits));
