@@ -29,12 +29,12 @@
 
 namespace {
 
-constexpr int kThreads = 256, kDrawThreads = 1024;
+constexpr int kThreads = 256, kDrawThreads = 512;
 constexpr uint32_t kMaxSlices = 128, kMaxEpt = 32;
 constexpr uint32_t kMaxRowsV = kMaxSlices * kMaxEpt * kThreads;  // 2^20 tokens
 constexpr uint32_t kLeanK = 128;     // TOPK up to this k
 constexpr uint32_t kLeanCap = 256;   // TOPK: tokens a slice's list holds
-constexpr int kLeanRegs = 4, kDrawRegs = 8;  // tokens of a list that a thread holds
+constexpr int kLeanRegs = 4, kDrawRegs = 32;  // tokens of a list that a thread holds
 constexpr uint32_t kLeanList = kLeanRegs * kThreads, kListCap = kDrawRegs * kDrawThreads;  // tokens of a row's list
 constexpr uint32_t kFinish = 256;    // keys that are left to a key a thread
 constexpr uint32_t kBins = 512;     // of 1/8 in l / T; the last one takes all below e^-63.9 of the largest, never drawn
@@ -401,6 +401,60 @@ __device__ __forceinline__ void draw_exact(Shared& sh, uint32_t n, const RowPara
     });
 }
 
+// The same for at most a token a thread of k_rows_cut, list[0 .. n - 1]: put into their order by counting, so that each cut
+// is a number of tokens and the kept ones are the smallest of the three. 45 tokens (k = 40 of 32000) 14.8 us by draw_exact.
+__device__ __forceinline__ void draw_few(Shared& sh, uint64_t* list, uint32_t n, const RowParams& rp, double vmax, double u,
+                                         const RowOut& out) {
+    const uint32_t t = threadIdx.x;
+    const uint64_t mine = t < n ? list[t] : 0;
+    if (t >= n && t < ((n + 15) & ~15u)) list[t] = 0;  // up to a whole batch
+    const double w = weight_of(mine ? value_of(mine) : (float)vmax, vmax, rp.inv_t);
+    const bool heavy = w >= rp.m;
+    const uint64_t fixed = (uint64_t)(w * kListOne + 0.5);
+    __syncthreads();
+    uint32_t rank = 0;
+    for (uint32_t j0 = 0; j0 < n; j0 += 16) {
+        uint64_t x[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = list[j0 + j];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) rank += x[j] > mine;
+    }
+    // by rank: inverted index + 1 and weight; whether the weight is below min-p in the key's top bit
+    if (t < n) sh.keyed[rank] = Keyed{((mine & 0xFFFFFFFFull) + 1) | (heavy ? 0 : 1ull << 63), fixed};
+    __syncthreads();
+    const Keyed k = t < n ? sh.keyed[t] : Keyed{0, 0};
+    const bool first = t < min(n, rp.k);
+    uint64_t total;
+    const uint64_t incl = block_scan<kThreads>(sh, first ? k.weight : 0, total), before = incl - k.weight;
+    const uint64_t target_p = rp.cut_p ? (uint64_t)ceil((double)total * rp.p) : ~0ull;
+    const bool keep = first && (t == 0 || (before < target_p && !(k.key >> 63)));
+    // the kept ones are the ranks below the first that is not
+    const uint64_t m64 = __builtin_amdgcn_ballot_w64(keep);
+    if ((t & 63) == 0) sh.counts[t >> 6] = (uint32_t)__builtin_popcountll(m64);
+    __syncthreads();
+    uint32_t kept = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) kept += sh.counts[i];
+    if (t == kept - 1) sh.sel_left = incl;
+    if (t >= kept && t < ((kept + 7) & ~7u) && t < kFinish) sh.keyed[t] = Keyed{0, 0};
+    __syncthreads();
+    const uint64_t sum = sh.sel_left;
+    if (t >= kept) return;
+    uint64_t target = (uint64_t)((double)sum * u);
+    if (target >= sum) target = sum - 1;
+    const uint64_t key = k.key & ~(1ull << 63);
+    uint64_t below = 0;  // weights of lower indices
+    for (uint32_t j0 = 0; j0 < kept; j0 += 8) {
+        Keyed x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = sh.keyed[j0 + j];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) below += (x[j].key & ~(1ull << 63)) > key ? x[j].weight : 0;
+    }
+    if (below <= target && below + k.weight > target) put(out, ~(uint32_t)(key - 1), (double)k.weight / (double)sum);
+}
+
 // Bin of a value on the grid that all slices share: floor(8 l / T), as a double (exact to 2^53, and monotone above).
 __device__ __forceinline__ double bin_of(float v, double inv_t) { return floor((double)v * inv_t * 8.0); }
 __device__ __forceinline__ uint32_t bin_below(double top_bin, double bin) { return (uint32_t)fmin(top_bin - bin, (double)(kBins - 1)); }
@@ -415,6 +469,34 @@ __device__ __forceinline__ double one_less_exp(double y) {
     p = fma(p, y, 0.5);
     p = fma(p, y, 1.0);
     return -p * y;
+}
+
+// Values between vmax and vmin in kBins - 1 bins (NaN, of an infinite range, and what lies below: the last one).
+struct ValueBins {
+    float vmax, step;
+    __device__ ValueBins(float hi, float lo) : vmax(hi), step(hi - lo > 0.f ? (float)(kBins - 2) / (hi - lo) : 0.f) {}
+    __device__ uint32_t operator()(float x) const {
+        const float b = (vmax - x) * step;
+        return b < (float)(kBins - 1) ? (uint32_t)b : kBins - 1;
+    }
+};
+// The bin of counts that holds the k-th value, to *cut (unchanged where there are fewer); the first wave calls.
+__device__ __forceinline__ void find_kth(const uint32_t* count, uint32_t k, uint32_t* cut) {
+    constexpr int N = kBins / 64;
+    const uint32_t t = threadIdx.x;
+    uint32_t c[N];
+    uint64_t s = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        c[j] = count[t * N + j];
+        s += c[j];
+    }
+    uint64_t run = wave_scan(s) - s;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        if (run < k && run + c[j] >= k) *cut = t * N + j;
+        run += c[j];
+    }
 }
 
 template <class T, int EPT>
@@ -456,31 +538,12 @@ __global__ __launch_bounds__(kThreads) void k_rows_scan(const T* __restrict__ lo
     if (t == 0) rec->top = top;
     if (rp.mode == MODE_GREEDY || rp.mode == MODE_SUM) return;
     if (rp.mode == MODE_TOPK) {
-        // threads' maxima in 512 bins between their largest and their smallest: the bin of the k-th bounds the k-th token
-        const float vmax = top ? value_of(top) : 0.f, vmin = top ? value_of(~low_key) : 0.f, range = vmax - vmin;
-        const float step = range > 0.f ? (float)(kBins - 2) / range : 0.f;
-        auto bin = [&](float x) {
-            const float b = (vmax - x) * step;
-            return b < (float)(kBins - 1) ? (uint32_t)b : kBins - 1;  // NaN (an infinite range): the last
-        };
+        // threads' maxima in bins between their largest and their smallest: the bin of the k-th bounds the k-th token
+        const ValueBins bin(top ? value_of(top) : 0.f, top ? value_of(~low_key) : 0.f);
         uint32_t* count = reinterpret_cast<uint32_t*>(s_hist);
         if (best) atomicAdd(&count[bin(mx)], 1u);
         __syncthreads();
-        if (t < 64) {
-            uint32_t c[kBins / 64];
-            uint64_t s = 0;
-#pragma unroll
-            for (int j = 0; j < (int)kBins / 64; ++j) {
-                c[j] = count[t * (kBins / 64) + j];
-                s += c[j];
-            }
-            uint64_t run = wave_scan(s) - s;
-#pragma unroll
-            for (int j = 0; j < (int)kBins / 64; ++j) {
-                if (run < rp.k && run + c[j] >= rp.k) sh.sel_count = t * (kBins / 64) + j;
-                run += c[j];
-            }
-        }
+        if (t < 64) find_kth(count, rp.k, &sh.sel_count);
         __syncthreads();
         const uint32_t cut = sh.sel_count;  // the last bin: fewer than k threads hold a token
         uint64_t* list = ws.lists + (size_t)row * ws.list_stride + (size_t)slice * kLeanCap;
@@ -535,9 +598,21 @@ __global__ __launch_bounds__(kThreads) void k_rows_cut(const T* __restrict__ log
     __shared__ uint32_t s_cum_n[kBins];
     __shared__ uint32_t s_count[kMaxSlices], s_off[kMaxSlices], s_n, s_plo, s_phi, s_kb, s_base;
     const uint32_t row = blockIdx.y, slice = blockIdx.x, nsl = gridDim.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const RowParams rp = row_params(params[row], V);
-    if (rp.mode <= MODE_TOPK && slice != 0) return;
     SliceRec* rec = ws.rec + (size_t)row * nsl;
+    // requested together: parameters, u and the slices' records
+    const vsl_row_sampler ps = params[row];
+    const float uf = us[row];
+    uint64_t my_top = 0, top, bound = 0;
+    uint32_t my_count = 0;
+    float my_floor = -INFINITY;
+    if (t < nsl) {
+        my_top = rec[t].top;
+        my_count = rec[t].count;
+        my_floor = rec[t].floor_v;
+    }
+    const RowParams rp = row_params(ps, V);
+    const double u = uf > 0.f ? fmin((double)uf, 1.0 - 0x1p-24) : 0.0;  // NaN and below 0: 0; 1 and above: the float below 1
+    if (rp.mode <= MODE_TOPK && slice != 0) return;
     const T* l = logits + (size_t)row * stride;
     const uint32_t first = slice * (EPT * kThreads);
     float v[EPT];
@@ -549,13 +624,8 @@ __global__ __launch_bounds__(kThreads) void k_rows_cut(const T* __restrict__ log
         }
     }
     const RowOut out{tokens + row, probs ? probs + row : nullptr};
-    uint64_t my_top = 0, top, bound = 0;
-    uint32_t my_count = 0;
-    if (t < nsl) {
-        my_top = rec[t].top;
-        if (rp.mode == MODE_TOPK || rp.mode == MODE_HIST) my_count = rec[t].count;
-        if (rp.mode == MODE_TOPK) bound = rank_of(rec[t].floor_v, 0xFFFFFFFFu);  // the smallest rank of that value
-    }
+    // (count and floor_v are this call's in the modes that use them)
+    if (rp.mode == MODE_TOPK) bound = rank_of(my_floor, 0xFFFFFFFFu);  // the smallest rank of that value
     if (t < kMaxSlices) s_count[t] = my_count;
     if (t == 0) {
         s_n = 0;
@@ -601,11 +671,40 @@ __global__ __launch_bounds__(kThreads) void k_rows_cut(const T* __restrict__ log
         const bool whole = over || n > kLeanList;
         if (t == 0) ws.row[row].whole = whole;
         if (whole) return;
+        // each slice's k-th bounds them: of k = 40 from 16 slices 490 are left, so they are binned once more
+        uint32_t m = n;
+        uint64_t* few = s_list;
+        if (n > rp.k && n > 64) {
+            const ValueBins bin((float)vmax, bound ? value_of(bound) : (float)vmax);
+            few = reinterpret_cast<uint64_t*>(s_cum_w);
+#pragma unroll
+            for (uint32_t b = 0; b < kBins; b += NT) s_cum_n[b + t] = 0;
+            if (t == 0) {
+                sh.sel_count = kBins - 1;
+                sh.n = 0;
+            }
+            __syncthreads();
+            for (uint32_t i = t; i < n; i += NT) atomicAdd(&s_cum_n[bin(value_of(s_list[i]))], 1u);
+            __syncthreads();
+            if (t < 64) find_kth(s_cum_n, rp.k, &sh.sel_count);
+            __syncthreads();
+            const uint32_t cut = sh.sel_count;
+            for (uint32_t i = t; i < n; i += NT) {
+                const uint64_t x = s_list[i];
+                if (bin(value_of(x)) > cut) continue;
+                const uint32_t at = atomicAdd(&sh.n, 1u);
+                if (at < kThreads) few[at] = x;
+            }
+            __syncthreads();
+            m = sh.n;
+        }
+        if (m <= kThreads) {
+            draw_few(sh, few, m, rp, vmax, u, out);
+            return;
+        }
         uint64_t r[kLeanRegs];
 #pragma unroll
         for (int i = 0; i < kLeanRegs; ++i) r[i] = i * NT + t < n ? s_list[i * NT + t] : 0;
-        const float uf = us[row];
-        const double u = uf > 0.f ? fmin((double)uf, 1.0 - 0x1p-24) : 0.0;
         draw_exact<NT>(sh, n, rp, vmax, u, kListOne, out, n > rp.k, [&](auto f) {
 #pragma unroll
             for (int i = 0; i < kLeanRegs; ++i)
@@ -760,14 +859,19 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
     __shared__ Shared sh;
     __shared__ uint64_t s_slice[kMaxSlices];
     const uint32_t row = blockIdx.x, t = threadIdx.x;
-    const RowParams rp = row_params(params[row], V);
+    const vsl_row_sampler ps = params[row];
     const RowRec& rr = ws.row[row];
-    if (rp.mode == MODE_GREEDY || (rp.mode == MODE_TOPK && !rr.whole)) return;
+    // requested together with the parameters; each is this call's in the modes that use it
+    const uint32_t kb = rr.kb, plo = rr.plo, phi = rr.phi, rec_sure = rr.sure, rec_cut_k = rr.cut_k, k_left = rr.k_left, whole = rr.whole;
+    const double lo_total = rr.lo_total, hi_total = rr.hi_total;
+    const float uf = us[row];
+    const uint32_t listed = ws.counters[row];
+    const RowParams rp = row_params(ps, V);
+    if (rp.mode == MODE_GREEDY || (rp.mode == MODE_TOPK && !whole)) return;
     const T* l = logits + (size_t)row * stride;
     const RowOut out{tokens + row, probs ? probs + row : nullptr};
-    const float uf = us[row];
-    const double u = uf > 0.f ? fmin((double)uf, 1.0 - 0x1p-24) : 0.0;  // NaN and below 0: 0; 1 and above: the float below 1
-    const uint32_t n_list = rp.mode == MODE_HIST ? ws.counters[row] : 0;
+    const double u = uf > 0.f ? fmin((double)uf, 1.0 - 0x1p-24) : 0.0;
+    const uint32_t n_list = rp.mode == MODE_HIST ? listed : 0;
     const SliceRec* rec = ws.rec + (size_t)row * nsl;
     uint64_t top = 0, none = 0;
     double slice_sum = 0.0;
@@ -814,11 +918,10 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
     uint32_t cb = kBins - 2, sure = 0;  // the last bin that keeps a token; the bins kept whole are in the slices' sums
     const bool hist = rp.mode == MODE_HIST;
     if (hist) {
-        const uint32_t kb = rr.kb, plo = rr.plo, phi = rr.phi;
-        sure = rr.sure;
-        double total = rr.hi_total;
-        if (rr.cut_k) {
-            low = select_key<NT>(sh, n_list, rr.k_left, visit, [&](uint64_t rank, uint64_t& key, uint64_t& w) {
+        sure = rec_sure;
+        double total = hi_total;
+        if (rec_cut_k) {
+            low = select_key<NT>(sh, n_list, k_left, visit, [&](uint64_t rank, uint64_t& key, uint64_t& w) {
                 key = rank;
                 w = 1;
                 return row_bin(value_of(rank)) == kb;
@@ -826,7 +929,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
             if (rp.cut_p) {
                 uint64_t part = 0;
                 visit([&](uint64_t rank) { part += rank >= low && row_bin(value_of(rank)) == kb ? fixed(rank) : 0; });
-                total = rr.lo_total + (double)block_add<NT>(sh, part) / kListOne;
+                total = lo_total + (double)block_add<NT>(sh, part) / kListOne;
             }
         }
         if (rp.cut_p) {
