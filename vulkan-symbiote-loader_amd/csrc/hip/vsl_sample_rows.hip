@@ -34,8 +34,8 @@ constexpr uint32_t kMaxSlices = 128, kMaxEpt = 32;
 constexpr uint32_t kMaxRowsV = kMaxSlices * kMaxEpt * kThreads;  // 2^20 tokens
 constexpr uint32_t kLeanK = 128;     // TOPK up to this k
 constexpr uint32_t kLeanCap = 256;   // TOPK: tokens a slice's list holds
-constexpr int kLeanRegs = 4, kDrawRegs = 32;  // tokens of a list that a thread holds
-constexpr uint32_t kLeanList = kLeanRegs * kThreads, kListCap = kDrawRegs * kDrawThreads;  // tokens of a row's list
+constexpr int kLeanRegs = 4, kDrawRegs = 4;  // tokens of a list that a thread holds
+constexpr uint32_t kLeanList = kLeanRegs * kThreads, kListCap = 32768;  // tokens of a row's list: TOPK, HIST
 constexpr uint32_t kFinish = 256;    // keys that are left to a key a thread
 constexpr uint32_t kBins = 512;     // of 1/8 in l / T; the last one takes all below e^-63.9 of the largest, never drawn
 constexpr double kBinSpan = 0.11751;  // above 1 - exp(-1/8), the most that a weight lies below its bin's upper edge
@@ -215,8 +215,8 @@ __device__ __forceinline__ T block_scan(Shared& sh, T v, T& total) {
 }
 
 // The last key of the shortest run of keys, in descending order, whose measures reach `target` (the smallest key of all if
-// they do not). visit(f) calls f(rank) for each of the thread's elements; map(rank, key, measure) is false where one takes no
-// part; measures are integers, keys differ and are not 0. `n` bounds the elements that take part. Narrowed down by
+// they do not). visit(f) calls f(rank, weight) for each of the thread's elements, weight() being its fixed-point weight;
+// map(rank, weight, key, measure) is false where one takes no part; measures are integers, keys differ and are not 0. `n` bounds the elements that take part. Narrowed down by
 // digits of 8 bits, from the highest bit in which keys differ, until kFinish keys are left, whose threads sum up the
 // measures before their own. All threads call; 0 without elements.
 template <int NT, class Visit, class Map>
@@ -225,9 +225,9 @@ __device__ __forceinline__ uint64_t select_key(Shared& sh, uint32_t n, uint64_t 
     uint64_t prefix = 0, mask = 0;
     if (n > kFinish) {
         uint64_t all_or = 0, none_or = 0;  // bits that some key has, that some key lacks
-        visit([&](uint64_t rank) {
+        visit([&](uint64_t rank, auto weight) {
             uint64_t key, w;
-            if (map(rank, key, w)) {
+            if (map(rank, weight, key, w)) {
                 all_or |= key;
                 none_or |= ~key;
             }
@@ -260,9 +260,9 @@ __device__ __forceinline__ uint64_t select_key(Shared& sh, uint32_t n, uint64_t 
                 sh.counts[t] = 0;
             }
             __syncthreads();
-            visit([&](uint64_t rank) {
+            visit([&](uint64_t rank, auto weight) {
                 uint64_t key, w;
-                if (map(rank, key, w) && (key & mask) == prefix) {
+                if (map(rank, weight, key, w) && (key & mask) == prefix) {
                     const uint32_t d = (uint32_t)(key >> shift) & 255u;
                     atomicAdd(reinterpret_cast<unsigned long long*>(&sh.digits[d]), (unsigned long long)w);
                     atomicAdd(&sh.counts[d], 1u);
@@ -319,9 +319,9 @@ __device__ __forceinline__ uint64_t select_key(Shared& sh, uint32_t n, uint64_t 
         sh.sel_left = 0;
     }
     __syncthreads();
-    visit([&](uint64_t rank) {
+    visit([&](uint64_t rank, auto weight) {
         uint64_t key, w;
-        if (map(rank, key, w) && (key & mask) == prefix) {
+        if (map(rank, weight, key, w) && (key & mask) == prefix) {
             const uint32_t at = atomicAdd(&sh.n, 1u);
             if (at < kFinish) sh.keyed[at] = Keyed{key, w};
         }
@@ -360,44 +360,47 @@ __device__ __forceinline__ void put(const RowOut& o, uint32_t token, double prob
 
 __device__ __forceinline__ double weight_of(float v, double vmax, double inv_t) { return exp(((double)v - vmax) * inv_t); }
 
+__device__ __forceinline__ uint64_t fixed_weight(uint64_t rank, double vmax, double inv_t, double one) {
+    return (uint64_t)(weight_of(value_of(rank), vmax, inv_t) * one + 0.5);
+}
+
 // The draw over elements (visit and n as for select_key) that hold every token of the first k: the three cuts, then the index
-// at which the running sum passes u. `one`: the fixed point of weights.
+// at which the running sum passes u.
 template <int NT, class Visit>
-__device__ __forceinline__ void draw_exact(Shared& sh, uint32_t n, const RowParams& rp, double vmax, double u, double one, const RowOut& out,
-                           bool cut_k, Visit visit) {
-    auto fixed = [&](uint64_t rank) { return (uint64_t)(weight_of(value_of(rank), vmax, rp.inv_t) * one + 0.5); };
+__device__ __forceinline__ void draw_exact(Shared& sh, uint32_t n, const RowParams& rp, double vmax, double u, const RowOut& out,
+                                           bool cut_k, Visit visit) {
     uint64_t low = 1;  // the smallest kept rank key
-    if (cut_k) low = select_key<NT>(sh, n, rp.k, visit, [&](uint64_t rank, uint64_t& key, uint64_t& w) {
+    if (cut_k) low = select_key<NT>(sh, n, rp.k, visit, [&](uint64_t rank, auto, uint64_t& key, uint64_t& w) {
         key = rank;
         w = 1;
         return true;
     });
     if (rp.cut_p) {
         uint64_t s = 0;
-        visit([&](uint64_t rank) { s += rank >= low ? fixed(rank) : 0; });
+        visit([&](uint64_t rank, auto weight) { s += rank >= low ? weight() : 0; });
         const uint64_t target = (uint64_t)ceil((double)block_add<NT>(sh, s) * rp.p);
-        low = select_key<NT>(sh, n, target, visit, [&](uint64_t rank, uint64_t& key, uint64_t& w) {
+        low = select_key<NT>(sh, n, target, visit, [&](uint64_t rank, auto weight, uint64_t& key, uint64_t& w) {
             key = rank;
-            w = rank >= low ? fixed(rank) : 0;
+            w = rank >= low ? weight() : 0;
             return rank >= low;
         });
     }
     // min-p: the weight itself decides
     auto heavy = [&](uint64_t rank) { return weight_of(value_of(rank), vmax, rp.inv_t) >= rp.m; };
     uint64_t s = 0;
-    visit([&](uint64_t rank) { s += rank >= low && heavy(rank) ? fixed(rank) : 0; });
+    visit([&](uint64_t rank, auto weight) { s += rank >= low && heavy(rank) ? weight() : 0; });
     const uint64_t total = block_add<NT>(sh, s);
     uint64_t target = (uint64_t)((double)total * u) + 1;
     if (target > total) target = total;
-    const uint64_t at = select_key<NT>(sh, n, target, visit, [&](uint64_t rank, uint64_t& key, uint64_t& w) {
+    const uint64_t at = select_key<NT>(sh, n, target, visit, [&](uint64_t rank, auto weight, uint64_t& key, uint64_t& w) {
         if (rank < low || !heavy(rank)) return false;
-        w = fixed(rank);
+        w = weight();
         key = (rank & 0xFFFFFFFFull) + 1;  // the inverted index: ascending indices are descending keys (+ 1: not 0)
         return w != 0;
     });
     const uint32_t idx = ~(uint32_t)(at - 1);
-    visit([&](uint64_t rank) {
-        if (index_of(rank) == idx) put(out, idx, (double)fixed(rank) / (double)total);
+    visit([&](uint64_t rank, auto weight) {
+        if (index_of(rank) == idx) put(out, idx, (double)weight() / (double)total);
     });
 }
 
@@ -705,10 +708,10 @@ __global__ __launch_bounds__(kThreads) void k_rows_cut(const T* __restrict__ log
         uint64_t r[kLeanRegs];
 #pragma unroll
         for (int i = 0; i < kLeanRegs; ++i) r[i] = i * NT + t < n ? s_list[i * NT + t] : 0;
-        draw_exact<NT>(sh, n, rp, vmax, u, kListOne, out, n > rp.k, [&](auto f) {
+        draw_exact<NT>(sh, n, rp, vmax, u, out, n > rp.k, [&](auto f) {
 #pragma unroll
             for (int i = 0; i < kLeanRegs; ++i)
-                if (r[i]) f(r[i]);
+                if (r[i]) f(r[i], [&] { return fixed_weight(r[i], vmax, rp.inv_t, kListOne); });
         });
         return;
     }
@@ -785,11 +788,15 @@ __global__ __launch_bounds__(kThreads) void k_rows_cut(const T* __restrict__ log
     const bool cut_k = kb < kBins - 1 && s_cum_n[kb] != rp.k;
     const double hi_total = s_cum_w[kb], lo_total = cut_k ? (kb ? s_cum_w[kb - 1] : 0.0) : hi_total;
     if (rp.cut_p) {
-        const double lo = lo_total * rp.p * (1.0 - kBinNoise), hi = hi_total * rp.p * (1.0 - kBinNoise);
-        if (n2[0] && cw0 >= lo) atomicMin(&s_plo, 2 * t);
-        if (n2[1] && cw1 >= lo) atomicMin(&s_plo, 2 * t + 1);
-        if (n2[0] && cw0 >= hi) atomicMin(&s_phi, 2 * t);
-        if (n2[1] && cw1 >= hi) atomicMin(&s_phi, 2 * t + 1);
+        // the first bin with a token whose running sum reaches the share, a lane of each wave (one address for all lanes
+        // that reach it took 4 us)
+        auto first_of = [&](double share, uint32_t* at) {
+            const bool r0 = n2[0] && cw0 >= share, r1 = n2[1] && cw1 >= share;
+            const uint64_t some = __builtin_amdgcn_ballot_w64(r0 || r1);
+            if (some && lane == (uint32_t)__builtin_ctzll(some)) atomicMin(at, 2 * t + (r0 ? 0 : 1));
+        };
+        first_of(lo_total * rp.p * (1.0 - kBinNoise), &s_plo);
+        first_of(hi_total * rp.p * (1.0 - kBinNoise), &s_phi);
     }
     __syncthreads();
     const uint32_t plo = s_plo, phi = s_phi;
@@ -882,38 +889,42 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
     const uint64_t* list = ws.lists + (size_t)row * ws.list_stride;
     uint64_t r[kDrawRegs];
 #pragma unroll
-    for (int i = 0; i < kDrawRegs; ++i) r[i] = 0;
-    if (n_list <= kListCap) {
-#pragma unroll
-        for (int i = 0; i < kDrawRegs; ++i)
-            if (i * NT + t < n_list) r[i] = list[i * NT + t];
-    }
+    for (int i = 0; i < kDrawRegs; ++i) r[i] = i * NT + t < min(n_list, kListCap) ? list[i * NT + t] : 0;
     block_max2<NT>(sh, top, none);
     if (top == 0) return;
     const double vmax = (double)value_of(top);
+    // batches of eight elements, requested together
+    auto in_batches = [&](uint32_t from, uint32_t n, auto load, double one, auto f) {
+        for (uint32_t i0 = from + t; i0 < n; i0 += 8 * NT) {
+            uint64_t x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = i0 + j * NT < n ? load(i0 + j * NT) : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (x[j]) f(x[j], [&] { return fixed_weight(x[j], vmax, rp.inv_t, one); });
+        }
+    };
     if (rp.mode == MODE_TOPK || (rp.mode == MODE_HIST && (n_list > kListCap || fabs(vmax * rp.inv_t) > kMaxTop))) {
-        draw_exact<NT>(sh, V, rp, vmax, u, kRowOne, out, rp.k < V, [&](auto f) {
-            for (uint32_t i0 = t; i0 < V; i0 += 8 * NT) {
-                uint64_t x[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = i0 + j * NT < V ? rank_of(load_logit(l, i0 + j * NT), i0 + j * NT) : 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (x[j]) f(x[j]);
-            }
+        draw_exact<NT>(sh, V, rp, vmax, u, out, rp.k < V, [&](auto f) {
+            in_batches(0, V, [&](uint32_t i) { return rank_of(load_logit(l, i), i); }, kRowOne, f);
         });
         return;
     }
+    // the list's tokens: the first ones from registers, their weights taken once, the others from memory
+    uint64_t fixed[kDrawRegs];
+#pragma unroll
+    for (int i = 0; i < kDrawRegs; ++i) {
+        fixed[i] = 0;
+        if ((uint32_t)i * NT < n_list) fixed[i] = r[i] ? fixed_weight(r[i], vmax, rp.inv_t, kListOne) : 0;
+    }
     auto visit = [&](auto f) {
 #pragma unroll
-        for (int i = 0; i < kDrawRegs; ++i) {
-            if ((uint32_t)i * NT >= n_list) break;
-            if (r[i]) f(r[i]);
-        }
+        for (int i = 0; i < kDrawRegs; ++i)
+            if (r[i]) f(r[i], [&] { return fixed[i]; });
+        in_batches(kDrawRegs * NT, n_list, [&](uint32_t i) { return list[i]; }, kListOne, f);
     };
     const double top_bin = bin_of(value_of(top), rp.inv_t);
     auto row_bin = [&](float x) { return bin_below(top_bin, bin_of(x, rp.inv_t)); };
-    auto fixed = [&](uint64_t rank) { return (uint64_t)(weight_of(value_of(rank), vmax, rp.inv_t) * kListOne + 0.5); };
     uint64_t low = 1;  // the smallest kept rank key
     uint32_t cb = kBins - 2, sure = 0;  // the last bin that keeps a token; the bins kept whole are in the slices' sums
     const bool hist = rp.mode == MODE_HIST;
@@ -921,14 +932,14 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
         sure = rec_sure;
         double total = hi_total;
         if (rec_cut_k) {
-            low = select_key<NT>(sh, n_list, k_left, visit, [&](uint64_t rank, uint64_t& key, uint64_t& w) {
+            low = select_key<NT>(sh, n_list, k_left, visit, [&](uint64_t rank, auto, uint64_t& key, uint64_t& w) {
                 key = rank;
                 w = 1;
                 return row_bin(value_of(rank)) == kb;
             });
             if (rp.cut_p) {
                 uint64_t part = 0;
-                visit([&](uint64_t rank) { part += rank >= low && row_bin(value_of(rank)) == kb ? fixed(rank) : 0; });
+                visit([&](uint64_t rank, auto weight) { part += rank >= low && row_bin(value_of(rank)) == kb ? weight() : 0; });
                 total = lo_total + (double)block_add<NT>(sh, part) / kListOne;
             }
         }
@@ -938,10 +949,10 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
             while (pb < phi && rr.cum_w[pb] < target) ++pb;
             const double base = pb ? rr.cum_w[pb - 1] : 0.0;
             const uint64_t left = target > base ? (uint64_t)ceil((target - base) * kListOne) : 1;
-            const uint64_t cut = select_key<NT>(sh, n_list, left, visit, [&](uint64_t rank, uint64_t& key, uint64_t& w) {
+            const uint64_t cut = select_key<NT>(sh, n_list, left, visit, [&](uint64_t rank, auto weight, uint64_t& key, uint64_t& w) {
                 if (rank < low || row_bin(value_of(rank)) != pb) return false;
                 key = rank;
-                w = fixed(rank);
+                w = weight();
                 return true;
             });
             if (cut > low) low = cut;
@@ -952,10 +963,12 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
     // the slices' kept weights, in fixed point; of the bins that a cut divides, the list's tokens
     if (t < kMaxSlices) s_slice[t] = (uint64_t)(slice_sum * kRowOne + 0.5);
     __syncthreads();
-    visit([&](uint64_t rank) {
-        const double w = weight_of(value_of(rank), vmax, rp.inv_t);
-        if (row_bin(value_of(rank)) >= sure && kept(rank, w))
-            atomicAdd(reinterpret_cast<unsigned long long*>(&s_slice[index_of(rank) / SL]), (unsigned long long)(w * kRowOne + 0.5));
+    visit([&](uint64_t rank, auto weight) {
+        if (rank < low) return;
+        const uint32_t b = row_bin(value_of(rank));
+        if (b < sure || b > cb || (rp.m > 0.0 && weight_of(value_of(rank), vmax, rp.inv_t) < rp.m)) return;
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s_slice[index_of(rank) / SL]),
+                  (unsigned long long)(((double)weight() * (kRowOne / kListOne)) + 0.5));
     });
     __syncthreads();
     // the slice in which their running sum passes u
@@ -1014,7 +1027,7 @@ uint64_t up256(uint64_t b) { return (b + 255) & ~255ull; }
 // Elements a thread: enough slices to fill the CUs with the rows there are, at most kMaxSlices of them.
 uint32_t elements_per_thread(uint32_t rows, uint32_t V) {
     for (uint32_t e : {8u, 16u})
-        if ((uint64_t)rows * ((V + e * kThreads - 1) / (e * kThreads)) <= 1024 && (V + e * kThreads - 1) / (e * kThreads) <= kMaxSlices)
+        if ((uint64_t)rows * ((V + e * kThreads - 1) / (e * kThreads)) <= (e == 8 ? 32 : 1024) && (V + e * kThreads - 1) / (e * kThreads) <= kMaxSlices)
             return e;
     return kMaxEpt;
 }
