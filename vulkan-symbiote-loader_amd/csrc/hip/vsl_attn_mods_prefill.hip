@@ -22,6 +22,8 @@ struct PrefillArgs {
     uint32_t S, pos0, n_q, n_kv, cap, G, n_chunk;
     float to_u;    // |scale| / softcap, or |scale| * log2(e) without a cap
     float from_u;  // softcap * log2(e)
+    float near;    // |q.k| up to which the polynomial is tanh (0: never)
+    float poly[kTanhTerms];  // its coefficients, in q.k and times softcap * log2(e)
     int negative;  // scale < 0: q is taken with the other sign
     int out_mode;  // 0 fp16, 1 hi / lo fp16 planes, 2 fp16 + fp8 planes
     const float* slopes;
@@ -142,9 +144,9 @@ __device__ __noinline__ void rows_one_by_one(const PrefillArgs& a, uint32_t rb, 
 // A row's keys are a range [lo, hi); tiles that lie within the ranges of all of a wave's rows take no masks, and tiles
 // outside all of them are skipped. In the others a masked probability is 0; where V then holds an infinity or a NaN, whose
 // product with 0 would reach the sums, the query tile's rows are computed again, one by one (rows_one_by_one).
-template <int HD, bool QX2, bool CAP>
+template <int HD, bool QX2, bool PX2, bool CAP>
 __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
-    constexpr int CPR = HD / 8, NCH = kTK * CPR / kThreads, QP = QX2 ? 2 : 1, ND = HD / 32;
+    constexpr int CPR = HD / 8, NCH = kTK * CPR / kThreads, QP = QX2 ? 2 : 1, PP = PX2 ? 2 : 1, ND = HD / 32;
     static_assert(NCH >= 1 && kTK * CPR % kThreads == 0, "a tile divides over the block");
     __shared__ __attribute__((aligned(16))) vsl_half Ks[kBufs][kTK * HD];
     __shared__ __attribute__((aligned(16))) vsl_half Vs[kBufs][kTK * HD];
@@ -242,53 +244,27 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
         for (int v = 0; v < 16; ++v) o[t][v] = 0.f;
     float m = -INFINITY, l = 0.f;
 
+    // LDS byte addresses: the swizzle is an xor of the chunk, so all chunks that a lane reads of a row are its first one's
+    // address xor a constant. (The address passes through an empty asm, or the compiler keeps all of them in registers.)
+    typedef __attribute__((address_space(3))) const char* lds_ptr;
+    constexpr int kTile = kTK * HD * 2;  // bytes
+    const uint32_t k_at = (uint32_t)(uintptr_t)(lds_ptr)&Ks[0][swizzle<HD>(share * 32 + (lane & 31), lane >> 5)];
     auto qk = [&](int buf, float16v& st) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) st[v] = 0.f;
         half8 kf[HD / 16];
+        uint32_t at = k_at;
+        asm volatile("" : "+v"(at));
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c)
-            kf[c] = *reinterpret_cast<const half8*>(&Ks[buf][swizzle<HD>(share * 32 + (lane & 31), 2 * c + (lane >> 5))]);
+            kf[c] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>((lds_ptr)(uintptr_t)(at ^ (c * 32)) + buf * kTile);
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c)
 #pragma unroll
             for (int p = 0; p < QP; ++p) st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[c], qf[p][c], st, 0, 0, 0);
     };
-    // scores of tile t in log2 units, modified, masked where the tile is not within all rows' ranges
-    auto modify = [&](float16v& st, uint32_t t, bool whole) {
-        if constexpr (CAP) {
-            float um = 0.f;
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                st[v] *= a.to_u;
-                um = fmaxf(um, fabsf(st[v]));
-            }
-            if (__builtin_amdgcn_ballot_w64(um > kTanhNear)) {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) st[v] = tanh_any(st[v]) * a.from_u;
-            } else {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) st[v] = tanh_near(st[v]) * a.from_u;
-            }
-        } else {
-#pragma unroll
-            for (int v = 0; v < 16; ++v) st[v] *= a.to_u;
-        }
-        const uint32_t k0 = t * kTK + share * 32;
-        if (a.slopes) {
-#pragma unroll
-            for (int v = 0; v < 16; ++v)
-                st[v] = fmaf(-slope, fabsf((float)((int)(k0 + d_row(v, lane)) - (int)my_pos)), st[v]);
-        }
-        if (!whole) {
-#pragma unroll
-            for (int v = 0; v < 16; ++v) st[v] = k0 + d_row(v, lane) - lo < hi - lo ? st[v] : -INFINITY;
-        }
-    };
-    auto raise = [&](const float16v& st) {
-        float bm = st[0];
-#pragma unroll
-        for (int v = 1; v < 16; ++v) bm = fmaxf(bm, st[v]);
+    // the reference raised to scores of up to bm (log2 units), where that is far above it in some row
+    auto raise = [&](float bm) {
         if (__builtin_amdgcn_ballot_w64(bm - m > kLazy + kRoom)) {  // m = -inf: any finite score raises it
             float a0, a1;
             lane_pair<32>(bm, a0, a1);
@@ -302,40 +278,48 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
             m = mn;
         }
     };
-    auto probs = [&](const float16v& st, half8 (&pf)[QP][2]) {
-        const float ref = m == -INFINITY ? 0.f : m;
+    auto largest = [&](const float16v& st) {
+        float bm = st[0];
 #pragma unroll
-        for (int v = 0; v < 16; v += 2) {
-            const float p0 = fast_exp2(st[v] - ref), p1 = fast_exp2(st[v + 1] - ref);
-            l += p0;
-            l += p1;
-            const half2v hi2 = round2(p0, p1);
-            pf[0][v >> 3][v & 7] = hi2[0];
-            pf[0][v >> 3][(v & 7) + 1] = hi2[1];
-            if constexpr (QX2) {
-                const half2v lo2 = round2(p0 - (float)hi2[0], p1 - (float)hi2[1]);
-                pf[QP - 1][v >> 3][v & 7] = lo2[0];
-                pf[QP - 1][v >> 3][(v & 7) + 1] = lo2[1];
-            }
+        for (int v = 1; v < 16; ++v) bm = fmaxf(bm, st[v]);
+        return bm;
+    };
+    // two probabilities 2^x into their place in P^T; the row's sum takes them as they are multiplied
+    auto put_probs = [&](int v, float x0, float x1, half8 (&pf)[PP][2]) {
+        const half2v one = {(vsl_half)1.f, (vsl_half)1.f};
+        const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+        const half2v hi2 = round2(p0, p1);
+        pf[0][v >> 3][v & 7] = hi2[0];
+        pf[0][v >> 3][(v & 7) + 1] = hi2[1];
+        l = __builtin_amdgcn_fdot2(hi2, one, l, false);
+        if constexpr (PX2) {
+            const half2v lo2 = round2(p0 - (float)hi2[0], p1 - (float)hi2[1]);
+            pf[PP - 1][v >> 3][v & 7] = lo2[0];
+            pf[PP - 1][v >> 3][(v & 7) + 1] = lo2[1];
+            l = __builtin_amdgcn_fdot2(lo2, one, l, false);
         }
     };
     // V^T operand of dims 32 tt .., keys 16 half ..: slots of P^T are the keys (v / 4) 8 + (lane / 32) 4 + v % 4, which the
     // transpose reads match: lane i of 16 addresses V[r0 + i / 4][d0 + 4 (i % 4) ..] and receives V[r0 + j][d0 + i] as value j
-    const int gi = lane & 15, gdim = ((lane >> 4) & 1) * 16 + 4 * (gi & 3);
-    auto v_frag = [&](int buf, int tt, int half) {
-        const int d = tt * 32 + gdim, r = share * 32 + half * 16 + (lane >> 5) * 4 + (gi >> 2);
-        const half4 x0 = lds_read_tr16(&Vs[buf][swizzle<HD>(r, d >> 3) + (d & 7)]);
-        const half4 x1 = lds_read_tr16(&Vs[buf][swizzle<HD>(r + 8, d >> 3) + (d & 7)]);
+    const int gi = lane & 15, gdim = ((lane >> 4) & 1) * 16 + 4 * (gi & 3), grow = share * 32 + (lane >> 5) * 4 + (gi >> 2);
+    const uint32_t v_at = (uint32_t)(uintptr_t)(lds_ptr)&Vs[0][swizzle<HD>(grow, gdim >> 3) + (gdim & 7)];
+    auto v_frag = [&](uint32_t at, int buf, int tt, int half) {
+        const int off = buf * kTile + half * 16 * HD * 2;
+        const auto* p0 = (const vsl_half*)((lds_ptr)(uintptr_t)(at ^ (tt * 64)) + off);
+        const auto* p1 = (const vsl_half*)((lds_ptr)(uintptr_t)(at ^ (tt * 64) ^ (HD == 128 ? 128 : 64)) + off + 8 * HD * 2);
+        const half4 x0 = lds_read_tr16(p0), x1 = lds_read_tr16(p1);
         return half8{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
     };
-    auto pv = [&](int buf, const half8 (&pf)[QP][2]) {
+    auto pv = [&](int buf, const half8 (&pf)[PP][2]) {
+        uint32_t at = v_at;
+        asm volatile("" : "+v"(at));
 #pragma unroll
         for (int tt = 0; tt < ND; ++tt)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const half8 af = v_frag(buf, tt, half);
+                const half8 af = v_frag(at, buf, tt, half);
 #pragma unroll
-                for (int p = 0; p < QP; ++p) o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af, pf[p][half], o[tt], 0, 0, 0);
+                for (int p = 0; p < PP; ++p) o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af, pf[p][half], o[tt], 0, 0, 0);
             }
     };
     // infinities and NaN in this wave's half of the tile's V
@@ -345,48 +329,86 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
         for (int tt = 0; tt < ND; ++tt)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const u32x4 w = __builtin_bit_cast(u32x4, v_frag(buf, tt, half));
+                const u32x4 w = __builtin_bit_cast(u32x4, v_frag(v_at, buf, tt, half));
                 odd |= odd_halfs(w[0]) | odd_halfs(w[1]) | odd_halfs(w[2]) | odd_halfs(w[3]);
             }
         asm volatile("" ::: "memory");  // the products read V again: nothing of it is kept in registers here
     };
+    const float to_u = a.to_u, from_u = a.from_u, near = a.near;
+    auto poly = [&](float x) {  // x polynomial(x^2) = the capped score
+        const float z = x * x;
+        float p = a.poly[kTanhTerms - 1];
+#pragma unroll
+        for (int i = kTanhTerms - 2; i >= 0; --i) p = fmaf(p, z, a.poly[i]);
+        return p;
+    };
 
-    // Tiles t and t + 1 are in LDS and the scores of t in registers at the top of iteration t; t + 2 goes where t - 1 was.
+    // Tiles t and t + 1 are in LDS and the products of t in registers at the top of a step; t + 2 goes where t - 1 was.
     // Each wave waits for its own copies, then the block meets: all copies have landed and all waves are done with buffer t.
+    // BUF, NEXT, FREE: the buffers of t, t + 1 and t + 2.
+    float16v st;
+    auto step = [&](uint32_t t, int BUF, int NEXT, int FREE) {
+        issue(FREE, min(t + 2, t1 - 1));
+        const uint32_t k0 = t * kTK + share * 32;
+        const bool any = k0 < some_hi && k0 + 32 > some_lo, whole = k0 >= all_lo && k0 + 32 <= all_hi;  // wave-uniform
+        bool plain = any && whole && !a.slopes;
+        if (plain) {
+            // no score raises the reference; capped: of either sign, and the polynomial serves them all
+            if constexpr (CAP) {
+                float most = 0.f;
+#pragma unroll
+                for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(st[v]));
+                plain = !__builtin_amdgcn_ballot_w64(!(most <= near) || !(most * poly(most) - m <= kLazy + kRoom));
+            } else {
+                plain = !__builtin_amdgcn_ballot_w64(!(largest(st) * to_u - m <= kLazy + kRoom));
+            }
+        }
+        if (plain) {
+            float16v sn;
+            qk(NEXT, sn);
+            half8 pf[PP][2];
+#pragma unroll
+            for (int v = 0; v < 16; v += 2) {
+                if constexpr (CAP) put_probs(v, fmaf(st[v], poly(st[v]), -m), fmaf(st[v + 1], poly(st[v + 1]), -m), pf);
+                else put_probs(v, fmaf(st[v], to_u, -m), fmaf(st[v + 1], to_u, -m), pf);
+            }
+            pv(BUF, pf);
+            st = sn;
+        } else {
+            if (any) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    float x = st[v] * to_u;
+                    if constexpr (CAP) x = tanh_any(x) * from_u;
+                    x = fmaf(-slope, fabsf((float)((int)(k0 + d_row(v, lane)) - (int)my_pos)), x);
+                    st[v] = whole || k0 + d_row(v, lane) - lo < hi - lo ? x : -INFINITY;
+                }
+                raise(largest(st));
+                const float ref = m == -INFINITY ? 0.f : m;
+                half8 pf[PP][2];
+#pragma unroll
+                for (int v = 0; v < 16; v += 2) put_probs(v, st[v] - ref, st[v + 1] - ref, pf);
+                if (!whole) note_odd(BUF);
+                pv(BUF, pf);
+            }
+            qk(NEXT, st);
+        }
+        VSL_VMCNT_WAIT(0);
+        __syncthreads();
+    };
     if (t1 > t0) {
-        auto buf_of = [&](uint32_t t) { return (int)((t - t0) % kBufs); };
         issue(0, t0);
         issue(1, min(t0 + 1, t1 - 1));
         VSL_VMCNT_WAIT(0);
         __syncthreads();
-        float16v st;
         qk(0, st);
-        for (uint32_t t = t0; t < t1; ++t) {
-            issue(buf_of(t + 2), min(t + 2, t1 - 1));
-            const uint32_t k0 = t * kTK + share * 32;
-            const bool any = k0 < some_hi && k0 + 32 > some_lo, whole = k0 >= all_lo && k0 + 32 <= all_hi;  // wave-uniform
-            if (any && whole) {
-                float16v sn;
-                modify(st, t, true);
-                raise(st);
-                qk(buf_of(t + 1), sn);
-                half8 pf[QP][2];
-                probs(st, pf);
-                pv(buf_of(t), pf);
-                st = sn;
-            } else {
-                if (any) {
-                    modify(st, t, false);
-                    raise(st);
-                    half8 pf[QP][2];
-                    probs(st, pf);
-                    note_odd(buf_of(t));
-                    pv(buf_of(t), pf);
-                }
-                qk(buf_of(t + 1), st);
-            }
-            VSL_VMCNT_WAIT(0);
-            __syncthreads();
+        for (uint32_t t = t0;;) {  // in threes, so that the buffers are known
+            step(t, 0, 1, 2);
+            if (++t >= t1) break;
+            step(t, 1, 2, 0);
+            if (++t >= t1) break;
+            step(t, 2, 0, 1);
+            if (++t >= t1) break;
         }
     }
     // a row's weights lie in two lanes
@@ -415,7 +437,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
         __syncthreads();
         if (share) return;
         if (any_odd || s_lo[wave + 1]) {
-            if (active) rows_one_by_one<HD, QX2, CAP>(a, rb, h, chunk, t0 * kTK, t1 * kTK);
+            if (active) {
+                // the arguments where the launch put them: the address of `a` would move them all to scratch memory
+                const auto* args = reinterpret_cast<const PrefillArgs*>((const void*)__builtin_amdgcn_kernarg_segment_ptr());
+                rows_one_by_one<HD, QX2, CAP>(*args, rb, h, chunk, t0 * kTK, t1 * kTK);
+            }
             return;
         }
         const float mb = x[OSZ + lane], mm = fmaxf(m, mb), ref = mm == -INFINITY ? 0.f : mm;
@@ -523,26 +549,48 @@ extern "C" int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kca
     const float mag = std::fabs(scale);
     uint32_t chunks = workspace ? chunks_of(S, pos0, n_q, n_kv) : 1;
     if (chunks > 1 && ws_bytes < (uint64_t)chunks * S * n_q * (hd + 2) * 4) chunks = 1;
-    PrefillArgs a{static_cast<const vsl_half*>(q), static_cast<const vsl_half*>(kcache), static_cast<const vsl_half*>(vcache),
-                  S, pos0, n_q, n_kv, cap, G, chunks, capped ? mag / md.softcap : mag * kLog2e, md.softcap * kLog2e, scale < 0.f,
-                  out_dtype == VSL_DT_F16X2 ? 1 : out_dtype == VSL_DT_F16F8 ? 2 : 0, md.slopes, md.ranges,
-                  static_cast<vsl_half*>(out), static_cast<float*>(workspace),
-                  static_cast<float*>(workspace) + (size_t)chunks * S * n_q * hd};
+    PrefillArgs a{};
+    a.q = static_cast<const vsl_half*>(q);
+    a.kc = static_cast<const vsl_half*>(kcache);
+    a.vc = static_cast<const vsl_half*>(vcache);
+    a.S = S;
+    a.pos0 = pos0;
+    a.n_q = n_q;
+    a.n_kv = n_kv;
+    a.cap = cap;
+    a.G = G;
+    a.n_chunk = chunks;
+    a.to_u = capped ? mag / md.softcap : mag * kLog2e;
+    a.from_u = md.softcap * kLog2e;
+    // the polynomial in q.k itself, while its highest power of to_u is far from underflow (a cap of 50 at head_dim 128: 2^-9.1)
+    if (capped && a.to_u >= 0x1p-10f && a.to_u <= 0x1p10f) {
+        a.near = kTanhNear / a.to_u;
+        double f = (double)a.from_u * a.to_u;
+        for (int i = 0; i < kTanhTerms; ++i, f *= (double)a.to_u * a.to_u) a.poly[i] = (float)(kTanhPoly[i] * f);
+    }
+    a.negative = scale < 0.f;
+    a.out_mode = out_dtype == VSL_DT_F16X2 ? 1 : out_dtype == VSL_DT_F16F8 ? 2 : 0;
+    a.slopes = md.slopes;
+    a.ranges = md.ranges;
+    a.out = static_cast<vsl_half*>(out);
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + (size_t)chunks * S * n_q * hd;
     const dim3 grid((uint32_t)blocks, chunks);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    auto go = [&](auto hdc, auto x2, auto cc) {
+    // Probabilities in one fp16 plane where q or the output is one: their rounding is as large as the output's (with the split
+    // q and an fp16 output 2.5e-4 of the norm in all, 2.1e-4 by two planes), and a quarter of the products is saved.
+    const bool p2 = q_dtype == VSL_DT_F16X2 && out_dtype != VSL_DT_F16;
+    auto go = [&](auto hdc, auto x2, auto px2, auto cc) {
         constexpr int HD = decltype(hdc)::value;
-        k_prefill_mods<HD, decltype(x2)::value, decltype(cc)::value><<<grid, kThreads, 0, s>>>(a);
+        k_prefill_mods<HD, decltype(x2)::value, decltype(px2)::value, decltype(cc)::value><<<grid, kThreads, 0, s>>>(a);
         if (chunks > 1) k_join_prefill<HD><<<(uint32_t)(((uint64_t)S * n_q + 1024 / HD - 1) / (1024 / HD)), 256, 0, s>>>(a);
     };
+    using T = std::true_type;
+    using F = std::false_type;
     auto pick = [&](auto hdc) {
-        if (q_dtype == VSL_DT_F16X2) {
-            if (capped) go(hdc, std::true_type{}, std::true_type{});
-            else go(hdc, std::true_type{}, std::false_type{});
-        } else {
-            if (capped) go(hdc, std::false_type{}, std::true_type{});
-            else go(hdc, std::false_type{}, std::false_type{});
-        }
+        if (q_dtype == VSL_DT_F16) capped ? go(hdc, F{}, F{}, T{}) : go(hdc, F{}, F{}, F{});
+        else if (!p2) capped ? go(hdc, T{}, F{}, T{}) : go(hdc, T{}, F{}, F{});
+        else capped ? go(hdc, T{}, T{}, T{}) : go(hdc, T{}, T{}, F{});
     };
     if (hd == 128) pick(std::integral_constant<int, 128>{});
     else pick(std::integral_constant<int, 64>{});
