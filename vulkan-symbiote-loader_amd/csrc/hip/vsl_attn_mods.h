@@ -42,12 +42,18 @@ __device__ __forceinline__ half2v round2(float a, float b) {
     return h;
 }
 
-// LDS position (in halfs) of 16-byte chunk c of row r of a [rows][HD] tile: the chunks of a row exchanged so that the rows
-// that a wave reads at one column lie in different banks.
+// LDS position (in halfs) of 16-byte chunk c of row r of a [rows][HD] tile: the chunks of a row exchanged (an xor by bits of
+// the row) so that what a half wave reads at once lies in different banks: 16 bytes of one column of 16 rows (the operand
+// K), and 64 bytes of four rows (a transpose read of V). The row's two low bits move whole 64-byte groups; with its bits in
+// order (an xor by r & 15) four rows' 64 bytes fell onto the same 16 banks, 59 % of the LDS cycles of prompt attention.
+template <int HD>
+__device__ __forceinline__ constexpr int swizzle_bits(int r) {
+    if constexpr (HD == 128) return (r & 3) << 2 | ((r >> 2) & 3);          // 256-byte rows
+    else return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);                        // 128-byte rows: by pairs
+}
 template <int HD>
 __device__ __forceinline__ int swizzle(int r, int c) {
-    if constexpr (HD == 128) return r * HD + ((c ^ (r & 15)) * 8);  // 256-byte rows
-    else return r * HD + ((c ^ ((r >> 1) & 7)) * 8);                 // 128-byte rows: by pairs
+    return r * HD + ((c ^ swizzle_bits<HD>(r)) * 8);
 }
 
 // Whether a word of two halfs holds an infinity or a NaN: the carry out of an exponent of ones, in bit 15 of either half.

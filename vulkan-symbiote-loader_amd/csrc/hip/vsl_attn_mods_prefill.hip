@@ -306,7 +306,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
     auto v_frag = [&](uint32_t at, int buf, int tt, int half) {
         const int off = buf * kTile + half * 16 * HD * 2;
         const auto* p0 = (const vsl_half*)((lds_ptr)(uintptr_t)(at ^ (tt * 64)) + off);
-        const auto* p1 = (const vsl_half*)((lds_ptr)(uintptr_t)(at ^ (tt * 64) ^ (HD == 128 ? 128 : 64)) + off + 8 * HD * 2);
+        const auto* p1 = (const vsl_half*)((lds_ptr)(uintptr_t)(at ^ (tt * 64) ^ (swizzle_bits<HD>(8) * 16)) + off + 8 * HD * 2);
         const half4 x0 = lds_read_tr16(p0), x1 = lds_read_tr16(p1);
         return half8{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
     };
