@@ -20,11 +20,10 @@ struct PrefillArgs {
     const vsl_half* kc;
     const vsl_half* vc;
     uint32_t S, pos0, n_q, n_kv, cap, G, n_chunk;
-    float to_u;    // |scale| / softcap, or |scale| * log2(e) without a cap
+    float to_u;    // scale / softcap, or scale * log2(e) without a cap
     float from_u;  // softcap * log2(e)
     float near;    // |q.k| up to which the polynomial is tanh (0: never)
     float poly[kTanhTerms];  // its coefficients, in q.k and times softcap * log2(e)
-    int negative;  // scale < 0: q is taken with the other sign
     int out_mode;  // 0 fp16, 1 hi / lo fp16 planes, 2 fp16 + fp8 planes
     const float* slopes;
     const uint32_t* ranges;
@@ -97,7 +96,7 @@ __device__ __noinline__ void rows_one_by_one(const PrefillArgs& a, uint32_t rb, 
                 for (int d = 0; d < HD; ++d) {
                     float x = (float)q[d];
                     if constexpr (QX2) x += (float)q[(size_t)a.S * qw + d];
-                    sc = fmaf(a.negative ? -x : x, (float)Kb[(size_t)k * HD + d], sc);
+                    sc = fmaf(x, (float)Kb[(size_t)k * HD + d], sc);
                 }
             }
             sc *= a.to_u;
@@ -166,38 +165,47 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
     const size_t qplane = (size_t)a.S * qw;
     const uint32_t my_pos = a.pos0 + row;
 
-    // this row's keys [lo, lo + n); the wave's: within some row's and within all rows'
-    uint32_t lo, hi;
+    // this row's keys, the wave's (within some row's and within all rows') and the block's
+    uint32_t lo, hi, some_lo, some_hi, all_lo, all_hi, blk_lo, blk_hi;
     row_range(a, row, lo, hi);
-    uint32_t some_lo = hi > lo ? lo : 0xFFFFFFFFu, some_hi = hi, all_lo = hi > lo ? lo : 0xFFFFFFFFu, all_hi = hi;
+    if (!a.ranges) {
+        some_lo = all_lo = blk_lo = 0;
+        some_hi = active ? a.pos0 + min(a.S, rb * 32 + 32) : 0;
+        all_hi = a.pos0 + rb * 32 + 1;
+        blk_hi = a.pos0 + min(a.S, (min(grp * kTiles + kTiles, n_qt) - 1) / a.G * 32 + 32);
+    } else {
+        some_lo = all_lo = hi > lo ? lo : 0xFFFFFFFFu;
+        some_hi = all_hi = hi;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {  // the two half waves hold the same rows
-        some_lo = min(some_lo, (uint32_t)__shfl_xor((int)some_lo, o, 64));
-        some_hi = max(some_hi, (uint32_t)__shfl_xor((int)some_hi, o, 64));
-        all_lo = max(all_lo, (uint32_t)__shfl_xor((int)all_lo, o, 64));
-        all_hi = min(all_hi, (uint32_t)__shfl_xor((int)all_hi, o, 64));
-    }
-    if (!active) {
-        some_lo = 0xFFFFFFFFu;
-        some_hi = 0;
-    }
-    some_lo = __builtin_amdgcn_readfirstlane(some_lo);
-    some_hi = __builtin_amdgcn_readfirstlane(some_hi);
-    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-    if (lane == 0) {
-        s_lo[wave] = some_lo;
-        s_hi[wave] = some_hi;
-    }
-    __syncthreads();
-    uint32_t blk_lo = 0xFFFFFFFFu, blk_hi = 0;
+        for (int o = 16; o; o >>= 1) {  // the two half waves hold the same rows
+            some_lo = min(some_lo, (uint32_t)__shfl_xor((int)some_lo, o, 64));
+            some_hi = max(some_hi, (uint32_t)__shfl_xor((int)some_hi, o, 64));
+            all_lo = max(all_lo, (uint32_t)__shfl_xor((int)all_lo, o, 64));
+            all_hi = min(all_hi, (uint32_t)__shfl_xor((int)all_hi, o, 64));
+        }
+        if (!active) {
+            some_lo = 0xFFFFFFFFu;
+            some_hi = 0;
+        }
+        some_lo = __builtin_amdgcn_readfirstlane(some_lo);
+        some_hi = __builtin_amdgcn_readfirstlane(some_hi);
+        all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+        all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+        if (lane == 0) {
+            s_lo[wave] = some_lo;
+            s_hi[wave] = some_hi;
+        }
+        __syncthreads();
+        blk_lo = 0xFFFFFFFFu;
+        blk_hi = 0;
 #pragma unroll
-    for (int w = 0; w < kTiles * kShares; ++w) {
-        blk_lo = min(blk_lo, s_lo[w]);
-        blk_hi = max(blk_hi, s_hi[w]);
+        for (int w = 0; w < kTiles * kShares; ++w) {
+            blk_lo = min(blk_lo, s_lo[w]);
+            blk_hi = max(blk_hi, s_hi[w]);
+        }
+        blk_lo = __builtin_amdgcn_readfirstlane(blk_lo);
+        blk_hi = __builtin_amdgcn_readfirstlane(blk_hi);
     }
-    blk_lo = __builtin_amdgcn_readfirstlane(blk_lo);
-    blk_hi = __builtin_amdgcn_readfirstlane(blk_hi);
     // the block's key tiles, or its chunk of them
     uint32_t t0 = 0, t1 = 0;
     if (blk_hi > blk_lo) {
@@ -226,6 +234,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
             lds_load16(src + (size_t)min(t * kTK + crow[i], blk_hi - 1) * HD + coff[i], 0, buf + (i * kThreads + wave * 64) * 8);
     };
 
+    // the first tiles' copies run under what follows
+    if (t1 > t0) {
+        issue(Kb, Ks[0], t0);
+        issue(Kb, Ks[1], min(t0 + 1, t1 - 1));
+        issue(Vb, Vs[0], t0);
+    }
     // Q^T as the B operand: lane holds row lane % 32, dims 16 c + 8 (lane / 32) ..
     half8 qf[QP][HD / 16];
 #pragma unroll
@@ -233,7 +247,6 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c) {
             qf[p][c] = *reinterpret_cast<const half8*>(a.q + p * qplane + (size_t)row * qw + (size_t)h * HD + c * 16 + (lane >> 5) * 8);
-            if (a.negative) qf[p][c] = -qf[p][c];
         }
     const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.f;
     float16v o[ND];
@@ -352,14 +365,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
         const bool whole = whole_of(t);
         bool plain = whole && !a.slopes;
         if (plain) {
-            if constexpr (CAP) {
-                float most = 0.f;
+            float most = 0.f;
 #pragma unroll
-                for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(st[v]));
-                plain = !__builtin_amdgcn_ballot_w64(!(most <= near) || !(most * poly(most) - m <= kLazy + kRoom));
-            } else {
-                plain = !__builtin_amdgcn_ballot_w64(!(largest(st) * to_u - m <= kLazy + kRoom));
-            }
+            for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(st[v]));
+            plain = !__builtin_amdgcn_ballot_w64((CAP && !(most <= near)) || !(fabsf(most * (CAP ? poly(most) : to_u)) - m <= kLazy + kRoom));
         }
         if (plain) {
 #pragma unroll
@@ -410,9 +419,6 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
         __syncthreads();
     };
     if (t1 > t0) {
-        issue(Kb, Ks[0], t0);
-        issue(Kb, Ks[1], min(t0 + 1, t1 - 1));
-        issue(Vb, Vs[0], t0);
         VSL_VMCNT_WAIT(0);
         __syncthreads();
         if (any_of(t0)) qk(0, st);
@@ -498,17 +504,33 @@ __global__ __launch_bounds__(256) void k_join_prefill(PrefillArgs a) {
     const uint64_t at = (uint64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR, n = (uint64_t)a.S * a.n_q;
     if (at >= n) return;
     const int dim = threadIdx.x % LPR * 4;
-    float M = -INFINITY;
-    for (uint32_t c = 0; c < a.n_chunk; ++c) M = fmaxf(M, a.part_ml[(c * n + at) * 2]);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float L = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t c = 0; c < a.n_chunk; ++c) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (c * n + at) * 2);
-        const float4v v = *reinterpret_cast<const float4v*>(a.part_o + (c * n + at) * HD + dim);
-        const float f = fast_exp2(ml.x - ref);
-        L = fmaf(ml.y, f, L);
+    float M = -INFINITY, L = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t c0 = 0; c0 < a.n_chunk; c0 += 8) {  // eight chunks' sums are requested at once
+        float2 ml[8];
+        float4v v[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = fmaf(v[i], f, y[i]);
+        for (int j = 0; j < 8; ++j) {
+            const uint64_t c = min(c0 + j, a.n_chunk - 1);
+            ml[j] = *reinterpret_cast<const float2*>(a.part_ml + (c * n + at) * 2);
+            v[j] = *reinterpret_cast<const float4v*>(a.part_o + (c * n + at) * HD + dim);
+        }
+        float top = M;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, ml[j].x);
+        const float ref = top == -INFINITY ? 0.f : top, old = fast_exp2(M - ref);
+        M = top;
+        L *= old;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] *= old;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float f = c0 + j < a.n_chunk ? fast_exp2(ml[j].x - ref) : 0.f;
+            if (c0 + j < a.n_chunk) {
+                L = fmaf(ml[j].y, f, L);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = fmaf(v[j][i], f, y[i]);
+            }
+        }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
@@ -521,11 +543,12 @@ uint32_t blocks_of(uint32_t S, uint32_t n_q, uint32_t n_kv) {
     return (uint32_t)((n_qt + kTiles - 1) / kTiles * n_kv);
 }
 
-// Key chunks: as many as fill the CUs, none shorter than four tiles of the longest rows.
+// Key chunks: as many as fill the CUs, none shorter than three tiles of the longest rows; calls of less than 12 tiles are not
+// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8; 45 rows at 3001 26.1 in 16 chunks, 31.9 in 6).
 uint32_t chunks_of(uint32_t S, uint32_t pos0, uint32_t n_q, uint32_t n_kv) {
     const uint64_t blocks = blocks_of(S, n_q, n_kv), tiles = ((uint64_t)pos0 + S + kTK - 1) / kTK;
-    if (blocks >= 256) return 1;
-    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({256 / blocks, tiles / 4, 32}));
+    if (blocks >= 256 || tiles < 12) return 1;
+    return (uint32_t)std::min<uint64_t>({256 / blocks, tiles / 3, 32});
 }
 
 bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
@@ -563,7 +586,6 @@ extern "C" int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kca
     const uint64_t blocks = ((uint64_t)((S + 31) / 32) * G + kTiles - 1) / kTiles * n_kv;
     if (blocks > 1u << 23 || (uint64_t)S * n_q > 1u << 26) return vsl_unsupported("%s: %u rows in one call", fn, S);
     const bool capped = md.softcap > 0.f;
-    const float mag = std::fabs(scale);
     uint32_t chunks = workspace ? chunks_of(S, pos0, n_q, n_kv) : 1;
     if (chunks > 1 && ws_bytes < (uint64_t)chunks * S * n_q * (hd + 2) * 4) chunks = 1;
     PrefillArgs a{};
@@ -577,15 +599,14 @@ extern "C" int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kca
     a.cap = cap;
     a.G = G;
     a.n_chunk = chunks;
-    a.to_u = capped ? mag / md.softcap : mag * kLog2e;
+    a.to_u = capped ? scale / md.softcap : scale * kLog2e;
     a.from_u = md.softcap * kLog2e;
     // the polynomial in q.k itself, while its highest power of to_u is far from underflow (a cap of 50 at head_dim 128: 2^-9.1)
-    if (capped && a.to_u >= 0x1p-10f && a.to_u <= 0x1p10f) {
-        a.near = kTanhNear / a.to_u;
+    if (capped && std::fabs(a.to_u) >= 0x1p-10f && std::fabs(a.to_u) <= 0x1p10f) {
+        a.near = kTanhNear / std::fabs(a.to_u);
         double f = (double)a.from_u * a.to_u;
         for (int i = 0; i < kTanhTerms; ++i, f *= (double)a.to_u * a.to_u) a.poly[i] = (float)(kTanhPoly[i] * f);
     }
-    a.negative = scale < 0.f;
     a.out_mode = out_dtype == VSL_DT_F16X2 ? 1 : out_dtype == VSL_DT_F16F8 ? 2 : 0;
     a.slopes = md.slopes;
     a.ranges = md.ranges;
