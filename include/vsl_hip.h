@@ -548,11 +548,12 @@ int vsl_attn_prefill_kv4_window(const void* q, int q_dtype, const void* kcache, 
  *                   documents, prefixes that see themselves whole, windows, padding; NULL: 0 <= k <= p)
  * then softmax over the keys attended to.  `end` counts up to the positions that the call can know: pos0 + S in
  * vsl_attn_prefill_mods, ctrl->pos + 1 in vsl_attn_decode_mods.  A row without keys gives zeros.  What masked
- * positions hold, infinities and NaN among it, reaches no result; an infinity or a NaN among the values attended to makes
- * the outputs that it reaches infinite or NaN.
+ * positions hold, infinities and NaN among it, reaches no result.  Among the keys attended to, a NaN or an infinity makes
+ * its rows NaN, or a weight 0 or 1 where the sum of its products is infinite; among the values, it makes the outputs
+ * that it reaches infinite or NaN.
  * ------------------------------------------------------------------------------------------ */
 typedef struct vsl_attn_mods { /* host memory, read during the call; NULL for the call: no modification */
-    float softcap;             /* 0: none */
+    float softcap;             /* 0: none; scale / softcap and softcap * log2(e) finite */
     uint32_t pad;
     const float* slopes;
     const uint32_t* ranges;
@@ -562,9 +563,10 @@ typedef struct vsl_attn_mods { /* host memory, read during the call; NULL for th
 int vsl_attn_decode_mods(const float* q, const void* kcache, const void* vcache, int kv_dtype, uint32_t n_q, uint32_t n_kv,
                          uint32_t hd, uint32_t cap, float scale, uint32_t nsplit, float* part_o, float* part_ml, float* out,
                          vsl_ctrl* ctrl, const vsl_attn_mods* mods, void* stream);
-/* vsl_attn_prefill with modified scores: arguments as there, all pointers 16-byte aligned (slopes 4, ranges 8).  With a
- * workspace of vsl_attn_prefill_mods_ws_bytes calls of few rows split the keys over more blocks and join their sums in
- * a second launch; with less (NULL, 0) they run unsplit. */
+/* vsl_attn_prefill with modified scores: arguments as there, all pointers 16-byte aligned (slopes 4, ranges 8), up to
+ * 65535 heads.  The probabilities are split as q is where the output is F16X2 or F16F8; with an F16 output they are one fp16
+ * plane (2^-11 of each, as the output's own rounding).  With a workspace of vsl_attn_prefill_mods_ws_bytes calls of few
+ * rows split the keys over more blocks and join their sums in a second launch; with less (NULL, 0) they run unsplit. */
 int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kcache, const void* vcache, uint32_t S, uint32_t pos0,
                           uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t cap, float scale, void* out, int out_dtype,
                           const vsl_attn_mods* mods, void* workspace, uint64_t ws_bytes, void* stream);

@@ -77,7 +77,8 @@ def test_decode_attention(vsl, H):
     for kw in (dict(q=None), dict(kc=None), dict(vc=None), dict(po=None), dict(pml=None), dict(out=None), dict(ctrl=None),
                dict(nkv=0), dict(nq=0), dict(nq=7), dict(cap=0), dict(cap=0x80000000), dict(nsplit=0), dict(nsplit=1025),
                dict(q=ptr(4)), dict(kc=ptr(8)), dict(po=ptr(4)), dict(pml=ptr(4)), dict(out=ptr(8)), dict(softcap=-1.0),
-               dict(softcap=float("nan")), dict(softcap=float("inf")), dict(slopes=ptr(2)), dict(ranges=ptr(4))):
+               dict(softcap=float("nan")), dict(softcap=float("inf")), dict(softcap=3e38), dict(softcap=1e-40), dict(slopes=ptr(2)),
+               dict(ranges=ptr(4))):
         assert call(**kw) == -100, kw
     for kw in (dict(nq=18), dict(hd=96), dict(kvdt=7), dict(kvdt=2)):
         assert call(**kw) == -103, kw
@@ -91,9 +92,9 @@ def test_prompt_attention(vsl, H):
     assert call(S=0) == 0
     for kw in (dict(q=None), dict(kc=None), dict(vc=None), dict(out=None), dict(nkv=0), dict(nq=0), dict(nq=7), dict(q=ptr(8)),
                dict(out=ptr(8)), dict(kc=ptr(8)), dict(ws=ptr(8)), dict(cap=0x80000000), dict(softcap=-1.0), dict(slopes=ptr(1)),
-               dict(ranges=ptr(4))):
+               dict(ranges=ptr(4)), dict(softcap=3e38), dict(softcap=1e-40), dict(softcap=float("inf"))):
         assert call(**kw) == -100, kw
-    for kw in (dict(nq=18), dict(hd=96), dict(qdt=0), dict(odt=0), dict(qdt=3), dict(S=1 << 24, cap=1 << 25)):
+    for kw in (dict(nq=65536, nkv=8192), dict(nq=18), dict(hd=96), dict(qdt=0), dict(odt=0), dict(qdt=3), dict(S=1 << 24, cap=1 << 25)):
         assert call(**kw) == -103, kw
     assert call(pos0=61) == -104
     assert call(pos0=0xFFFFFFFF) == -104

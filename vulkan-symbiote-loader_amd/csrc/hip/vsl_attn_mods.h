@@ -1,5 +1,7 @@
 // vsl_attn_mods.h -- device helpers of attention with modified scores (vsl_attn_mods.hip, vsl_attn_mods_prefill.hip).
 #pragma once
+#include <cmath>
+
 #include "vsl_device.h"
 
 namespace attn_mods {
@@ -58,5 +60,10 @@ __device__ __forceinline__ int swizzle(int r, int c) {
 
 // Whether a word of two halfs holds an infinity or a NaN: the carry out of an exponent of ones, in bit 15 of either half.
 __device__ __forceinline__ uint32_t odd_halfs(uint32_t w) { return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
+
+// Whether a cap can be used with a scale: both factors of a score, scale / softcap and softcap * log2(e), within 32 bits.
+inline bool softcap_ok(float softcap, float scale) {
+    return softcap == 0.f || (softcap > 0.f && std::isfinite(softcap * kLog2e) && (std::isfinite(scale / softcap) || !std::isfinite(scale)));
+}
 
 }  // namespace attn_mods

@@ -422,7 +422,7 @@ extern "C" int vsl_attn_decode_mods(const float* q, const void* kcache, const vo
     const vsl_attn_mods none{};
     const vsl_attn_mods& md = mods ? *mods : none;
     if (!aligned_to(part_ml, 8) || !aligned_to(md.slopes, 4) || !aligned_to(md.ranges, 8)) return vsl_invalid("%s: misaligned pointer", fn);
-    if (!(md.softcap >= 0.f) || md.softcap == INFINITY) return vsl_invalid("%s: softcap %g", fn, (double)md.softcap);
+    if (!softcap_ok(md.softcap, scale)) return vsl_invalid("%s: softcap %g with scale %g", fn, (double)md.softcap, (double)scale);
     const bool capped = md.softcap > 0.f;
     const DecodeArgs a{q, kcache, vcache, G, cap, nsplit, capped ? scale / md.softcap : scale * kLog2e, md.softcap * kLog2e,
                        md.slopes, md.ranges, part_o, part_ml, ctrl};

@@ -573,7 +573,7 @@ extern "C" int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kca
         return vsl_unsupported("%s: dtypes %d/%d", fn, q_dtype, out_dtype);
     if (hd != 64 && hd != 128) return vsl_unsupported("%s: head_dim %u (64 or 128)", fn, hd);
     const uint32_t G = n_q / n_kv;
-    if (G > 8) return vsl_unsupported("%s: GQA ratio %u (supported 1..8)", fn, G);
+    if (G > 8 || n_q > 65535) return vsl_unsupported("%s: GQA ratio %u (supported 1..8), %u heads", fn, G, n_q);
     if (cap > 0x7FFFFFFFu) return vsl_invalid("%s: capacity %u", fn, cap);
     if ((uint64_t)pos0 + S > cap) return vsl_capacity("%s: %u positions from %u exceed capacity %u", fn, S, pos0, cap);
     for (const void* p : {q, kcache, vcache, static_cast<const void*>(out), static_cast<const void*>(workspace)})
@@ -581,7 +581,7 @@ extern "C" int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kca
     const vsl_attn_mods none{};
     const vsl_attn_mods& md = mods ? *mods : none;
     if (!aligned_to(md.slopes, 4) || !aligned_to(md.ranges, 8)) return vsl_invalid("%s: misaligned pointer", fn);
-    if (!(md.softcap >= 0.f) || md.softcap == INFINITY) return vsl_invalid("%s: softcap %g", fn, (double)md.softcap);
+    if (!softcap_ok(md.softcap, scale)) return vsl_invalid("%s: softcap %g with scale %g", fn, (double)md.softcap, (double)scale);
     if (S == 0) return VSL_OK;
     const uint64_t blocks = ((uint64_t)((S + 31) / 32) * G + kTiles - 1) / kTiles * n_kv;
     if (blocks > 1u << 23 || (uint64_t)S * n_q > 1u << 26) return vsl_unsupported("%s: %u rows in one call", fn, S);
