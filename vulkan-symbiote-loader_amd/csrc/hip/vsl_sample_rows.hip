@@ -6,7 +6,7 @@
 // of the three filters cuts that order somewhere, and the shortest run counts. So nothing is sorted: a cut is one 64-bit
 // rank key (the float's order, then the inverted index), found by narrowing down, and the draw walks the kept tokens by
 // index. Weights are summed in 64 bits (fixed point where atomics add them, so that no order of arrival matters): the
-// token is that of exact sums but where u falls within about 1e-12 of a border.
+// token is that of exact sums but where u falls within about 1e-10 of a border.
 //
 // Three launches. k_rows_scan reads the row's slices (a block each) once and leaves, by what the row asks for,
 //   GREEDY  the slice's maximum
@@ -20,6 +20,11 @@
 // row, finds the cuts among the collected tokens, the slice in which u falls and the token there. Where ties or ranges make
 // a list too long, it narrows the cuts down over the whole row instead. (The last block of the second kernel to arrive
 // took the draw at first: its fences write the L2 caches back, and a pass over one row of 131072 took 66 us.)
+//
+// What bounds it: for few rows the three launches and, within each, a chain of loads, sums over the block and code run for the
+// first time: 1 x 32000 with k = 40 14.9 us, 1 x 131072 with top-p 32 (7 + 11 + 14). For many the two passes over the logits
+// with 64-bit arithmetic per token, and a block a row in the draw: 64 x 131072 of mixed parameters 59 us (20.5 + 20.4 + 20.3;
+// one read of the 33.6 MB takes about 7).
 #include <float.h>
 
 #include <cmath>
@@ -38,8 +43,7 @@ constexpr int kLeanRegs = 4, kDrawRegs = 4;  // tokens of a list that a thread h
 constexpr uint32_t kLeanList = kLeanRegs * kThreads, kListCap = 32768;  // tokens of a row's list: TOPK, HIST
 constexpr uint32_t kFinish = 256;    // keys that are left to a key a thread
 constexpr uint32_t kBins = 512;     // of 1/8 in l / T; the last one takes all below e^-63.9 of the largest, never drawn
-constexpr double kBinSpan = 0.11751;  // above 1 - exp(-1/8), the most that a weight lies below its bin's upper edge
-constexpr int kBinFrac = 36;        // weights in a bin: what they lie below it, in units of 2^-36
+constexpr int kBinFrac = 36;        // weights in a bin: what they lie below its upper edge (up to .1175), in units of 2^-36
 constexpr int kCountShift = 46;     // 8192 of them stay below 2^46; the count above
 // Sums over bins are off by up to 2^-37 of their weights, and a little of the grid's rounding. Cuts and draws that meet a
 // border exactly (equal logits: whole numbers of equal weights) are decided as exact sums are: a share is reached a little
@@ -76,21 +80,22 @@ struct SliceRec {
     uint32_t count;   // TOPK: tokens found (kLeanCap of them stored); HIST: bins up to the last one that holds a token
     float floor_v;    // TOPK: all tokens of the slice at or above this value are in its list, and there are k of them (-inf: all)
     double sum;       // weights kept for sure
-    uint64_t pad;
 };
 
 struct RowRec {
     uint32_t kb, plo, phi, sure;  // HIST: the bin of the k-th token, those in which the top-p cut can fall, those kept whole
     uint32_t cut_k, k_left;       // whether k ends within its bin, and how many of that bin's tokens count
     double lo_total, hi_total;    // the first k tokens' weights, without and with the k-th's bin
-    uint32_t whole, pad;          // TOPK: the lists do not hold the tokens
+    uint32_t whole;               // TOPK: the lists do not hold the tokens
     double cum_w[kBins];          // HIST: weights up to and with each bin
 };
 
+constexpr uint32_t kCounter = 64;
 struct Work {
     SliceRec* rec;       // [rows][nsl]
     RowRec* row;         // [rows]
-    uint32_t* counters;  // [rows]: the row list's length
+    uint32_t* counters;  // [rows][kCounter]: the row list's length, in lines of their own (side by side 1024 blocks' atomics
+                         // met in two lines)
     uint64_t* lists;     // [rows][list_stride]
     uint64_t* hist;      // [rows][nsl][kBins]
     uint32_t list_stride;
@@ -518,7 +523,7 @@ __global__ __launch_bounds__(kThreads) void k_rows_scan(const T* __restrict__ lo
         v[i] = e < V ? load_logit(l, e) : -INFINITY;
     }
     const RowParams rp = row_params(params[row], V);
-    if (slice == 0 && t == 0) ws.counters[row] = 0;
+    if (slice == 0 && t == 0) ws.counters[row * kCounter] = 0;
 #pragma unroll
     for (uint32_t b = 0; b < kBins; b += kThreads) s_hist[b + t] = 0;
     if (t == 0) {
@@ -572,10 +577,11 @@ __global__ __launch_bounds__(kThreads) void k_rows_scan(const T* __restrict__ lo
         if (v[i] == -INFINITY) continue;
         const double x = (double)v[i] * rp.inv_t, b = floor(x * 8.0);
         const uint32_t r = bin_below(top_bin, b);
-        const double d = fmin(fmax(one_less_exp(x - (b + 1.0) * 0.125), 0.0), kBinSpan);
+        // what the weight lies below its bin's upper edge, 0 .. 1 - exp(-1/8), in units of 2^-36: the mantissa behind 2^16
+        const double d = one_less_exp(x - (b + 1.0) * 0.125) + 0x1p16;
         if (r < kBins - 1)
             atomicAdd(reinterpret_cast<unsigned long long*>(&s_hist[r]),
-                      (unsigned long long)((1ull << kCountShift) + (uint64_t)(d * (double)(1ull << kBinFrac) + 0.5)));
+                      __builtin_bit_cast(unsigned long long, d) + ((1ull << kCountShift) - __builtin_bit_cast(unsigned long long, 0x1p16)));
     }
     __syncthreads();
     uint64_t* h = ws.hist + ((size_t)row * nsl + slice) * kBins;
@@ -801,11 +807,8 @@ __global__ __launch_bounds__(kThreads) void k_rows_cut(const T* __restrict__ log
     __syncthreads();
     const uint32_t plo = s_plo, phi = s_phi;
     const uint32_t mb = rp.m > 0.0 ? bin_below(top_bin, fmin(floor((vmax * rp.inv_t + log(rp.m)) * 8.0), top_bin)) : kBins - 1;
-    auto wanted = [&](uint32_t b) {
-        return b < kBins - 1 && ((cut_k && b == kb) || (rp.cut_p && b >= plo && b <= phi) || b == mb);
-    };
-    // Bins that are kept whole whatever the cuts turn out to be: those before the first in which one can fall (all bins up to
-    // that of the last one kept are then wanted ones). This slice's weight in them, and its tokens in the wanted bins.
+    // Bins that are kept whole whatever the cuts turn out to be: those before the first in which one can fall (from there
+    // on to the last one kept, a cut can fall in every bin, or they lie below min-p). This slice's weight in them, and its tokens in the others.
     const uint32_t sure = min(min(rp.cut_p ? plo : kBins - 1, mb), kb < kBins - 1 ? (cut_k ? kb : kb + 1) : kBins - 1);
     if (slice == 0) {
         RowRec& r = ws.row[row];
@@ -837,15 +840,27 @@ __global__ __launch_bounds__(kThreads) void k_rows_cut(const T* __restrict__ log
         if (t == 0) rec[slice].sum = sum;
     }
     uint64_t* list = ws.lists + (size_t)row * ws.list_stride;
+    // The tokens of bins b1 .. b2, by value: within some 2^-21 of an edge also the next bins' (the draw takes no token by its
+    // being listed). In 64 bits, bin by bin, this took 9000 cycles of 32 tokens a thread.
     uint32_t mine = 0;
+    auto collect = [&](uint32_t b1, uint32_t b2) {
+        b2 = min(b2, kBins - 2);
+        if (b1 > b2) return;
+        const double eighth = 0.125 * (double)ps.temperature, most = (double)FLT_MAX;
+        const double lo = fmax((top_bin - (double)b2) * eighth, -most), hi = fmin((top_bin - (double)b1 + 1.0) * eighth, most);
+        const float mid = (float)(0.5 * (lo + hi));
+        const float reach = (float)fmin((hi - lo) * 0.5 + (hi - lo + fabs(lo + hi)) * 0x1p-22 + 0x1p-140, most);
 #pragma unroll
-    for (int i = 0; i < EPT; ++i)
-        if (v[i] != -INFINITY && wanted(bin_below(top_bin, bin_of(v[i], rp.inv_t)))) mine |= 1u << i;
+        for (int i = 0; i < EPT; ++i) mine |= fabsf(v[i] - mid) <= reach ? 1u << i : 0u;
+    };
+    if (rp.cut_p) collect(plo, phi);
+    if (cut_k) collect(kb, kb);
+    if (mb <= min(rp.cut_p ? phi : kBins, kb)) collect(mb, mb);
     uint64_t total;
     const uint64_t c = __builtin_popcount(mine);
     uint32_t at = (uint32_t)(block_scan<NT>(sh, c, total) - c);
     if (total == 0) return;
-    if (t == 0) s_base = atomicAdd(&ws.counters[row], (uint32_t)total);
+    if (t == 0) s_base = atomicAdd(&ws.counters[row * kCounter], (uint32_t)total);
     __syncthreads();
     at += s_base;
 #pragma unroll
@@ -872,7 +887,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
     const uint32_t kb = rr.kb, plo = rr.plo, phi = rr.phi, rec_sure = rr.sure, rec_cut_k = rr.cut_k, k_left = rr.k_left, whole = rr.whole;
     const double lo_total = rr.lo_total, hi_total = rr.hi_total;
     const float uf = us[row];
-    const uint32_t listed = ws.counters[row];
+    const uint32_t listed = ws.counters[row * kCounter];
     const RowParams rp = row_params(ps, V);
     if (rp.mode == MODE_GREEDY || (rp.mode == MODE_TOPK && !whole)) return;
     const T* l = logits + (size_t)row * stride;
@@ -996,7 +1011,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         const float x = from + i < V ? load_logit(l, from + i) : -INFINITY;
-        const double wx = weight_of(x, vmax, rp.inv_t);
+        const double wx = weight_of(x, vmax, rp.inv_t);  // (a select: zeroed in a branch, an element kept an old value in the built code)
         w[i] = x != -INFINITY && kept(rank_of(x, from + i), wx) ? wx : 0.0;
         mine += w[i];
         if (w[i] > 0.0) last = from + i + 1;
@@ -1044,7 +1059,7 @@ Layout layout(uint32_t rows, uint32_t V) {
     y.list_stride = y.nsl * kLeanCap > wide ? y.nsl * kLeanCap : wide;
     y.row = up256((uint64_t)rows * y.nsl * sizeof(SliceRec));
     y.counters = y.row + up256((uint64_t)rows * sizeof(RowRec));
-    y.lists = y.counters + up256((uint64_t)rows * 4);
+    y.lists = y.counters + up256((uint64_t)rows * kCounter * 4);
     y.hist = y.lists + up256((uint64_t)rows * y.list_stride * 8);
     y.bytes = y.hist + up256((uint64_t)rows * y.nsl * kBins * 8);
     return y;
