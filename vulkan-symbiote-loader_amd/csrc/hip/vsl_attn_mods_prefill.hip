@@ -137,9 +137,15 @@ __device__ __noinline__ void rows_one_by_one(const PrefillArgs& a, uint32_t rb, 
 
 // Block: four query tiles (32 rows of one head) of one KV head, numbered row block by row block with the group's heads
 // within; two waves each, a wave the one 32-key half of every 64-key tile. Key tiles go from the cache straight into LDS
-// (three buffers, two tiles ahead), shared by the four query tiles. Per tile a wave takes S^T = K Q^T (its D: a lane has 16
-// keys of one row), turns the scores into probabilities, which are the operand of O^T += V^T P^T as they lie, and the next
-// tile's S^T is issued under this one's softmax. The halves are joined through LDS at the end.
+// (two buffers of K and two of V), shared by the four query tiles. Per tile a wave takes S^T = K Q^T (its D: a lane has 16
+// keys of one row) and turns the scores into probabilities, which are the operand of O^T += V^T P^T as they lie. The halves
+// are joined through LDS at the end.
+// Bound: the two products (4 head_dim flops a row and key, half as many again for a split q) and, for every score, 12 vector
+// instructions of cap, exponential and rounding, which take longer than its share of the products; LDS, which each query tile
+// reads anew, is as busy as the matrix cores. 2048 rows at 6144 of the 8B shape, split q, cap 30: 442 to 475 us (the same
+// code on different days), 760 to 820 TFLOP/s in products where a large plain fp16 product reaches 1080 on this card; the matrix
+// cores are busy a third of the time, the vector unit 45 %, LDS without bank conflicts. Slower there: the next tile's K in
+// registers ahead of its product 451 to 470, products and vector code mixed by scheduling barriers 485.
 // A row's keys are a range [lo, hi); tiles that lie within the ranges of all of a wave's rows take no masks, and tiles
 // outside all of them are skipped. In the others a masked probability is 0; where V then holds an infinity or a NaN, whose
 // product with 0 would reach the sums, the query tile's rows are computed again, one by one (rows_one_by_one).
@@ -544,7 +550,7 @@ uint32_t blocks_of(uint32_t S, uint32_t n_q, uint32_t n_kv) {
 }
 
 // Key chunks: as many as fill the CUs, none shorter than three tiles of the longest rows; calls of less than 12 tiles are not
-// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8; 45 rows at 3001 26.1 in 16 chunks, 31.9 in 6).
+// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8; 45 rows at 3001 26.1 in 16 chunks, 27.9 in 12, 35.7 in 6).
 uint32_t chunks_of(uint32_t S, uint32_t pos0, uint32_t n_q, uint32_t n_kv) {
     const uint64_t blocks = blocks_of(S, n_q, n_kv), tiles = ((uint64_t)pos0 + S + kTK - 1) / kTK;
     if (blocks >= 256 || tiles < 12) return 1;

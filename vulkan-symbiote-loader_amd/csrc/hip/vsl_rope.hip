@@ -21,7 +21,9 @@ struct FreqArgs {
 };
 
 // A thread takes a pair at kRun positions: the angles of the first and of one step in 64 bits, the others by rotation
-// (each adds under 2^-52; 16 of them stay 2^24 below the results' rounding).
+// (each adds under 2^-52; 16 of them stay 2^24 below the results' rounding). Bound by the
+// stores: 131072 positions of 32 pairs 8.1 us (4.1 TB/s); of fewer values a thread's two sincos show: 32768 positions of 64 pairs
+// 6.0 us (2.8 TB/s). Runs of 8 / 32 / 64 positions 8.9 / 8.2 / 9.6 and 6.3 / 6.5 / 7.8, of 4 11.8 and 7.7.
 constexpr uint32_t kRun = 16;
 __global__ __launch_bounds__(256) void k_rope_tables(uint32_t half, uint32_t pos0, uint32_t rows, FreqArgs a, double rot,
                                                      const float* __restrict__ ff, float* __restrict__ cos_out,
@@ -77,7 +79,8 @@ struct PartArgs {
 
 // Four dims a lane; bpr blocks a row. A rotated dim's partner is read again from the row (it is in the same lines).
 // VEC: rot % 8 == 0, so that four dims are rotated or not as one and the partners and angles of a halves' rotation are
-// aligned vectors; otherwise dim by dim.
+// aligned vectors; otherwise dim by dim. Bound by the projection read and the outputs written: 2048 rows of the 8B shape, 32
+// dims of each head, split q: 92 MB in 16.4 us (5.6 TB/s; 19.2 with the launch); a token 4.0.
 template <bool VEC, int QM, typename KT, bool DEC>
 __global__ __launch_bounds__(256) void k_rope_part(PartArgs a, uint32_t bpr, vsl_ctrl* ctrl) {
     const uint32_t s = blockIdx.x / bpr;
