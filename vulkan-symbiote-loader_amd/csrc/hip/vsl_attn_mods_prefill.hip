@@ -142,8 +142,8 @@ __device__ __noinline__ void rows_one_by_one(const PrefillArgs& a, uint32_t rb, 
 // are joined through LDS at the end.
 // Bound: the two products (4 head_dim flops a row and key, half as many again for a split q) and, for every score, 12 vector
 // instructions of cap, exponential and rounding, which take longer than its share of the products; LDS, which each query tile
-// reads anew, is as busy as the matrix cores. 2048 rows at 6144 of the 8B shape, split q, cap 30: 442 to 475 us (the same
-// code on different days), 760 to 820 TFLOP/s in products where a large plain fp16 product reaches 1080 on this card; the matrix
+// reads anew, is as busy as the matrix cores. 2048 rows at 6144 of the 8B shape, split q, cap 30: 432 us (cards and days
+// differ by 7 %), 835 TFLOP/s in products where a large plain fp16 product reaches 1080 on this card; the matrix
 // cores are busy a third of the time, the vector unit 45 %, LDS without bank conflicts. Slower there: the next tile's K in
 // registers ahead of its product 451 to 470, products and vector code mixed by scheduling barriers 485.
 // A row's keys are a range [lo, hi); tiles that lie within the ranges of all of a wave's rows take no masks, and tiles
@@ -271,11 +271,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) st[v] = 0.f;
         half8 kf[HD / 16];
-        uint32_t at = k_at;
+        uint32_t at = k_at + buf * kTile;
         asm volatile("" : "+v"(at));
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c)
-            kf[c] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>((lds_ptr)(uintptr_t)(at ^ (c * 32)) + buf * kTile);
+            kf[c] = *reinterpret_cast<const __attribute__((address_space(3))) half8*>((lds_ptr)(uintptr_t)(at ^ (c * 32)));
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c)
 #pragma unroll
@@ -302,6 +302,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
         for (int v = 1; v < 16; ++v) bm = fmaxf(bm, st[v]);
         return bm;
     };
+    auto largest_size = [&](const float16v& st) __attribute__((always_inline)) {
+        float most = 0.f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(st[v]));
+        return most;
+    };
     // two probabilities 2^x into their place in P^T; the row's sum takes them as they are multiplied
     auto put_probs = [&](int v, float x0, float x1, half8 (&pf)[PP][2]) __attribute__((always_inline)) {
         const half2v one = {(vsl_half)1.f, (vsl_half)1.f};
@@ -321,21 +327,21 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
     // transpose reads match: lane i of 16 addresses V[r0 + i / 4][d0 + 4 (i % 4) ..] and receives V[r0 + j][d0 + i] as value j
     const int gi = lane & 15, gdim = ((lane >> 4) & 1) * 16 + 4 * (gi & 3), grow = share * 32 + (lane >> 5) * 4 + (gi >> 2);
     const uint32_t v_at = (uint32_t)(uintptr_t)(lds_ptr)&Vs[0][swizzle<HD>(grow, gdim >> 3) + (gdim & 7)];
-    auto v_frag = [&](uint32_t at, int buf, int tt, int half) {
-        const int off = buf * kTile + half * 16 * HD * 2;
+    auto v_frag = [&](uint32_t at, int tt, int half) {
+        const int off = half * 16 * HD * 2;
         const auto* p0 = (const vsl_half*)((lds_ptr)(uintptr_t)(at ^ (tt * 64)) + off);
         const auto* p1 = (const vsl_half*)((lds_ptr)(uintptr_t)(at ^ (tt * 64) ^ (swizzle_bits<HD>(8) * 16)) + off + 8 * HD * 2);
         const half4 x0 = lds_read_tr16(p0), x1 = lds_read_tr16(p1);
         return half8{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
     };
     auto pv = [&](int buf, const half8 (&pf)[PP][2]) __attribute__((always_inline)) {
-        uint32_t at = v_at;
+        uint32_t at = v_at + buf * kTile;
         asm volatile("" : "+v"(at));
 #pragma unroll
         for (int tt = 0; tt < ND; ++tt)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const half8 af = v_frag(at, buf, tt, half);
+                const half8 af = v_frag(at, tt, half);
 #pragma unroll
                 for (int p = 0; p < PP; ++p) o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af, pf[p][half], o[tt], 0, 0, 0);
             }
@@ -347,7 +353,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
         for (int tt = 0; tt < ND; ++tt)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const u32x4 w = __builtin_bit_cast(u32x4, v_frag(v_at, buf, tt, half));
+                const u32x4 w = __builtin_bit_cast(u32x4, v_frag(v_at + buf * kTile, tt, half));
                 odd |= odd_halfs(w[0]) | odd_halfs(w[1]) | odd_halfs(w[2]) | odd_halfs(w[3]);
             }
         asm volatile("" ::: "memory");  // the products read V again: nothing of it is kept in registers here
@@ -371,9 +377,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
         const bool whole = whole_of(t);
         bool plain = whole && !a.slopes;
         if (plain) {
-            float most = 0.f;
-#pragma unroll
-            for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(st[v]));
+            const float most = largest_size(st);
             plain = !__builtin_amdgcn_ballot_w64((CAP && !(most <= near)) || !(fabsf(most * (CAP ? poly(most) : to_u)) - m <= kLazy + kRoom));
         }
         if (plain) {
@@ -384,12 +388,26 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
             }
             return;
         }
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            float x = st[v] * to_u;
-            if constexpr (CAP) x = tanh_any(x) * from_u;
+        auto masked = [&](int v, float x) {
             x = fmaf(-slope, fabsf((float)((int)(k0 + d_row(v, lane)) - (int)my_pos)), x);
-            st[v] = whole || k0 + d_row(v, lane) - lo < hi - lo ? x : -INFINITY;
+            return whole || k0 + d_row(v, lane) - lo < hi - lo ? x : -INFINITY;
+        };
+        if constexpr (!CAP) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) st[v] = masked(v, st[v] * to_u);
+        } else {  // a wave's first tile comes here, its code fetched for the first time: what does not apply is branched over (45
+                  // rows at 3001 25.8 -> 23.3 us; without a cap, where less is to skip, 512 packed rows 12.4 -> 13.2)
+            if (__builtin_amdgcn_ballot_w64(!(largest_size(st) <= near))) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) st[v] = tanh_any(st[v] * to_u) * from_u;
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) st[v] *= poly(st[v]);
+            }
+            if (!whole || a.slopes) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) st[v] = masked(v, st[v]);
+            }
         }
         raise(largest(st));
         const float ref = m == -INFINITY ? 0.f : m;
@@ -430,12 +448,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
         if (any_of(t0)) qk(0, st);
         __syncthreads();  // (K of t0 is overwritten in the first turn but one)
         if (late) __syncthreads();
-        for (uint32_t t = t0;;) {  // in pairs, so that the buffers are known
-            step(t, 0);
-            if (++t >= t1) break;
-            step(t, 1);
-            if (++t >= t1) break;
-        }
+        int buf = 0;
+        for (uint32_t t = t0; t < t1; ++t, buf ^= 1) step(t, buf);
         if (!late) __syncthreads();
         VSL_VMCNT_WAIT(0);
         __syncthreads();  // the buffers are free
@@ -458,7 +472,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
 #pragma unroll
             for (int t = 0; t < ND; ++t)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) x[(t * 16 + v) * 64 + lane] = o[t][v];
+                for (int v = 0; v < 16; v += 4)
+                    *reinterpret_cast<float4v*>(x + ((t * 4 + v / 4) * 64 + lane) * 4) = float4v{o[t][v], o[t][v + 1], o[t][v + 2], o[t][v + 3]};
             s_m[w][lane] = m;
             s_l[w][lane] = l;
             if (lane == 0) s_lo[wave] = any_odd;
@@ -480,7 +495,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
 #pragma unroll
         for (int t = 0; t < ND; ++t)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) o[t][v] = o[t][v] * ca + x[(t * 16 + v) * 64 + lane] * cb;
+            for (int v = 0; v < 16; v += 4) {
+                const float4v y = *reinterpret_cast<const float4v*>(x + ((t * 4 + v / 4) * 64 + lane) * 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[t][v + i] = o[t][v + i] * ca + y[i] * cb;
+            }
     }
     if (!active || my_s >= a.S) return;
     if (a.n_chunk > 1) {
@@ -550,7 +569,7 @@ uint32_t blocks_of(uint32_t S, uint32_t n_q, uint32_t n_kv) {
 }
 
 // Key chunks: as many as fill the CUs, none shorter than three tiles of the longest rows; calls of less than 12 tiles are not
-// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8; 45 rows at 3001 26.1 in 16 chunks, 27.9 in 12, 35.7 in 6).
+// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8; 45 rows at 3001 26.1 in 16 chunks, 27.9 in 12, 35.7 in 6; 23.3 now).
 uint32_t chunks_of(uint32_t S, uint32_t pos0, uint32_t n_q, uint32_t n_kv) {
     const uint64_t blocks = blocks_of(S, n_q, n_kv), tiles = ((uint64_t)pos0 + S + kTK - 1) / kTK;
     if (blocks >= 256 || tiles < 12) return 1;
