@@ -28,8 +28,8 @@ struct PrefillArgs {
     const float* slopes;
     const uint32_t* ranges;
     vsl_half* out;
-    float* part_o;   // [n_chunk][S][n_q][HD], where the keys are split over blocks
-    float* part_ml;  // [n_chunk][S][n_q][2]
+    float* part_o;   // where the keys are split over blocks: a query tile's sums as its wave holds them (part_tile)
+    float* part_ml;  // its rows' references and weights
 };
 
 // row of D of a 32 x 32 product in register v
@@ -56,6 +56,13 @@ __device__ __forceinline__ void store4(const PrefillArgs& a, uint32_t s, uint32_
     }
     *reinterpret_cast<half4*>(a.out + at) = hv;
     if (a.out_mode == 1) *reinterpret_cast<half4*>(a.out + plane + at) = lv;
+}
+
+// A query tile's place in the partial sums, [n_chunk][row blocks][n_q]: 32 rows of references and weights, and of sums as
+// [HD / 4 groups of four dims in pairs][64 lanes][4], so that a wave stores and loads whole lines. (By rows, every store of a
+// wave went to 64 of them: 45 rows at 3001 23.3 us.)
+__device__ __forceinline__ size_t part_tile(const PrefillArgs& a, uint32_t chunk, uint32_t rb, uint32_t h) {
+    return ((size_t)chunk * ((a.S + 31) / 32) + rb) * a.n_q + h;
 }
 
 // keys [lo, hi) of row s
@@ -117,10 +124,13 @@ __device__ __noinline__ void rows_one_by_one(const PrefillArgs& a, uint32_t rb, 
         }
         if (m == -INFINITY && l != 0.f) m = 0.f;
         if (a.n_chunk > 1) {
-            const size_t at = ((size_t)chunk * a.S + s) * a.n_q + h;
+            const size_t tile = part_tile(a, chunk, rb, h);
 #pragma unroll
-            for (int i = 0; i < D; ++i) a.part_o[at * HD + 64 * i + lane] = acc[i];
-            if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+            for (int i = 0; i < D; ++i) {
+                const uint32_t dim = 64 * i + lane;
+                a.part_o[tile * 32 * HD + (dim / 8 * 64 + (dim & 4) * 8 + s % 32) * 4 + dim % 4] = acc[i];
+            }
+            if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + (tile * 32 + s % 32) * 2) = make_float2(m, l);
             continue;
         }
         // four consecutive dims in every fourth lane, for the output's types
@@ -503,13 +513,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
     }
     if (!active || my_s >= a.S) return;
     if (a.n_chunk > 1) {
-        const size_t at = ((size_t)chunk * a.S + my_s) * a.n_q + h;
+        const size_t tile = part_tile(a, chunk, rb, h);
 #pragma unroll
         for (int t = 0; t < ND; ++t)
 #pragma unroll
-            for (int v = 0; v < 16; v += 4)
-                *reinterpret_cast<float4v*>(a.part_o + at * HD + t * 32 + d_row(v, lane)) = float4v{o[t][v], o[t][v + 1], o[t][v + 2], o[t][v + 3]};
-        if (lane < 32) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+            for (int v = 0; v < 16; v += 4)  // dims 32 t + 2 v + 4 (lane / 32) ..
+                *reinterpret_cast<float4v*>(a.part_o + tile * 32 * HD + ((t * 4 + v / 4) * 64 + lane) * 4) =
+                    float4v{o[t][v], o[t][v + 1], o[t][v + 2], o[t][v + 3]};
+        if (lane < 32) *reinterpret_cast<float2*>(a.part_ml + (tile * 32 + lane) * 2) = make_float2(m, l);
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -522,22 +533,23 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
         }
 }
 
-// The chunks' sums of a row and head joined: HD / 4 lanes each.
+// The chunks' sums joined: a block 32 dims of a query tile, a wave 8 of them, its lanes as those that stored them.
 template <int HD>
 __global__ __launch_bounds__(256) void k_join_prefill(PrefillArgs a) {
-    constexpr uint32_t LPR = HD / 4;
-    const uint64_t at = (uint64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR, n = (uint64_t)a.S * a.n_q;
-    if (at >= n) return;
-    const int dim = threadIdx.x % LPR * 4;
+    constexpr uint32_t ND = HD / 32;
+    const uint32_t lane = threadIdx.x & 63, group = blockIdx.x % ND * 4 + threadIdx.x / 64;
+    const uint32_t in_chunk = blockIdx.x / ND, h = in_chunk % a.n_q, s = in_chunk / a.n_q * 32 + (lane & 31);
+    if (s >= a.S) return;
+    const size_t n = (size_t)((a.S + 31) / 32) * a.n_q;
     float M = -INFINITY, L = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
     for (uint32_t c0 = 0; c0 < a.n_chunk; c0 += 8) {  // eight chunks' sums are requested at once
         float2 ml[8];
         float4v v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const uint64_t c = min(c0 + j, a.n_chunk - 1);
-            ml[j] = *reinterpret_cast<const float2*>(a.part_ml + (c * n + at) * 2);
-            v[j] = *reinterpret_cast<const float4v*>(a.part_o + (c * n + at) * HD + dim);
+            const size_t tile = min(c0 + j, a.n_chunk - 1) * n + in_chunk;
+            ml[j] = *reinterpret_cast<const float2*>(a.part_ml + (tile * 32 + (lane & 31)) * 2);
+            v[j] = *reinterpret_cast<const float4v*>(a.part_o + tile * 32 * HD + (group * 64 + lane) * 4);
         }
         float top = M;
 #pragma unroll
@@ -560,7 +572,7 @@ __global__ __launch_bounds__(256) void k_join_prefill(PrefillArgs a) {
     const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] *= inv;
-    store4<HD>(a, (uint32_t)(at / a.n_q), (uint32_t)(at % a.n_q), dim, y);
+    store4<HD>(a, s, h, (int)(group * 8 + lane / 32 * 4), y);
 }
 
 uint32_t blocks_of(uint32_t S, uint32_t n_q, uint32_t n_kv) {
@@ -569,12 +581,15 @@ uint32_t blocks_of(uint32_t S, uint32_t n_q, uint32_t n_kv) {
 }
 
 // Key chunks: as many as fill the CUs, none shorter than three tiles of the longest rows; calls of less than 12 tiles are not
-// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8; 45 rows at 3001 26.1 in 16 chunks, 27.9 in 12, 35.7 in 6; 23.3 now).
+// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8; 45 rows at 3001 26.1 in 16 chunks, 27.9 in 12, 35.7 in 6; 21.6 now).
 uint32_t chunks_of(uint32_t S, uint32_t pos0, uint32_t n_q, uint32_t n_kv) {
     const uint64_t blocks = blocks_of(S, n_q, n_kv), tiles = ((uint64_t)pos0 + S + kTK - 1) / kTK;
     if (blocks >= 256 || tiles < 12) return 1;
     return (uint32_t)std::min<uint64_t>({256 / blocks, tiles / 3, 32});
 }
+
+// A chunk's partial sums: whole query tiles.
+uint64_t part_bytes(uint32_t S, uint32_t n_q, uint32_t hd) { return ((uint64_t)S + 31) / 32 * 32 * n_q * (hd + 2) * 4; }
 
 bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
@@ -583,7 +598,7 @@ bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t
 extern "C" uint64_t vsl_attn_prefill_mods_ws_bytes(uint32_t S, uint32_t pos0, uint32_t n_q, uint32_t n_kv, uint32_t hd) {
     if (S == 0 || n_kv == 0 || n_q == 0 || n_q % n_kv || (hd != 64 && hd != 128)) return 0;
     const uint64_t c = chunks_of(S, pos0, n_q, n_kv);
-    return c > 1 ? c * S * n_q * (hd + 2) * 4 : 0;
+    return c > 1 ? c * part_bytes(S, n_q, hd) : 0;
 }
 
 extern "C" int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kcache, const void* vcache, uint32_t S,
@@ -611,8 +626,9 @@ extern "C" int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kca
     const uint64_t blocks = ((uint64_t)((S + 31) / 32) * G + kTiles - 1) / kTiles * n_kv;
     if (blocks > 1u << 23 || (uint64_t)S * n_q > 1u << 26) return vsl_unsupported("%s: %u rows in one call", fn, S);
     const bool capped = md.softcap > 0.f;
+    const uint32_t n_rb = (S + 31) / 32;
     uint32_t chunks = workspace ? chunks_of(S, pos0, n_q, n_kv) : 1;
-    if (chunks > 1 && ws_bytes < (uint64_t)chunks * S * n_q * (hd + 2) * 4) chunks = 1;
+    if (chunks > 1 && ws_bytes < chunks * part_bytes(S, n_q, hd)) chunks = 1;
     PrefillArgs a{};
     a.q = static_cast<const vsl_half*>(q);
     a.kc = static_cast<const vsl_half*>(kcache);
@@ -637,7 +653,7 @@ extern "C" int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kca
     a.ranges = md.ranges;
     a.out = static_cast<vsl_half*>(out);
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + (size_t)chunks * S * n_q * hd;
+    a.part_ml = a.part_o + (size_t)chunks * n_rb * 32 * n_q * hd;
     const dim3 grid((uint32_t)blocks, chunks);
     hipStream_t s = static_cast<hipStream_t>(stream);
     // Probabilities in one fp16 plane where q or the output is one: their rounding is as large as the output's (with the split
@@ -646,7 +662,7 @@ extern "C" int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kca
     auto go = [&](auto hdc, auto x2, auto px2, auto cc) {
         constexpr int HD = decltype(hdc)::value;
         k_prefill_mods<HD, decltype(x2)::value, decltype(px2)::value, decltype(cc)::value><<<grid, kThreads, 0, s>>>(a);
-        if (chunks > 1) k_join_prefill<HD><<<(uint32_t)(((uint64_t)S * n_q + 1024 / HD - 1) / (1024 / HD)), 256, 0, s>>>(a);
+        if (chunks > 1) k_join_prefill<HD><<<n_rb * n_q * (HD / 32), 256, 0, s>>>(a);
     };
     using T = std::true_type;
     using F = std::false_type;
