@@ -152,8 +152,8 @@ __device__ __noinline__ void rows_one_by_one(const PrefillArgs& a, uint32_t rb, 
 // are joined through LDS at the end.
 // Bound: the two products (4 head_dim flops a row and key, half as many again for a split q) and, for every score, 12 vector
 // instructions of cap, exponential and rounding, which take longer than its share of the products; LDS, which each query tile
-// reads anew, is as busy as the matrix cores. 2048 rows at 6144 of the 8B shape, split q, cap 30: 432 us (cards and days
-// differ by 7 %), 835 TFLOP/s in products where a large plain fp16 product reaches 1080 on this card; the matrix
+// reads anew, is as busy as the matrix cores. 2048 rows at 6144 of the 8B shape, split q, cap 30: 423 us (cards and days
+// differ by 7 %), 850 TFLOP/s in products where a large plain fp16 product reaches 1080 on this card; the matrix
 // cores are busy a third of the time, the vector unit 45 %, LDS without bank conflicts. Slower there: the next tile's K in
 // registers ahead of its product 451 to 470, products and vector code mixed by scheduling barriers 485.
 // A row's keys are a range [lo, hi); tiles that lie within the ranges of all of a wave's rows take no masks, and tiles
@@ -166,6 +166,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
     __shared__ __attribute__((aligned(16))) vsl_half s_tiles[2 * kBufs][kTK * HD];  // K's buffers, then V's
     vsl_half(*Ks)[kTK * HD] = s_tiles;
     vsl_half(*Vs)[kTK * HD] = s_tiles + kBufs;
+    __shared__ __attribute__((aligned(16))) vsl_half s_q[kTiles][QP * 32 * HD];
     __shared__ uint32_t s_lo[kTiles * kShares], s_hi[kTiles * kShares];
     __shared__ float s_m[kTiles][64], s_l[kTiles][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -250,20 +251,21 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
             lds_load16(src + (size_t)min(t * kTK + crow[i], blk_hi - 1) * HD + coff[i], 0, buf + (i * kThreads + wave * 64) * 8);
     };
 
-    // the first tiles' copies run under what follows
+    // q's rows by way of LDS too, each wave half of its query tile's: a lane needs 16 bytes of its row at a time, and 32 rows'
+    // lines for each such load kept a block for 4000 cycles (45 rows at 3001 21.6 -> 19.2 us). The first tiles' copies follow.
+    constexpr int NQ = QP * CPR / 4;
     if (t1 > t0) {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const int at = (share * NQ + i) * 64, P = at + lane, r = P / CPR % 32;
+            lds_load16(a.q + P / (32 * CPR) * qplane + (size_t)min(rb * 32 + r, a.S - 1) * qw + (size_t)h * HD + (swizzle<HD>(r, P % CPR) - r * HD), 0,
+                       &s_q[wave / kShares][at * 8]);
+        }
         issue(Kb, Ks[0], t0);
         issue(Kb, Ks[1], min(t0 + 1, t1 - 1));
         issue(Vb, Vs[0], t0);
     }
-    // Q^T as the B operand: lane holds row lane % 32, dims 16 c + 8 (lane / 32) ..
     half8 qf[QP][HD / 16];
-#pragma unroll
-    for (int p = 0; p < QP; ++p)
-#pragma unroll
-        for (int c = 0; c < HD / 16; ++c) {
-            qf[p][c] = *reinterpret_cast<const half8*>(a.q + p * qplane + (size_t)row * qw + (size_t)h * HD + c * 16 + (lane >> 5) * 8);
-        }
     const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.f;
     float16v o[ND];
 #pragma unroll
@@ -455,6 +457,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
     if (t1 > t0) {
         VSL_VMCNT_WAIT(0);
         __syncthreads();
+        // Q^T as the B operand: lane holds row lane % 32, dims 16 c + 8 (lane / 32) ..
+#pragma unroll
+        for (int p = 0; p < QP; ++p)
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c)
+                qf[p][c] = *reinterpret_cast<const half8*>(&s_q[wave / kShares][p * 32 * HD + swizzle<HD>(lane & 31, 2 * c + (lane >> 5))]);
         if (any_of(t0)) qk(0, st);
         __syncthreads();  // (K of t0 is overwritten in the first turn but one)
         if (late) __syncthreads();
@@ -581,7 +589,7 @@ uint32_t blocks_of(uint32_t S, uint32_t n_q, uint32_t n_kv) {
 }
 
 // Key chunks: as many as fill the CUs, none shorter than three tiles of the longest rows; calls of less than 12 tiles are not
-// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8; 45 rows at 3001 26.1 in 16 chunks, 27.9 in 12, 35.7 in 6; 21.6 now).
+// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8; 45 rows at 3001 26.1 in 16 chunks, 27.9 in 12, 35.7 in 6; 19.2 now).
 uint32_t chunks_of(uint32_t S, uint32_t pos0, uint32_t n_q, uint32_t n_kv) {
     const uint64_t blocks = blocks_of(S, n_q, n_kv), tiles = ((uint64_t)pos0 + S + kTK - 1) / kTK;
     if (blocks >= 256 || tiles < 12) return 1;
