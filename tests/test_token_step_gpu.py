@@ -263,3 +263,54 @@ def test_sequences_at_once(vsl, H, dev):
     vsl.check(H.vsl_graph_destroy(graph))
     for st in streams:
         vsl.check(H.vsl_stream_destroy(st))
+
+
+def test_offsets_past_32_bits(vsl, H, dev):
+    """Caches of more than 2^31 values and rows of logits more than 2^32 bytes apart: bit for bit what small ones give."""
+    rng = np.random.default_rng(23)
+    m = Model(vsl, H, dev, rng)
+    S, small, large = 3, 128, 64 * 33000
+    assert N_KV * 4 * large * HD > 2 ** 31
+    x, at = dev.put(rng.normal(0, 1, (S, N_Q + 8 * N_KV, HD)).astype(np.float32)), dev.put(np.array([7, 8, 9], np.uint32))
+    row, place = dev.put(rng.normal(0, 1, (N_Q + 8 * N_KV, HD)).astype(np.float32)), dev.put(np.array([10], np.uint32))
+    old = [dev.torch.randn(4 * N_KV, 60, HD, device="cuda").half() for _ in range(2)]
+    p, nkv, outs = dev.p, 4 * N_KV, []
+    for cap in (small, large):
+        kc, vc = (dev.empty((nkv, cap, HD), np.float16) for _ in range(2))
+        pos0 = cap - 4
+        for c, o in zip((kc, vc), old):
+            c[:, pos0 - 60:pos0] = o
+        rg = dev.put(np.array([(pos0 - 60, pos0 + 1), (pos0 - 1, pos0 + 2), (0, 0)], np.uint32))
+        mods = vsl.AttnMods(softcap=SOFTCAP, slopes=p(m.slopes), ranges=p(rg))
+        q, out = dev.empty((2, S, N_Q, HD), np.float16), dev.empty((2, S, N_Q, HD), np.float16)
+        vsl.check(H.vsl_rope_part_append(p(x), S, N_Q, nkv, HD, ROT, 1, pos0, p(at), p(m.cos), p(m.sin), TABLE, p(q), 2, p(kc), p(vc),
+                                         1, cap, None))
+        vsl.check(H.vsl_attn_prefill_mods(p(q), 2, p(kc), p(vc), S, pos0, N_Q, nkv, HD, cap, SCALE, p(out), 2, ctypes.byref(mods),
+                                          None, 0, None))
+        ctrl, q1, o1 = dev.put(np.array([cap - 1, 0, 0, 0, 9, 0, cap, 0], np.uint32)), *(dev.empty((N_Q, HD), np.float32) for _ in range(2))
+        po, pml = dev.empty((N_Q, NSPLIT, HD), np.float32), dev.empty((N_Q, NSPLIT, 2), np.float32)
+        vsl.check(H.vsl_rope_part_append_decode(p(row), N_Q, nkv, HD, ROT, 1, p(place), p(m.cos), p(m.sin), TABLE, p(q1), p(kc), p(vc),
+                                                1, cap, p(ctrl), None))
+        rg1 = dev.put(np.array([(pos0 - 50, 0xFFFFFFFF)], np.uint32))
+        mods = vsl.AttnMods(softcap=SOFTCAP, slopes=p(m.slopes), ranges=p(rg1))
+        vsl.check(H.vsl_attn_decode_mods(p(q1), p(kc), p(vc), 1, N_Q, nkv, HD, cap, SCALE, NSPLIT, p(po), p(pml), p(o1), p(ctrl),
+                                         ctypes.byref(mods), None))
+        outs.append([dev.get(t).copy() for t in (q, out, q1, o1, kc[:, pos0 - 60:], vc[:, pos0 - 60:])])
+    assert all(np.array_equal(a, b) for a, b in zip(*outs)) and all(a.any() for a in outs[0])
+    rows_n, n, stride = len(SAMPLERS), 700, 1 << 28
+    logits = rng.normal(0, 2, (rows_n, n)).astype(np.float32)
+    far = dev.empty(((rows_n - 1) * stride + n,), np.float32)
+    for r in range(rows_n):
+        far[r * stride:r * stride + n].copy_(dev.torch.from_numpy(logits[r]))
+    par = np.zeros((rows_n, 4), np.float32)
+    for r, s in enumerate(SAMPLERS):
+        par[r] = (s[0], 0, s[2], s[3])
+        par[r, 1:2].view(np.uint32)[0] = s[1]
+    u, par = dev.put(rng.random(rows_n).astype(np.float32)), dev.put(par)
+    size = H.vsl_sample_rows_ws_bytes(rows_n, n)
+    ws, got = dev.empty((size,), np.uint8), []
+    for l, st in ((dev.put(logits), n), (far, stride)):
+        tok, share = dev.empty((rows_n,), np.uint32), dev.empty((rows_n,), np.float32)
+        vsl.check(H.vsl_sample_rows(p(l), 0, rows_n, n, st, p(par), p(u), p(tok), p(share), p(ws), size, None))
+        got.append((dev.get(tok), dev.get(share)))
+    assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][1], got[1][1]) and len(set(got[0][0])) > 1
