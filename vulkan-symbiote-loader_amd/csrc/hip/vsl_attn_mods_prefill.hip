@@ -152,8 +152,8 @@ __device__ __noinline__ void rows_one_by_one(const PrefillArgs& a, uint32_t rb, 
 // are joined through LDS at the end.
 // Bound: the two products (4 head_dim flops a row and key, half as many again for a split q) and, for every score, 12 vector
 // instructions of cap, exponential and rounding, which take longer than its share of the products; LDS, which each query tile
-// reads anew, is as busy as the matrix cores. 2048 rows at 6144 of the 8B shape, split q, cap 30: 423 us (cards and days
-// differ by 7 %), 850 TFLOP/s in products where a large plain fp16 product reaches 1080 on this card; the matrix
+// reads anew, is as busy as the matrix cores. 2048 rows at 6144 of the 8B shape, split q, cap 30: 423 to 434 us (cards and
+// days differ by more), 830 to 850 TFLOP/s in products where a large plain fp16 product reaches 1080 on this card; the matrix
 // cores are busy a third of the time, the vector unit 45 %, LDS without bank conflicts. Slower there: the next tile's K in
 // registers ahead of its product 451 to 470, products and vector code mixed by scheduling barriers 485.
 // A row's keys are a range [lo, hi); tiles that lie within the ranges of all of a wave's rows take no masks, and tiles
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
     vsl_half(*Vs)[kTK * HD] = s_tiles + kBufs;
     __shared__ __attribute__((aligned(16))) vsl_half s_q[kTiles][QP * 32 * HD];
     __shared__ uint32_t s_lo[kTiles * kShares], s_hi[kTiles * kShares];
-    __shared__ float s_m[kTiles][64], s_l[kTiles][64];
+    __shared__ float s_m[kTiles * kShares][64], s_l[kTiles * kShares][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // blocks in the order of their rows, the last (longest under the causal mask) first, KV heads next to each other
     const uint32_t n_rb = (a.S + 31) / 32, n_qt = n_rb * a.G, n_grp = (n_qt + kTiles - 1) / kTiles;
@@ -479,66 +479,68 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
         l = a0 + a1;
         if (m == -INFINITY && l != 0.f) m = 0.f;  // only NaN scores: keep the sum in the join
     }
-    // the halves of each query tile joined: the second leaves its sums in the tile buffers (every read and copy is over)
+    // the halves of each query tile joined: each wave takes half of the dims, and leaves the other half of its sums in the tile
+    // buffers (every read and copy is over)
     const bool any_odd = __builtin_amdgcn_ballot_w64(odd != 0) != 0;
-    constexpr int OSZ = ND * 16 * 64;
-    static_assert(kTiles * OSZ * 4 <= 2 * kBufs * kTK * HD * 2, "every query tile's sums in the tile buffers");
-    {
-        const int w = wave / kShares;
-        float* x = reinterpret_cast<float*>(&s_tiles[0][0]) + w * OSZ;
-        if (share) {
+    constexpr int NJ = ND / 2, OSZ = NJ * 16 * 64;
+    static_assert(kTiles * kShares * OSZ * 4 <= 2 * kBufs * kTK * HD * 2, "every query tile's sums in the tile buffers");
+    const int w = wave / kShares;
+    float* sums = reinterpret_cast<float*>(&s_tiles[0][0]) + (w * kShares) * OSZ;
+    auto leave = [&](auto first) __attribute__((always_inline)) {  // tiles of dims first .. for the other wave
+        float* x = sums + (share ^ 1) * OSZ;
 #pragma unroll
-            for (int t = 0; t < ND; ++t)
-#pragma unroll
-                for (int v = 0; v < 16; v += 4)
-                    *reinterpret_cast<float4v*>(x + ((t * 4 + v / 4) * 64 + lane) * 4) = float4v{o[t][v], o[t][v + 1], o[t][v + 2], o[t][v + 3]};
-            s_m[w][lane] = m;
-            s_l[w][lane] = l;
-            if (lane == 0) s_lo[wave] = any_odd;
-        }
-        __syncthreads();
-        if (share) return;
-        if (any_odd || s_lo[wave + 1]) {
-            if (active) {
-                // the arguments where the launch put them: the address of `a` would move them all to scratch memory
-                const auto* args = reinterpret_cast<const PrefillArgs*>((const void*)__builtin_amdgcn_kernarg_segment_ptr());
-                rows_one_by_one<HD, QX2, CAP>(*args, rb, h, chunk, t0 * kTK, t1 * kTK);
-            }
-            return;
-        }
-        const float mb = s_m[w][lane], mm = fmaxf(m, mb), ref = mm == -INFINITY ? 0.f : mm;
-        const float ca = fast_exp2(m - ref), cb = fast_exp2(mb - ref);
-        l = l * ca + s_l[w][lane] * cb;
-        m = mm;
-#pragma unroll
-        for (int t = 0; t < ND; ++t)
+        for (int t = 0; t < NJ; ++t)
 #pragma unroll
             for (int v = 0; v < 16; v += 4) {
-                const float4v y = *reinterpret_cast<const float4v*>(x + ((t * 4 + v / 4) * 64 + lane) * 4);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[t][v + i] = o[t][v + i] * ca + y[i] * cb;
+                const float16v& from = o[decltype(first)::value + t];
+                *reinterpret_cast<float4v*>(x + ((t * 4 + v / 4) * 64 + lane) * 4) = float4v{from[v], from[v + 1], from[v + 2], from[v + 3]};
             }
-    }
-    if (!active || my_s >= a.S) return;
-    if (a.n_chunk > 1) {
-        const size_t tile = part_tile(a, chunk, rb, h);
-#pragma unroll
-        for (int t = 0; t < ND; ++t)
-#pragma unroll
-            for (int v = 0; v < 16; v += 4)  // dims 32 t + 2 v + 4 (lane / 32) ..
-                *reinterpret_cast<float4v*>(a.part_o + tile * 32 * HD + ((t * 4 + v / 4) * 64 + lane) * 4) =
-                    float4v{o[t][v], o[t][v + 1], o[t][v + 2], o[t][v + 3]};
-        if (lane < 32) *reinterpret_cast<float2*>(a.part_ml + (tile * 32 + lane) * 2) = make_float2(m, l);
+    };
+    using std::integral_constant;
+    if (share) leave(integral_constant<int, 0>());
+    else leave(integral_constant<int, NJ>());
+    s_m[wave][lane] = m;
+    s_l[wave][lane] = l;
+    if (lane == 0) s_lo[wave] = any_odd;
+    __syncthreads();
+    if (!active) return;
+    if (s_lo[w * kShares] || s_lo[w * kShares + 1]) {
+        if (share) return;
+        // the arguments where the launch put them: the address of `a` would move them all to scratch memory
+        const auto* args = reinterpret_cast<const PrefillArgs*>((const void*)__builtin_amdgcn_kernarg_segment_ptr());
+        rows_one_by_one<HD, QX2, CAP>(*args, rb, h, chunk, t0 * kTK, t1 * kTK);
         return;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float mb = s_m[wave ^ 1][lane], mm = fmaxf(m, mb), ref = mm == -INFINITY ? 0.f : mm;
+    const float ca = fast_exp2(m - ref), cb = fast_exp2(mb - ref);
+    l = l * ca + s_l[wave ^ 1][lane] * cb;
+    m = mm;
+    if (my_s >= a.S) return;
+    auto finish = [&](auto first) __attribute__((always_inline)) {
+        constexpr int F = decltype(first)::value;
+        const float* x = sums + share * OSZ;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const size_t tile = part_tile(a, chunk, rb, h);
 #pragma unroll
-    for (int t = 0; t < ND; ++t)
+        for (int t = 0; t < NJ; ++t)
 #pragma unroll
-        for (int v = 0; v < 16; v += 4) {
-            const float y[4] = {o[t][v] * inv, o[t][v + 1] * inv, o[t][v + 2] * inv, o[t][v + 3] * inv};
-            store4<HD>(a, my_s, h, t * 32 + d_row(v, lane), y);
-        }
+            for (int v = 0; v < 16; v += 4) {
+                const float4v b = *reinterpret_cast<const float4v*>(x + ((t * 4 + v / 4) * 64 + lane) * 4);
+                float y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = o[F + t][v + i] * ca + b[i] * cb;
+                if (a.n_chunk > 1) {  // dims 32 t + 2 v + 4 (lane / 32) ..
+                    *reinterpret_cast<float4v*>(a.part_o + tile * 32 * HD + (((F + t) * 4 + v / 4) * 64 + lane) * 4) = float4v{y[0], y[1], y[2], y[3]};
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] *= inv;
+                    store4<HD>(a, my_s, h, (F + t) * 32 + d_row(v, lane), y);
+                }
+            }
+        if (a.n_chunk > 1 && F == 0 && lane < 32) *reinterpret_cast<float2*>(a.part_ml + (tile * 32 + lane) * 2) = make_float2(m, l);
+    };
+    if (share) finish(integral_constant<int, NJ>());
+    else finish(integral_constant<int, 0>());
 }
 
 // The chunks' sums joined: a block 32 dims of a query tile, a wave 8 of them, its lanes as those that stored them.
@@ -589,7 +591,7 @@ uint32_t blocks_of(uint32_t S, uint32_t n_q, uint32_t n_kv) {
 }
 
 // Key chunks: as many as fill the CUs, none shorter than three tiles of the longest rows; calls of less than 12 tiles are not
-// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8; 45 rows at 3001 26.1 in 16 chunks, 27.9 in 12, 35.7 in 6; 19.2 now).
+// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8 at the time; 45 rows at 3001 26.1 in 16 chunks, 27.9 in 12, 35.7 in 6; 18.8 now).
 uint32_t chunks_of(uint32_t S, uint32_t pos0, uint32_t n_q, uint32_t n_kv) {
     const uint64_t blocks = blocks_of(S, n_q, n_kv), tiles = ((uint64_t)pos0 + S + kTK - 1) / kTK;
     if (blocks >= 256 || tiles < 12) return 1;
