@@ -270,6 +270,25 @@ def test_prompt_split_keys(vsl, H, dev, S, pos0):
             assert prompt_ok(got, qv, K, V, pos0, 0.09, True, 1, 30.0, slopes_of(4), rg), (ws, rg is None)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_split_keys_of_short_ranges(vsl, H, dev, hd):
+    """Ranges of fewer tiles than a call has chunks, far into the cache: most blocks have no tiles at all, and a wave that is
+    through before the others of its block changes nothing of theirs."""
+    rng = np.random.default_rng(77)
+    S, pos0, n_q, n_kv = 45, 2900, 8, 2
+    K, V, kc, vc = caches(rng, n_kv, pos0 + S, hd, pos0 + S, np.float16)
+    q = rng.normal(0, 2, (S, n_q, hd)).astype(np.float32)
+    at = rng.integers(2600, 2700, S)
+    rg = np.stack([at, at + rng.integers(0, 70, S)], 1).astype(np.uint32)
+    rg[32:] = [(2000, 2001)] * (S - 32)
+    assert H.vsl_attn_prefill_mods_ws_bytes(S, pos0, n_q, n_kv, hd) >= 8 * 64 * n_q * (hd + 2) * 4
+    m = mods(vsl, dev, 0.0, slopes_of(n_q), rg)
+    first, qv = prompt(vsl, H, dev, q, kc, vc, pos0, 0.09, m)
+    assert prompt_ok(first, qv, K, V, pos0, 0.09, True, 1, 0.0, slopes_of(n_q), rg)
+    for _ in range(20):
+        assert np.array_equal(prompt(vsl, H, dev, q, kc, vc, pos0, 0.09, m)[0], first)
+
+
 @pytest.mark.parametrize("hd,n_q,n_kv", [(64, 4, 4), (128, 4, 1), (128, 3, 1)])
 @pytest.mark.parametrize("pos0", [0, 900])
 def test_prompt_masked_values_stay_out(vsl, H, dev, hd, n_q, n_kv, pos0):

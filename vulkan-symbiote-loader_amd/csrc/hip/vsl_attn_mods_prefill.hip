@@ -168,6 +168,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
     vsl_half(*Vs)[kTK * HD] = s_tiles + kBufs;
     __shared__ __attribute__((aligned(16))) vsl_half s_q[kTiles][QP * 32 * HD];
     __shared__ uint32_t s_lo[kTiles * kShares], s_hi[kTiles * kShares];
+    // (not in s_lo's place: where a chunk has no tiles, no barrier lies between the reads of s_lo and these flags)
+    __shared__ uint32_t s_odd[kTiles * kShares];
     __shared__ float s_m[kTiles * kShares][64], s_l[kTiles * kShares][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // blocks in the order of their rows, the last (longest under the causal mask) first, KV heads next to each other
@@ -501,10 +503,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
     else leave(integral_constant<int, NJ>());
     s_m[wave][lane] = m;
     s_l[wave][lane] = l;
-    if (lane == 0) s_lo[wave] = any_odd;
+    if (lane == 0) s_odd[wave] = any_odd;
     __syncthreads();
     if (!active) return;
-    if (s_lo[w * kShares] || s_lo[w * kShares + 1]) {
+    if (s_odd[w * kShares] || s_odd[w * kShares + 1]) {
         if (share) return;
         // the arguments where the launch put them: the address of `a` would move them all to scratch memory
         const auto* args = reinterpret_cast<const PrefillArgs*>((const void*)__builtin_amdgcn_kernarg_segment_ptr());
