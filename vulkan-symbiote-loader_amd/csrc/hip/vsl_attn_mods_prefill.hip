@@ -152,8 +152,8 @@ __device__ __noinline__ void rows_one_by_one(const PrefillArgs& a, uint32_t rb, 
 // are joined through LDS at the end.
 // Bound: the two products (4 head_dim flops a row and key, half as many again for a split q) and, for every score, 12 vector
 // instructions of cap, exponential and rounding, which take longer than its share of the products; LDS, which each query tile
-// reads anew, is as busy as the matrix cores. 2048 rows at 6144 of the 8B shape, split q, cap 30: 423 to 434 us (cards and
-// days differ by more), 830 to 850 TFLOP/s in products where a large plain fp16 product reaches 1080 on this card; the matrix
+// reads anew, is as busy as the matrix cores. 2048 rows at 6144 of the 8B shape, split q, cap 30: 417 to 434 us (cards and
+// days differ by more), 830 to 865 TFLOP/s in products where a large plain fp16 product reaches 1080 on this card; the matrix
 // cores are busy a third of the time, the vector unit 45 %, LDS without bank conflicts. Slower there: the next tile's K in
 // registers ahead of its product 451 to 470, products and vector code mixed by scheduling barriers 485.
 // A row's keys are a range [lo, hi); tiles that lie within the ranges of all of a wave's rows take no masks, and tiles
