@@ -145,23 +145,25 @@ __device__ __noinline__ void rows_one_by_one(const PrefillArgs& a, uint32_t rb, 
     }
 }
 
+// Planes: a split q has split probabilities (2^-22 of each is lost), as in attention without modifications. A caller who passes one
+// plane has q in fp16 already: the probabilities are then one plane too, 2^-11 of each, for half the matrix work.
+//
 // Block: four query tiles (32 rows of one head) of one KV head, numbered row block by row block with the group's heads
 // within; two waves each, a wave the one 32-key half of every 64-key tile. Key tiles go from the cache straight into LDS
 // (two buffers of K and two of V), shared by the four query tiles. Per tile a wave takes S^T = K Q^T (its D: a lane has 16
 // keys of one row) and turns the scores into probabilities, which are the operand of O^T += V^T P^T as they lie. The halves
 // are joined through LDS at the end.
-// Bound: the two products (4 head_dim flops a row and key, half as many again for a split q) and, for every score, 12 vector
-// instructions of cap, exponential and rounding, which take longer than its share of the products; LDS, which each query tile
-// reads anew, is as busy as the matrix cores. 2048 rows at 6144 of the 8B shape, split q, cap 30: 417 to 434 us (cards and
-// days differ by more), 830 to 865 TFLOP/s in products where a large plain fp16 product reaches 1080 on this card; the matrix
-// cores are busy a third of the time, the vector unit 45 %, LDS without bank conflicts. Slower there: the next tile's K in
-// registers ahead of its product 451 to 470, products and vector code mixed by scheduling barriers 485.
+// Bound: the two products (4 head_dim flops a row and key, twice as many for a split q) and, for every score, a dozen vector
+// instructions of cap, exponential and rounding; LDS, which each query tile reads anew, is as busy as the matrix cores. 2048 rows
+// at 6144 of the 8B shape, split q, cap 30: 509 us, 946 TFLOP/s in products where a large plain fp16 product reaches 1080 on this
+// card. With the probabilities in one plane, 424 there, slower were: the next tile's K in registers ahead of its product 451 to
+// 470, products and vector code mixed by scheduling barriers 485.
 // A row's keys are a range [lo, hi); tiles that lie within the ranges of all of a wave's rows take no masks, and tiles
 // outside all of them are skipped. In the others a masked probability is 0; where V then holds an infinity or a NaN, whose
 // product with 0 would reach the sums, the query tile's rows are computed again, one by one (rows_one_by_one).
-template <int HD, bool QX2, bool PX2, bool CAP>
+template <int HD, bool QX2, bool CAP>
 __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
-    constexpr int CPR = HD / 8, NCH = kTK * CPR / kThreads, QP = QX2 ? 2 : 1, PP = PX2 ? 2 : 1, ND = HD / 32;
+    constexpr int CPR = HD / 8, NCH = kTK * CPR / kThreads, QP = QX2 ? 2 : 1, ND = HD / 32;
     static_assert(NCH >= 1 && kTK * CPR % kThreads == 0, "a tile divides over the block");
     __shared__ __attribute__((aligned(16))) vsl_half s_tiles[2 * kBufs][kTK * HD];  // K's buffers, then V's
     vsl_half(*Ks)[kTK * HD] = s_tiles;
@@ -323,17 +325,17 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
         return most;
     };
     // two probabilities 2^x into their place in P^T; the row's sum takes them as they are multiplied
-    auto put_probs = [&](int v, float x0, float x1, half8 (&pf)[PP][2]) __attribute__((always_inline)) {
+    auto put_probs = [&](int v, float x0, float x1, half8 (&pf)[QP][2]) __attribute__((always_inline)) {
         const half2v one = {(vsl_half)1.f, (vsl_half)1.f};
         const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
         const half2v hi2 = round2(p0, p1);
         pf[0][v >> 3][v & 7] = hi2[0];
         pf[0][v >> 3][(v & 7) + 1] = hi2[1];
         l = __builtin_amdgcn_fdot2(hi2, one, l, false);
-        if constexpr (PX2) {
+        if constexpr (QX2) {
             const half2v lo2 = round2(p0 - (float)hi2[0], p1 - (float)hi2[1]);
-            pf[PP - 1][v >> 3][v & 7] = lo2[0];
-            pf[PP - 1][v >> 3][(v & 7) + 1] = lo2[1];
+            pf[QP - 1][v >> 3][v & 7] = lo2[0];
+            pf[QP - 1][v >> 3][(v & 7) + 1] = lo2[1];
             l = __builtin_amdgcn_fdot2(lo2, one, l, false);
         }
     };
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
         const half4 x0 = lds_read_tr16(p0), x1 = lds_read_tr16(p1);
         return half8{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
     };
-    auto pv = [&](int buf, const half8 (&pf)[PP][2]) __attribute__((always_inline)) {
+    auto pv = [&](int buf, const half8 (&pf)[QP][2]) __attribute__((always_inline)) {
         uint32_t at = v_at + buf * kTile;
         asm volatile("" : "+v"(at));
 #pragma unroll
@@ -357,7 +359,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
             for (int half = 0; half < 2; ++half) {
                 const half8 af = v_frag(at, tt, half);
 #pragma unroll
-                for (int p = 0; p < PP; ++p) o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af, pf[p][half], o[tt], 0, 0, 0);
+                for (int p = 0; p < QP; ++p) o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af, pf[p][half], o[tt], 0, 0, 0);
             }
     };
     // infinities and NaN in this wave's half of the tile's V
@@ -384,7 +386,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
     // probabilities of tile t from its products: the short way where no mask or bias applies, the polynomial serves all its
     // scores and none, of either sign, raises the reference
     float16v st;
-    half8 pf[PP][2];
+    half8 pf[QP][2];
     auto whole_of = [&](uint32_t t) { return t * kTK + share * 32 >= all_lo && t * kTK + share * 32 + 32 <= all_hi; };
     auto softmax = [&](uint32_t t) __attribute__((always_inline)) {
         const uint32_t k0 = t * kTK + share * 32;
@@ -593,7 +595,7 @@ uint32_t blocks_of(uint32_t S, uint32_t n_q, uint32_t n_kv) {
 }
 
 // Key chunks: as many as fill the CUs, none shorter than three tiles of the longest rows; calls of less than 12 tiles are not
-// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8 at the time; 45 rows at 3001 26.1 in 16 chunks, 27.9 in 12, 35.7 in 6; 18.8 now).
+// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8 at the time; 45 rows at 3001 26.1 in 16 chunks, 27.9 in 12, 35.7 in 6; 19.6 now).
 uint32_t chunks_of(uint32_t S, uint32_t pos0, uint32_t n_q, uint32_t n_kv) {
     const uint64_t blocks = blocks_of(S, n_q, n_kv), tiles = ((uint64_t)pos0 + S + kTK - 1) / kTK;
     if (blocks >= 256 || tiles < 12) return 1;
@@ -668,20 +670,16 @@ extern "C" int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kca
     a.part_ml = a.part_o + (size_t)chunks * n_rb * 32 * n_q * hd;
     const dim3 grid((uint32_t)blocks, chunks);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    // Probabilities in one fp16 plane where q or the output is one: their rounding is as large as the output's (with the split
-    // q and an fp16 output 2.5e-4 of the norm in all, 2.1e-4 by two planes), and a quarter of the products is saved.
-    const bool p2 = q_dtype == VSL_DT_F16X2 && out_dtype != VSL_DT_F16;
-    auto go = [&](auto hdc, auto x2, auto px2, auto cc) {
+    auto go = [&](auto hdc, auto x2, auto cc) {
         constexpr int HD = decltype(hdc)::value;
-        k_prefill_mods<HD, decltype(x2)::value, decltype(px2)::value, decltype(cc)::value><<<grid, kThreads, 0, s>>>(a);
+        k_prefill_mods<HD, decltype(x2)::value, decltype(cc)::value><<<grid, kThreads, 0, s>>>(a);
         if (chunks > 1) k_join_prefill<HD><<<n_rb * n_q * (HD / 32), 256, 0, s>>>(a);
     };
     using T = std::true_type;
     using F = std::false_type;
     auto pick = [&](auto hdc) {
-        if (q_dtype == VSL_DT_F16) capped ? go(hdc, F{}, F{}, T{}) : go(hdc, F{}, F{}, F{});
-        else if (!p2) capped ? go(hdc, T{}, F{}, T{}) : go(hdc, T{}, F{}, F{});
-        else capped ? go(hdc, T{}, T{}, T{}) : go(hdc, T{}, T{}, F{});
+        if (q_dtype == VSL_DT_F16) capped ? go(hdc, F{}, T{}) : go(hdc, F{}, F{});
+        else capped ? go(hdc, T{}, T{}) : go(hdc, T{}, F{});
     };
     if (hd == 128) pick(std::integral_constant<int, 128>{});
     else pick(std::integral_constant<int, 64>{});
