@@ -50,7 +50,10 @@ constexpr int kCountShift = 46;     // 8192 of them stay below 2^46; the count a
 // below it, a draw has passed a border a little above it.
 constexpr double kBinNoise = 4e-11;
 constexpr double kMaxTop = 16384.0;  // l / T up to which the grid's rounding (2^-39) is far below a weight's
-constexpr double kListOne = 0x1p48, kRowOne = 0x1p42;  // fixed point of weights in lists (<= 2^15 tokens) and rows (<= 2^20)
+// Fixed point of weights: so many units for a weight of 1 that the sum of those that take part stays below 2^62. For lists of a
+// known length from that (k_rows_cut), else from their sum (unit_of): units for a row of 2^20 weights of 1 would leave 2^-42, and
+// as many weights of that size 2^-22 of the sum.
+constexpr double kFewOne = 0x1p54, kLeanOne = 0x1p52;
 
 enum { MODE_GREEDY = 0, MODE_TOPK = 1, MODE_SUM = 2, MODE_HIST = 3 };
 
@@ -220,7 +223,7 @@ __device__ __forceinline__ T block_scan(Shared& sh, T v, T& total) {
 }
 
 // The last key of the shortest run of keys, in descending order, whose measures reach `target` (the smallest key of all if
-// they do not). visit(f) calls f(rank, weight) for each of the thread's elements, weight() being its fixed-point weight;
+// they do not). visit(f) calls f(rank, weight) for each of the thread's elements, weight() being its weight;
 // map(rank, weight, key, measure) is false where one takes no part; measures are integers, keys differ and are not 0. `n` bounds the elements that take part. Narrowed down by
 // digits of 8 bits, from the highest bit in which keys differ, until kFinish keys are left, whose threads sum up the
 // measures before their own. All threads call; 0 without elements.
@@ -365,15 +368,19 @@ __device__ __forceinline__ void put(const RowOut& o, uint32_t token, double prob
 
 __device__ __forceinline__ double weight_of(float v, double vmax, double inv_t) { return exp(((double)v - vmax) * inv_t); }
 
-__device__ __forceinline__ uint64_t fixed_weight(uint64_t rank, double vmax, double inv_t, double one) {
-    return (uint64_t)(weight_of(value_of(rank), vmax, inv_t) * one + 0.5);
+__device__ __forceinline__ uint64_t units(double w, double one) { return (uint64_t)(w * one + 0.5); }
+// Units for weights whose sum is `sum`, about 1 or above: the power of two that makes it 2^61 to 2^62. 2^20 roundings are 2^-42 of it,
+// and as much of the sum of any first ones in descending order, each of which is no smaller than the others.
+__device__ __forceinline__ double unit_of(double sum) {
+    const uint64_t e = __builtin_bit_cast(uint64_t, sum) >> 52;  // 1023 + its exponent
+    return __builtin_bit_cast(double, (2 * 1023 + 61 - e) << 52);
 }
 
 // The draw over elements (visit and n as for select_key) that hold every token of the first k: the three cuts, then the index
-// at which the running sum passes u.
+// at which the running sum passes u. one: units of a weight of 1.
 template <int NT, class Visit>
 __device__ __forceinline__ void draw_exact(Shared& sh, uint32_t n, const RowParams& rp, double vmax, double u, const RowOut& out,
-                                           bool cut_k, Visit visit) {
+                                           bool cut_k, double one, Visit visit) {
     uint64_t low = 1;  // the smallest kept rank key
     if (cut_k) low = select_key<NT>(sh, n, rp.k, visit, [&](uint64_t rank, auto, uint64_t& key, uint64_t& w) {
         key = rank;
@@ -382,30 +389,30 @@ __device__ __forceinline__ void draw_exact(Shared& sh, uint32_t n, const RowPara
     });
     if (rp.cut_p) {
         uint64_t s = 0;
-        visit([&](uint64_t rank, auto weight) { s += rank >= low ? weight() : 0; });
+        visit([&](uint64_t rank, auto weight) { s += rank >= low ? units(weight(), one) : 0; });
         const uint64_t target = (uint64_t)ceil((double)block_add<NT>(sh, s) * rp.p);
         low = select_key<NT>(sh, n, target, visit, [&](uint64_t rank, auto weight, uint64_t& key, uint64_t& w) {
             key = rank;
-            w = rank >= low ? weight() : 0;
+            w = rank >= low ? units(weight(), one) : 0;
             return rank >= low;
         });
     }
     // min-p: the weight itself decides
     auto heavy = [&](uint64_t rank) { return weight_of(value_of(rank), vmax, rp.inv_t) >= rp.m; };
     uint64_t s = 0;
-    visit([&](uint64_t rank, auto weight) { s += rank >= low && heavy(rank) ? weight() : 0; });
+    visit([&](uint64_t rank, auto weight) { s += rank >= low && heavy(rank) ? units(weight(), one) : 0; });
     const uint64_t total = block_add<NT>(sh, s);
     uint64_t target = (uint64_t)((double)total * u) + 1;
     if (target > total) target = total;
     const uint64_t at = select_key<NT>(sh, n, target, visit, [&](uint64_t rank, auto weight, uint64_t& key, uint64_t& w) {
         if (rank < low || !heavy(rank)) return false;
-        w = weight();
+        w = units(weight(), one);
         key = (rank & 0xFFFFFFFFull) + 1;  // the inverted index: ascending indices are descending keys (+ 1: not 0)
         return w != 0;
     });
     const uint32_t idx = ~(uint32_t)(at - 1);
     visit([&](uint64_t rank, auto weight) {
-        if (index_of(rank) == idx) put(out, idx, (double)weight() / (double)total);
+        if (index_of(rank) == idx) put(out, idx, weight() * one / (double)total);
     });
 }
 
@@ -418,7 +425,7 @@ __device__ __forceinline__ void draw_few(Shared& sh, uint64_t* list, uint32_t n,
     if (t >= n && t < ((n + 15) & ~15u)) list[t] = 0;  // up to a whole batch
     const double w = weight_of(mine ? value_of(mine) : (float)vmax, vmax, rp.inv_t);
     const bool heavy = w >= rp.m;
-    const uint64_t fixed = (uint64_t)(w * kListOne + 0.5);
+    const uint64_t fixed = units(w, kFewOne);
     __syncthreads();
     uint32_t rank = 0;
     for (uint32_t j0 = 0; j0 < n; j0 += 16) {
@@ -448,19 +455,22 @@ __device__ __forceinline__ void draw_few(Shared& sh, uint64_t* list, uint32_t n,
     if (t >= kept && t < ((kept + 7) & ~7u) && t < kFinish) sh.keyed[t] = Keyed{0, 0};
     __syncthreads();
     const uint64_t sum = sh.sel_left;
-    if (t >= kept) return;
-    uint64_t target = (uint64_t)((double)sum * u);
-    if (target >= sum) target = sum - 1;
-    const uint64_t key = k.key & ~(1ull << 63);
-    uint64_t below = 0;  // weights of lower indices
-    for (uint32_t j0 = 0; j0 < kept; j0 += 8) {
-        Keyed x[8];
+    if (t < kept) {
+        uint64_t target = (uint64_t)((double)sum * u);
+        if (target >= sum) target = sum - 1;
+        const uint64_t key = k.key & ~(1ull << 63);
+        uint64_t below = 0;  // weights of lower indices
+        for (uint32_t j0 = 0; j0 < kept; j0 += 8) {
+            Keyed x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = sh.keyed[j0 + j];
+            for (int j = 0; j < 8; ++j) x[j] = sh.keyed[j0 + j];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) below += (x[j].key & ~(1ull << 63)) > key ? x[j].weight : 0;
+            for (int j = 0; j < 8; ++j) below += (x[j].key & ~(1ull << 63)) > key ? x[j].weight : 0;
+        }
+        if (below <= target && below + k.weight > target) sh.sel_key = key;
     }
-    if (below <= target && below + k.weight > target) put(out, ~(uint32_t)(key - 1), (double)k.weight / (double)sum);
+    __syncthreads();
+    if (t < n && (mine & 0xFFFFFFFFull) + 1 == sh.sel_key) put(out, index_of(mine), w * kFewOne / (double)sum);
 }
 
 // Bin of a value on the grid that all slices share: floor(8 l / T), as a double (exact to 2^53, and monotone above).
@@ -714,10 +724,10 @@ __global__ __launch_bounds__(kThreads) void k_rows_cut(const T* __restrict__ log
         uint64_t r[kLeanRegs];
 #pragma unroll
         for (int i = 0; i < kLeanRegs; ++i) r[i] = i * NT + t < n ? s_list[i * NT + t] : 0;
-        draw_exact<NT>(sh, n, rp, vmax, u, out, n > rp.k, [&](auto f) {
+        draw_exact<NT>(sh, n, rp, vmax, u, out, n > rp.k, kLeanOne, [&](auto f) {
 #pragma unroll
             for (int i = 0; i < kLeanRegs; ++i)
-                if (r[i]) f(r[i], [&] { return fixed_weight(r[i], vmax, rp.inv_t, kListOne); });
+                if (r[i]) f(r[i], [&] { return weight_of(value_of(r[i]), vmax, rp.inv_t); });
         });
         return;
     }
@@ -909,40 +919,43 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
     if (top == 0) return;
     const double vmax = (double)value_of(top);
     // batches of eight elements, requested together
-    auto in_batches = [&](uint32_t from, uint32_t n, auto load, double one, auto f) {
+    auto in_batches = [&](uint32_t from, uint32_t n, auto load, auto f) {
         for (uint32_t i0 = from + t; i0 < n; i0 += 8 * NT) {
             uint64_t x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = i0 + j * NT < n ? load(i0 + j * NT) : 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (x[j]) f(x[j], [&] { return fixed_weight(x[j], vmax, rp.inv_t, one); });
+                if (x[j]) f(x[j], [&] { return weight_of(value_of(x[j]), vmax, rp.inv_t); });
         }
     };
     if (rp.mode == MODE_TOPK || (rp.mode == MODE_HIST && (n_list > kListCap || fabs(vmax * rp.inv_t) > kMaxTop))) {
-        draw_exact<NT>(sh, V, rp, vmax, u, out, rp.k < V, [&](auto f) {
-            in_batches(0, V, [&](uint32_t i) { return rank_of(load_logit(l, i), i); }, kRowOne, f);
-        });
+        auto visit = [&](auto f) { in_batches(0, V, [&](uint32_t i) { return rank_of(load_logit(l, i), i); }, f); };
+        double one = kFewOne;  // TOPK: only the first k count
+        if (rp.mode == MODE_HIST) {
+            double sum = 0.0;
+            visit([&](uint64_t, auto weight) { sum += weight(); });
+            one = unit_of(block_add<NT>(sh, sum));
+        }
+        draw_exact<NT>(sh, V, rp, vmax, u, out, rp.k < V, one, visit);
         return;
     }
     // the list's tokens: the first ones from registers, their weights taken once, the others from memory
-    uint64_t fixed[kDrawRegs];
+    double wts[kDrawRegs];
 #pragma unroll
-    for (int i = 0; i < kDrawRegs; ++i) {
-        fixed[i] = 0;
-        if ((uint32_t)i * NT < n_list) fixed[i] = r[i] ? fixed_weight(r[i], vmax, rp.inv_t, kListOne) : 0;
-    }
+    for (int i = 0; i < kDrawRegs; ++i) wts[i] = (uint32_t)i * NT < n_list ? weight_of(r[i] ? value_of(r[i]) : (float)vmax, vmax, rp.inv_t) : 0.0;
     auto visit = [&](auto f) {
 #pragma unroll
         for (int i = 0; i < kDrawRegs; ++i)
-            if (r[i]) f(r[i], [&] { return fixed[i]; });
-        in_batches(kDrawRegs * NT, n_list, [&](uint32_t i) { return list[i]; }, kListOne, f);
+            if (r[i]) f(r[i], [&] { return wts[i]; });
+        in_batches(kDrawRegs * NT, n_list, [&](uint32_t i) { return list[i]; }, f);
     };
     const double top_bin = bin_of(value_of(top), rp.inv_t);
     auto row_bin = [&](float x) { return bin_below(top_bin, bin_of(x, rp.inv_t)); };
     uint64_t low = 1;  // the smallest kept rank key
     uint32_t cb = kBins - 2, sure = 0;  // the last bin that keeps a token; the bins kept whole are in the slices' sums
     const bool hist = rp.mode == MODE_HIST;
+    const double one = unit_of(hist ? hi_total : block_add<NT>(sh, slice_sum));  // kept weights add up to no more
     if (hist) {
         sure = rec_sure;
         double total = hi_total;
@@ -954,8 +967,8 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
             });
             if (rp.cut_p) {
                 uint64_t part = 0;
-                visit([&](uint64_t rank, auto weight) { part += rank >= low && row_bin(value_of(rank)) == kb ? weight() : 0; });
-                total = lo_total + (double)block_add<NT>(sh, part) / kListOne;
+                visit([&](uint64_t rank, auto weight) { part += rank >= low && row_bin(value_of(rank)) == kb ? units(weight(), one) : 0; });
+                total = lo_total + (double)block_add<NT>(sh, part) / one;
             }
         }
         if (rp.cut_p) {
@@ -963,11 +976,11 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
             uint32_t pb = plo;
             while (pb < phi && rr.cum_w[pb] < target) ++pb;
             const double base = pb ? rr.cum_w[pb - 1] : 0.0;
-            const uint64_t left = target > base ? (uint64_t)ceil((target - base) * kListOne) : 1;
+            const uint64_t left = target > base ? (uint64_t)ceil((target - base) * one) : 1;
             const uint64_t cut = select_key<NT>(sh, n_list, left, visit, [&](uint64_t rank, auto weight, uint64_t& key, uint64_t& w) {
                 if (rank < low || row_bin(value_of(rank)) != pb) return false;
                 key = rank;
-                w = weight();
+                w = units(weight(), one);
                 return true;
             });
             if (cut > low) low = cut;
@@ -976,14 +989,13 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
     }
     auto kept = [&](uint64_t rank, double w) { return rank >= low && w >= rp.m && (!hist || row_bin(value_of(rank)) <= cb); };
     // the slices' kept weights, in fixed point; of the bins that a cut divides, the list's tokens
-    if (t < kMaxSlices) s_slice[t] = (uint64_t)(slice_sum * kRowOne + 0.5);
+    if (t < kMaxSlices) s_slice[t] = units(slice_sum, one);
     __syncthreads();
     visit([&](uint64_t rank, auto weight) {
         if (rank < low) return;
         const uint32_t b = row_bin(value_of(rank));
         if (b < sure || b > cb || (rp.m > 0.0 && weight_of(value_of(rank), vmax, rp.inv_t) < rp.m)) return;
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s_slice[index_of(rank) / SL]),
-                  (unsigned long long)(((double)weight() * (kRowOne / kListOne)) + 0.5));
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s_slice[index_of(rank) / SL]), (unsigned long long)units(weight(), one));
     });
     __syncthreads();
     // the slice in which their running sum passes u
@@ -1003,8 +1015,8 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
     }
     __syncthreads();
     // the token in it: thread t takes E neighbours
-    const double total = (double)sh.sel_left / kRowOne;
-    const double target = total * (hist ? u * (1.0 + kBinNoise) : u) - (double)sh.sel_key / kRowOne;
+    const double total = (double)sh.sel_left / one;
+    const double target = total * (hist ? u * (1.0 + kBinNoise) : u) - (double)sh.sel_key / one;
     const uint32_t first = sh.sel_count * SL, from = first + t * E;
     double w[E], mine = 0.0, all;
     uint64_t last = 0;  // the last kept index + 1
