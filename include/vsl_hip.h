@@ -421,8 +421,9 @@ int vsl_sample_logits(const float* logits, uint32_t V, vsl_sampler sampler, uint
  * share w / total goes to probs (may be NULL).  temperature <= 0 or NaN, top_k = 1, top_p <= 0 and min_p > 1 give the first
  * maximum, with share 1.  u below 0 or NaN counts as 0, 1 and above as the largest float below 1.  NaN logits count as
  * -infinity, +infinity as the largest float; a row of -infinity gives token 0 with share 0.  Weights below about 2^-91
- * of the largest may count as 0.  Weights are summed in 64 bits.  V up to 2^20, up to 65535 rows; workspace 16-byte aligned,
- * vsl_sample_rows_ws_bytes(rows, V) bytes (0 for sizes that are not served). */
+ * of the largest may count as 0.  Weights are summed in 64 bits: the token is that of exact sums but where u or the top-p cut
+ * lies within 1e-10 of a border, as a share of the total; u = 0 gives the first kept token.  V up to 2^20, up to 65535 rows;
+ * workspace 16-byte aligned, vsl_sample_rows_ws_bytes(rows, V) bytes (0 for sizes that are not served). */
 typedef struct vsl_row_sampler {
     float temperature;
     uint32_t top_k;

@@ -1,10 +1,12 @@
-"""Sampling of rows where weights are far apart: rows whose small weights add up.
+"""Sampling of rows where weights are far apart: kept tokens of very small weight, and rows whose small weights add up.
 
-Tolerances: tokens are equal, u lying further than 1e-10 from every border; a share is one fp32 rounding (2^-24) off, and 1e-10."""
+Tolerances: tokens are equal, u lying further than 1e-10 from every border, or being 0 (or so small that the first kept token has
+it); a share is one fp32 rounding (2^-24) off, and 1e-10 of itself for the sums."""
 import numpy as np
 import pytest
 
 import test_sample_rows_gpu as base
+import token_step_ref as ref
 import vsl_testlib
 
 pytestmark = pytest.mark.gpu
@@ -31,6 +33,38 @@ def row(V, *values, rest=-np.inf):
     for at, x in values:
         l[at] = x
     return l
+
+
+def lists(n, *starts):
+    return np.concatenate([np.arange(s, s + n) for s in starts])
+
+
+# name: (logits, (temperature, top_k, top_p, min_p), first kept token). Weights of that token, relative to the largest's: e^-31 to
+# e^-42 (2^-44.7 to 2^-60.6).
+FIRST = {
+    "few of a list": (row(2, (0, 0), (1, 40)), (1.0, 2, 1.0, 0.0), 0),
+    "list of two slices": (row(5000, (3, 0), (4000, 39)), (1.0, 40, 1.0, 0.0), 3),
+    "list with ties": (row(5000, (lists(200, 0, 2048, 4096), 0), (4990, 40)), (1.0, 40, 1.0, 0.0), 0),
+    "top-k over the whole row": (row(30000, (29999, 40), rest=0), (1.0, 40, 1.0, 0.0), 0),
+    "a slice's sum": (row(5000, (0, 0), (3000, 31)), (1.0, 0, 1.0, 0.0), 0),
+    "a slice's sum, min-p": (row(5000, (0, -20), (5, 0), (3000, 40)), (1.0, 0, 1.0, 1e-20), 5),
+    "a bin kept whole": (row(5000, (0, 0), (slice(2048, 2348), -5), (3000, 36)), (1.0, 150, 1.0, 0.0), 0),
+    "the bin of the cut": (row(5000, (slice(0, 300), -1.5), (4000, 40.5)), (1.0, 250, 1.0, 0.0), 0),
+    "the whole row": (row(5000, (0, 19965), (slice(2048, 2348), 19963), (3000, 20000)), (1.0, 150, 1.0, 0.0), 0),
+}
+
+
+@pytest.mark.parametrize("name", FIRST)
+def test_first_kept_token(vsl, H, dev, name):
+    """u of 0 (and what counts as 0) and one below its share give the first kept token, however small its weight."""
+    logits, params, first = FIRST[name]
+    us = [0.0, np.nan, -1.0, 1e-30]
+    tok, share = base.run(vsl, H, dev, np.tile(logits, (4, 1)), [params] * 4, us)
+    t, k, p, m = (float(np.float32(x)) for x in params)
+    want, ws, _ = ref.sample(logits.astype(np.float64), t, int(k), p, m, 0.0)
+    assert want == first and 2.0 ** -62 < ws < 2.0 ** -44
+    assert list(tok) == [first] * 4
+    assert np.all(np.abs(share.astype(np.float64) - ws) <= (2.0 ** -24 * 1.001 + 1e-10) * ws)
 
 
 def test_sum_of_small_weights_over_the_whole_row(vsl, H, dev):

@@ -368,8 +368,12 @@ __device__ __forceinline__ void put(const RowOut& o, uint32_t token, double prob
 
 __device__ __forceinline__ double weight_of(float v, double vmax, double inv_t) { return exp(((double)v - vmax) * inv_t); }
 
-__device__ __forceinline__ uint64_t units(double w, double one) { return (uint64_t)(w * one + 0.5); }
-// Units for weights whose sum is `sum`, about 1 or above: the power of two that makes it 2^61 to 2^62. 2^20 roundings are 2^-42 of it,
+// A weight in units: none above 0 counts as 0, so that u = 0 gives the first kept token however small its weight.
+__device__ __forceinline__ uint64_t units(double w, double one) {
+    const uint64_t n = (uint64_t)(w * one + 0.5);
+    return n || !(w > 0.0) ? n : 1;
+}
+// Units for weights whose sum is `sum`, about 1 or above: the power of two that makes it 2^61 to 2^62. 2^20 roundings are 2^-41 of it,
 // and as much of the sum of any first ones in descending order, each of which is no smaller than the others.
 __device__ __forceinline__ double unit_of(double sum) {
     const uint64_t e = __builtin_bit_cast(uint64_t, sum) >> 52;  // 1023 + its exponent
