@@ -589,9 +589,9 @@ __global__ __launch_bounds__(256) void k_join_prefill(PrefillArgs a) {
     store4<HD>(a, s, h, (int)(group * 8 + lane / 32 * 4), y);
 }
 
-uint32_t blocks_of(uint32_t S, uint32_t n_q, uint32_t n_kv) {
-    const uint64_t n_qt = (uint64_t)((S + 31) / 32) * (n_q / n_kv);
-    return (uint32_t)((n_qt + kTiles - 1) / kTiles * n_kv);
+uint64_t blocks_of(uint32_t S, uint32_t n_q, uint32_t n_kv) {
+    const uint64_t n_qt = ((uint64_t)S + 31) / 32 * (n_q / n_kv);
+    return (n_qt + kTiles - 1) / kTiles * n_kv;
 }
 
 // Key chunks: as many as fill the CUs, none shorter than three tiles of the longest rows; calls of less than 12 tiles are not
@@ -637,7 +637,7 @@ extern "C" int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kca
     if (!aligned_to(md.slopes, 4) || !aligned_to(md.ranges, 8)) return vsl_invalid("%s: misaligned pointer", fn);
     if (!softcap_ok(md.softcap, scale)) return vsl_invalid("%s: softcap %g with scale %g", fn, (double)md.softcap, (double)scale);
     if (S == 0) return VSL_OK;
-    const uint64_t blocks = ((uint64_t)((S + 31) / 32) * G + kTiles - 1) / kTiles * n_kv;
+    const uint64_t blocks = blocks_of(S, n_q, n_kv);
     if (blocks > 1u << 23 || (uint64_t)S * n_q > 1u << 26) return vsl_unsupported("%s: %u rows in one call", fn, S);
     const bool capped = md.softcap > 0.f;
     const uint32_t n_rb = (S + 31) / 32;
