@@ -565,9 +565,12 @@ int vsl_attn_decode_mods(const float* q, const void* kcache, const void* vcache,
                          uint32_t hd, uint32_t cap, float scale, uint32_t nsplit, float* part_o, float* part_ml, float* out,
                          vsl_ctrl* ctrl, const vsl_attn_mods* mods, void* stream);
 /* vsl_attn_prefill with modified scores: arguments as there, all pointers 16-byte aligned (slopes 4, ranges 8), up to
- * 65535 heads.  With F16X2 q the probabilities are split as well; with F16 q they are one fp16 plane
- * (2^-11 of each).  With a workspace of vsl_attn_prefill_mods_ws_bytes calls of few
- * rows split the keys over more blocks and join their sums in a second launch; with less (NULL, 0) they run unsplit. */
+ * 65535 heads and S * n_q up to 2^26.  With F16X2 q the probabilities are split as well; with F16 q they are one fp16 plane
+ * (2^-11 of each).  With a workspace of vsl_attn_prefill_mods_ws_bytes calls of few rows split the keys over more blocks and
+ * join their sums in a second launch; with less (NULL, 0) they run unsplit (45 rows at 3001 101 us instead of 20, at 20000
+ * 628 instead of 54).  The size is that of one call: one of more rows may take less, or nothing.  No call takes more than
+ * VSL_ATTN_MODS_WS_MAX(hd) bytes: a program whose calls differ keeps that much. */
+#define VSL_ATTN_MODS_WS_MAX(hd) (131072ull * ((hd) + 2))
 int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kcache, const void* vcache, uint32_t S, uint32_t pos0,
                           uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t cap, float scale, void* out, int out_dtype,
                           const vsl_attn_mods* mods, void* workspace, uint64_t ws_bytes, void* stream);

@@ -1,4 +1,7 @@
-"""Workspace sizes of prompt attention with modified scores: for any arguments."""
+"""Workspace sizes of prompt attention with modified scores: for any arguments, and never more than
+what serves every call."""
+import random
+
 import pytest
 
 
@@ -13,3 +16,17 @@ def ws(vsl):
 def test_sizes_that_no_call_takes(ws, S, pos0, n_q, n_kv):
     """A number of blocks that does not fit 32 bits is many blocks, not none."""
     assert ws(S, pos0, n_q, n_kv, 128) == 0
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_one_size_serves_every_call(vsl, ws, hd):
+    rng = random.Random(hd)
+    most, some = vsl.ATTN_MODS_WS_MAX(hd), 0
+    for n_kv in (1, 2, 3, 8, 40, 256, 1000):
+        for g in range(1, 9):
+            for _ in range(200):
+                S, pos0 = int(2 ** rng.uniform(0, 14)), int(2 ** rng.uniform(0, 24))
+                n = ws(S, pos0, n_kv * g, n_kv, hd)
+                assert n <= most, (S, pos0, n_kv * g, n_kv)
+                some = max(some, n)
+    assert some > most // 2

@@ -34,6 +34,13 @@ GEMM_A_X2, GEMM_C_X2, GEMM_A_F8, GEMM_C_F8 = 0x100, 0x200, 0x400, 0x800
 def GEMM_B8_SHIFT(s):
     """VSL_GEMM_B8_SHIFT(s): the weight shift of the fp8 lo product (B rounded to e4m3 as B * 2^s)."""
     return ((s + 128) & 0xFF) << 16
+
+
+def ATTN_MODS_WS_MAX(hd):
+    """VSL_ATTN_MODS_WS_MAX(hd): bytes of workspace that serve every call of vsl_attn_prefill_mods."""
+    return 131072 * (hd + 2)
+
+
 SAMPLE_GREEDY, SAMPLE_REFERENCE, SAMPLE_TOPK_SEEDED = 0, 1, 2
 MAX_TOP_K = 262144  # VSL_MAX_TOP_K: the seeded top-k serves 1 <= min(top_k, V) <= MAX_TOP_K
 EPI_STORE_F32, EPI_STORE_F16, EPI_RESID, EPI_SWIGLU = 0, 1, 2, 3

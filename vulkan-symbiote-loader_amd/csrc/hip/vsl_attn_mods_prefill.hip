@@ -602,7 +602,8 @@ uint32_t chunks_of(uint32_t S, uint32_t pos0, uint32_t n_q, uint32_t n_kv) {
     return (uint32_t)std::min<uint64_t>({256 / blocks, tiles / 3, 32});
 }
 
-// A chunk's partial sums: whole query tiles.
+// A chunk's partial sums: whole query tiles. With at most 256 / blocks chunks, and a block for four query tiles at most, all of them
+// together are VSL_ATTN_MODS_WS_MAX(hd) = 256 * 4 * 32 * (hd + 2) * 4 bytes or less, whatever the call.
 uint64_t part_bytes(uint32_t S, uint32_t n_q, uint32_t hd) { return ((uint64_t)S + 31) / 32 * 32 * n_q * (hd + 2) * 4; }
 
 bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
