@@ -165,7 +165,7 @@ template <int HD, bool QX2, bool CAP>
 __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
     constexpr int CPR = HD / 8, NCH = kTK * CPR / kThreads, QP = QX2 ? 2 : 1, ND = HD / 32;
     static_assert(NCH >= 1 && kTK * CPR % kThreads == 0, "a tile divides over the block");
-    __shared__ __attribute__((aligned(16))) vsl_half s_tiles[2 * kBufs][kTK * HD];  // K's buffers, then V's
+    __shared__ __attribute__((aligned(256))) vsl_half s_tiles[2 * kBufs][kTK * HD];  // K's buffers, then V's
     vsl_half(*Ks)[kTK * HD] = s_tiles;
     vsl_half(*Vs)[kTK * HD] = s_tiles + kBufs;
     __shared__ __attribute__((aligned(16))) vsl_half s_q[kTiles][QP * 32 * HD];
@@ -282,6 +282,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_prefill_mods(PrefillArgs a) {
     // address xor a constant. (The address passes through an empty asm, or the compiler keeps all of them in registers.)
     typedef __attribute__((address_space(3))) const char* lds_ptr;
     constexpr int kTile = kTK * HD * 2;  // bytes
+    static_assert(__alignof__(s_tiles) >= HD * 2, "an xor of the address is one of the chunk where rows start at multiples of their size");
     const uint32_t k_at = (uint32_t)(uintptr_t)(lds_ptr)&Ks[0][swizzle<HD>(share * 32 + (lane & 31), lane >> 5)];
     auto qk = [&](int buf, float16v& st) __attribute__((always_inline)) {
 #pragma unroll
