@@ -554,7 +554,7 @@ int vsl_attn_prefill_kv4_window(const void* q, int q_dtype, const void* kcache, 
  * that it reaches infinite or NaN.
  * ------------------------------------------------------------------------------------------ */
 typedef struct vsl_attn_mods { /* host memory, read during the call; NULL for the call: no modification */
-    float softcap;             /* 0: none; scale / softcap and softcap * log2(e) finite */
+    float softcap;             /* 0: none; scale / softcap (but for a scale of 0) and softcap * log2(e) normal numbers */
     uint32_t pad;
     const float* slopes;
     const uint32_t* ranges;

@@ -92,3 +92,30 @@ def test_masked_values_stay_out_in_every_form(vsl, H, dev, x2, odt, hd, pos0):
             ok = close(got, qv, K, V, pos0, 0.1, x2, odt, **kw)
             assert np.all(ok[np.r_[0:32, 41:100]]), (bad, ws)
             assert not got[99].any()
+
+
+@pytest.mark.parametrize("x2", [True, False])
+def test_caps_from_small_to_large(vsl, H, dev, x2):
+    """Caps on both sides of those whose polynomial has coefficients within fp32's range, scores from far below to far above them."""
+    rng = np.random.default_rng(31)
+    S, hd = 70, 128
+    K, V, kc, vc = base.caches(rng, 2, S, hd, S, np.float16)
+    q = rng.normal(0, 30, (S, 4, hd)).astype(np.float32)
+    for cap in (0.01, 2.0, 89.0, 92.0, 500.0, 2000.0, 2500.0, 1e5, 1e30):
+        for scale in (0.0884, 0.002):
+            got, qv = base.prompt(vsl, H, dev, q, kc, vc, 0, scale, base.mods(vsl, dev, cap), x2)
+            assert np.all(close(got, qv, K, V, 0, scale, x2, 1, softcap=cap)), (cap, scale)
+
+
+def test_scale_and_cap_near_the_largest_number(vsl, H, dev):
+    """Keys of zeros: every score is 0, whatever the scale and the cap, and rows are means of the values."""
+    rng = np.random.default_rng(32)
+    S, hd = 40, 64
+    K, V, kc, vc = base.caches(rng, 1, S, hd, S, np.float16)
+    K[:], kc[:] = 0, 0
+    q = rng.normal(0, 1, (S, 2, hd)).astype(np.float32)
+    for scale, cap in ((3e38, 3e37), (-3e38, 3e37), (3e38, 2e38), (1e-30, 1e-30), (0.0, 2e38), (2e-20, 1e15)):
+        got, qv = base.prompt(vsl, H, dev, q, kc, vc, 0, scale, base.mods(vsl, dev, cap), True, 2)
+        assert np.all(close(got, qv, K, V, 0, scale, True, 2, softcap=cap)), (scale, cap)
+        row = base.decode(vsl, H, dev, q[-1], kc, vc, S - 1, scale, base.mods(vsl, dev, cap), nsplit=3)
+        assert base.decode_ok(row, q[-1], K, V, S - 1, scale, np.float16, cap), (scale, cap)

@@ -1,5 +1,6 @@
-"""Workspace sizes of prompt attention with modified scores: for any arguments, and never more than
-what serves every call."""
+"""Limits of attention with modified scores that the host checks: workspace sizes, which never divide by zero and never exceed
+what serves every call, and caps."""
+import ctypes
 import random
 
 import pytest
@@ -30,3 +31,14 @@ def test_one_size_serves_every_call(vsl, ws, hd):
                 assert n <= most, (S, pos0, n_kv * g, n_kv)
                 some = max(some, n)
     assert some > most // 2
+
+
+def test_factors_below_the_normal_numbers_are_refused(vsl):
+    """scale / softcap and softcap * log2(e) would lose digits."""
+    H = vsl.hip()
+    buf = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(buf) + 255) & ~255
+    for scale, cap in ((0.09, 2e38), (-0.09, 2e38), (1e-20, 1e19), (1e-38, 2e38), (1e-45, 1.0), (1e-40, 1e-40), (1e-39, 7e-39)):
+        m = ctypes.byref(vsl.AttnMods(softcap=cap))
+        assert H.vsl_attn_prefill_mods(p, 1, p, p, 4, 0, 8, 2, 128, 64, scale, p, 1, m, None, 0, None) == -100, (scale, cap)
+        assert H.vsl_attn_decode_mods(p, p, p, 1, 8, 2, 128, 64, scale, 4, p, p, p, p, m, None) == -100, (scale, cap)

@@ -61,9 +61,10 @@ __device__ __forceinline__ int swizzle(int r, int c) {
 // Whether a word of two halfs holds an infinity or a NaN: the carry out of an exponent of ones, in bit 15 of either half.
 __device__ __forceinline__ uint32_t odd_halfs(uint32_t w) { return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
 
-// Whether a cap can be used with a scale: both factors of a score, scale / softcap and softcap * log2(e), within 32 bits.
+// Whether a cap can be used with a scale: both factors of a score, scale / softcap and softcap * log2(e), normal numbers of 32 bits
+// (below, they have fewer digits).
 inline bool softcap_ok(float softcap, float scale) {
-    return softcap == 0.f || (softcap > 0.f && std::isfinite(softcap * kLog2e) && (std::isfinite(scale / softcap) || !std::isfinite(scale)));
+    return softcap == 0.f || (softcap > 0.f && std::isnormal(softcap * kLog2e) && (std::isnormal(scale / softcap) || scale == 0.f || !std::isfinite(scale)));
 }
 
 }  // namespace attn_mods

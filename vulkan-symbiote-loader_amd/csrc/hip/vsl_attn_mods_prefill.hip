@@ -22,7 +22,7 @@ struct PrefillArgs {
     uint32_t S, pos0, n_q, n_kv, cap, G, n_chunk;
     float to_u;    // scale / softcap, or scale * log2(e) without a cap
     float from_u;  // softcap * log2(e)
-    float near;    // |q.k| up to which the polynomial is tanh (0: never)
+    float near;    // |q.k| up to which the polynomial is tanh (below 0: never)
     float poly[kTanhTerms];  // its coefficients, in q.k and times softcap * log2(e)
     int out_mode;  // 0 fp16, 1 hi / lo fp16 planes, 2 fp16 + fp8 planes
     const float* slopes;
@@ -658,11 +658,15 @@ extern "C" int vsl_attn_prefill_mods(const void* q, int q_dtype, const void* kca
     a.n_chunk = chunks;
     a.to_u = capped ? scale / md.softcap : scale * kLog2e;
     a.from_u = md.softcap * kLog2e;
-    // the polynomial in q.k itself, while its highest power of to_u is far from underflow (a cap of 50 at head_dim 128: 2^-9.1)
-    if (capped && std::fabs(a.to_u) >= 0x1p-10f && std::fabs(a.to_u) <= 0x1p10f) {
-        a.near = kTanhNear / std::fabs(a.to_u);
+    // the polynomial in q.k itself, where its coefficients are normal numbers (at head_dim 128 caps of 4e-5 to 2200)
+    if (capped) {
+        bool normal = true;
         double f = (double)a.from_u * a.to_u;
-        for (int i = 0; i < kTanhTerms; ++i, f *= (double)a.to_u * a.to_u) a.poly[i] = (float)(kTanhPoly[i] * f);
+        for (int i = 0; i < kTanhTerms; ++i, f *= (double)a.to_u * a.to_u) {
+            a.poly[i] = (float)(kTanhPoly[i] * f);
+            normal = normal && std::isnormal(a.poly[i]);
+        }
+        a.near = normal ? kTanhNear / std::fabs(a.to_u) : -1.f;
     }
     a.out_mode = out_dtype == VSL_DT_F16X2 ? 1 : out_dtype == VSL_DT_F16F8 ? 2 : 0;
     a.slopes = md.slopes;
