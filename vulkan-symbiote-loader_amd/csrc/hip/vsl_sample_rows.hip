@@ -81,7 +81,7 @@ __device__ __forceinline__ RowParams row_params(const vsl_row_sampler& s, uint32
 struct SliceRec {
     uint64_t top;     // the largest rank key (0: nothing above -inf)
     uint32_t count;   // TOPK: tokens found (kLeanCap of them stored); HIST: bins up to the last one that holds a token
-    float floor_v;    // TOPK: all tokens of the slice at or above this value are in its list, and there are k of them (-inf: all)
+    float floor_v;    // TOPK: all tokens of the slice at or above this value are in its list, and there are k of them (-inf: all that can be drawn)
     double sum;       // weights kept for sure
 };
 
@@ -477,6 +477,14 @@ __device__ __forceinline__ void draw_few(Shared& sh, uint64_t* list, uint32_t n,
     if (t < n && (mine & 0xFFFFFFFFull) + 1 == sh.sel_key) put(out, index_of(mine), w * kFewOne / (double)sum);
 }
 
+// The smallest value that can be drawn beside one of vmax: 64 temperatures below it weights are 2^-92. Top-k lists leave out what
+// lies further down, or a mask of finite values (-1e9, the type's lowest) would count among the k largest where fewer are allowed,
+// fill the lists and send the row to the draw over the whole row: 1 x 32000 with 20 allowed 567 us,
+// 30 now (slices of masked tokens alone still list theirs), 11 with -infinity; with 1000 allowed 15 either way.
+__device__ __forceinline__ float least_drawn(float vmax, float temperature) {
+    return (float)((double)vmax - 64.0 * (double)temperature);
+}
+
 // Bin of a value on the grid that all slices share: floor(8 l / T), as a double (exact to 2^53, and monotone above).
 __device__ __forceinline__ double bin_of(float v, double inv_t) { return floor((double)v * inv_t * 8.0); }
 __device__ __forceinline__ uint32_t bin_below(double top_bin, double bin) { return (uint32_t)fmin(top_bin - bin, (double)(kBins - 1)); }
@@ -536,7 +544,8 @@ __global__ __launch_bounds__(kThreads) void k_rows_scan(const T* __restrict__ lo
         const uint32_t e = first + i * kThreads + t;
         v[i] = e < V ? load_logit(l, e) : -INFINITY;
     }
-    const RowParams rp = row_params(params[row], V);
+    const vsl_row_sampler ps = params[row];
+    const RowParams rp = row_params(ps, V);
     if (slice == 0 && t == 0) ws.counters[row * kCounter] = 0;
 #pragma unroll
     for (uint32_t b = 0; b < kBins; b += kThreads) s_hist[b + t] = 0;
@@ -561,9 +570,10 @@ __global__ __launch_bounds__(kThreads) void k_rows_scan(const T* __restrict__ lo
     if (rp.mode == MODE_GREEDY || rp.mode == MODE_SUM) return;
     if (rp.mode == MODE_TOPK) {
         // threads' maxima in bins between their largest and their smallest: the bin of the k-th bounds the k-th token
-        const ValueBins bin(top ? value_of(top) : 0.f, top ? value_of(~low_key) : 0.f);
+        const float hi = top ? value_of(top) : 0.f, least = least_drawn(hi, ps.temperature);
+        const ValueBins bin(hi, top ? fmaxf(value_of(~low_key), least) : 0.f);
         uint32_t* count = reinterpret_cast<uint32_t*>(s_hist);
-        if (best) atomicAdd(&count[bin(mx)], 1u);
+        if (best && mx >= least) atomicAdd(&count[bin(mx)], 1u);
         __syncthreads();
         if (t < 64) find_kth(count, rp.k, &sh.sel_count);
         __syncthreads();
@@ -571,7 +581,7 @@ __global__ __launch_bounds__(kThreads) void k_rows_scan(const T* __restrict__ lo
         uint64_t* list = ws.lists + (size_t)row * ws.list_stride + (size_t)slice * kLeanCap;
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
-            if (v[i] == -INFINITY || bin(v[i]) > cut) continue;
+            if (v[i] == -INFINITY || v[i] < least || bin(v[i]) > cut) continue;
             const uint32_t at = atomicAdd(&s_n, 1u);
             const uint64_t r = rank_of(v[i], first + i * kThreads + t);
             if (at < kLeanCap) list[at] = r;
@@ -667,7 +677,9 @@ __global__ __launch_bounds__(kThreads) void k_rows_cut(const T* __restrict__ log
     const double vmax = (double)value_of(top);
 
     if (rp.mode == MODE_TOPK) {
-        // the slices' tokens at or above the highest of their bounds
+        // the slices' tokens at or above the highest of their bounds, and of what can be drawn
+        const uint64_t drawn = rank_of(least_drawn((float)vmax, ps.temperature), 0xFFFFFFFFu);
+        bound = drawn > bound ? drawn : bound;
         const uint64_t* lists = ws.lists + (size_t)row * ws.list_stride;
         auto take = [&](uint64_t r) {
             if (r < bound || r == 0) return;
@@ -689,7 +701,7 @@ __global__ __launch_bounds__(kThreads) void k_rows_cut(const T* __restrict__ log
                     for (uint32_t i = 64 + lane; i < min(s_count[s], kLeanCap); i += 64) take(lists[(size_t)s * kLeanCap + i]);
             }
         }
-        const bool over = __syncthreads_or(my_count > kLeanCap);
+        const bool over = __syncthreads_or(my_count > kLeanCap && my_top >= bound);
         const uint32_t n = s_n;
         const bool whole = over || n > kLeanList;
         if (t == 0) ws.row[row].whole = whole;
