@@ -1039,7 +1039,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         const float x = from + i < V ? load_logit(l, from + i) : -INFINITY;
-        const double wx = weight_of(x, vmax, rp.inv_t);  // (a select: zeroed in a branch, an element kept an old value in the built code)
+        const double wx = weight_of(x, vmax, rp.inv_t);
         w[i] = x != -INFINITY && kept(rank_of(x, from + i), wx) ? wx : 0.0;
         mine += w[i];
         if (w[i] > 0.0) last = from + i + 1;
