@@ -118,25 +118,48 @@ def test_finite_masks_are_masks(vsl, H, dev, V, dt):
     assert not tok.any()
 
 
+def fastest(H, vsl, dev, logits, params):
+    """The shortest of nine times of 20 calls, in ms."""
+    torch, (rows, V) = dev.torch, logits.shape
+    n = H.vsl_sample_rows_ws_bytes(rows, V)
+    ws, par, u = dev.empty((n,), np.uint8), dev.put(base.structs(params)), dev.put(np.full(rows, 0.4, np.float32))
+    tok, l, took = dev.empty((rows,), np.int32), dev.put(logits), []
+    for _ in range(9):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        for _ in range(20):
+            vsl.check(H.vsl_sample_rows(dev.p(l), 0, rows, V, V, dev.p(par), dev.p(u), dev.p(tok), None, dev.p(ws), n, None))
+        b.record()
+        dev.sync()
+        took.append(a.elapsed_time(b))
+    return min(took)
+
+
 def test_cost_of_a_finite_mask(vsl, H, dev):
     """A step with 20 tokens allowed takes about as long with a finite mask as with -infinity: 2.6 times, where it took 48 times as
     long when the masked tokens counted among the k largest."""
-    torch, rng = dev.torch, np.random.default_rng(5)
-    V, times = 32000, []
-    allowed = rng.permutation(V)[:20]
-    n = H.vsl_sample_rows_ws_bytes(1, V)
-    ws, par, u = dev.empty((n,), np.uint8), dev.put(base.structs([(0.7, 40, 0.9, 0.0)])), dev.put(np.array([0.4], np.float32))
-    tok = dev.empty((1,), np.int32)
-    for value in (-np.inf, -1e9, np.finfo(np.float32).min):
-        l = dev.put(masked(rng.normal(0, 2.5, V).astype(np.float32), allowed, value))
-        took = []
-        for _ in range(9):
-            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
-            a.record()
-            for _ in range(20):
-                vsl.check(H.vsl_sample_rows(dev.p(l), 0, 1, V, V, dev.p(par), dev.p(u), dev.p(tok), None, dev.p(ws), n, None))
-            b.record()
-            dev.sync()
-            took.append(a.elapsed_time(b))
-        times.append(min(took))
+    rng = np.random.default_rng(5)
+    allowed, logits = rng.permutation(32000)[:20], rng.normal(0, 2.5, 32000).astype(np.float32)
+    times = [fastest(H, vsl, dev, masked(logits, allowed, v)[None], [(0.7, 40, 0.9, 0.0)]) for v in (-np.inf, -1e9, np.finfo(np.float32).min)]
     assert max(times[1:]) < 8 * times[0], times
+
+
+@pytest.mark.parametrize("rows,V", [(1, 32000), (1, 131072), (16, 131072), (64, 32000)])
+def test_cost_of_a_larger_k(vsl, H, dev, rows, V):
+    """A row with k up to 128, whose tokens come from the slices' lists, takes no longer than one with k = 200, which is cut by bins
+    (7 to 35 times as long when the lists together held more than 1024 tokens)."""
+    logits = np.random.default_rng(V).normal(0, 2.5, (rows, V)).astype(np.float32)
+    times = [fastest(H, vsl, dev, logits, [(0.7, k, 0.9, 0.0)] * rows) for k in (200, 40, 64, 100, 128)]
+    assert max(times[1:]) < 3 * times[0], times
+
+
+@pytest.mark.parametrize("rows,V", [(1, 32000), (3, 50000), (1, 131072), (16, 131072), (2, 1 << 20)])
+def test_long_lists(vsl, H, dev, rows, V):
+    """k up to 128 from few and many slices, with ties where the lists end."""
+    rng = np.random.default_rng(rows + V)
+    for k in (40, 64, 100, 127, 128):
+        for step in (0.0, 0.25):
+            logits = rng.normal(0, 2.5, (rows, V)).astype(np.float32)
+            if step:
+                logits = (np.round(logits / step) * step).astype(np.float32)
+            base.check(vsl, H, dev, logits, [(0.9, k, 0.95, 0.0)] * rows, rng.random(rows))

@@ -37,10 +37,12 @@ namespace {
 constexpr int kThreads = 256, kDrawThreads = 512;
 constexpr uint32_t kMaxSlices = 128, kMaxEpt = 32;
 constexpr uint32_t kMaxRowsV = kMaxSlices * kMaxEpt * kThreads;  // 2^20 tokens
-constexpr uint32_t kLeanK = 128;     // TOPK up to this k
+// TOPK up to this k, HIST above. us, TOPK / HIST: k = 40 of 32000 15 / 22, of 131072 19 / 27, 64 rows of it 30 / 58; k = 128 25 / 23,
+// 39 / 30, 47 / 59.
+constexpr uint32_t kLeanK = 128;
 constexpr uint32_t kLeanCap = 256;   // TOPK: tokens a slice's list holds
 constexpr int kLeanRegs = 4, kDrawRegs = 4;  // tokens of a list that a thread holds
-constexpr uint32_t kLeanList = kLeanRegs * kThreads, kListCap = 32768;  // tokens of a row's list: TOPK, HIST
+constexpr uint32_t kLeanList = kLeanRegs * kThreads, kListCap = 32768;  // tokens of a row's list: TOPK (in LDS), HIST
 constexpr uint32_t kFinish = 256;    // keys that are left to a key a thread
 constexpr uint32_t kBins = 512;     // of 1/8 in l / T; the last one takes all below e^-63.9 of the largest, never drawn
 constexpr int kBinFrac = 36;        // weights in a bin: what they lie below its upper edge (up to .1175), in units of 2^-36
@@ -89,7 +91,7 @@ struct RowRec {
     uint32_t kb, plo, phi, sure;  // HIST: the bin of the k-th token, those in which the top-p cut can fall, those kept whole
     uint32_t cut_k, k_left;       // whether k ends within its bin, and how many of that bin's tokens count
     double lo_total, hi_total;    // the first k tokens' weights, without and with the k-th's bin
-    uint32_t whole;               // TOPK: the lists do not hold the tokens
+    uint32_t whole;               // TOPK: the lists do not hold the tokens, or too many of the same size
     double cum_w[kBins];          // HIST: weights up to and with each bin
 };
 
@@ -681,35 +683,42 @@ __global__ __launch_bounds__(kThreads) void k_rows_cut(const T* __restrict__ log
         const uint64_t drawn = rank_of(least_drawn((float)vmax, ps.temperature), 0xFFFFFFFFu);
         bound = drawn > bound ? drawn : bound;
         const uint64_t* lists = ws.lists + (size_t)row * ws.list_stride;
-        auto take = [&](uint64_t r) {
-            if (r < bound || r == 0) return;
+        auto each = [&](auto f) {
+            auto take = [&](uint64_t r) {
+                if (r >= bound && r != 0) f(r);
+            };
+            for (uint32_t s0 = wave; s0 < nsl; s0 += 4 * (NT / 64)) {  // four slices' first 64 entries at a time
+                uint64_t r[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t s = s0 + j * (NT / 64);
+                    r[j] = s < nsl && lane < s_count[s] ? lists[(size_t)s * kLeanCap + lane] : 0;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t s = s0 + j * (NT / 64);
+                    take(r[j]);
+                    if (s < nsl)
+                        for (uint32_t i = 64 + lane; i < min(s_count[s], kLeanCap); i += 64) take(lists[(size_t)s * kLeanCap + i]);
+                }
+            }
+        };
+        each([&](uint64_t r) {
             const uint32_t at = atomicAdd(&s_n, 1u);
             if (at < kLeanList) s_list[at] = r;
-        };
-        for (uint32_t s0 = wave; s0 < nsl; s0 += 4 * (NT / 64)) {  // four slices' first 64 entries at a time
-            uint64_t r[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t s = s0 + j * (NT / 64);
-                r[j] = s < nsl && lane < s_count[s] ? lists[(size_t)s * kLeanCap + lane] : 0;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t s = s0 + j * (NT / 64);
-                take(r[j]);
-                if (s < nsl)
-                    for (uint32_t i = 64 + lane; i < min(s_count[s], kLeanCap); i += 64) take(lists[(size_t)s * kLeanCap + i]);
-            }
-        }
+        });
         const bool over = __syncthreads_or(my_count > kLeanCap && my_top >= bound);
         const uint32_t n = s_n;
-        const bool whole = over || n > kLeanList;
-        if (t == 0) ws.row[row].whole = whole;
-        if (whole) return;
-        // each slice's k-th bounds them: of k = 40 from 16 slices 490 are left, so they are binned once more
+        // each slice's k-th bounds them: of k = 40 from 16 slices 490 are left, from 32 slices 1000, so they are binned once more; what
+        // s_list does not hold is read again for that (16 x 131072 with k = 40 took 741 us when it sent a row to the draw over the
+        // whole row, 1 x 32000 with k = 100 211)
+        auto listed = [&](auto f) {
+            if (n > kLeanList) return each(f);
+            for (uint32_t i = t; i < n; i += NT) f(s_list[i]);
+        };
         uint32_t m = n;
         uint64_t* few = s_list;
-        if (n > rp.k && n > 64) {
+        if (n > rp.k && n > 64 && !over) {
             const ValueBins bin((float)vmax, bound ? value_of(bound) : (float)vmax);
             few = reinterpret_cast<uint64_t*>(s_cum_w);
 #pragma unroll
@@ -719,20 +728,22 @@ __global__ __launch_bounds__(kThreads) void k_rows_cut(const T* __restrict__ log
                 sh.n = 0;
             }
             __syncthreads();
-            for (uint32_t i = t; i < n; i += NT) atomicAdd(&s_cum_n[bin(value_of(s_list[i]))], 1u);
+            listed([&](uint64_t x) { atomicAdd(&s_cum_n[bin(value_of(x))], 1u); });
             __syncthreads();
             if (t < 64) find_kth(s_cum_n, rp.k, &sh.sel_count);
             __syncthreads();
             const uint32_t cut = sh.sel_count;
-            for (uint32_t i = t; i < n; i += NT) {
-                const uint64_t x = s_list[i];
-                if (bin(value_of(x)) > cut) continue;
+            listed([&](uint64_t x) {
+                if (bin(value_of(x)) > cut) return;
                 const uint32_t at = atomicAdd(&sh.n, 1u);
                 if (at < kThreads) few[at] = x;
-            }
+            });
             __syncthreads();
             m = sh.n;
         }
+        const bool whole = over || (m > kThreads && n > kLeanList);
+        if (t == 0) ws.row[row].whole = whole;
+        if (whole) return;
         if (m <= kThreads) {
             draw_few(sh, few, m, rp, vmax, u, out);
             return;
