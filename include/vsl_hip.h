@@ -422,8 +422,10 @@ int vsl_sample_logits(const float* logits, uint32_t V, vsl_sampler sampler, uint
  * maximum, with share 1.  u below 0 or NaN counts as 0, 1 and above as the largest float below 1.  NaN logits count as
  * -infinity, +infinity as the largest float; a row of -infinity gives token 0 with share 0.  Weights below about 2^-91
  * of the largest may count as 0.  Weights are summed in 64 bits: the token is that of exact sums but where u or the top-p cut
- * lies within 1e-10 of a border, as a share of the total; u = 0 gives the first kept token.  V up to 2^20, up to 65535 rows;
- * workspace 16-byte aligned, vsl_sample_rows_ws_bytes(rows, V) bytes (0 for sizes that are not served). */
+ * lies within 1e-10 of a border, as a share of the total; u = 0 gives the first kept token.  Rows whose cut falls among more
+ * than 32768 tokens of nearly equal logits (256 in 2048 for top_k up to 128), or with |max l / temperature| above 16384, are cut
+ * by one block, 10 to 50 times slower (1 x 131072 up to 1.7 ms); finite masks cost up to 3 times what -infinity does.  V up to
+ * 2^20, up to 65535 rows; workspace 16-byte aligned, vsl_sample_rows_ws_bytes(rows, V) bytes (0 for sizes not served). */
 typedef struct vsl_row_sampler {
     float temperature;
     uint32_t top_k;
@@ -549,9 +551,10 @@ int vsl_attn_prefill_kv4_window(const void* q, int q_dtype, const void* kcache, 
  *                   documents, prefixes that see themselves whole, windows, padding; NULL: 0 <= k <= p)
  * then softmax over the keys attended to.  `end` counts up to the positions that the call can know: pos0 + S in
  * vsl_attn_prefill_mods, ctrl->pos + 1 in vsl_attn_decode_mods.  A row without keys gives zeros.  What masked
- * positions hold, infinities and NaN among it, reaches no result.  Among the keys attended to, a NaN or an infinity makes
- * its rows NaN, or a weight 0 or 1 where the sum of its products is infinite; among the values, it makes the outputs
- * that it reaches infinite or NaN.
+ * positions hold, infinities and NaN among it, reaches no result.  (Values that are not finite within 64 positions of a
+ * range's begin or end, or of a row's own position, slow vsl_attn_prefill_mods down, 20 to 100 times: clear a cache whose
+ * padding is never written.)  Among the keys attended to, a NaN or an infinity makes its rows NaN, or a weight 0 or 1 where
+ * the sum of its products is infinite; among the values, it makes the outputs that it reaches infinite or NaN.
  * ------------------------------------------------------------------------------------------ */
 typedef struct vsl_attn_mods { /* host memory, read during the call; NULL for the call: no modification */
     float softcap;             /* 0: none; scale / softcap (but for a scale of 0) and softcap * log2(e) normal numbers */
@@ -560,7 +563,8 @@ typedef struct vsl_attn_mods { /* host memory, read during the call; NULL for th
     const uint32_t* ranges;
 } vsl_attn_mods;
 /* vsl_attn_decode with modified scores: arguments as there; caches VSL_DT_F16 or VSL_DT_F32, head_dim 64 or 128, any GQA
- * ratio 1..8, 1..1024 splits; over fp16 caches |q| < 65504 (two fp16 planes); q, caches, part_o and out 16-byte, part_ml 8-byte aligned. */
+ * ratio 1..8, 1..1024 splits; over fp16 caches |q| < 65504, taken as two fp16 planes (2^-22 of each value or 2^-25); q, caches,
+ * part_o and out 16-byte, part_ml 8-byte aligned. */
 int vsl_attn_decode_mods(const float* q, const void* kcache, const void* vcache, int kv_dtype, uint32_t n_q, uint32_t n_kv,
                          uint32_t hd, uint32_t cap, float scale, uint32_t nsplit, float* part_o, float* part_ml, float* out,
                          vsl_ctrl* ctrl, const vsl_attn_mods* mods, void* stream);

@@ -155,9 +155,12 @@ __device__ __noinline__ void rows_one_by_one(const PrefillArgs& a, uint32_t rb, 
 // are joined through LDS at the end.
 // Bound: the two products (4 head_dim flops a row and key, twice as many for a split q) and, for every score, a dozen vector
 // instructions of cap, exponential and rounding; LDS, which each query tile reads anew, is as busy as the matrix cores. 2048 rows
-// at 6144 of the 8B shape, split q, cap 30: 509 us, 946 TFLOP/s in products where a large plain fp16 product reaches 1080 on this
-// card. With the probabilities in one plane, 424 there, slower were: the next tile's K in registers ahead of its product 451 to
-// 470, products and vector code mixed by scheduling barriers 485.
+// at 6144 of the 8B shape, split q, cap 30: 506 us whatever the output's type, 951 TFLOP/s in products where a large plain fp16
+// product reaches 1084 on this card. Under the counters the clock is 2.05 GHz, the matrix cores are busy 44 % of the cycles and
+// vector instructions are issued in 50 %; LDS has no bank conflicts. Single-plane q 350; without a cap 479; scores past 0.64 of the
+// cap (tanh by its exponential) 630; a distance bias, whose tiles take the general way, 528, with the cap 595. With the
+// probabilities in one plane, 424 there, slower were: the next tile's K in registers ahead of its product 451 to 470, products and
+// vector code mixed by scheduling barriers 485.
 // A row's keys are a range [lo, hi); tiles that lie within the ranges of all of a wave's rows take no masks, and tiles
 // outside all of them are skipped. In the others a masked probability is 0; where V then holds an infinity or a NaN, whose
 // product with 0 would reach the sums, the query tile's rows are computed again, one by one (rows_one_by_one).
@@ -595,8 +598,11 @@ uint64_t blocks_of(uint32_t S, uint32_t n_q, uint32_t n_kv) {
     return (n_qt + kTiles - 1) / kTiles * n_kv;
 }
 
-// Key chunks: as many as fill the CUs, none shorter than three tiles of the longest rows; calls of less than 12 tiles are not
-// worth the join (512 rows of the 1B shape 12.4 us, in two chunks 16.8 at the time; 45 rows at 3001 26.1 in 16 chunks, 27.9 in 12, 35.7 in 6; 19.6 now).
+// Key chunks: as many as fill the CUs (45 rows at 3001 of the 8B shape 19.4 us, half as many 23.1; at 20000 59.6, half as many 98.7, up
+// to two blocks a CU 66.8), none shorter than three tiles of the longest rows (45 rows at 3001 two tiles 19.4, four 20.7, six 23.1; 5
+// rows at 2500 16.3, 19.0 and 22.7 against 18.2). Calls of less than 12 tiles run unsplit: 512 packed rows of the 1B shape 11.4,
+// in two chunks 15.4; the rule goes by pos0 + S, not by what rows see, and 45 rows at 600 of the 8B shape would take 17.2 split
+// instead of 28.
 uint32_t chunks_of(uint32_t S, uint32_t pos0, uint32_t n_q, uint32_t n_kv) {
     const uint64_t blocks = blocks_of(S, n_q, n_kv), tiles = ((uint64_t)pos0 + S + kTK - 1) / kTK;
     if (blocks >= 256 || tiles < 12) return 1;

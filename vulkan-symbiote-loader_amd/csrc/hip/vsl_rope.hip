@@ -79,8 +79,8 @@ struct PartArgs {
 
 // Four dims a lane; bpr blocks a row. A rotated dim's partner is read again from the row (it is in the same lines).
 // VEC: rot % 8 == 0, so that four dims are rotated or not as one and the partners and angles of a halves' rotation are
-// aligned vectors; otherwise dim by dim. Bound by the projection read and the outputs written: 2048 rows of the 8B shape, 32
-// dims of each head, split q: 92 MB in 16.4 us (5.6 TB/s; 19.2 with the launch); a token 4.0.
+// aligned vectors; otherwise dim by dim (36 dims instead of 32: by halves 30.3 us instead of 19.2, by pairs 19.7). Bound by the projection read and the outputs written: 2048 rows of the 8B shape, 32
+// dims of each head, split q: 92 MB in 16.4 us (5.6 TB/s; 19.2 with the launch; fp32 caches 21.8); a token 4.0.
 template <bool VEC, int QM, typename KT, bool DEC>
 __global__ __launch_bounds__(256) void k_rope_part(PartArgs a, uint32_t bpr, vsl_ctrl* ctrl) {
     const uint32_t s = blockIdx.x / bpr;

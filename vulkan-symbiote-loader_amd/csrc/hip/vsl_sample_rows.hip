@@ -17,13 +17,16 @@
 //           that no slice has to know the row's maximum
 // k_rows_cut ends GREEDY and TOPK rows in one block; for SUM its blocks sum the kept weights of the slices, for HIST each
 // joins the slices' bins, which tells in which bins a cut falls, and collects its tokens of those. k_rows_draw, a block a
-// row, finds the cuts among the collected tokens, the slice in which u falls and the token there. Where ties or ranges make
-// a list too long, it narrows the cuts down over the whole row instead. (The last block of the second kernel to arrive
-// took the draw at first: its fences write the L2 caches back, and a pass over one row of 131072 took 66 us.)
+// row, finds the cuts among the collected tokens, the slice in which u falls and the token there. (The last
+// block of the second kernel to arrive took the draw at first: its fences write the L2 caches back, and a pass over one row of
+// 131072 took 66 us.) Where ties or ranges make a list too long, it narrows the cuts down over the whole row instead, which is
+// slow, one block and several passes: more than 32768 tokens in the cut's bin (a flat row of 131072 by top-p 1.7 ms, 64 of them
+// 1.8), |max l / T| above 16384 (1.0 ms), a top-k list of more than 256 tokens of a slice within 1/510 of its range (flat, k = 40:
+// 32000 .24 ms, 131072 .9).
 //
 // What bounds it: for few rows the three launches and, within each, a chain of loads, sums over the block and code run for the
-// first time: 1 x 32000 with k = 40 14.9 us, 1 x 131072 with top-p 32 (7 + 11 + 14). For many the two passes over the logits
-// with 64-bit arithmetic per token, and a block a row in the draw: 64 x 131072 of mixed parameters 59 us (20.5 + 20.4 + 20.3;
+// first time: 1 x 32000 with k = 40 14.8 us, 1 x 131072 with top-p 32.5 (7 + 12 + 14). For many the two passes over the logits
+// with 64-bit arithmetic per token, and a block a row in the draw: 64 x 131072 of mixed parameters 59 us (20.9 + 19.6 + 20.5;
 // one read of the 33.6 MB takes about 7).
 #include <float.h>
 
@@ -1078,7 +1081,9 @@ __global__ __launch_bounds__(kDrawThreads) void k_rows_draw(const T* __restrict_
 
 uint64_t up256(uint64_t b) { return (b + 255) & ~255ull; }
 
-// Elements a thread: enough slices to fill the CUs with the rows there are, at most kMaxSlices of them.
+// Elements a thread: enough slices to fill the CUs with the rows there are, at most kMaxSlices of them. us for 8 / 16 / 32, k = 40 and
+// top-p: 1 x 32000 15 / 17 / 19 and 23 / 29 / 39, 1 x 131072 24 / 19 / 20 and 29 / 32 / 42, 64 x 131072 59 / 42 / 30 and
+// 88 / 64 / 62. Between, rows of 32000 would do better with 8: 16 rows 16 / 17 / 20 and 24 / 30 / 41.
 uint32_t elements_per_thread(uint32_t rows, uint32_t V) {
     for (uint32_t e : {8u, 16u})
         if ((uint64_t)rows * ((V + e * kThreads - 1) / (e * kThreads)) <= (e == 8 ? 32 : 1024) && (V + e * kThreads - 1) / (e * kThreads) <= kMaxSlices)
